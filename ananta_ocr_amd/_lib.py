@@ -100,6 +100,23 @@ SIGNATURES = {
     "dash_page_rope_pos": (_i, [_p, _l, _i, _i, _l, _l, _i, _p, _p, _p, _l, _p, _p, _l, _p]),
     "dash_rope2d_cos_sin": (_i, [_p, _p, _l, _i, _i, _p, _i, _p, _i, _i, _p, _p, _i, _l, _l,
                                  _p]),
+    "dash_kbar_pages": (_i, [_p, _l, _l, _p, _p, _p, _p, _l, _p, _i, _i, _i, _i, _i, _p]),
+    "dash_tree_masks": (_i, [_p, _p, _i, _l, _i, _i, _p, _p, _p]),
+    "dash_tree_scores": (_i, [_p, _l, _p, _p, _p, _p, _l, _p, _i, _i, _i, _i, _i, _i, _i, _i, _p, _p,
+                              _p, _l, _p]),
+    "dash_attn_tree_workspace_size": (_i, [_i, _i, _i, _l, _i, _i, _i, _i, _i, ctypes.POINTER(_l)]),
+    "dash_attn_tree": (_i, [_p, _l, _l, _p, _l, _l, _l, _p, _l, _l, _l, _p, _l, _i, _i, _p, _p,
+                            _p, _p, _p, _i, _p, _i, _p, _p, _i, _l, _l, _p, _l, _l,
+                            _i, _i, _i, _l, _i, _i, _i, _i, _i, _f, _p, _l, _p]),
+    "dash_verify_tree_workspace_size": (_i, [_i, _l, _i, _i, ctypes.POINTER(_l)]),
+    "dash_verify_tree": (_i, [_p, _l, _p, _l, _i, _p, _i, _p, _p, _p, _i, _l, _i, _i, _p, _p, _l, _p,
+                              _p, _l, _p]),
+    "dash_copy_pages": (_i, [_i, _p, _p, _p, _p, _i, _i, _p]),
+    "dash_keep_rows": (_i, [_i, _p, _p, _p, _l, _p, _p, _p, _l, _i, _i, _i, _i, _i, _p]),
+    "dash_fork_pages": (_i, [_p, _i, _p, _l, _i, _i, _p, _p, _p, _i, _i, _p, _p, _p, _p]),
+    "dash_reserve_pages": (_i, [_p, _i, _p, _l, _i, _i, _p, _p, _i, _p, _p, _p, _p]),
+    "dash_free_pages": (_i, [_p, _i, _p, _l, _i, _i, _p, _p, _i, _p]),
+    "dash_compact_pages": (_i, [_p, _i, _p, _l, _i, _i, _p, _i, _p, _p, _p, _p, _p, _p]),
     "dash_page_rope_advance": (_i, [_p, _l, _i, _l, _p, _p, _p, _l, _p, _p, _p, _p]),
 }
 

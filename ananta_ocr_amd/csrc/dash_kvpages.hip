@@ -1,0 +1,581 @@
+// Pages of a paged cache on gfx950: copied, shared between sequences (fork), handed out
+// (reserve), given back (free) and moved together (compact), and the rows of accepted drafted
+// tokens moved up in the last pages (keep).
+//
+// The state is three int32 arrays: refs [num_pages], how many block-table entries name a page
+// (0: free); table [R, P], the pages of every sequence row; lens [R], its tokens.  Entry i of a
+// row is in use for i < ceil(len / page).  Free pages are handed out lowest first, to the rows
+// in order, so that a result does not depend on how a launch ran: what is added up by atomics
+// is whole numbers.
+//
+// The table kernels run as one work-group: their data (a few kilobytes) lives in one L2, and
+// what bounds them is the latency of three or four dependent passes, not bandwidth.  The copies
+// are bound by HBM: 16 bytes a lane, several loads in flight before the first store.
+
+#include "dash_common.h"
+
+namespace dash {
+
+constexpr int kKvThreads = 1024;
+constexpr int kKvMaxRows = 8192;      // rows of a table (prefix sums in LDS)
+constexpr int kKvMaxCaches = 32;      // caches per launch (kernel argument space)
+
+// One cache: page p of layer l starts at base + l * layer + p * page bytes; a page holds
+// n1 x n2 pieces of seg bytes at strides s1 and s2.  For rows, s1 is the stride of a token.
+struct KvCache {
+  char* base;
+  int64_t layer, page, s1, s2;
+  int32_t layers, n1, n2, seg;
+};
+struct KvCaches {
+  KvCache c[kKvMaxCaches];
+  int32_t task0[kKvMaxCaches + 1];    // first task of each cache
+  int n;
+};
+
+// The cache that task t belongs to.
+__device__ __forceinline__ int kv_cache_of(const KvCaches& a, int t) {
+  int i = 0;
+  while (i + 1 < a.n && t >= a.task0[i + 1]) ++i;
+  return i;
+}
+
+constexpr int kCpThreads = 256, kCpUnroll = 4;
+
+// One work-group per (pair, task); a task is kCpThreads * kCpUnroll units of one layer's page.
+template <typename U>
+__global__ __launch_bounds__(kCpThreads) void copy_pages_kernel(KvCaches a, const int32_t* frm,
+                                                                const int32_t* to, int num_pages) {
+  const int tasks = a.task0[a.n];
+  const int pair = blockIdx.x / tasks, t = blockIdx.x % tasks;
+  const int f = frm[pair], d = to[pair];
+  if (f < 0 || d < 0 || f >= num_pages || d >= num_pages || f == d) return;
+  const int i = kv_cache_of(a, t);
+  const KvCache& c = a.c[i];
+  const int per = (int)(((int64_t)c.n1 * c.n2 * c.seg / (int)sizeof(U) + kCpThreads * kCpUnroll - 1) /
+                        (kCpThreads * kCpUnroll));
+  const int rel = t - a.task0[i];
+  const int l = rel / per, ch = rel % per;
+  char* const lb = c.base + l * c.layer;
+  const char* const sp = lb + f * c.page;
+  char* const dp = lb + d * c.page;
+  const int segu = c.seg / (int)sizeof(U);
+  const int64_t units = (int64_t)c.n1 * c.n2 * segu;
+  const int64_t u0 = (int64_t)ch * (kCpThreads * kCpUnroll) + threadIdx.x;
+  U x[kCpUnroll];
+  int64_t off[kCpUnroll];
+#pragma unroll
+  for (int k = 0; k < kCpUnroll; ++k) {
+    const int64_t u = u0 + k * kCpThreads;
+    if (c.n1 == 1 && c.n2 == 1) {
+      off[k] = u * (int)sizeof(U);
+    } else {
+      const int64_t piece = u / segu;
+      off[k] = (piece / c.n2) * c.s1 + (piece % c.n2) * c.s2 + (u - piece * segu) * (int)sizeof(U);
+    }
+    if (u < units) x[k] = *(const U*)(sp + off[k]);
+  }
+#pragma unroll
+  for (int k = 0; k < kCpUnroll; ++k)
+    if (u0 + k * kCpThreads < units) *(U*)(dp + off[k]) = x[k];
+}
+
+// Rows ctx + path[i] -> ctx + i, 1 <= i < count, of one sequence and one unit column of one
+// cache and layer per lane.  Parents come before their children, so path is strictly
+// increasing and path[i] >= i: the source of a row is never a place that an earlier row moved
+// to, and ascending order needs no copy kept aside.
+constexpr int kKeepRows = 8;
+template <typename U>
+__global__ __launch_bounds__(kWave) void keep_rows_kernel(KvCaches a, const int32_t* path,
+                                                          int64_t path_st, const int32_t* count,
+                                                          const int32_t* ctx, const int32_t* table,
+                                                          int64_t table_st, int P, int page,
+                                                          int num_pages, int max_n) {
+  const int b = blockIdx.y, lane = threadIdx.x;
+  const int n = min(count[b], max_n);
+  const int c0 = ctx[b];
+  if (n <= 0 || c0 < 0) return;
+  const int i0 = kv_cache_of(a, blockIdx.x);
+  const KvCache& c = a.c[i0];
+  const int segu = c.seg / (int)sizeof(U);
+  const int units = c.n2 * segu;
+  const int per = (units + kWave - 1) / kWave;
+  const int rel = blockIdx.x - a.task0[i0];
+  const int l = rel / per, u = (rel % per) * kWave + lane;
+  char* const lb = c.base + l * c.layer;
+  const int64_t col = (int64_t)(u / segu) * c.s2 + (int64_t)(u % segu) * (int)sizeof(U);
+  const int32_t* tr = table + (int64_t)b * table_st;
+  // byte offset of a slot's row in this layer, -1 where there is none
+  auto row_of = [&](int64_t s) -> int64_t {
+    if (s < 0 || s >= (int64_t)P * page) return -1;
+    const int p = tr[s / page];
+    if (p < 0 || p >= num_pages) return -1;
+    return p * c.page + (int64_t)(s % page) * c.s1;
+  };
+  for (int r0 = 0; r0 < n; r0 += kWave) {
+    // this lane's row of the next 64
+    int64_t so = -1, dn = -1;
+    if (r0 + lane < n) {
+      const int p = path[b * path_st + r0 + lane];
+      if (p > r0 + lane) {
+        so = row_of((int64_t)c0 + p);
+        dn = row_of((int64_t)c0 + r0 + lane);
+      }
+    }
+    uint64_t todo = __ballot(so >= 0 && dn >= 0);
+    while (todo) {
+      U x[kKeepRows];
+      int64_t d[kKeepRows];
+#pragma unroll
+      for (int k = 0; k < kKeepRows; ++k) {
+        const int s = todo ? __builtin_ctzll(todo) : -1;
+        d[k] = s >= 0 ? __shfl(dn, s, kWave) : -1;
+        const int64_t f = s >= 0 ? __shfl(so, s, kWave) : -1;
+        if (f >= 0 && u < units) x[k] = *(const U*)(lb + f + col);
+        if (todo) todo &= todo - 1;
+      }
+#pragma unroll
+      for (int k = 0; k < kKeepRows; ++k)
+        if (d[k] >= 0 && u < units) *(U*)(lb + d[k] + col) = x[k];
+    }
+  }
+}
+
+// Sum of v over the work-group's earlier threads; `total` gets the sum over all.
+__device__ __forceinline__ int block_exclusive(int v, int* sW, int& total) {
+  const int lane = wave_lane(), wv = threadIdx.x / kWave;
+  int x = v;
+#pragma unroll
+  for (int s = 1; s < kWave; s <<= 1) {
+    const int y = __shfl_up(x, s, kWave);
+    if (lane >= s) x += y;
+  }
+  __syncthreads();
+  if (lane == kWave - 1) sW[wv] = x;
+  __syncthreads();
+  int before = 0;
+  total = 0;
+  for (int w = 0; w < kKvThreads / kWave; ++w) {
+    const int t = sW[w];
+    if (w < wv) before += t;
+    total += t;
+  }
+  return before + x - v;
+}
+
+__device__ __forceinline__ int kv_blocks(int len, int page) { return (len + page - 1) / page; }
+
+__device__ __forceinline__ int kv_count_free(const int32_t* refs, int num_pages, int* sW) {
+  int mine = 0, total;
+  for (int p = threadIdx.x; p < num_pages; p += kKvThreads) mine += refs[p] == 0;
+  block_exclusive(mine, sW, total);
+  return total;
+}
+
+// Hands the lowest free pages out: want[i] .. want[i + 1] - 1 are the ranks of item i;
+// give(item, k, page) takes the k-th page of an item.
+template <typename Give>
+__device__ __forceinline__ void kv_hand_out(int32_t* refs, int num_pages, const int* want, int items,
+                                            int total, int* sW, Give give) {
+  int given = 0;
+  for (int p0 = 0; p0 < num_pages && given < total; p0 += kKvThreads) {
+    const int p = p0 + threadIdx.x;
+    const bool is_free = p < num_pages && refs[p] == 0;
+    int got;
+    const int rank = given + block_exclusive(is_free ? 1 : 0, sW, got);
+    if (is_free && rank < total) {
+      int lo = 0, hi = items;              // the last item with want[item] <= rank
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (want[mid] <= rank) lo = mid; else hi = mid;
+      }
+      refs[p] = 1;
+      give(lo, rank - want[lo], p);
+    }
+    given += got;
+  }
+}
+
+// Prefix sums of n values value(i) into want [n + 1] in LDS.
+template <typename Value>
+__device__ __forceinline__ int kv_prefix(int n, int* want, int* sW, Value value) {
+  int base = 0;
+  for (int i0 = 0; i0 < n; i0 += kKvThreads) {
+    const int i = i0 + threadIdx.x;
+    int total;
+    const int before = block_exclusive(i < n ? value(i) : 0, sW, total);
+    if (i < n) want[i] = base + before;
+    base += total;
+  }
+  if (threadIdx.x == 0) want[n] = base;
+  __syncthreads();
+  return base;
+}
+
+// Row dst[i] becomes row src[i]: its whole pages shared, its last, partly filled one a page of
+// its own, to be copied (frm[i] -> to[i]; -1 where there is none).  All pairs or none: ok is 0
+// and nothing changes where a row is out of range or named wrongly (a filled or repeated target, a
+// source that is a target, a table entry that is no page) or the free pages do not suffice.
+__global__ __launch_bounds__(kKvThreads) void fork_pages_kernel(
+    int32_t* refs, int num_pages, int32_t* table, int64_t table_st, int R, int P, int32_t* lens,
+    const int32_t* src, const int32_t* dst, int n, int page, int32_t* ok, int32_t* frm, int32_t* to) {
+  __shared__ int sW[kKvThreads / kWave];
+  __shared__ int sWant[kKvMaxRows + 1];
+  __shared__ uint32_t sDst[kKvMaxRows / 32];
+  const int tid = threadIdx.x;
+  for (int i = tid; i < kKvMaxRows / 32; i += kKvThreads) sDst[i] = 0u;
+  __syncthreads();
+  bool bad = false;
+  for (int i = tid; i < n; i += kKvThreads) {
+    const int d = dst[i];
+    if (d < 0 || d >= R || lens[d] != 0) { bad = true; continue; }
+    bad |= (atomicOr(&sDst[d >> 5], 1u << (d & 31)) >> (d & 31)) & 1u;
+  }
+  __syncthreads();
+  for (int i = tid; i < n; i += kKvThreads) {
+    const int s = src[i];
+    if (s < 0 || s >= R || (sDst[s >> 5] >> (s & 31)) & 1u || lens[s] < 0 ||
+        kv_blocks(lens[s], page) > P)
+      bad = true;
+  }
+  if (__syncthreads_or(bad)) {
+    for (int i = tid; i < n; i += kKvThreads) frm[i] = to[i] = -1;
+    if (tid == 0) *ok = 0;
+    return;
+  }
+  // every entry that is shared or copied names a page
+  for (int i = 0; i < n; ++i) {
+    const int s = src[i], nb = kv_blocks(lens[s], page);
+    for (int k = tid; k < nb; k += kKvThreads) {
+      const int p = table[(int64_t)s * table_st + k];
+      bad |= p < 0 || p >= num_pages;
+    }
+  }
+  const int total = kv_prefix(n, sWant, sW, [&](int i) { return lens[src[i]] % page != 0 ? 1 : 0; });
+  const int n_free = kv_count_free(refs, num_pages, sW);
+  if (__syncthreads_or(bad || total > n_free)) {
+    for (int i = tid; i < n; i += kKvThreads) frm[i] = to[i] = -1;
+    if (tid == 0) *ok = 0;
+    return;
+  }
+  for (int i = tid; i < n; i += kKvThreads) {
+    const int s = src[i], len = lens[s];
+    frm[i] = len % page != 0 ? table[(int64_t)s * table_st + len / page] : -1;
+    if (len % page == 0) to[i] = -1;
+  }
+  kv_hand_out(refs, num_pages, sWant, n, total, sW, [&](int i, int, int p) {
+    // an item without a page has an empty range, and the last of equal starts is taken
+    to[i] = p;
+    table[(int64_t)dst[i] * table_st + lens[src[i]] / page] = p;
+  });
+  __syncthreads();
+  for (int i = 0; i < n; ++i) {
+    const int s = src[i], full = lens[s] / page;
+    for (int k = tid; k < full; k += kKvThreads) {
+      const int p = table[(int64_t)s * table_st + k];
+      table[(int64_t)dst[i] * table_st + k] = p;
+      atomicAdd(&refs[p], 1);
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < n; i += kKvThreads) lens[dst[i]] = lens[src[i]];
+  if (tid == 0) *ok = 1;
+}
+
+// Rows grow to new_lens (shorter ones stay): new pages for the blocks they lack, and a page of
+// its own for a partly filled last page that another row shares, to be copied (frm[r] -> to[r]).
+// All rows or none, as above.
+__global__ __launch_bounds__(kKvThreads) void reserve_pages_kernel(
+    int32_t* refs, int num_pages, int32_t* table, int64_t table_st, int R, int P, int32_t* lens,
+    const int32_t* new_lens, int page, int32_t* ok, int32_t* frm, int32_t* to) {
+  __shared__ int sW[kKvThreads / kWave];
+  __shared__ int sWant[kKvMaxRows + 1];
+  const int tid = threadIdx.x;
+  bool bad = false;
+  for (int r = tid; r < R; r += kKvThreads) {
+    const int len = lens[r], want = new_lens[r];
+    frm[r] = to[r] = -1;
+    if (len < 0 || kv_blocks(len, page) > P) { bad = true; continue; }
+    if (want <= len) continue;
+    if (want > (int64_t)P * page) { bad = true; continue; }
+    if (len % page != 0) {
+      const int p = table[(int64_t)r * table_st + len / page];
+      if (p < 0 || p >= num_pages) bad = true;
+      else if (refs[p] > 1) frm[r] = p;
+    }
+  }
+  // each row was read and written by its own thread alone; the barrier in the prefix orders
+  // these before the loops of other threads
+  if (__syncthreads_or(bad)) {
+    for (int r = tid; r < R; r += kKvThreads) frm[r] = -1;
+    if (tid == 0) *ok = 0;
+    return;
+  }
+  const int total = kv_prefix(R, sWant, sW, [&](int r) {
+    const int len = lens[r], want = new_lens[r];
+    return want <= len ? 0 : kv_blocks(want, page) - kv_blocks(len, page) + (frm[r] >= 0 ? 1 : 0);
+  });
+  const int n_free = kv_count_free(refs, num_pages, sW);
+  if (total > n_free) {
+    __syncthreads();
+    for (int r = tid; r < R; r += kKvThreads) frm[r] = -1;
+    if (tid == 0) *ok = 0;
+    return;
+  }
+  // several rows may leave one shared page: all of them get a page of their own but, where no
+  // other row keeps it, the page loses its last name here and is free again
+  kv_hand_out(refs, num_pages, sWant, R, total, sW, [&](int r, int k, int p) {
+    const int have = kv_blocks(lens[r], page);
+    int at = have + k;
+    if (frm[r] >= 0) {
+      at -= 1;
+      if (k == 0) to[r] = p;
+    }
+    table[(int64_t)r * table_st + at] = p;
+  });
+  __syncthreads();
+  for (int r = tid; r < R; r += kKvThreads) {
+    if (frm[r] >= 0) atomicSub(&refs[frm[r]], 1);
+    if (new_lens[r] > lens[r]) lens[r] = new_lens[r];
+  }
+  if (tid == 0) *ok = 1;
+}
+
+// Rows are cut to keep[r] tokens (longer ones; below 0 counts as 0) and the pages above given up.
+__global__ __launch_bounds__(256) void free_pages_kernel(int32_t* refs, int num_pages, int32_t* table,
+                                                         int64_t table_st, int P, int32_t* lens,
+                                                         const int32_t* keep, int page) {
+  const int r = blockIdx.x;
+  const int len = lens[r], k = max(keep[r], 0);
+  if (k >= len) return;
+  const int b1 = (int)min((int64_t)P, ((int64_t)len + page - 1) / page);
+  for (int i = kv_blocks(k, page) + threadIdx.x; i < b1; i += 256) {
+    const int p = table[(int64_t)r * table_st + i];
+    if (p >= 0 && p < num_pages) atomicSub(&refs[p], 1);
+    table[(int64_t)r * table_st + i] = -1;
+  }
+  __syncthreads();                          // every thread read the length
+  if (threadIdx.x == 0) lens[r] = k;
+}
+
+// The live pages move to the lowest places: with `live` of them, the i-th live page at or above
+// `live` goes to the i-th free page below it.  new_refs and the moves (frm, to; -1 past them);
+// place [num_pages]: where each page went.
+__global__ __launch_bounds__(kKvThreads) void compact_plan_kernel(const int32_t* refs, int num_pages,
+                                                                  int32_t* new_refs, int32_t* frm,
+                                                                  int32_t* to, int32_t* place) {
+  __shared__ int sW[kKvThreads / kWave];
+  const int tid = threadIdx.x;
+  const int live = num_pages - kv_count_free(refs, num_pages, sW);
+  int highs = 0, lows = 0;
+  for (int p0 = 0; p0 < num_pages; p0 += kKvThreads) {
+    const int p = p0 + tid;
+    const int rc = p < num_pages ? refs[p] : 0;
+    const bool in = p < num_pages;
+    const bool low = in && rc == 0 && p < live, high = in && rc != 0 && p >= live;
+    // at most 1024 of each: both counts in one scan
+    int both;
+    const int before = block_exclusive((low ? 1 : 0) | (high ? 1 << 16 : 0), sW, both);
+    if (low) to[lows + (before & 0xffff)] = p;
+    if (high) frm[highs + (before >> 16)] = p;
+    if (in) {
+      new_refs[p] = p < live ? rc : 0;
+      place[p] = p;
+    }
+    lows += both & 0xffff;
+    highs += both >> 16;
+  }
+  __syncthreads();
+  for (int i = tid; i < num_pages / 2; i += kKvThreads) {
+    if (i < highs) {
+      const int f = frm[i], t = to[i];
+      new_refs[t] = refs[f];
+      place[f] = t;
+    } else {
+      frm[i] = to[i] = -1;
+    }
+  }
+}
+
+__global__ __launch_bounds__(256) void compact_table_kernel(const int32_t* table, int64_t table_st,
+                                                            int R, int P, const int32_t* lens,
+                                                            int page, const int32_t* place,
+                                                            int num_pages, int32_t* out) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (int64_t)R * P) return;
+  const int r = (int)(i / P), k = (int)(i % P);
+  const int p = table[(int64_t)r * table_st + k];
+  // entries past a row's pages, and those that name no page, come out as -1
+  out[i] = (int64_t)k * page < lens[r] && p >= 0 && p < num_pages ? place[p] : -1;
+}
+
+static int kv_status() {
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? kOk : (int)e;
+}
+
+// The kernel of the unit's size: 16 bytes where every address and size allows it, else the
+// largest that does.
+template <typename K16, typename K4, typename K2, typename K1, typename... Args>
+static int kv_launch(int unit, K16 k16, K4 k4, K2 k2, K1 k1, dim3 grid, dim3 block, void* stream,
+                     Args... args) {
+  hipStream_t st = (hipStream_t)stream;
+  if (unit == 16) hipLaunchKernelGGL(k16, grid, block, 0, st, args...);
+  else if (unit == 4) hipLaunchKernelGGL(k4, grid, block, 0, st, args...);
+  else if (unit == 2) hipLaunchKernelGGL(k2, grid, block, 0, st, args...);
+  else hipLaunchKernelGGL(k1, grid, block, 0, st, args...);
+  return kv_status();
+}
+
+// The caches of one launch: descriptors first .. first + n - 1 of desc [.., 8] (layers, layer
+// stride, page stride, n1, s1, n2, s2, seg; bytes), tasks of `task_units` units of a layer's page
+// (or row).  Returns the unit's bytes, 0 if a number does not fit.
+static int kv_fill(KvCaches& a, void* const* base, const int64_t* desc, int n, bool rows,
+                   int task_units, int64_t* tasks) {
+  int unit = 16;
+  for (int i = 0; i < n; ++i) {
+    const int64_t* d = desc + 8 * i;
+    const int64_t m = (int64_t)(uintptr_t)base[i] | d[1] | d[2] | d[4] | d[6] | d[7];
+    while (m % unit) unit >>= 1;
+  }
+  if (unit == 8) unit = 4;
+  a.n = n;
+  int64_t t = 0;
+  for (int i = 0; i < n; ++i) {
+    const int64_t* d = desc + 8 * i;
+    if (!base[i] || d[0] < 0 || d[3] < 1 || d[5] < 1 || d[7] < 1 || d[0] > INT32_MAX ||
+        d[3] > INT32_MAX || d[5] > INT32_MAX || d[7] > INT32_MAX || d[1] < 0 || d[2] < 0)
+      return 0;
+    a.c[i] = KvCache{(char*)base[i], d[1], d[2], d[4], d[6], (int)d[0], (int)d[3], (int)d[5],
+                     (int)d[7]};
+    a.task0[i] = (int)t;
+    const int64_t units = (rows ? 1 : d[3]) * d[5] * (d[7] / unit);
+    if (d[5] * (d[7] / unit) > INT32_MAX - 64) return 0;
+    t += d[0] * ((units + task_units - 1) / task_units);
+    if (t > INT32_MAX) return 0;
+  }
+  a.task0[n] = (int)t;
+  *tasks = t;
+  return unit;
+}
+
+}  // namespace dash
+
+extern "C" int dash_copy_pages(int num_caches, void* const* caches, const int64_t* desc,
+                               const int32_t* from_pages, const int32_t* to_pages, int num_pairs,
+                               int num_pages, void* stream) {
+  using namespace dash;
+  if (num_caches < 0 || num_pairs < 0 || num_pages < 0) return kErrInvalid;
+  if (num_caches == 0 || num_pairs == 0 || num_pages == 0) return kOk;
+  if (!caches || !desc || !from_pages || !to_pages) return kErrInvalid;
+  for (int c0 = 0; c0 < num_caches; c0 += kKvMaxCaches) {
+    KvCaches a;
+    int64_t tasks = 0;
+    const int n = std::min(kKvMaxCaches, num_caches - c0);
+    const int unit = kv_fill(a, caches + c0, desc + 8 * c0, n, false, kCpThreads * kCpUnroll, &tasks);
+    if (unit == 0) return kErrInvalid;
+    if (tasks == 0) continue;
+    if (tasks * num_pairs > INT32_MAX) return kErrUnsupported;
+    const int s = kv_launch(unit, copy_pages_kernel<uint4>, copy_pages_kernel<uint32_t>,
+                            copy_pages_kernel<uint16_t>, copy_pages_kernel<uint8_t>,
+                            dim3((unsigned)(tasks * num_pairs)), dim3(kCpThreads), stream, a,
+                            from_pages, to_pages, num_pages);
+    if (s != kOk) return s;
+  }
+  return kOk;
+}
+
+extern "C" int dash_keep_rows(int num_caches, void* const* caches, const int64_t* desc,
+                              const int32_t* path, int64_t path_stride, const int32_t* count,
+                              const int32_t* context_lens, const int32_t* block_table,
+                              int64_t table_stride, int B, int P, int page_size, int num_pages,
+                              int max_query_len, void* stream) {
+  using namespace dash;
+  if (num_caches < 0 || B < 0 || P < 0 || page_size <= 0 || num_pages < 0 || max_query_len < 0)
+    return kErrInvalid;
+  if (num_caches == 0 || B == 0 || P == 0 || num_pages == 0 || max_query_len == 0) return kOk;
+  if (!caches || !desc || !path || !count || !context_lens || !block_table) return kErrInvalid;
+  if (B > 65535) return kErrUnsupported;
+  for (int c0 = 0; c0 < num_caches; c0 += kKvMaxCaches) {
+    KvCaches a;
+    int64_t tasks = 0;
+    const int n = std::min(kKvMaxCaches, num_caches - c0);
+    const int unit = kv_fill(a, caches + c0, desc + 8 * c0, n, true, kWave, &tasks);
+    if (unit == 0) return kErrInvalid;
+    if (tasks == 0) continue;
+    const int s = kv_launch(unit, keep_rows_kernel<uint4>, keep_rows_kernel<uint32_t>,
+                            keep_rows_kernel<uint16_t>, keep_rows_kernel<uint8_t>,
+                            dim3((unsigned)tasks, B), dim3(kWave), stream, a, path, path_stride,
+                            count, context_lens, block_table, table_stride, P, page_size, num_pages,
+                            max_query_len);
+    if (s != kOk) return s;
+  }
+  return kOk;
+}
+
+extern "C" int dash_fork_pages(int32_t* refs, int num_pages, int32_t* block_table,
+                               int64_t table_stride, int R, int P, int32_t* lens,
+                               const int32_t* src_rows, const int32_t* dst_rows, int n,
+                               int page_size, int32_t* ok, int32_t* from_pages, int32_t* to_pages,
+                               void* stream) {
+  using namespace dash;
+  if (!refs || !block_table || !lens || !ok || num_pages < 0 || R < 0 || P < 0 || n < 0 ||
+      page_size <= 0)
+    return kErrInvalid;
+  if (n > 0 && (!src_rows || !dst_rows || !from_pages || !to_pages)) return kErrInvalid;
+  if (R > kKvMaxRows || n > kKvMaxRows) return kErrUnsupported;
+  hipLaunchKernelGGL(fork_pages_kernel, dim3(1), dim3(kKvThreads), 0, (hipStream_t)stream, refs,
+                     num_pages, block_table, table_stride, R, P, lens, src_rows, dst_rows, n,
+                     page_size, ok, from_pages, to_pages);
+  return kv_status();
+}
+
+extern "C" int dash_reserve_pages(int32_t* refs, int num_pages, int32_t* block_table,
+                                  int64_t table_stride, int R, int P, int32_t* lens,
+                                  const int32_t* new_lens, int page_size, int32_t* ok,
+                                  int32_t* from_pages, int32_t* to_pages, void* stream) {
+  using namespace dash;
+  if (!refs || !block_table || !lens || !new_lens || !ok || !from_pages || !to_pages ||
+      num_pages < 0 || R < 0 || P < 0 || page_size <= 0)
+    return kErrInvalid;
+  if (R > kKvMaxRows) return kErrUnsupported;
+  hipLaunchKernelGGL(reserve_pages_kernel, dim3(1), dim3(kKvThreads), 0, (hipStream_t)stream, refs,
+                     num_pages, block_table, table_stride, R, P, lens, new_lens, page_size, ok,
+                     from_pages, to_pages);
+  return kv_status();
+}
+
+extern "C" int dash_free_pages(int32_t* refs, int num_pages, int32_t* block_table,
+                               int64_t table_stride, int R, int P, int32_t* lens,
+                               const int32_t* keep_lens, int page_size, void* stream) {
+  using namespace dash;
+  if (!refs || !block_table || !lens || !keep_lens || num_pages < 0 || R < 0 || P < 0 ||
+      page_size <= 0)
+    return kErrInvalid;
+  if (R == 0) return kOk;
+  hipLaunchKernelGGL(free_pages_kernel, dim3(R), dim3(256), 0, (hipStream_t)stream, refs, num_pages,
+                     block_table, table_stride, P, lens, keep_lens, page_size);
+  return kv_status();
+}
+
+extern "C" int dash_compact_pages(const int32_t* refs, int num_pages, const int32_t* block_table,
+                                  int64_t table_stride, int R, int P, const int32_t* lens,
+                                  int page_size, int32_t* new_refs, int32_t* new_table,
+                                  int32_t* from_pages, int32_t* to_pages, int32_t* place,
+                                  void* stream) {
+  using namespace dash;
+  if (num_pages < 0 || R < 0 || P < 0 || page_size <= 0) return kErrInvalid;
+  if (num_pages > 0 && (!refs || !new_refs || !from_pages || !to_pages || !place)) return kErrInvalid;
+  const int64_t entries = (int64_t)R * P;
+  if (entries > 0 && (!block_table || !lens || !new_table || (num_pages > 0 && !place)))
+    return kErrInvalid;
+  if ((entries + 255) / 256 > INT32_MAX) return kErrUnsupported;
+  hipStream_t st = (hipStream_t)stream;
+  if (num_pages > 0)
+    hipLaunchKernelGGL(compact_plan_kernel, dim3(1), dim3(kKvThreads), 0, st, refs, num_pages,
+                       new_refs, from_pages, to_pages, place);
+  if (entries > 0)
+    hipLaunchKernelGGL(compact_table_kernel, dim3((unsigned)((entries + 255) / 256)), dim3(256), 0, st,
+                       block_table, table_stride, R, P, lens, page_size, place, num_pages, new_table);
+  return kv_status();
+}

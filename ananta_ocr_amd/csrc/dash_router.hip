@@ -1325,13 +1325,14 @@ extern "C" int dash_block_scores(const float* idx_q, int64_t iq_sb, int64_t iq_s
 // ---------------------------------------------------------------------------
 namespace dash {
 // Position and block count of every query row: row cu[b] + i is position ctx[b] + i of
-// sequence b.  Without ctx the rows are whole packed documents, whose block counts alone
-// are written.
+// sequence b, or ctx[b] + depth[row] with depths (the nodes of a tree).  Without ctx the rows
+// are whole packed documents, whose block counts alone are written.
 __global__ __launch_bounds__(256) void extend_rows_kernel(const int32_t* __restrict__ cu,
                                                           const int32_t* __restrict__ ctx,
                                                           const int32_t* __restrict__ lens, int B,
                                                           int T, int bs, int32_t* __restrict__ q_pos,
-                                                          int32_t* __restrict__ row_nblk) {
+                                                          int32_t* __restrict__ row_nblk,
+                                                          const int32_t* __restrict__ depth) {
   const int r = blockIdx.x * 256 + threadIdx.x;
   if (r >= T) return;
   int b = 0, hi = B;                       // the last sequence b with cu[b] <= r
@@ -1339,7 +1340,7 @@ __global__ __launch_bounds__(256) void extend_rows_kernel(const int32_t* __restr
     const int mid = (b + hi) >> 1;
     if (cu[mid] <= r) b = mid; else hi = mid;
   }
-  if (ctx) q_pos[r] = ctx[b] + r - cu[b];
+  if (ctx) q_pos[r] = ctx[b] + (depth ? depth[r] : r - cu[b]);
   row_nblk[r] = ((ctx ? lens[b] : cu[b + 1] - cu[b]) + bs - 1) / bs;
 }
 }  // namespace dash
@@ -1351,7 +1352,7 @@ extern "C" int dash_packed_row_blocks(const int32_t* cu_seqlens, int B, int T, i
   if (B == 0 || T == 0) return kOk;
   hipLaunchKernelGGL(extend_rows_kernel, dim3((T + 255) / 256), dim3(256), 0, (hipStream_t)stream,
                      cu_seqlens, (const int32_t*)nullptr, (const int32_t*)nullptr, B, T, block_size,
-                     (int32_t*)nullptr, row_nblk);
+                     (int32_t*)nullptr, row_nblk, (const int32_t*)nullptr);
   return launch_status();
 }
 
@@ -1381,13 +1382,61 @@ extern "C" int dash_extend_scores(const float* idx_q, int64_t iq_st, const float
                      pool, (int64_t)0, KbarPages{context_lens, block_size, pool_rows});
   if (T == 0 || max_query_len == 0) return launch_status();
   hipLaunchKernelGGL(extend_rows_kernel, dim3((T + 255) / 256), dim3(256), 0, st, cu_seqlens_q,
-                     context_lens, seq_lens, B, T, block_size, q_pos, row_nblk);
+                     context_lens, seq_lens, B, T, block_size, q_pos, row_nblk, (const int32_t*)nullptr);
   const SeqLayout lq{cu_seqlens_q, nullptr, 0, 0, 0, iq_st, 1};
   dim3 grid((max_query_len + kSmRows - 1) / kSmRows, (nblk + kSmBlk - 1) / kSmBlk, B);
   hipLaunchKernelGGL(scores_mfma_kernel, grid, dim3(256), 0, st, idx_q, lq, cu_seqlens_q,
                      max_query_len, q_pos, pool, (int64_t)0, (const int32_t*)nullptr, seq_lens,
                      nblk * block_size, block_size, local_blocks, nblk, inv, z, z_stride, block_table,
                      table_stride, pool_rows);
+  return launch_status();
+}
+
+extern "C" int dash_kbar_pages(const float* idx_k, int64_t ik_st, int64_t ik_sp,
+                               const float* head_cls, const int32_t* first_tokens,
+                               const int32_t* seq_lens, const int32_t* block_table,
+                               int64_t table_stride, float* pool, int pool_rows, int B, int nblk,
+                               int d, int block_size, void* stream) {
+  using namespace dash;
+  if (B < 0 || nblk < 0 || pool_rows < 0) return kErrInvalid;
+  if (B == 0 || nblk == 0 || pool_rows == 0) return kOk;
+  if (!idx_k || !head_cls || !first_tokens || !seq_lens || !block_table || !pool) return kErrInvalid;
+  if (d != kKbD || block_size <= 0 || block_size > kKbMaxBs || ik_st % 4 != 0 || ik_sp % 4 != 0 ||
+      (uintptr_t)idx_k % 16 != 0 || (uintptr_t)head_cls % 16 != 0 || (uintptr_t)pool % 16 != 0 ||
+      B > 65535)
+    return kErrUnsupported;
+  const SeqLayout lk{nullptr, block_table, table_stride, 0, ik_sp, ik_st, block_size};
+  hipLaunchKernelGGL(kbar128_kernel, dim3(nblk, B), dim3(256), 0, (hipStream_t)stream, idx_k, lk,
+                     (const int32_t*)nullptr, seq_lens, head_cls, nblk * block_size, block_size, 0,
+                     (float)(1.0 / sqrt((double)d)), pool, (int64_t)0,
+                     KbarPages{first_tokens, block_size, pool_rows});
+  return launch_status();
+}
+
+extern "C" int dash_tree_scores(const float* idx_q, int64_t iq_st, const int32_t* cu_seqlens_q,
+                                const int32_t* context_lens, const int32_t* depth,
+                                const int32_t* block_table, int64_t table_stride, const float* pool,
+                                int pool_rows, int B, int T, int max_query_len, int nblk, int d,
+                                int block_size, int local_blocks, int32_t* q_pos, int32_t* row_nblk,
+                                float* z, int64_t z_stride, void* stream) {
+  using namespace dash;
+  if (B < 0 || T < 0 || max_query_len < 0 || nblk < 0 || pool_rows <= 0) return kErrInvalid;
+  if (B == 0 || T == 0 || max_query_len == 0 || nblk == 0) return kOk;
+  if (!idx_q || !cu_seqlens_q || !context_lens || !depth || !block_table || !pool || !q_pos ||
+      !row_nblk || !z)
+    return kErrInvalid;
+  if (d != kKbD || block_size <= 0 || iq_st % 4 != 0 || (uintptr_t)idx_q % 16 != 0 ||
+      (uintptr_t)pool % 16 != 0 || B > 65535)
+    return kErrUnsupported;
+  hipStream_t st = (hipStream_t)stream;
+  hipLaunchKernelGGL(extend_rows_kernel, dim3((T + 255) / 256), dim3(256), 0, st, cu_seqlens_q,
+                     context_lens, context_lens, B, T, block_size, q_pos, row_nblk, depth);
+  const SeqLayout lq{cu_seqlens_q, nullptr, 0, 0, 0, iq_st, 1};
+  dim3 grid((max_query_len + kSmRows - 1) / kSmRows, (nblk + kSmBlk - 1) / kSmBlk, B);
+  hipLaunchKernelGGL(scores_mfma_kernel, grid, dim3(256), 0, st, idx_q, lq, cu_seqlens_q,
+                     max_query_len, q_pos, pool, (int64_t)0, (const int32_t*)nullptr, context_lens,
+                     nblk * block_size, block_size, local_blocks, nblk,
+                     (float)(1.0 / sqrt((double)d)), z, z_stride, block_table, table_stride, pool_rows);
   return launch_status();
 }
 

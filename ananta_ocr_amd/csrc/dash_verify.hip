@@ -1,0 +1,468 @@
+// Verification of drafted tokens on gfx950: which nodes of a sequence's tree the target's
+// distribution accepts, from given random numbers, and the token that follows the last of them.
+//
+// Row r = cu[b] + i is node i of sequence b; node 0 is the root (the newest sampled token), and
+// p[r] the target's distribution of the token after it.  At a node, its children are tried in
+// order.  With draft probabilities q (the children were drawn from q[node], each by itself) what is
+// left of p after some rejections is max(p - a q, 0) for one number a: taking max(x - Z q, 0) of
+// x = max(p - a q, 0) gives max(p - (a + Z) q, 0).  So with a = 0 and Z = 1 at first, child x is
+// accepted if u Z q(x) < max(p(x) - a q(x), 0), and a rejection sets a += Z and
+// Z = sum_v max(p - a q, 0).  Without draft probabilities a child is a certain proposal: accepted
+// if u Z < p(x), else its token's probability leaves p and Z.  The root's number draws the next
+// token from what is left at the last accepted node, in order of the token ids.  Greedy: a
+// child that is the row's best token (the lowest of equals) is accepted.
+//
+// Sums and products are taken in 64 bits: products of 32-bit inputs are then exact, and a
+// different order of a sum moves a border by 1e-16 of the row's mass, not by the 1e-7 that would
+// change a drawn token in every few thousandth row of 131,072 tokens.
+//
+// Probabilities that are not above 0 (NaN too) count as 0.
+
+#include <hip/hip_fp16.h>
+
+#include "dash_common.h"
+
+namespace dash {
+
+constexpr int kVfMaxNodes = 256;      // nodes of a sequence
+constexpr int kVfChunk = 4096;        // tokens per work-group of the sums
+constexpr int kVfThreads = 256;
+
+struct VerifyArgs {
+  const void* p; int64_t p_st;
+  const void* q; int64_t q_st;          // null: certain proposals
+  const void* tok; int tok64;
+  const int32_t* parents; const int32_t* cu;
+  const float* u;                       // null: greedy
+  int B, V, max_n, chunks;              // chunks of a row (sums, or greedy partials)
+  int chunk;                            // tokens of a greedy partial
+  int64_t T;
+  int32_t* count; int32_t* path; int64_t path_st; int64_t* token;
+  // workspace
+  int32_t* stop;                        // [B] the last accepted node
+  double* gone;                         // [B] a at that node
+  double2* sums;                        // [B, chunks] (what is left, the row itself)
+  float* best_v; int32_t* best_i;       // [T, chunks] greedy partials
+};
+
+template <typename T> __device__ __forceinline__ float vf_load(const T* x) { return (float)*x; }
+template <> __device__ __forceinline__ float vf_load<__half>(const __half* x) { return __half2float(*x); }
+
+__device__ __forceinline__ int64_t vf_token(const VerifyArgs& a, int64_t row) {
+  return a.tok64 ? ((const int64_t*)a.tok)[row] : ((const int32_t*)a.tok)[row];
+}
+
+// What is left of probability p where the draft's is q.
+__device__ __forceinline__ double vf_left(float p, float q, double gone) {
+  const double x = p > 0.f ? (double)p : 0.0;
+  if (gone == 0.0) return x;
+  const double r = x - gone * (double)q;
+  return r > 0.0 ? r : 0.0;
+}
+
+// Sum over the work-group, the same on every thread.
+template <int THREADS>
+__device__ __forceinline__ double vf_block_sum(double v, double* sD) {
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m, kWave);
+  __syncthreads();
+  if (wave_lane() == 0) sD[threadIdx.x / kWave] = v;
+  __syncthreads();
+  double s = 0.0;
+#pragma unroll
+  for (int w = 0; w < THREADS / kWave; ++w) s += sD[w];
+  return s;
+}
+
+// Greedy: the best token of a piece of a row; the lowest of equals, NaN never.
+template <typename T, bool VEC>
+__global__ __launch_bounds__(kVfThreads) void verify_best_kernel(VerifyArgs a) {
+  __shared__ float sV[kVfThreads / kWave];
+  __shared__ int sI[kVfThreads / kWave];
+  const int64_t row = blockIdx.x / a.chunks;
+  const int ch = blockIdx.x % a.chunks, tid = threadIdx.x;
+  const int v0 = ch * a.chunk, v1 = (int)min((int64_t)a.V, (int64_t)v0 + a.chunk);
+  const T* p = (const T*)a.p + row * a.p_st;
+  float best = -INFINITY;
+  int at = INT32_MAX;
+  int v = v0;
+  if (VEC) {
+    constexpr int E = 16 / sizeof(T), U = 4;
+    for (; v + kVfThreads * E * U <= v1; v += kVfThreads * E * U) {
+      uint4 x[U];
+#pragma unroll
+      for (int k = 0; k < U; ++k) x[k] = *(const uint4*)(p + v + (k * kVfThreads + tid) * E);
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        const T* e = (const T*)&x[k];
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+          const float f = vf_load(e + j);
+          if (f > best) { best = f; at = v + (k * kVfThreads + tid) * E + j; }
+        }
+      }
+    }
+  }
+  for (int w = v + tid; w < v1; w += kVfThreads) {
+    const float f = vf_load(p + w);
+    if (f > best) { best = f; at = w; }
+  }
+  auto take = [&](float f, int i) {
+    if (f > best || (f == best && i < at)) { best = f; at = i; }
+  };
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) take(__shfl_xor(best, m, kWave), __shfl_xor(at, m, kWave));
+  if (wave_lane() == 0) { sV[tid / kWave] = best; sI[tid / kWave] = at; }
+  __syncthreads();
+  if (tid == 0) {
+#pragma unroll
+    for (int w = 1; w < kVfThreads / kWave; ++w) take(sV[w], sI[w]);
+    a.best_v[blockIdx.x] = best;
+    a.best_i[blockIdx.x] = at;
+  }
+}
+
+// The walk from the root.  Every wavefront walks by itself on the same values in LDS; the draft
+// and target probabilities of every drafted token are gathered first, in one round trip.  Only a
+// rejected child that has a later sibling, with draft probabilities, needs a pass over a row.
+template <typename T, int MODE, int THREADS>   // MODE 0 greedy, 1 certain proposals, 2 drawn ones
+__global__ __launch_bounds__(THREADS) void verify_walk_kernel(VerifyArgs a) {
+  __shared__ int sPar[kVfMaxNodes];
+  __shared__ int64_t sTok[kVfMaxNodes];
+  __shared__ float sP[kVfMaxNodes], sQ[kVfMaxNodes], sU[kVfMaxNodes];
+  __shared__ int sBest[MODE == 0 ? kVfMaxNodes : 1];
+  __shared__ int sPath[kVfMaxNodes];
+  __shared__ double sD[THREADS / kWave];
+  const int b = blockIdx.x, tid = threadIdx.x, lane = wave_lane();
+  const int64_t r0 = a.cu[b];
+  const int n = min((int)(a.cu[b + 1] - r0), a.max_n);
+  if (n <= 0) {
+    for (int i = tid; i < a.max_n; i += THREADS) a.path[b * a.path_st + i] = -1;
+    if (tid == 0) { a.count[b] = 0; a.token[b] = -1; if (MODE) a.stop[b] = -1; }
+    return;
+  }
+  for (int i = tid; i < n; i += THREADS) {
+    int par = a.parents[r0 + i];
+    if (i == 0 || par < 0 || par >= i) par = -1;
+    const int64_t t = vf_token(a, r0 + i);
+    sPar[i] = par;
+    sTok[i] = t;
+    if (MODE != 0) {
+      const bool in = par >= 0 && t >= 0 && t < a.V;
+      sP[i] = in ? vf_load((const T*)a.p + (r0 + par) * a.p_st + t) : 0.f;
+      sQ[i] = MODE == 2 && in ? vf_load((const T*)a.q + (r0 + par) * a.q_st + t) : 1.f;
+      sU[i] = a.u[r0 + i];
+    }
+  }
+  if (MODE == 0) {
+    for (int i = tid; i < n; i += THREADS) {
+      float best = -INFINITY;
+      int at = INT32_MAX;
+      for (int c = 0; c < a.chunks; ++c) {
+        const float f = a.best_v[(r0 + i) * a.chunks + c];
+        if (f > best) { best = f; at = a.best_i[(r0 + i) * a.chunks + c]; }
+      }
+      sBest[i] = at == INT32_MAX ? 0 : at;
+    }
+  }
+  __syncthreads();
+  int s = 0, cnt = 1;
+  double gone = 0.0;
+  if (tid == 0) sPath[0] = 0;
+  for (;;) {
+    int found = -1;
+    double Z = 1.0;
+    gone = 0.0;
+    for (int w = 0; w < n && found < 0; w += kWave) {
+      uint64_t kids = __ballot(w + lane < n && sPar[min(w + lane, n - 1)] == s);
+      while (kids) {
+        const int i = w + __builtin_ctzll(kids);
+        kids &= kids - 1;
+        if (MODE == 0) {
+          if (sTok[i] == sBest[s]) { found = i; break; }
+        } else if (MODE == 1) {
+          // a token that an earlier sibling named is no longer in p
+          bool again = false;
+          for (int k = 0; k <= w; k += kWave)
+            again |= __any(k + lane < i && sPar[min(k + lane, n - 1)] == s && sTok[min(k + lane, n - 1)] == sTok[i]);
+          const double e = again ? 0.0 : vf_left(sP[i], 0.f, 0.0);
+          if ((double)sU[i] * Z < e) { found = i; break; }
+          Z -= e;
+        } else {
+          const double e = vf_left(sP[i], sQ[i], gone);
+          if ((double)sU[i] * Z * (double)sQ[i] < e) { found = i; break; }
+          gone += Z;
+          bool more = kids != 0;
+          for (int k = w + kWave; k < n && !more; k += kWave)
+            more = __any(k + lane < n && sPar[min(k + lane, n - 1)] == s);
+          if (more) {
+            const T* p = (const T*)a.p + (r0 + s) * a.p_st;
+            const T* q = (const T*)a.q + (r0 + s) * a.q_st;
+            constexpr int U = 8;
+            double mine = 0.0;
+            int v = tid;
+            for (; v + (U - 1) * THREADS < a.V; v += U * THREADS) {
+              float x[U], y[U];
+#pragma unroll
+              for (int k = 0; k < U; ++k) { x[k] = vf_load(p + v + k * THREADS); y[k] = vf_load(q + v + k * THREADS); }
+#pragma unroll
+              for (int k = 0; k < U; ++k) mine += vf_left(x[k], y[k], gone);
+            }
+            for (; v < a.V; v += THREADS) mine += vf_left(vf_load(p + v), vf_load(q + v), gone);
+            Z = vf_block_sum<THREADS>(mine, sD);
+          }
+        }
+      }
+    }
+    if (found < 0) break;
+    s = found;
+    if (tid == 0) sPath[cnt] = s;
+    ++cnt;
+  }
+  __syncthreads();
+  for (int i = tid; i < a.max_n; i += THREADS) a.path[b * a.path_st + i] = i < cnt ? sPath[i] : -1;
+  if (tid == 0) {
+    a.count[b] = cnt;
+    if (MODE == 0) {
+      a.token[b] = sBest[s];
+    } else {
+      a.stop[b] = s;
+      a.gone[b] = gone;
+    }
+  }
+}
+
+// The tokens of a chunk that the children of the last accepted node named (certain proposals):
+// a bit each.
+__device__ __forceinline__ void vf_named(const VerifyArgs& a, int b, int s, int v0, uint32_t* sBits) {
+  for (int i = threadIdx.x; i < kVfChunk / 32; i += kVfThreads) sBits[i] = 0u;
+  __syncthreads();
+  if (!a.q) {
+    const int64_t r0 = a.cu[b];
+    const int n = min((int)(a.cu[b + 1] - r0), a.max_n);
+    for (int i = threadIdx.x + 1; i < n; i += kVfThreads) {
+      const int par = a.parents[r0 + i];
+      if (par != s || par >= i) continue;
+      const int64_t t = vf_token(a, r0 + i) - v0;
+      if (t >= 0 && t < kVfChunk) atomicOr(&sBits[t >> 5], 1u << (t & 31));
+    }
+  }
+  __syncthreads();
+}
+
+// (what is left, the row itself) of token v0 + e.
+template <typename T>
+__device__ __forceinline__ double2 vf_pair(const VerifyArgs& a, const T* p, const T* q, int v0, int e,
+                                           double gone, const uint32_t* sBits) {
+  const float x = vf_load(p + v0 + e);
+  const double whole = vf_left(x, 0.f, 0.0);
+  if (q) return make_double2(vf_left(x, vf_load(q + v0 + e), gone), whole);
+  return make_double2((sBits[e >> 5] >> (e & 31)) & 1u ? 0.0 : whole, whole);
+}
+
+template <typename T>
+__global__ __launch_bounds__(kVfThreads) void verify_sums_kernel(VerifyArgs a) {
+  __shared__ uint32_t sBits[kVfChunk / 32];
+  __shared__ double sD[kVfThreads / kWave];
+  const int b = blockIdx.y, v0 = blockIdx.x * kVfChunk;
+  const int s = a.stop[b];
+  if (s < 0) return;
+  const int64_t row = a.cu[b] + s;
+  const T* p = (const T*)a.p + row * a.p_st;
+  const T* q = a.q ? (const T*)a.q + row * a.q_st : nullptr;
+  const double gone = a.gone[b];
+  vf_named(a, b, s, v0, sBits);
+  const int m = min(kVfChunk, a.V - v0);
+  double left = 0.0, whole = 0.0;
+#pragma unroll 8
+  for (int e = threadIdx.x; e < m; e += kVfThreads) {
+    const double2 x = vf_pair<T>(a, p, q, v0, e, gone, sBits);
+    left += x.x;
+    whole += x.y;
+  }
+  left = vf_block_sum<kVfThreads>(left, sD);
+  whole = vf_block_sum<kVfThreads>(whole, sD);
+  if (threadIdx.x == 0) a.sums[(int64_t)b * a.chunks + blockIdx.x] = make_double2(left, whole);
+}
+
+// Sum over the work-group's earlier threads, and over all.
+__device__ __forceinline__ double vf_before(double v, double* sD, double& total) {
+  const int lane = wave_lane(), wv = threadIdx.x / kWave;
+  double x = v;
+#pragma unroll
+  for (int s = 1; s < kWave; s <<= 1) {
+    const double y = __shfl_up(x, s, kWave);
+    if (lane >= s) x += y;
+  }
+  __syncthreads();
+  if (lane == kWave - 1) sD[wv] = x;
+  __syncthreads();
+  double before = 0.0;
+  total = 0.0;
+#pragma unroll
+  for (int w = 0; w < kVfThreads / kWave; ++w) {
+    if (w < wv) before += sD[w];
+    total += sD[w];
+  }
+  return before + x - v;
+}
+
+// The chunk that the root's number falls into, then the token within it.
+template <typename T>
+__global__ __launch_bounds__(kVfThreads) void verify_draw_kernel(VerifyArgs a) {
+  __shared__ uint32_t sBits[kVfChunk / 32];
+  __shared__ double sD[kVfThreads / kWave];
+  __shared__ double sX[kVfChunk];
+  __shared__ double sBase;
+  __shared__ int sAt, sLast;
+  const int b = blockIdx.x, tid = threadIdx.x;
+  const int s = a.stop[b];
+  if (s < 0) return;
+  const double2* sums = a.sums + (int64_t)b * a.chunks;
+  // each thread's run of chunks
+  const int per = (a.chunks + kVfThreads - 1) / kVfThreads;
+  const int c0 = min(tid * per, a.chunks), c1 = min(c0 + per, a.chunks);
+  double left = 0.0, whole = 0.0, total, total_w;
+  for (int c = c0; c < c1; ++c) { left += sums[c].x; whole += sums[c].y; }
+  double before = vf_before(left, sD, total);
+  const double before_w = vf_before(whole, sD, total_w);
+  const bool rest = total > 0.0;            // nothing left by rounding: the row itself
+  if (!rest) { before = before_w; total = total_w; }
+  if (!(total > 0.0)) {
+    if (tid == 0) a.token[b] = -1;
+    return;
+  }
+  const double want = (double)a.u[a.cu[b]] * total;
+  if (tid == 0) { sAt = INT32_MAX; sLast = -1; }
+  __syncthreads();
+  {
+    double x = before;
+    for (int c = c0; c < c1; ++c) {
+      const double y = rest ? sums[c].x : sums[c].y;
+      if (y > 0.0) atomicMax(&sLast, c);
+      if (x + y > want) { atomicMin(&sAt, c); break; }
+      x += y;
+    }
+  }
+  __syncthreads();
+  const int at = sAt == INT32_MAX ? sLast : sAt;
+  if (at >= c0 && at < c1) {
+    double x = before;
+    for (int c = c0; c < at; ++c) x += rest ? sums[c].x : sums[c].y;
+    sBase = x;
+  }
+  __syncthreads();
+  const double base = sBase;
+  const int v0 = at * kVfChunk, m = min(kVfChunk, a.V - v0);
+  const int64_t row = a.cu[b] + s;
+  const T* p = (const T*)a.p + row * a.p_st;
+  const T* q = a.q ? (const T*)a.q + row * a.q_st : nullptr;
+  const double gone = a.gone[b];
+  vf_named(a, b, s, v0, sBits);
+  for (int e = tid; e < kVfChunk; e += kVfThreads) {
+    double2 x = make_double2(0.0, 0.0);
+    if (e < m) x = vf_pair<T>(a, p, q, v0, e, gone, sBits);
+    sX[e] = rest ? x.x : x.y;
+  }
+  if (tid == 0) { sAt = INT32_MAX; sLast = -1; }
+  __syncthreads();
+  constexpr int kPer = kVfChunk / kVfThreads;
+  double run = 0.0;
+  for (int k = 0; k < kPer; ++k) run += sX[tid * kPer + k];
+  double x = base + vf_before(run, sD, total);
+  for (int k = 0; k < kPer; ++k) {
+    const double y = sX[tid * kPer + k];
+    if (y > 0.0) atomicMax(&sLast, tid * kPer + k);
+    x += y;
+    if (x > want && y > 0.0) { atomicMin(&sAt, tid * kPer + k); break; }
+  }
+  __syncthreads();
+  if (tid == 0) a.token[b] = v0 + (sAt == INT32_MAX ? sLast : sAt);
+}
+
+static int verify_chunks(int64_t T, int V, bool greedy, int& chunk) {
+  if (!greedy) {
+    chunk = kVfChunk;
+    return (V + kVfChunk - 1) / kVfChunk;
+  }
+  // rows alone fill the chip from 1,024 on; below, a row is cut into pieces of 8,192 at least
+  const int64_t pieces = std::max<int64_t>(1, std::min<int64_t>((1024 + T - 1) / std::max<int64_t>(T, 1), (V + 8191) / 8192));
+  chunk = (int)(((V + pieces - 1) / pieces + 63) / 64 * 64);
+  return (V + chunk - 1) / chunk;
+}
+
+struct VerifyLayout { int64_t stop, gone, sums, best_v, best_i, total; int chunks, chunk; };
+static VerifyLayout verify_layout(int B, int64_t T, int V, bool greedy) {
+  VerifyLayout L;
+  L.chunks = verify_chunks(T, V, greedy, L.chunk);
+  auto align = [](int64_t x) { return (x + 255) / 256 * 256; };
+  int64_t o = 0;
+  L.stop = o; o = align(o + (int64_t)B * 4);
+  L.gone = o; o = align(o + (int64_t)B * 8);
+  L.sums = o; if (!greedy) o = align(o + (int64_t)B * L.chunks * 16);
+  L.best_v = o; if (greedy) o = align(o + T * L.chunks * 4);
+  L.best_i = o; if (greedy) o = align(o + T * L.chunks * 4);
+  L.total = o;
+  return L;
+}
+
+template <typename T>
+static void verify_launch(const VerifyArgs& a, hipStream_t st) {
+  if (!a.u) {
+    const bool vec = (uintptr_t)a.p % 16 == 0 && a.p_st * sizeof(T) % 16 == 0 && a.chunk % 64 == 0;
+    auto kern = vec ? verify_best_kernel<T, true> : verify_best_kernel<T, false>;
+    if (a.T > 0)
+      hipLaunchKernelGGL(kern, dim3((unsigned)(a.T * a.chunks)), dim3(kVfThreads), 0, st, a);
+    hipLaunchKernelGGL((verify_walk_kernel<T, 0, 256>), dim3(a.B), dim3(256), 0, st, a);
+    return;
+  }
+  if (a.q)
+    hipLaunchKernelGGL((verify_walk_kernel<T, 2, 1024>), dim3(a.B), dim3(1024), 0, st, a);
+  else
+    hipLaunchKernelGGL((verify_walk_kernel<T, 1, 256>), dim3(a.B), dim3(256), 0, st, a);
+  hipLaunchKernelGGL(verify_sums_kernel<T>, dim3(a.chunks, a.B), dim3(kVfThreads), 0, st, a);
+  hipLaunchKernelGGL(verify_draw_kernel<T>, dim3(a.B), dim3(kVfThreads), 0, st, a);
+}
+
+}  // namespace dash
+
+extern "C" int dash_verify_tree_workspace_size(int B, int64_t T, int V, int greedy, int64_t* bytes) {
+  using namespace dash;
+  if (!bytes || B < 0 || T < 0 || V <= 0) return kErrInvalid;
+  *bytes = verify_layout(B, T, V, greedy != 0).total;
+  return kOk;
+}
+
+extern "C" int dash_verify_tree(const void* target, int64_t target_stride, const void* draft,
+                                int64_t draft_stride, int dtype, const void* tokens, int tokens_int64,
+                                const int32_t* parents, const int32_t* cu_seqlens_q,
+                                const float* uniforms, int B, int64_t T, int V, int max_query_len,
+                                int32_t* count, int32_t* path, int64_t path_stride,
+                                int64_t* next_token, void* workspace, int64_t workspace_bytes,
+                                void* stream) {
+  using namespace dash;
+  if (B < 0 || T < 0 || V <= 0 || max_query_len < 0 || dtype < 0 || dtype > 2) return kErrInvalid;
+  if (B == 0) return kOk;
+  if (!cu_seqlens_q || !count || !next_token) return kErrInvalid;
+  if (T > 0 && (!target || !tokens || !parents)) return kErrInvalid;
+  if (max_query_len > 0 && !path) return kErrInvalid;
+  if (draft && !uniforms) return kErrInvalid;
+  if (max_query_len > kVfMaxNodes || B > 65535) return kErrUnsupported;
+  const VerifyLayout L = verify_layout(B, T, V, !uniforms);
+  if (T * L.chunks > INT32_MAX) return kErrUnsupported;
+  if (!workspace || workspace_bytes < L.total || (uintptr_t)workspace % 256 != 0) return kErrWorkspace;
+  char* w = (char*)workspace;
+  VerifyArgs a = {};
+  a.p = target; a.p_st = target_stride; a.q = draft; a.q_st = draft_stride;
+  a.tok = tokens; a.tok64 = tokens_int64; a.parents = parents; a.cu = cu_seqlens_q; a.u = uniforms;
+  a.B = B; a.V = V; a.max_n = max_query_len; a.chunks = L.chunks; a.chunk = L.chunk; a.T = T;
+  a.count = count; a.path = path; a.path_st = path_stride; a.token = next_token;
+  a.stop = (int32_t*)(w + L.stop); a.gone = (double*)(w + L.gone); a.sums = (double2*)(w + L.sums);
+  a.best_v = (float*)(w + L.best_v); a.best_i = (int32_t*)(w + L.best_i);
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == 0) verify_launch<float>(a, st);
+  else if (dtype == 1) verify_launch<bf16>(a, st);
+  else verify_launch<__half>(a, st);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? kOk : (int)e;
+}

@@ -1009,6 +1009,29 @@ def extend_scores(idx_q, idx_k, head_cls, cu_seqlens_q, context_lens, seq_lens, 
     return z[:, :P], rows[0], rows[1]
 
 
+def kbar_pages_ok(idx_k, pool, block_size):
+    """Whether kbar_pages takes these paged index keys and this k_bar pool."""
+    return (idx_k.dim() == 3 and idx_k.shape[1] == block_size and idx_k.shape[2] == 128
+            and pool.shape[-1] == 128 and 0 < block_size <= 64 and pool.shape[0] > 0
+            and pool.dtype == torch.float32 and pool.is_contiguous() and pool.data_ptr() % 16 == 0
+            and idx_k.dtype == torch.float32 and idx_k.stride(-1) == 1
+            and idx_k.data_ptr() % 16 == 0 and all(s % 4 == 0 for s in idx_k.stride()[:-1]))
+
+
+def kbar_pages(idx_k, head_cls, first_tokens, seq_lens, block_table, pool, block_size):
+    """The summaries of blocks first_tokens[b] // block_size .. of every sequence of seq_lens[b]
+    tokens, written to their pages' rows of the k_bar pool [pages, 128] in one launch
+    (KBarPageCache.refresh_from in its one-block pages)."""
+    _need_gpu(idx_k, head_cls, first_tokens, seq_lens, block_table, pool)
+    B, P = block_table.shape
+    first, lens, bt = (_i32(x) for x in (first_tokens, seq_lens, block_table))
+    hc = _aligned(head_cls.float())
+    _lib.check(_lib.load().dash_kbar_pages(
+        _ptr(idx_k), idx_k.stride(1), idx_k.stride(0), _ptr(hc), _ptr(first), _ptr(lens), _ptr(bt),
+        bt.stride(0), _ptr(pool), pool.shape[0], B, P, idx_k.shape[2], int(block_size), _stream()),
+        "dash_kbar_pages")
+
+
 def attn_extend_ok(q, k, v, K, block_size, page_size, num_blocks, scale):
     """Whether attn_extend takes these rows (else attn_rows).  Any number of rows: an extend
     step of 2 rows takes 107 us grouped and 138 row by row (caches of 13,650 tokens), of 128

@@ -4,14 +4,16 @@
 block scores -> route -> fused attention) and ``decode_step`` the decode step of
 modeling_deepseekv2.py:481-498, except that the k_bar cache is refreshed only at
 the tail block instead of being rebuilt from the whole index-key cache every step
-(the summaries of complete blocks never change).
+(the summaries of complete blocks never change).  ``extend_prefill``, ``tree_step`` and
+``commit_tree`` are the serving steps over a paged cache: a chunk of known tokens, and a tree of
+drafted ones with the update of the cache after its verification.
 """
 
 import math
 
 import torch
 
-from . import ops
+from . import ops, tree
 
 
 def prefill(q, k, v, idx_q, idx_k, head_cls, block_size, local_blocks, idx_scale, floor,
@@ -178,6 +180,76 @@ def extend_prefill(state, q, k_cache, v_cache, idx_q, idx_k, head_cls, block_siz
     if return_routing:
         return out, (idx, bias, valid.bool()), q_pos
     return out
+
+
+def tree_step(state, q, k_cache, v_cache, idx_q, block_size, local_blocks, idx_scale, floor,
+              sigma, K, topm, block_table, context_lens, cu_seqlens_q, parents, max_query_len,
+              scale=None, block_cand=None, out_dtype=torch.bfloat16, return_routing=False):
+    """One step of a tree of drafted tokens per request over a paged cache: the rows of request b
+    are the nodes of its tree (node 0 the newest sampled token, the others drafted; parents [T],
+    see tree.tree_masks), whose keys and values are already written at slots context_lens[b] + i.
+    Node i is at position context_lens[b] + depth and
+
+    * scores the summaries of its request's committed blocks (state, a KBarPageCache that holds
+      them: put_sequences after the prefill, commit_tree after each step);
+    * routes like a decode row at that position;
+    * attends the committed keys of its window and of its routed blocks, its ancestors and itself.
+
+    A chain gives extend_prefill's rows: no drafted key is remote while the tree is not deeper than
+    the window.  q [T,H,D] bf16, k_cache / v_cache [pages, block_size, Hkv, D] bf16 (H a multiple
+    of Hkv), idx_q [T,d] fp32, block_table [B,P] int32, context_lens [B], cu_seqlens_q [B+1],
+    max_query_len the largest tree.  Returns out [T,H,D] (out_dtype)."""
+    if not getattr(state, "paged", False):
+        raise NotImplementedError("tree_step takes a k_bar page pool (KBarPageCache)")
+    T, H, D = q.shape
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    ctx, cu, table = (x.to(device=q.device, dtype=torch.int32).contiguous()
+                      for x in (context_lens, cu_seqlens_q, block_table))
+    B, P = table.shape
+    mask, depth = tree.tree_masks(parents, cu, max_query_len)
+    idx_q = idx_q.reshape(T, -1)
+    pool = state.kbar
+    if idx_q.shape[1] == 128 and pool.shape[1] == 128 and pool.data_ptr() % 16 == 0:
+        idx_q = idx_q if idx_q.dtype == torch.float32 else idx_q.float()
+        z, q_pos, row_nblk = tree.tree_scores(ops._f4_rows(idx_q), cu, ctx, depth, table, pool,
+                                              block_size, local_blocks, max_query_len)
+    else:
+        kb_seq = pool.index_select(0, table.to(torch.int64).clamp(0, pool.shape[0] - 1)
+                                   .reshape(-1)).view(B, P, -1)
+        row_seq = _row_seq(cu, B, T)
+        q_pos = ctx.index_select(0, row_seq) + depth
+        z = ops.block_scores(idx_q.reshape(1, T, -1), kb_seq, block_size, local_blocks,
+                             q_pos=q_pos, cu_seqlens=cu, max_seqlen=max_query_len, key_lens=ctx,
+                             S=P * block_size)
+        row_nblk = ((ctx + block_size - 1) // block_size).index_select(0, row_seq)
+    width = max(1, min(int(K), int(topm))) if int(topm) > 0 else max(1, int(K))
+    idx, bias, valid = ops.route(z, block_cand, idx_scale, floor, sigma, K, topm,
+                                 row_nblk=row_nblk, width=width)
+    out = tree.attn_tree(q, k_cache, v_cache, idx, bias, valid, mask, depth, ctx, cu,
+                         max_query_len, block_size, local_blocks * block_size, scale,
+                         block_table=table, page_size=block_size, out_dtype=out_dtype)
+    if return_routing:
+        return out, (idx, bias, valid), q_pos
+    return out
+
+
+def commit_tree(pool, path, count, context_lens, layers=()):
+    """After a tree step's verification (path and count of tree.verify_tree): the accepted rows are
+    moved up in the caches of ``pool`` (kv_pages.PagePool, whose row b is request b), the others
+    given back with their pages, and for every (state, idx_k, head_cls) of ``layers`` (its
+    KBarPageCache and paged index keys) the block summaries are recomputed from the step's first
+    block on.  Returns the new context lengths [B] int32 (requests without nodes keep theirs)."""
+    ctx = context_lens.to(device=pool.lens.device, dtype=torch.int32)
+    kept = pool.keep(path, count, ctx)
+    new = torch.where(count > 0, kept, ctx)
+    bs = pool.page_size
+    for state, idx_k, head_cls in layers:
+        if ops.kbar_pages_ok(idx_k, state.kbar, bs):
+            ops.kbar_pages(idx_k, head_cls, ctx, new, pool.table, state.kbar, bs)
+        else:
+            state.refresh_from(idx_k, head_cls, bs, pool.table, new, ctx // bs)
+    return new
 
 
 def init_decode_state(idx_k, head_cls, block_size, nblk_cap, seq_lens=None, block_table=None,

@@ -639,6 +639,150 @@ int dash_decode_step_noalloc(const float* idx_q, int64_t iq_sb, const float* idx
 /* Bytes of the fixed scratch array dash_decode_step_noalloc uses (per GPU). */
 int64_t dash_decode_step_scratch_bytes(void);
 
+/*
+ * Trees of drafted tokens.  Row cu_seqlens_q[b] + i (cu_seqlens_q [B + 1], T rows in all, at most
+ * max_query_len <= 256 a sequence) is node i of sequence b, node 0 its root; parents [T] holds
+ * each node's parent within its sequence, an earlier node (anything else: none).  The key and
+ * value of node i lie in the cache at slot context_lens[b] + i.
+ */
+
+/* mask [T, words] (words = ceil(max_query_len / 64)): bit m of row (b, i) is set where node m is
+ * node i or one of its ancestors; depth [T]: the number of its ancestors. */
+int dash_tree_masks(const int32_t* parents, const int32_t* cu_seqlens_q, int B, int64_t T,
+                    int max_query_len, int words, int64_t* mask, int32_t* depth, void* stream);
+
+/*
+ * Router inputs of a tree's rows, as dash_extend_scores gives them for a chunk's: row r of
+ * sequence b is at position q_pos[r] = context_lens[b] + depth[r], its blocks are those of the
+ * context_lens[b] committed tokens (row_nblk [T]), whose summaries the k_bar pool holds.
+ */
+int dash_tree_scores(const float* idx_q, int64_t iq_st, const int32_t* cu_seqlens_q,
+                     const int32_t* context_lens, const int32_t* depth,
+                     const int32_t* block_table, int64_t table_stride, const float* pool,
+                     int pool_rows, int B, int T, int max_query_len, int nblk, int d,
+                     int block_size, int local_blocks, int32_t* q_pos, int32_t* row_nblk, float* z,
+                     int64_t z_stride, void* stream);
+
+/* The summaries of blocks first_tokens[b] / block_size .. of sequences of seq_lens[b] tokens,
+ * written to their pages' rows of the k_bar pool [pool_rows, 128] (pages of one block; idx_k as in
+ * dash_extend_scores).  block_size <= 64. */
+int dash_kbar_pages(const float* idx_k, int64_t ik_st, int64_t ik_sp, const float* head_cls,
+                    const int32_t* first_tokens, const int32_t* seq_lens,
+                    const int32_t* block_table, int64_t table_stride, float* pool, int pool_rows,
+                    int B, int nblk, int d, int block_size, void* stream);
+
+/* Workspace bytes dash_attn_tree needs (S: keys a sequence's table or cache row has room for). */
+int dash_attn_tree_workspace_size(int B, int H, int Hkv, int64_t T, int max_query_len, int K, int S,
+                                  int block_size, int local_window, int64_t* bytes);
+
+/*
+ * Attention of a tree's rows q [T, H, 128] bf16 over a cache with Hkv key heads (H a multiple;
+ * query head h reads key head h / (H / Hkv)): contiguous [B, Hkv, S, 128] (k_sb the sequence
+ * stride) or pages [num_pages, page_size, Hkv, 128] (k_sb the page stride) through block_table.
+ * With t = context_lens[b] + depth[r] and w = t - local_window + 1 a row sees
+ *   the committed keys j >= w                                               (j < context_lens[b])
+ *   the committed keys j < w of its routed blocks idx [T, K] (valid; a block's first slot), each
+ *   with the bias of its slot
+ *   the drafted keys m whose bit is set in its mask row (node m of its sequence)
+ * out [T, H, 128] fp32 (out_bf16 = 0) or bf16, lse [T, H] optional; a row that sees no key gives 0
+ * and -inf.  block_size 32 or a multiple of 64, page_size a multiple of it, K <= 64, at most
+ * 2,048 blocks.  workspace: dash_attn_tree_workspace_size bytes, any contents.
+ */
+int dash_attn_tree(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_sb,
+                   int64_t k_sh, int64_t k_st, const void* v, int64_t v_sb, int64_t v_sh,
+                   int64_t v_st, const int32_t* block_table, int64_t table_stride, int page_size,
+                   int num_pages, const int32_t* context_lens, const int32_t* cu_seqlens_q,
+                   const int32_t* idx, const uint8_t* valid, const float* bias, int K,
+                   const int64_t* mask, int words, const int32_t* depth, void* out, int out_bf16,
+                   int64_t o_st, int64_t o_sh, float* lse, int64_t lse_st, int64_t lse_sh, int B,
+                   int H, int Hkv, int64_t T, int max_query_len, int S, int D, int block_size,
+                   int local_window, float scale, void* workspace, int64_t workspace_bytes,
+                   void* stream);
+
+/* Workspace bytes dash_verify_tree needs (greedy: uniforms == NULL). */
+int dash_verify_tree_workspace_size(int B, int64_t T, int V, int greedy, int64_t* bytes);
+
+/*
+ * Verification of drafted tokens [T] (int32, or int64 with tokens_int64) against the target's
+ * distributions target [T, V] (row r: of the token after node r; dtype 0 fp32, 1 bf16, 2 fp16).
+ * At a node, from the root on, its children are tried in order:
+ *   uniforms NULL: greedy; a child that is the row's largest entry (lowest id of equals, NaN never)
+ *   uniforms [T], draft NULL: with Z = 1 at first, a child with token x is accepted if
+ *     uniforms[child] Z < p(x), else x leaves p and Z -= p(x)
+ *   uniforms [T], draft [T, V] (row r: the distribution node r's children were drawn from, each by
+ *     itself): with a = 0 and Z = 1, accepted if uniforms[child] Z q(x) < max(p(x) - a q(x), 0),
+ *     else a += Z and Z = sum_v max(p - a q, 0)
+ * path [B, max_query_len]: the accepted nodes, the root first, -1 past them; count [B]: their
+ * number (0 for a sequence without nodes, whose next_token is -1); next_token [B]: greedy, the last
+ * node's best token (0 for a row with nothing above -inf), else drawn by uniforms[root] from what is
+ * left at the last node: the first id whose running sum exceeds uniforms[root] times the whole (the
+ * row itself where nothing is left, -1 where that holds nothing above 0 either).  Probabilities that
+ * are not above 0 count as 0; a token outside [0, V) is rejected.  Sums in 64 bits.
+ */
+int dash_verify_tree(const void* target, int64_t target_stride, const void* draft,
+                     int64_t draft_stride, int dtype, const void* tokens, int tokens_int64,
+                     const int32_t* parents, const int32_t* cu_seqlens_q, const float* uniforms,
+                     int B, int64_t T, int V, int max_query_len, int32_t* count, int32_t* path,
+                     int64_t path_stride, int64_t* next_token, void* workspace,
+                     int64_t workspace_bytes, void* stream);
+
+/*
+ * Pages of a paged cache.  refs [num_pages]: how many table entries name a page (0: free);
+ * block_table [R, P] (rows of table_stride); lens [R]: tokens of a row, whose first
+ * ceil(lens / page_size) entries are in use.  Free pages are handed out lowest first, to the rows in
+ * order.  R <= 8192.
+ *
+ * Caches are given in host arrays: caches[i], the address of cache i, and desc[8 i ..] in bytes:
+ * layers, layer stride, page stride, n1, s1, n2, s2, seg.  A layer's page is n1 x n2 pieces of seg
+ * bytes at strides s1 and s2 (dash_keep_rows: n1 is not used, s1 is the stride of a token and a row
+ * n2 pieces).  Read before the call returns.
+ */
+
+/* Page from_pages[i] -> to_pages[i] in every layer of every cache, i < num_pairs; pairs with a
+ * number outside [0, num_pages) are left out.  No page may be a source and a target, or two
+ * pairs' target. */
+int dash_copy_pages(int num_caches, void* const* caches, const int64_t* desc,
+                    const int32_t* from_pages, const int32_t* to_pages, int num_pairs, int num_pages,
+                    void* stream);
+
+/* The rows of accepted nodes moved up: slot context_lens[b] + path[b][i] -> context_lens[b] + i for
+ * 1 <= i < count[b] (path [B, max_query_len] strictly increasing, as dash_verify_tree gives it; other
+ * entries are left out). */
+int dash_keep_rows(int num_caches, void* const* caches, const int64_t* desc, const int32_t* path,
+                   int64_t path_stride, const int32_t* count, const int32_t* context_lens,
+                   const int32_t* block_table, int64_t table_stride, int B, int P, int page_size,
+                   int num_pages, int max_query_len, void* stream);
+
+/* Row dst_rows[i] (empty) becomes row src_rows[i]: its filled pages shared, a partly filled last one
+ * replaced by a page of its own, whose content is to be copied from_pages[i] -> to_pages[i] (-1: none).
+ * ok = 1; or ok = 0 and nothing changed, where a row is out of range, a target filled, repeated or a
+ * source, an entry of a source no page, or the free pages do not suffice. */
+int dash_fork_pages(int32_t* refs, int num_pages, int32_t* block_table, int64_t table_stride, int R,
+                    int P, int32_t* lens, const int32_t* src_rows, const int32_t* dst_rows, int n,
+                    int page_size, int32_t* ok, int32_t* from_pages, int32_t* to_pages, void* stream);
+
+/* Rows grow to new_lens [R] (shorter ones stay): pages for the blocks they lack, and a page of its
+ * own for the partly filled last page of a growing row that another row shares, to be copied
+ * from_pages[r] -> to_pages[r] (-1: none).  ok = 1, or 0 and nothing changed, where a length does not
+ * fit the table, such a last entry names no page, or the free pages do not suffice. */
+int dash_reserve_pages(int32_t* refs, int num_pages, int32_t* block_table, int64_t table_stride, int R,
+                       int P, int32_t* lens, const int32_t* new_lens, int page_size, int32_t* ok,
+                       int32_t* from_pages, int32_t* to_pages, void* stream);
+
+/* Rows longer than keep_lens [R] are cut to it; the entries above come out as -1 and their pages lose
+ * a name (free at 0). */
+int dash_free_pages(int32_t* refs, int num_pages, int32_t* block_table, int64_t table_stride, int R,
+                    int P, int32_t* lens, const int32_t* keep_lens, int page_size, void* stream);
+
+/* With L pages in use, the i-th page in use at or above L moves to the i-th free page below it:
+ * new_refs [num_pages], new_table [R, P] (contiguous; entries not in use -1), and the moves
+ * from_pages / to_pages [num_pages / 2] (-1 past them).  place [num_pages] is scratch.  The inputs stay
+ * as they are. */
+int dash_compact_pages(const int32_t* refs, int num_pages, const int32_t* block_table,
+                       int64_t table_stride, int R, int P, const int32_t* lens, int page_size,
+                       int32_t* new_refs, int32_t* new_table, int32_t* from_pages,
+                       int32_t* to_pages, int32_t* place, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
