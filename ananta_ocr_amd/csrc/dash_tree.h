@@ -13,6 +13,7 @@
 namespace dash {
 
 constexpr int kTrMaxNodes = 256;
+constexpr int64_t kTrTarget = 1024;       // work-groups a call aims at
 
 struct TreeArgs {
   const bf16* q; int64_t q_st, q_sh;
@@ -25,6 +26,9 @@ struct TreeArgs {
   void* out; int out_bf16; int64_t o_st, o_sh;
   float* lse; int64_t lse_st, lse_sh;
   int B, H, Hkv, S, bs, lw, max_n;
+  int groups, nsplit;
+  float* part_o;                               // [T, H, nsplit, 128], not normalised
+  float2* part_ml;                             // [T, H, nsplit] base-2 reference and weight sum
   int64_t T;
   float scale_log2e;
 };
@@ -67,93 +71,518 @@ __global__ __launch_bounds__(kTrMaxNodes) void tree_masks_kernel(const int32_t* 
   depth[r0 + i] = d;
 }
 
-// One wavefront per (row, head): 16 lanes per key row, four keys per load.
-__global__ __launch_bounds__(kWave) void tree_rows_kernel(TreeArgs a) {
-  constexpr int D = 128;
-  const int h = blockIdx.x, lane = threadIdx.x;
-  const int64_t row = blockIdx.y;
-  int b = 0;
-  {
-    int hi = a.B;
-    while (hi - b > 1) {
-      const int mid = (b + hi) >> 1;
-      if (a.cu[mid] <= row) b = mid; else hi = mid;
-    }
-  }
+// ---------------------------------------------------------------------------
+// One work-group per (sequence, key head, 32 RT rows, split).  The rows of a key head are
+// (node, query head of its group) pairs, node first.  Keys come in halves of 32: the band from
+// the root's window to the last drafted key, then the blocks that the rows name, in ascending
+// order; an item is two halves, 64 keys of K and V in a double-buffered LDS stage filled by
+// direct loads.  The items of a (sequence, head) are divided evenly among its splits, each of which
+// writes an unnormalised fp32 partial that tree_merge_kernel adds up (one split writes the result).
+//
+// RT row tiles of 32 rows are the columns of S^T = K Q^T (v_mfma_f32_32x32x16_bf16); with KG = 2
+// two wavefronts share a row tile, one half of every item each, and meet at the end.  A half's
+// visible keys are 32 bits per row, so the band's edges, the drafted keys' mask and the routed
+// blocks of rows that do not name them are one test.  A weight enters the second product as three
+// bf16 parts (24 bits), as in the extend kernels: it is not rounded.
+// ---------------------------------------------------------------------------
+constexpr int kTrBatch = 32;              // routed blocks whose rows' slots are looked up at a time
+
+template <int RT, int KG>
+struct TreeShared {
+  __attribute__((aligned(16))) bf16 k[2][64 * 128];
+  __attribute__((aligned(16))) bf16 v[2][64 * 128];
+  uint32_t bits[kPfMaxBlocks / 32];       // the blocks that the rows name
+  int16_t list[kPfMaxBlocks];             // in ascending order
+  uint8_t sel[kTrBatch][32 * RT];         // slot + 1 of (block, node), 0: not named
+  uint32_t bad[RT * KG];
+  int total;
+};
+
+template <int RT, int KG>
+__global__ __launch_bounds__(64 * RT * KG, 2) void tree_attn_kernel(TreeArgs a) {
+  constexpr int D = 128, NW = RT * KG, TH = 64 * NW;
+  constexpr int NH = 2 / KG;              // halves of an item that a wavefront takes
+  __shared__ TreeShared<RT, KG> sm;
+  const int tid = threadIdx.x, lane = wave_lane(), wv = tid / kWave;
+  const int rt = wv % RT, kg = wv / RT;
+  int id = blockIdx.x;
+  const int hk = id % a.Hkv; id /= a.Hkv;
+  const int split = id % a.nsplit; id /= a.nsplit;
+  const int rg = id % a.groups, b = id / a.groups;
+  const int G = a.H / a.Hkv;
+  const int64_t r0 = a.cu[b];
   const int ctx = tree_ctx(a, b);
-  const int n = min(min((int)(a.cu[b + 1] - a.cu[b]), a.max_n), a.S - ctx);
-  const int hk = h / (a.H / a.Hkv);
-  const int w0 = ctx + a.depth[row] - a.lw + 1;
-  const int g = lane >> 4, dl = (lane & 15) * 8;
-  const bf16x8 q = *(const bf16x8*)(a.q + row * a.q_st + (int64_t)h * a.q_sh + dl);
-  float m = -INFINITY, l = 0.f, o[8];
-  for (int e = 0; e < 8; ++e) o[e] = 0.f;
-  // keys j0 .. j1 - 1; sees(j) the mask, blog the log2 bias
-  auto keys = [&](int j0, int j1, float blog, auto sees) {
-    for (int j = j0; j < j1; j += 4) {
-      const int key = min(j + g, j1 - 1);
+  const int nn = min((int)(a.cu[b + 1] - r0), a.max_n);   // nodes
+  const int n = min(nn, a.S - ctx);                       // with a slot in the cache
+  const int R = nn * G, rb = rg * RT * 32;
+  if (rb >= R) return;
+  const int node0 = rb / G, node1 = min(nn, (rb + RT * 32 - 1) / G + 1);
+  const int nblk = (a.S + a.bs - 1) / a.bs;
+
+  // this lane's row
+  const int hl = lane >> 5, col = lane & 31;
+  const int rr = min(rb + rt * 32 + col, R - 1);
+  const bool rvalid = rb + rt * 32 + col < R;
+  const int node = rr / G;
+  const int64_t row = r0 + node;
+  const int h = hk * G + rr % G;
+  const int w_row = ctx + a.depth[row] - a.lw + 1;
+  const int top = min(w_row, ctx);
+  bf16x8 qop[D / 16];
+  {
+    const bf16* qb = a.q + row * a.q_st + (int64_t)h * a.q_sh;
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) qop[kk] = *(const bf16x8*)(qb + kk * 16 + hl * 8);
+  }
+
+  // the blocks that the rows name, and their order
+  auto usable = [&](int64_t at, int node_top, int& c) {
+    c = a.idx[at];
+    return c >= 0 && c < nblk && c * a.bs < node_top && (!a.valid || a.valid[at]);
+  };
+  int n_blocks = 0;
+  if (a.K > 0) {
+    for (int i = tid; i < kPfMaxBlocks / 32; i += TH) sm.bits[i] = 0u;
+    __syncthreads();
+    for (int i = tid; i < (node1 - node0) * a.K; i += TH) {
+      const int64_t rw = r0 + node0 + i / a.K;
+      int c;
+      if (usable(rw * a.K + i % a.K, min(ctx + a.depth[rw] - a.lw + 1, ctx), c))
+        atomicOr(&sm.bits[c >> 5], 1u << (c & 31));
+    }
+    __syncthreads();
+    if (wv == 0) {
+      uint32_t w = sm.bits[lane];
+      int x = __popc(w);
+      const int own = x;
+#pragma unroll
+      for (int s = 1; s < kWave; s <<= 1) {
+        const int y = __shfl_up(x, s, kWave);
+        if (lane >= s) x += y;
+      }
+      if (lane == kWave - 1) sm.total = x;
+      for (int at = x - own; w; w &= w - 1) sm.list[at++] = (int16_t)(32 * lane + __builtin_ctz(w));
+    }
+    __syncthreads();
+    n_blocks = sm.total;
+  }
+
+  // items: the band's, then the blocks'
+  const int hpb = a.bs / 32;              // halves of a block
+  const int jw0 = max(ctx - a.lw + 1, 0) & ~31;
+  const int jend = ctx + n;
+  const int n_wi = (jend - jw0 + 63) / 64;
+  const int n_items = n_wi + (n_blocks * hpb + 1) / 2;
+  const int i0 = (int)((int64_t)n_items * split / a.nsplit);
+  const int i1 = (int)((int64_t)n_items * (split + 1) / a.nsplit);
+
+  // half hf of item i: its first key, the place of its block in the list (-1: the band; -2: no keys)
+  auto half_of = [&](int i, int hf, int& at) -> int {
+    if (i < n_wi) {
+      const int j = jw0 + 64 * i + 32 * hf;
+      at = j < jend ? -1 : -2;
+      return j < jend ? j : j - 32;
+    }
+    const int x = 2 * (i - n_wi) + hf;
+    at = x / hpb;
+    if (at >= n_blocks) { at = -2; return sm.list[(x - 1) / hpb] * a.bs + (x - 1) % hpb * 32; }
+    return sm.list[at] * a.bs + x % hpb * 32;
+  };
+  auto fetch = [&](int i, int buf) {
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      int at;
+      const int j = __builtin_amdgcn_readfirstlane(half_of(i, hf, at));
+      const int last = (i < n_wi ? jend : ctx) - 1;
       int64_t kr, vr;
       if (a.table) {
-        const int p = tree_page(a, a.table[(int64_t)b * a.table_stride + key / a.page]);
-        kr = (int64_t)p * a.k_sb + (int64_t)(key % a.page) * a.k_st;
-        vr = (int64_t)p * a.v_sb + (int64_t)(key % a.page) * a.v_st;
+        const int p = tree_page(a, a.table[(int64_t)b * a.table_stride + j / a.page]);
+        kr = (int64_t)p * a.k_sb + (int64_t)(j % a.page) * a.k_st;
+        vr = (int64_t)p * a.v_sb + (int64_t)(j % a.page) * a.v_st;
       } else {
-        kr = (int64_t)b * a.k_sb + (int64_t)key * a.k_st;
-        vr = (int64_t)b * a.v_sb + (int64_t)key * a.v_st;
+        kr = (int64_t)b * a.k_sb + (int64_t)j * a.k_st;
+        vr = (int64_t)b * a.v_sb + (int64_t)j * a.v_st;
       }
-      const bf16x8 kx = *(const bf16x8*)(a.k + kr + (int64_t)hk * a.k_sh + dl);
-      const bf16x8 vx = *(const bf16x8*)(a.v + vr + (int64_t)hk * a.v_sh + dl);
-      float s = 0.f;
-      for (int e = 0; e < 8; ++e) s += (float)q[e] * (float)kx[e];
-      for (int x = 1; x < 16; x <<= 1) s += __shfl_xor(s, x, kWave);
-      const bool ok = j + g < j1 && sees(key);
-      s = ok ? s * a.scale_log2e + blog : -INFINITY;
-      const float mn = fmaxf(m, s);
-      const float mu = mn == -INFINITY ? 0.f : mn;
-      const float al = fast_exp2(m - mu), p = fast_exp2(s - mu);
-      l = l * al + p;
-      for (int e = 0; e < 8; ++e) o[e] = o[e] * al + (ok ? p * (float)vx[e] : 0.f);
-      m = mn;
+      const bf16* kb = a.k + kr + (int64_t)hk * a.k_sh;
+      const bf16* vb = a.v + vr + (int64_t)hk * a.v_sh;
+#pragma unroll
+      for (int u = 0; u < 8 / NW; ++u) {
+        const int grp = NW * u + wv;      // four rows a wavefront
+        const int r = 4 * grp + (lane >> 4);
+        const int off = min(j + r, last) - j;
+        __builtin_amdgcn_global_load_lds(
+            (const void*)(kb + (int64_t)off * a.k_st + k_slot(r, lane & 15) * 8),
+            (__attribute__((address_space(3))) void*)(sm.k[buf] + (hf * 32 + grp * 4) * D), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds(
+            (const void*)(vb + (int64_t)off * a.v_st + v_slot(r, lane & 15) * 8),
+            (__attribute__((address_space(3))) void*)(sm.v[buf] + (hf * 32 + grp * 4) * D), 16, 0, 0);
+      }
     }
   };
-  keys(max(w0, 0), ctx, 0.f, [](int) { return true; });
-  keys(ctx, ctx + n, 0.f, [&](int j) {
-    const int x = j - ctx;
-    return ((a.mask[row * a.words + (x >> 6)] >> (x & 63)) & 1ull) != 0;
-  });
-  const int top = min(w0, ctx);             // routed keys lie below it
-  for (int s = 0; s < a.K; ++s) {
-    auto usable = [&](int x) {
-      const int c = a.idx[row * a.K + x];
-      return c >= 0 && c < (a.S + a.bs - 1) / a.bs && c * a.bs < top && (!a.valid || a.valid[row * a.K + x]);
-    };
-    if (!usable(s)) continue;
-    const int c = a.idx[row * a.K + s];
-    bool first = true;
-    for (int x = 0; x < s; ++x) first = first && !(a.idx[row * a.K + x] == c && usable(x));
-    if (first)
-      keys(c * a.bs, min((c + 1) * a.bs, top), a.bias[row * a.K + s] * 1.4426950408889634f,
-           [](int) { return true; });
+  // the keys of a half that this lane's row sees, a bit each, and their log2 bias
+  auto visible = [&](int i, int hf, float& blog) -> uint32_t {
+    int at;
+    const int j = half_of(i, hf, at);
+    blog = 0.f;
+    if (at == -2 || !rvalid) return 0u;
+    auto below = [](int x) -> uint32_t { return x >= 32 ? ~0u : x <= 0 ? 0u : (1u << x) - 1u; };
+    if (at == -1) {
+      uint32_t v = below(ctx - j) & ~below(w_row - j);
+      const int m0 = j - ctx;
+      if (m0 > -32) {
+        uint64_t m;
+        if (m0 < 0) {
+          m = a.mask[row * a.words] << -m0;
+        } else {
+          const int wd = m0 >> 6, sh = m0 & 63;
+          m = a.mask[row * a.words + wd] >> sh;
+          if (sh > 32 && wd + 1 < a.words) m |= a.mask[row * a.words + wd + 1] << (64 - sh);
+        }
+        v |= (uint32_t)m & below(jend - j) & ~below(ctx - j);
+      }
+      return v;
+    }
+    const int s = sm.sel[at % kTrBatch][node - node0];
+    if (s == 0) return 0u;
+    blog = a.bias[row * a.K + s - 1] * 1.4426950408889634f;
+    return below(top - j);
+  };
+  // the slots of the blocks at list places of one batch
+  auto look_up = [&](int batch) {
+    for (int x = tid; x < kTrBatch * 32 * RT / 4; x += TH) ((uint32_t*)sm.sel)[x] = 0u;
+    __syncthreads();
+    const int l0 = batch * kTrBatch, l1 = min(l0 + kTrBatch, n_blocks);
+    for (int nd = node0 + tid; nd < node1; nd += TH) {
+      const int64_t rw = r0 + nd;
+      const int nt = min(ctx + a.depth[rw] - a.lw + 1, ctx);
+      for (int s = a.K - 1; s >= 0; --s) {        // the first slot of a block is written last
+        int c;
+        if (!usable(rw * a.K + s, nt, c) || c < sm.list[l0] || c > sm.list[l1 - 1]) continue;
+        int lo = l0, hi = l1;
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) >> 1;
+          if (sm.list[mid] <= c) lo = mid; else hi = mid;
+        }
+        sm.sel[lo - l0][nd - node0] = (uint8_t)(s + 1);
+      }
+    }
+    __syncthreads();
+  };
+
+  floatx16 acc_o[D / 32];
+  float m_run, l_run;
+  auto reset = [&] {
+    m_run = -INFINITY;
+    l_run = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc_o[dt][r] = 0.f;
+  };
+  const uint32_t kl0 = k_lane_off(col, hl), vl0 = v_lane_off(lane);
+  const float csc = a.scale_log2e;
+
+  // this wavefront's halves of item i in stage `buf`
+  auto item = [&](int i, int buf, uint32_t (&vis)[NH]) __attribute__((always_inline)) {
+    float blog[NH];
+    bool any = false;
+#pragma unroll
+    for (int x = 0; x < NH; ++x) {
+      vis[x] = visible(i, KG == 2 ? kg : x, blog[x]);
+      any = any || vis[x] != 0u;
+    }
+    if (!__any(any)) return;
+    floatx16 s[NH];
+    float mloc = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < NH; ++x) {
+      const int hf = KG == 2 ? kg : x;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[x][r] = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk)
+        s[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k_frag_at(sm.k[buf], kl0, hf, kk), qop[kk], s[x],
+                                                       0, 0, 0);
+      const uint32_t vb = vis[x] >> (4 * hl);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[x][r] = (vb >> (8 * (r >> 2) + (r & 3))) & 1u ? fmaf(s[x][r], csc, blog[x]) : -INFINITY;
+        mloc = fmaxf(mloc, s[x][r]);
+      }
+    }
+    mloc = xor32_max(mloc);
+    // the reference moves only when a row's maximum exceeds it by more than 8
+    const bool up = mloc > m_run + 8.f;
+    if (__any(up)) {
+      const float alpha = up ? fast_exp2(m_run - mloc) : 1.f;
+      l_run *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc_o[dt][r] *= alpha;
+      m_run = up ? mloc : m_run;
+    }
+    const float off = m_run == -INFINITY ? 0.f : m_run;
+#pragma unroll
+    for (int x = 0; x < NH; ++x) {
+      const int hf = KG == 2 ? kg : x;
+      bf16x8 ph[2], pm[2], pl[2];
+#pragma unroll
+      for (int jj = 0; jj < 2; ++jj) {
+        float p[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) p[e] = fast_exp2(s[x][8 * jj + e] - off);
+        l_run += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+        ext_split3(p, ph[jj], pm[jj], pl[jj]);
+      }
+      // the half's products sum from zero, smallest parts first, before they meet the row's total
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt) {
+        bf16x8 vop[2];
+#pragma unroll
+        for (int jj = 0; jj < 2; ++jj) {
+          const char* vp = (const char*)sm.v[buf] + (32 * hf + 16 * jj) * 256 + (vl0 ^ (uint32_t)(dt << 6));
+          const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (lds_short4*)(__attribute__((address_space(3))) void*)vp);
+          const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (lds_short4*)(__attribute__((address_space(3))) void*)(vp + 2048));
+          const bf16x4 l4 = __builtin_bit_cast(bf16x4, lo);
+          const bf16x4 h4 = __builtin_bit_cast(bf16x4, hi);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) { vop[jj][e] = l4[e]; vop[jj][e + 4] = h4[e]; }
+        }
+        floatx16 t;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) t[r] = 0.f;
+#pragma unroll
+        for (int jj = 0; jj < 2; ++jj) t = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vop[jj], pl[jj], t, 0, 0, 0);
+#pragma unroll
+        for (int jj = 0; jj < 2; ++jj) t = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vop[jj], pm[jj], t, 0, 0, 0);
+#pragma unroll
+        for (int jj = 0; jj < 2; ++jj) t = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vop[jj], ph[jj], t, 0, 0, 0);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc_o[dt][r] += t[r];
+      }
+    }
+  };
+  // the batch of list places that item i's blocks belong to (items do not straddle: a batch is
+  // a whole number of items' halves), -1 for the band
+  auto batch_of = [&](int i) { return i < n_wi ? -1 : 2 * (i - n_wi) / hpb / kTrBatch; };
+
+  reset();
+  uint32_t vis[NH];
+  int batch = -1;
+  if (i0 < i1) fetch(i0, 0);
+  for (int i = i0; i < i1; ++i) {
+    const int nb = batch_of(i);
+    if (nb != batch) {                    // before the barrier below: no wavefront is past it
+      __syncthreads();
+      look_up(nb);
+      batch = nb;
+    }
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();                      // item i landed; every wavefront left item i - 1
+    if (i + 1 < i1) fetch(i + 1, (i + 1 - i0) & 1);
+    item(i, (i - i0) & 1, vis);
   }
-  // the four lane groups
-  for (int x = 16; x <= 32; x <<= 1) {
-    const float m2 = __shfl_xor(m, x, kWave), l2 = __shfl_xor(l, x, kWave);
-    const float mn = fmaxf(m, m2), mu = mn == -INFINITY ? 0.f : mn;
-    const float al = fast_exp2(m - mu), be = fast_exp2(m2 - mu);
-    for (int e = 0; e < 8; ++e) o[e] = o[e] * al + __shfl_xor(o[e], x, kWave) * be;
-    l = l * al + l2 * be;
-    m = mn;
-  }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-  if (g == 0) {
-    const int64_t at = row * a.o_st + (int64_t)h * a.o_sh + dl;
-    for (int e = 0; e < 8; ++e) {
-      if (a.out_bf16) ((bf16*)a.out)[at + e] = (bf16)(o[e] * inv);
-      else ((float*)a.out)[at + e] = o[e] * inv;
+
+  // V values that are not finite reached every row of the tile through masked weights: the items
+  // again, with V's finite values in the products and the others for the rows that see them
+  float z = 0.f;
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) z = fmaf(acc_o[dt][r], 0.f, z);
+  if (__syncthreads_or(z != 0.f)) {
+    reset();
+    batch = -1;
+    for (int i = i0; i < i1; ++i) {
+      __syncthreads();                    // every wavefront left the stage
+      fetch(i, 0);
+      const int nb = batch_of(i);
+      if (nb != batch) { look_up(nb); batch = nb; }
+      __builtin_amdgcn_s_waitcnt(0);
+      // each wavefront clears the rows it loaded; bit 8 hf + u: its group u of half hf holds some
+      uint32_t bad = 0;
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+        for (int u = 0; u < 8 / NW; ++u) {
+          uint4* p = (uint4*)(sm.v[0] + (hf * 32 + (NW * u + wv) * 4) * D) + lane;
+          uint4 x = *p;
+          bool is = false;
+          auto fix = [&](uint32_t& w) {
+            if ((w & 0x7f80u) == 0x7f80u) { w &= 0xffff0000u; is = true; }
+            if ((w & 0x7f800000u) == 0x7f800000u) { w &= 0xffffu; is = true; }
+          };
+          fix(x.x); fix(x.y); fix(x.z); fix(x.w);
+          if (is) *p = x;
+          if (__any(is)) bad |= 1u << (8 * hf + u);
+        }
+      if (lane == 0) sm.bad[wv] = bad;
+      __syncthreads();
+#pragma unroll
+      for (int y = 0; y < NH; ++y) vis[y] = 0u;
+      item(i, 0, vis);
+#pragma unroll
+      for (int y = 0; y < NH; ++y) {
+        const int hf = KG == 2 ? kg : y;
+        int at;
+        const int j = half_of(i, hf, at);
+        const int last = (i < n_wi ? jend : ctx) - 1;
+        for (int w = 0; w < NW; ++w)
+          for (uint32_t todo = (sm.bad[w] >> (8 * hf)) & 0xffu; todo; todo &= todo - 1)
+            for (int q4 = 0; q4 < 4; ++q4) {
+              const int r = 4 * (NW * __builtin_ctz(todo) + w) + q4;
+              if (j + r > last) continue;          // a repeated row
+              const bool sees = (vis[y] >> r) & 1u;
+              const int64_t vr = a.table
+                  ? (int64_t)tree_page(a, a.table[(int64_t)b * a.table_stride + j / a.page]) * a.v_sb +
+                        (int64_t)(j % a.page + r) * a.v_st
+                  : (int64_t)b * a.v_sb + (int64_t)(j + r) * a.v_st;
+              const bf16* vp = a.v + vr + (int64_t)hk * a.v_sh + 4 * hl;
+#pragma unroll
+              for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                  const bf16x4 x = *(const bf16x4*)(vp + 32 * dt + 8 * q);
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) {
+                    const float f = (float)x[e];
+                    if (sees && !(fabsf(f) <= 3.402823466e38f)) acc_o[dt][4 * q + e] += f;
+                  }
+                }
+            }
+      }
     }
   }
+  float l_tot = xor32_sum(l_run);
+  if (KG == 2) {
+    // the second half's wavefronts hand their sums to the first's (through both stages' K, and V)
+    __syncthreads();
+    float* so = (float*)sm.k + rt * 32 * (D + 2);
+    if (kg == 1) {
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) so[(16 * dt + r) * 64 + lane] = acc_o[dt][r];
+      so[64 * 64 + lane] = hl ? l_tot : m_run;
+    }
+    __syncthreads();
+    if (kg == 1) return;
+    const float m2 = so[64 * 64 + col], l2 = so[64 * 64 + 32 + col];
+    const float mn = fmaxf(m_run, m2), mu = mn == -INFINITY ? 0.f : mn;
+    const float al = fast_exp2(m_run - mu), be = fast_exp2(m2 - mu);
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc_o[dt][r] = acc_o[dt][r] * al + so[(16 * dt + r) * 64 + lane] * be;
+    l_tot = l_tot * al + l2 * be;
+    m_run = mn;
+  }
+  if (!rvalid) return;
+  const int64_t rh = row * a.H + h;
+  if (a.nsplit > 1) {
+    float* po = a.part_o + (rh * a.nsplit + split) * D + 4 * hl;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *(float4*)(po + dt * 32 + 8 * q) = make_float4(acc_o[dt][4 * q], acc_o[dt][4 * q + 1],
+                                                       acc_o[dt][4 * q + 2], acc_o[dt][4 * q + 3]);
+    if (hl == 0) a.part_ml[rh * a.nsplit + split] = make_float2(m_run, l_tot);
+    return;
+  }
+  const bool none = m_run == -INFINITY && l_tot == 0.f;     // (a NaN score leaves m as it was)
+  const float inv = none ? 0.f : 1.f / l_tot;
+  const int64_t at = row * a.o_st + (int64_t)h * a.o_sh + 4 * hl;
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float x[4] = {acc_o[dt][4 * q] * inv, acc_o[dt][4 * q + 1] * inv, acc_o[dt][4 * q + 2] * inv,
+                          acc_o[dt][4 * q + 3] * inv};
+      if (a.out_bf16) {
+        bf16x4 y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = (bf16)x[e];
+        *(bf16x4*)((bf16*)a.out + at + 32 * dt + 8 * q) = y;
+      } else {
+        *(float4*)((float*)a.out + at + 32 * dt + 8 * q) = make_float4(x[0], x[1], x[2], x[3]);
+      }
+    }
+  if (a.lse && hl == 0)
+    a.lse[row * a.lse_st + (int64_t)h * a.lse_sh] =
+        none ? -INFINITY : (m_run + log2f(l_tot)) * 0.6931471805599453f;
+}
+
+// One wavefront per (row, head), two dims a lane; lane s holds the weight of split s (at most 64).
+// A split that saw no key wrote m = -inf and is not read.
+__global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
+  constexpr int D = 128;
+  const int64_t rh = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
+  if (rh >= a.T * a.H) return;
+  const int lane = wave_lane();
+  const float2 ml = lane < a.nsplit ? a.part_ml[rh * a.nsplit + lane] : make_float2(-INFINITY, 0.f);
+  const float M = wave_max(ml.x);
+  // NaN in a score leaves the maximum and comes in through the sums
+  const bool seen = lane < a.nsplit && !(ml.x == -INFINITY && ml.y == 0.f);
+  const float w = seen ? fast_exp2(ml.x - (M == -INFINITY ? 0.f : M)) : 0.f;
+  const float L = wave_sum(seen ? ml.y * w : 0.f);
+  const float* po = a.part_o + rh * a.nsplit * D + 2 * lane;
+  float2 acc = make_float2(0.f, 0.f);
+  uint64_t todo = __ballot(seen);
+  const bool any = todo != 0;
+  while (todo) {
+    float2 x[8];
+    float u[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int s = todo ? __builtin_ctzll(todo) : 0;
+      u[i] = todo ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), s)) : 0.f;
+      x[i] = make_float2(0.f, 0.f);
+      if (todo) x[i] = *(const float2*)(po + s * D);
+      todo &= todo - 1;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      acc.x = fmaf(u[i], x[i].x, acc.x);
+      acc.y = fmaf(u[i], x[i].y, acc.y);
+    }
+  }
+  const float inv = any ? 1.f / L : 0.f;
+  const int64_t row = rh / a.H;
+  const int h = (int)(rh % a.H);
+  const int64_t at = row * a.o_st + (int64_t)h * a.o_sh + 2 * lane;
+  if (a.out_bf16) {
+    bf16x2 r;
+    r[0] = (bf16)(acc.x * inv);
+    r[1] = (bf16)(acc.y * inv);
+    *(bf16x2*)((bf16*)a.out + at) = r;
+  } else {
+    *(float2*)((float*)a.out + at) = make_float2(acc.x * inv, acc.y * inv);
+  }
   if (a.lse && lane == 0)
-    a.lse[row * a.lse_st + (int64_t)h * a.lse_sh] = l > 0.f ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
+    a.lse[row * a.lse_st + (int64_t)h * a.lse_sh] = any ? (M + log2f(L)) * 0.6931471805599453f : -INFINITY;
+}
+
+// Rows of a work-group, row groups and splits of a call: 32 rows per wavefront pair up to 64, then
+// 128 rows; splits until the grid is about two rounds of two work-groups per CU.
+struct TreePlan { int rt, groups, nsplit; };
+inline TreePlan tree_plan(int B, int H, int Hkv, int max_n, int K, int S, int bs, int lw) {
+  TreePlan p;
+  const int64_t rows = (int64_t)max_n * (H / Hkv);
+  p.rt = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
+  p.groups = (int)((rows + 32 * p.rt - 1) / (32 * p.rt));
+  const int64_t nodes = std::min<int64_t>(max_n, (32 * p.rt - 1) / (H / Hkv) + 2);
+  const int64_t blocks = std::min<int64_t>((S + bs - 1) / bs, nodes * K);
+  const int64_t items = (std::min<int64_t>(S, (int64_t)lw + max_n) + 95) / 64 + (blocks * (bs / 32) + 1) / 2;
+  const int64_t streams = std::max<int64_t>(1, (int64_t)B * Hkv * p.groups);
+  p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({64, items, (kTrTarget + streams - 1) / streams}));
+  return p;
+}
+inline int64_t tree_workspace(const TreePlan& p, int64_t T, int H) {
+  return p.nsplit > 1 ? T * H * p.nsplit * (128 * 4 + 8) : 0;
 }
 
 }  // namespace dash
@@ -178,7 +607,8 @@ extern "C" int dash_attn_tree_workspace_size(int B, int H, int Hkv, int64_t T, i
   using namespace dash;
   if (!bytes || B < 0 || H <= 0 || Hkv <= 0 || T < 0 || max_query_len < 0 || K < 0 || S < 0)
     return kErrInvalid;
-  *bytes = 0;
+  if (H % Hkv != 0 || block_size < 32 || local_window < 1) return kErrUnsupported;
+  *bytes = tree_workspace(tree_plan(B, H, Hkv, max_query_len, K, S, block_size, local_window), T, H);
   return kOk;
 }
 
@@ -201,7 +631,7 @@ extern "C" int dash_attn_tree(
   if (max_query_len == 0 || S == 0) return kErrInvalid;
   if (D != 128 || H % Hkv != 0 || K > kPfMaxSlots || max_query_len > kTrMaxNodes ||
       words != (max_query_len + 63) / 64 || block_size <= 0 ||
-      (block_size != 32 && block_size % 64 != 0) || !(scale > 0.f) || B > 65535 || T > 65535)
+      (block_size != 32 && block_size % 64 != 0) || !(scale > 0.f))
     return kErrUnsupported;
   if ((S + block_size - 1) / block_size > kPfMaxBlocks) return kErrUnsupported;
   if (block_table && num_pages <= 0) return kErrInvalid;
@@ -226,7 +656,25 @@ extern "C" int dash_attn_tree(
   a.B = B; a.H = H; a.Hkv = Hkv; a.S = S; a.bs = block_size; a.lw = local_window;
   a.max_n = max_query_len; a.T = T;
   a.scale_log2e = scale * 1.4426950408889634f;
-  hipLaunchKernelGGL(tree_rows_kernel, dim3(H, (unsigned)T), dim3(kWave), 0, (hipStream_t)stream, a);
+  const TreePlan p = tree_plan(B, H, Hkv, max_query_len, K, S, block_size, local_window);
+  a.groups = p.groups; a.nsplit = p.nsplit;
+  const int64_t wgs = (int64_t)B * Hkv * p.groups * p.nsplit;
+  if (wgs > INT32_MAX || T * H > INT32_MAX) return kErrUnsupported;
+  if (p.nsplit > 1) {
+    if (!workspace || workspace_bytes < tree_workspace(p, T, H) || (uintptr_t)workspace % 16 != 0)
+      return kErrWorkspace;
+    a.part_o = (float*)workspace;
+    a.part_ml = (float2*)(a.part_o + T * H * p.nsplit * 128);
+  }
+  hipStream_t st = (hipStream_t)stream;
+  if (p.rt == 1)
+    hipLaunchKernelGGL((tree_attn_kernel<1, 2>), dim3((unsigned)wgs), dim3(128), 0, st, a);
+  else if (p.rt == 2)
+    hipLaunchKernelGGL((tree_attn_kernel<2, 2>), dim3((unsigned)wgs), dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL((tree_attn_kernel<4, 1>), dim3((unsigned)wgs), dim3(256), 0, st, a);
+  if (p.nsplit > 1)
+    hipLaunchKernelGGL(tree_merge_kernel, dim3((unsigned)((T * H + 3) / 4)), dim3(256), 0, st, a);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? kOk : (int)e;
 }
