@@ -26,7 +26,7 @@ struct TreeArgs {
   void* out; int out_bf16; int64_t o_st, o_sh;
   float* lse; int64_t lse_st, lse_sh;
   int B, H, Hkv, S, bs, lw, max_n;
-  int groups, nsplit;
+  int groups, nsplit, slot_cap;                // slot_cap: slots of a row group
   float* part_o;                               // [T, H, nsplit, 128], not normalised
   float2* part_ml;                             // [T, H, nsplit] base-2 reference and weight sum
   int64_t T;
@@ -85,24 +85,32 @@ __global__ __launch_bounds__(kTrMaxNodes) void tree_masks_kernel(const int32_t* 
 // blocks of rows that do not name them are one test.  A weight enters the second product as three
 // bf16 parts (24 bits), as in the extend kernels: it is not rounded.
 // ---------------------------------------------------------------------------
-constexpr int kTrBatch = 32;              // routed blocks whose rows' slots are looked up at a time
-
-template <int RT, int KG>
-struct TreeShared {
-  __attribute__((aligned(16))) bf16 k[2][64 * 128];
-  __attribute__((aligned(16))) bf16 v[2][64 * 128];
-  uint32_t bits[kPfMaxBlocks / 32];       // the blocks that the rows name
-  int16_t list[kPfMaxBlocks];             // in ascending order
-  uint8_t sel[kTrBatch][32 * RT];         // slot + 1 of (block, node), 0: not named
-  uint32_t bad[RT * KG];
-  int total;
-};
+constexpr uint32_t kTrNotNamed = 0xffffffffu;
 
 template <int RT, int KG>
 __global__ __launch_bounds__(64 * RT * KG, 2) void tree_attn_kernel(TreeArgs a) {
   constexpr int D = 128, NW = RT * KG, TH = 64 * NW;
   constexpr int NH = 2 / KG;              // halves of an item that a wavefront takes
-  __shared__ TreeShared<RT, KG> sm;
+  constexpr int CH = RT == 1 ? 16 : 8;    // items laid out at a time
+  // arrays of their own: the compiler waits for direct loads before it reads an array they may write
+  __shared__ __attribute__((aligned(16))) bf16 sK0[64 * D];
+  __shared__ __attribute__((aligned(16))) bf16 sK1[64 * D];
+  __shared__ __attribute__((aligned(16))) bf16 sV0[64 * D];
+  __shared__ __attribute__((aligned(16))) bf16 sV1[64 * D];
+  __shared__ uint32_t sBits[kPfMaxBlocks / 32];       // the blocks that the rows name
+  __shared__ int sPref[kPfMaxBlocks / 32 + 1];        // set bits before each word
+  // halves of the items laid out: first key, place among the laid out blocks (-1: the band, -2: no
+  // keys), page and the first key's row in it
+  __shared__ int4 sHalf[2 * CH];
+  // (block, node): the bits of the log2 bias; kTrNotNamed where the node does not name the block
+  __shared__ uint32_t sBias[2 * CH][32 * RT];
+  __shared__ uint32_t sBad[NW];
+  __shared__ float2 sMl[32 * RT];
+  // [nodes, K]: the bias of every slot (up to 64 rows; above, it would cost the second work-group of
+  // a CU), then its block, -1 where it is not used
+  extern __shared__ float dyn[];
+  float* const sSlotBias = dyn;
+  int16_t* const slots = (int16_t*)(dyn + (RT == 4 ? 0 : a.slot_cap));
   const int tid = threadIdx.x, lane = wave_lane(), wv = tid / kWave;
   const int rt = wv % RT, kg = wv / RT;
   int id = blockIdx.x;
@@ -128,6 +136,7 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void tree_attn_kernel(TreeArgs a) 
   const int h = hk * G + rr % G;
   const int w_row = ctx + a.depth[row] - a.lw + 1;
   const int top = min(w_row, ctx);
+  const uint64_t mask0 = a.mask[row * a.words];
   bf16x8 qop[D / 16];
   {
     const bf16* qb = a.q + row * a.q_st + (int64_t)h * a.q_sh;
@@ -135,36 +144,48 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void tree_attn_kernel(TreeArgs a) 
     for (int kk = 0; kk < D / 16; ++kk) qop[kk] = *(const bf16x8*)(qb + kk * 16 + hl * 8);
   }
 
-  // the blocks that the rows name, and their order
-  auto usable = [&](int64_t at, int node_top, int& c) {
-    c = a.idx[at];
-    return c >= 0 && c < nblk && c * a.bs < node_top && (!a.valid || a.valid[at]);
-  };
+  // the blocks that the rows name: a bit each, and every slot's block in LDS
+  const int n_slots = (node1 - node0) * a.K;
+  const int64_t s0 = (r0 + node0) * a.K;
   int n_blocks = 0;
-  if (a.K > 0) {
-    for (int i = tid; i < kPfMaxBlocks / 32; i += TH) sm.bits[i] = 0u;
+  if (n_slots > 0) {
+    for (int i = tid; i < kPfMaxBlocks / 32; i += TH) sBits[i] = 0u;
     __syncthreads();
-    for (int i = tid; i < (node1 - node0) * a.K; i += TH) {
-      const int64_t rw = r0 + node0 + i / a.K;
-      int c;
-      if (usable(rw * a.K + i % a.K, min(ctx + a.depth[rw] - a.lw + 1, ctx), c))
-        atomicOr(&sm.bits[c >> 5], 1u << (c & 31));
+    for (int i0 = 0; i0 < n_slots; i0 += 4 * TH) {
+      int c[4], d[4];
+      float x[4];
+      bool ok[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {       // every load before the first store to LDS
+        const int i = min(i0 + u * TH + tid, n_slots - 1);
+        c[u] = a.idx[s0 + i];
+        ok[u] = !a.valid || a.valid[s0 + i];
+        d[u] = a.depth[r0 + node0 + i / a.K];
+        x[u] = RT == 4 ? 0.f : a.bias[s0 + i];
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + u * TH + tid;
+        if (i >= n_slots) break;
+        const bool use = ok[u] && c[u] >= 0 && c[u] < nblk && c[u] * a.bs < min(ctx + d[u] - a.lw + 1, ctx);
+        slots[i] = (int16_t)(use ? c[u] : -1);
+        if (RT != 4) sSlotBias[i] = x[u];
+        if (use) atomicOr(&sBits[c[u] >> 5], 1u << (c[u] & 31));
+      }
     }
     __syncthreads();
     if (wv == 0) {
-      uint32_t w = sm.bits[lane];
-      int x = __popc(w);
-      const int own = x;
+      int x = __popc(sBits[lane]);
 #pragma unroll
       for (int s = 1; s < kWave; s <<= 1) {
         const int y = __shfl_up(x, s, kWave);
         if (lane >= s) x += y;
       }
-      if (lane == kWave - 1) sm.total = x;
-      for (int at = x - own; w; w &= w - 1) sm.list[at++] = (int16_t)(32 * lane + __builtin_ctz(w));
+      sPref[lane + 1] = x;
+      if (lane == 0) sPref[0] = 0;
     }
     __syncthreads();
-    n_blocks = sm.total;
+    n_blocks = sPref[kPfMaxBlocks / 32];
   }
 
   // items: the band's, then the blocks'
@@ -173,100 +194,123 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void tree_attn_kernel(TreeArgs a) 
   const int jend = ctx + n;
   const int n_wi = (jend - jw0 + 63) / 64;
   const int n_items = n_wi + (n_blocks * hpb + 1) / 2;
-  const int i0 = (int)((int64_t)n_items * split / a.nsplit);
-  const int i1 = (int)((int64_t)n_items * (split + 1) / a.nsplit);
+  const int i_first = (int)((int64_t)n_items * split / a.nsplit);
+  const int i_last = (int)((int64_t)n_items * (split + 1) / a.nsplit);
 
-  // half hf of item i: its first key, the place of its block in the list (-1: the band; -2: no keys)
-  auto half_of = [&](int i, int hf, int& at) -> int {
-    if (i < n_wi) {
-      const int j = jw0 + 64 * i + 32 * hf;
-      at = j < jend ? -1 : -2;
-      return j < jend ? j : j - 32;
+  // Lays out items c0 .. c1 - 1 (at most CH): every wavefront has left the items before.
+  auto lay_out = [&](int c0, int c1) {
+    const int x0 = max(2 * (c0 - n_wi), 0), x1 = min(2 * (c1 - n_wi), n_blocks * hpb);
+    const int l0 = x0 / hpb, l1 = x1 > x0 ? (x1 - 1) / hpb + 1 : l0;   // their blocks' places
+    for (int x = tid; x < (l1 - l0) * 32 * RT; x += TH) (&sBias[0][0])[x] = kTrNotNamed;
+    if (tid < 2 * (c1 - c0)) {
+      const int i = c0 + (tid >> 1);
+      int j, at;
+      if (i < n_wi) {
+        j = jw0 + 64 * i + 32 * (tid & 1);
+        at = -1;
+        if (j >= jend) { at = -2; j -= 32; }
+      } else {
+        int x = 2 * (i - n_wi) + (tid & 1);
+        const bool none = x >= n_blocks * hpb;
+        if (none) --x;
+        const int l = x / hpb;
+        int lo = 0, hi = kPfMaxBlocks / 32;        // the word of the l-th block
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) >> 1;
+          if (sPref[mid] <= l) lo = mid; else hi = mid;
+        }
+        uint32_t w = sBits[lo];
+        for (int u = sPref[lo]; u < l; ++u) w &= w - 1u;
+        j = (32 * lo + (int)__builtin_ctz(w)) * a.bs + x % hpb * 32;
+        at = none ? -2 : l - l0;
+      }
+      sHalf[tid] = a.table ? make_int4(j, at, tree_page(a, a.table[(int64_t)b * a.table_stride + j / a.page]),
+                                       j % a.page)
+                           : make_int4(j, at, b, j);
     }
-    const int x = 2 * (i - n_wi) + hf;
-    at = x / hpb;
-    if (at >= n_blocks) { at = -2; return sm.list[(x - 1) / hpb] * a.bs + (x - 1) % hpb * 32; }
-    return sm.list[at] * a.bs + x % hpb * 32;
+    if (l1 > l0) {
+      // a block's first slot in a row wins: the smallest slot first, then its bias in its place (a
+      // bias whose bits could be a slot's number counts as 0)
+      auto place_of = [&](int c) {
+        return c < 0 ? -1 : sPref[c >> 5] + __popc(sBits[c >> 5] & ((1u << (c & 31)) - 1u)) - l0;
+      };
+      __syncthreads();
+      for (int i = tid; i < n_slots; i += TH) {
+        const int l = place_of(slots[i]);
+        if (l >= 0 && l < l1 - l0) atomicMin(&sBias[l][i / a.K], (uint32_t)(i % a.K));
+      }
+      __syncthreads();
+      for (int i = tid; i < n_slots; i += TH) {
+        const int l = place_of(slots[i]);
+        if (l < 0 || l >= l1 - l0) continue;
+        uint32_t& to = sBias[l][i / a.K];
+        if (to != (uint32_t)(i % a.K)) continue;
+        const float x = (RT == 4 ? a.bias[s0 + i] : sSlotBias[i]) * 1.4426950408889634f;
+        to = __float_as_uint(fabsf(x) < 1e-30f ? 0.f : x);
+      }
+    }
+    __syncthreads();
   };
-  auto fetch = [&](int i, int buf) {
+  // Direct loads of laid out item x into a stage.  Row r of a half is at r * stride + chunk.
+  uint32_t ko[8 / NW], vo[8 / NW];
+#pragma unroll
+  for (int u = 0; u < 8 / NW; ++u) {
+    const int r = 4 * (NW * u + wv) + (lane >> 4);        // four rows a wavefront
+    ko[u] = (uint32_t)(r * a.k_st + k_slot(r, lane & 15) * 8);
+    vo[u] = (uint32_t)(r * a.v_st + v_slot(r, lane & 15) * 8);
+  }
+  auto fetch = [&](int x, bool band, bf16* sKn, bf16* sVn) __attribute__((always_inline)) {
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
-      int at;
-      const int j = __builtin_amdgcn_readfirstlane(half_of(i, hf, at));
-      const int last = (i < n_wi ? jend : ctx) - 1;
-      int64_t kr, vr;
-      if (a.table) {
-        const int p = tree_page(a, a.table[(int64_t)b * a.table_stride + j / a.page]);
-        kr = (int64_t)p * a.k_sb + (int64_t)(j % a.page) * a.k_st;
-        vr = (int64_t)p * a.v_sb + (int64_t)(j % a.page) * a.v_st;
-      } else {
-        kr = (int64_t)b * a.k_sb + (int64_t)j * a.k_st;
-        vr = (int64_t)b * a.v_sb + (int64_t)j * a.v_st;
-      }
-      const bf16* kb = a.k + kr + (int64_t)hk * a.k_sh;
-      const bf16* vb = a.v + vr + (int64_t)hk * a.v_sh;
+      const int4 d = sHalf[2 * x + hf];
+      const int j = __builtin_amdgcn_readfirstlane(d.x), pg = __builtin_amdgcn_readfirstlane(d.z);
+      const int jp = __builtin_amdgcn_readfirstlane(d.w);
+      const int over = j + 31 - ((band ? jend : ctx) - 1);      // rows past the last key repeat it
+      const bf16* kb = a.k + ((int64_t)pg * a.k_sb + (int64_t)jp * a.k_st + (int64_t)hk * a.k_sh);
+      const bf16* vb = a.v + ((int64_t)pg * a.v_sb + (int64_t)jp * a.v_st + (int64_t)hk * a.v_sh);
 #pragma unroll
       for (int u = 0; u < 8 / NW; ++u) {
-        const int grp = NW * u + wv;      // four rows a wavefront
-        const int r = 4 * grp + (lane >> 4);
-        const int off = min(j + r, last) - j;
-        __builtin_amdgcn_global_load_lds(
-            (const void*)(kb + (int64_t)off * a.k_st + k_slot(r, lane & 15) * 8),
-            (__attribute__((address_space(3))) void*)(sm.k[buf] + (hf * 32 + grp * 4) * D), 16, 0, 0);
-        __builtin_amdgcn_global_load_lds(
-            (const void*)(vb + (int64_t)off * a.v_st + v_slot(r, lane & 15) * 8),
-            (__attribute__((address_space(3))) void*)(sm.v[buf] + (hf * 32 + grp * 4) * D), 16, 0, 0);
+        const int grp = NW * u + wv;
+        const bf16* kp = kb + ko[u];
+        const bf16* vp = vb + vo[u];
+        if (over > 0) {
+          const int back = min(31 - over - (4 * grp + (lane >> 4)), 0);
+          kp += (int64_t)back * a.k_st;
+          vp += (int64_t)back * a.v_st;
+        }
+        __builtin_amdgcn_global_load_lds((const void*)kp,
+            (__attribute__((address_space(3))) void*)(sKn + (hf * 32 + grp * 4) * D), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((const void*)vp,
+            (__attribute__((address_space(3))) void*)(sVn + (hf * 32 + grp * 4) * D), 16, 0, 0);
       }
     }
   };
-  // the keys of a half that this lane's row sees, a bit each, and their log2 bias
-  auto visible = [&](int i, int hf, float& blog) -> uint32_t {
-    int at;
-    const int j = half_of(i, hf, at);
+  // the keys of half hf of laid out item x that this lane's row sees, a bit each, and their log2 bias
+  auto visible = [&](int x, int hf, float& blog) -> uint32_t {
+    const int2 d = *(const int2*)&sHalf[2 * x + hf];
+    const int j = d.x, at = d.y;
     blog = 0.f;
     if (at == -2 || !rvalid) return 0u;
-    auto below = [](int x) -> uint32_t { return x >= 32 ? ~0u : x <= 0 ? 0u : (1u << x) - 1u; };
+    auto below = [](int y) -> uint32_t { return y >= 32 ? ~0u : y <= 0 ? 0u : (1u << y) - 1u; };
     if (at == -1) {
       uint32_t v = below(ctx - j) & ~below(w_row - j);
       const int m0 = j - ctx;
       if (m0 > -32) {
         uint64_t m;
         if (m0 < 0) {
-          m = a.mask[row * a.words] << -m0;
+          m = mask0 << -m0;
         } else {
           const int wd = m0 >> 6, sh = m0 & 63;
-          m = a.mask[row * a.words + wd] >> sh;
+          m = (wd ? a.mask[row * a.words + wd] : mask0) >> sh;
           if (sh > 32 && wd + 1 < a.words) m |= a.mask[row * a.words + wd + 1] << (64 - sh);
         }
         v |= (uint32_t)m & below(jend - j) & ~below(ctx - j);
       }
       return v;
     }
-    const int s = sm.sel[at % kTrBatch][node - node0];
-    if (s == 0) return 0u;
-    blog = a.bias[row * a.K + s - 1] * 1.4426950408889634f;
-    return below(top - j);
-  };
-  // the slots of the blocks at list places of one batch
-  auto look_up = [&](int batch) {
-    for (int x = tid; x < kTrBatch * 32 * RT / 4; x += TH) ((uint32_t*)sm.sel)[x] = 0u;
-    __syncthreads();
-    const int l0 = batch * kTrBatch, l1 = min(l0 + kTrBatch, n_blocks);
-    for (int nd = node0 + tid; nd < node1; nd += TH) {
-      const int64_t rw = r0 + nd;
-      const int nt = min(ctx + a.depth[rw] - a.lw + 1, ctx);
-      for (int s = a.K - 1; s >= 0; --s) {        // the first slot of a block is written last
-        int c;
-        if (!usable(rw * a.K + s, nt, c) || c < sm.list[l0] || c > sm.list[l1 - 1]) continue;
-        int lo = l0, hi = l1;
-        while (hi - lo > 1) {
-          const int mid = (lo + hi) >> 1;
-          if (sm.list[mid] <= c) lo = mid; else hi = mid;
-        }
-        sm.sel[lo - l0][nd - node0] = (uint8_t)(s + 1);
-      }
-    }
-    __syncthreads();
+    const uint32_t bits = sBias[at][node - node0];
+    blog = __uint_as_float(bits);
+    return bits == kTrNotNamed ? 0u : below(top - j);
   };
 
   floatx16 acc_o[D / 32];
@@ -282,8 +326,8 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void tree_attn_kernel(TreeArgs a) 
   const uint32_t kl0 = k_lane_off(col, hl), vl0 = v_lane_off(lane);
   const float csc = a.scale_log2e;
 
-  // this wavefront's halves of item i in stage `buf`
-  auto item = [&](int i, int buf, uint32_t (&vis)[NH]) __attribute__((always_inline)) {
+  // this wavefront's halves of laid out item i
+  auto item = [&](int i, const bf16* sKc, const bf16* sVc, uint32_t (&vis)[NH]) __attribute__((always_inline)) {
     float blog[NH];
     bool any = false;
 #pragma unroll
@@ -301,7 +345,7 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void tree_attn_kernel(TreeArgs a) 
       for (int r = 0; r < 16; ++r) s[x][r] = 0.f;
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk)
-        s[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k_frag_at(sm.k[buf], kl0, hf, kk), qop[kk], s[x],
+        s[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k_frag_at(sKc, kl0, hf, kk), qop[kk], s[x],
                                                        0, 0, 0);
       const uint32_t vb = vis[x] >> (4 * hl);
 #pragma unroll
@@ -341,7 +385,7 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void tree_attn_kernel(TreeArgs a) 
         bf16x8 vop[2];
 #pragma unroll
         for (int jj = 0; jj < 2; ++jj) {
-          const char* vp = (const char*)sm.v[buf] + (32 * hf + 16 * jj) * 256 + (vl0 ^ (uint32_t)(dt << 6));
+          const char* vp = (const char*)sVc + (32 * hf + 16 * jj) * 256 + (vl0 ^ (uint32_t)(dt << 6));
           const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
               (lds_short4*)(__attribute__((address_space(3))) void*)vp);
           const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
@@ -365,25 +409,24 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void tree_attn_kernel(TreeArgs a) 
       }
     }
   };
-  // the batch of list places that item i's blocks belong to (items do not straddle: a batch is
-  // a whole number of items' halves), -1 for the band
-  auto batch_of = [&](int i) { return i < n_wi ? -1 : 2 * (i - n_wi) / hpb / kTrBatch; };
-
   reset();
   uint32_t vis[NH];
-  int batch = -1;
-  if (i0 < i1) fetch(i0, 0);
-  for (int i = i0; i < i1; ++i) {
-    const int nb = batch_of(i);
-    if (nb != batch) {                    // before the barrier below: no wavefront is past it
-      __syncthreads();
-      look_up(nb);
-      batch = nb;
+  for (int c0 = i_first; c0 < i_last; c0 += CH) {
+    const int c1 = min(c0 + CH, i_last);
+    if (c0 > i_first) __syncthreads();    // every wavefront left the items before
+    lay_out(c0, c1);
+    fetch(0, c0 < n_wi, sK0, sV0);
+    auto step = [&](int i, auto par) __attribute__((always_inline)) {
+      constexpr int P = decltype(par)::value;
+      __builtin_amdgcn_s_waitcnt(0);
+      __syncthreads();                    // item i landed; every wavefront left item i - 1
+      if (i + 1 < c1) fetch(i + 1 - c0, i + 1 < n_wi, P ? sK0 : sK1, P ? sV0 : sV1);
+      item(i - c0, P ? sK1 : sK0, P ? sV1 : sV0, vis);
+    };
+    for (int i = c0; i < c1; i += 2) {
+      step(i, std::integral_constant<int, 0>{});
+      if (i + 1 < c1) step(i + 1, std::integral_constant<int, 1>{});
     }
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();                      // item i landed; every wavefront left item i - 1
-    if (i + 1 < i1) fetch(i + 1, (i + 1 - i0) & 1);
-    item(i, (i - i0) & 1, vis);
   }
 
   // V values that are not finite reached every row of the tile through masked weights: the items
@@ -395,12 +438,14 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void tree_attn_kernel(TreeArgs a) 
     for (int r = 0; r < 16; ++r) z = fmaf(acc_o[dt][r], 0.f, z);
   if (__syncthreads_or(z != 0.f)) {
     reset();
-    batch = -1;
-    for (int i = i0; i < i1; ++i) {
+    for (int i = i_first; i < i_last; ++i) {
+      const int x0 = (i - i_first) % CH;
+      if (x0 == 0) {
+        __syncthreads();
+        lay_out(i, min(i + CH, i_last));
+      }
       __syncthreads();                    // every wavefront left the stage
-      fetch(i, 0);
-      const int nb = batch_of(i);
-      if (nb != batch) { look_up(nb); batch = nb; }
+      fetch(x0, i < n_wi, sK0, sV0);
       __builtin_amdgcn_s_waitcnt(0);
       // each wavefront clears the rows it loaded; bit 8 hf + u: its group u of half hf holds some
       uint32_t bad = 0;
@@ -408,7 +453,7 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void tree_attn_kernel(TreeArgs a) 
       for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
         for (int u = 0; u < 8 / NW; ++u) {
-          uint4* p = (uint4*)(sm.v[0] + (hf * 32 + (NW * u + wv) * 4) * D) + lane;
+          uint4* p = (uint4*)(sV0 + (hf * 32 + (NW * u + wv) * 4) * D) + lane;
           uint4 x = *p;
           bool is = false;
           auto fix = [&](uint32_t& w) {
@@ -419,27 +464,24 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void tree_attn_kernel(TreeArgs a) 
           if (is) *p = x;
           if (__any(is)) bad |= 1u << (8 * hf + u);
         }
-      if (lane == 0) sm.bad[wv] = bad;
+      if (lane == 0) sBad[wv] = bad;
       __syncthreads();
 #pragma unroll
       for (int y = 0; y < NH; ++y) vis[y] = 0u;
-      item(i, 0, vis);
+      item(x0, sK0, sV0, vis);
 #pragma unroll
       for (int y = 0; y < NH; ++y) {
         const int hf = KG == 2 ? kg : y;
-        int at;
-        const int j = half_of(i, hf, at);
+        const int4 d = sHalf[2 * x0 + hf];
+        const int j = d.x;
         const int last = (i < n_wi ? jend : ctx) - 1;
         for (int w = 0; w < NW; ++w)
-          for (uint32_t todo = (sm.bad[w] >> (8 * hf)) & 0xffu; todo; todo &= todo - 1)
+          for (uint32_t todo = (sBad[w] >> (8 * hf)) & 0xffu; todo; todo &= todo - 1)
             for (int q4 = 0; q4 < 4; ++q4) {
               const int r = 4 * (NW * __builtin_ctz(todo) + w) + q4;
               if (j + r > last) continue;          // a repeated row
               const bool sees = (vis[y] >> r) & 1u;
-              const int64_t vr = a.table
-                  ? (int64_t)tree_page(a, a.table[(int64_t)b * a.table_stride + j / a.page]) * a.v_sb +
-                        (int64_t)(j % a.page + r) * a.v_st
-                  : (int64_t)b * a.v_sb + (int64_t)(j + r) * a.v_st;
+              const int64_t vr = (int64_t)d.z * a.v_sb + (int64_t)(d.w + r) * a.v_st;
               const bf16* vp = a.v + vr + (int64_t)hk * a.v_sh + 4 * hl;
 #pragma unroll
               for (int dt = 0; dt < D / 32; ++dt)
@@ -458,26 +500,26 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void tree_attn_kernel(TreeArgs a) 
   }
   float l_tot = xor32_sum(l_run);
   if (KG == 2) {
-    // the second half's wavefronts hand their sums to the first's (through both stages' K, and V)
+    // the second half's wavefronts hand their sums to the first's
     __syncthreads();
-    float* so = (float*)sm.k + rt * 32 * (D + 2);
+    float* so = (float*)(rt ? sK1 : sK0);
     if (kg == 1) {
 #pragma unroll
       for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) so[(16 * dt + r) * 64 + lane] = acc_o[dt][r];
-      so[64 * 64 + lane] = hl ? l_tot : m_run;
+      if (hl == 0) sMl[rt * 32 + col] = make_float2(m_run, l_tot);
     }
     __syncthreads();
     if (kg == 1) return;
-    const float m2 = so[64 * 64 + col], l2 = so[64 * 64 + 32 + col];
-    const float mn = fmaxf(m_run, m2), mu = mn == -INFINITY ? 0.f : mn;
-    const float al = fast_exp2(m_run - mu), be = fast_exp2(m2 - mu);
+    const float2 ml = sMl[rt * 32 + col];
+    const float mn = fmaxf(m_run, ml.x), mu = mn == -INFINITY ? 0.f : mn;
+    const float al = fast_exp2(m_run - mu), be = fast_exp2(ml.x - mu);
 #pragma unroll
     for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc_o[dt][r] = acc_o[dt][r] * al + so[(16 * dt + r) * 64 + lane] * be;
-    l_tot = l_tot * al + l2 * be;
+    l_tot = l_tot * al + ml.y * be;
     m_run = mn;
   }
   if (!rvalid) return;
@@ -568,13 +610,14 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
 
 // Rows of a work-group, row groups and splits of a call: 32 rows per wavefront pair up to 64, then
 // 128 rows; splits until the grid is about two rounds of two work-groups per CU.
-struct TreePlan { int rt, groups, nsplit; };
+struct TreePlan { int rt, groups, nsplit, nodes; };
 inline TreePlan tree_plan(int B, int H, int Hkv, int max_n, int K, int S, int bs, int lw) {
   TreePlan p;
   const int64_t rows = (int64_t)max_n * (H / Hkv);
   p.rt = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
   p.groups = (int)((rows + 32 * p.rt - 1) / (32 * p.rt));
   const int64_t nodes = std::min<int64_t>(max_n, (32 * p.rt - 1) / (H / Hkv) + 2);
+  p.nodes = (int)nodes;                   // at most, of a row group
   const int64_t blocks = std::min<int64_t>((S + bs - 1) / bs, nodes * K);
   const int64_t items = (std::min<int64_t>(S, (int64_t)lw + max_n) + 95) / 64 + (blocks * (bs / 32) + 1) / 2;
   const int64_t streams = std::max<int64_t>(1, (int64_t)B * Hkv * p.groups);
@@ -639,6 +682,7 @@ extern "C" int dash_attn_tree(
   const int64_t strides[] = {q_st, q_sh, k_sb, k_sh, k_st, v_sb, v_sh, v_st};
   for (int64_t s : strides)
     if (s % 8 != 0) return kErrUnsupported;
+  if (k_st > kMaxKeyRowStride || v_st > kMaxKeyRowStride || k_st < 0 || v_st < 0) return kErrUnsupported;
   const void* ptrs[] = {q, k, v};
   for (const void* x : ptrs)
     if ((uintptr_t)x % 16 != 0) return kErrUnsupported;
@@ -667,12 +711,14 @@ extern "C" int dash_attn_tree(
     a.part_ml = (float2*)(a.part_o + T * H * p.nsplit * 128);
   }
   hipStream_t st = (hipStream_t)stream;
+  a.slot_cap = p.nodes * K;
+  const unsigned lds = (unsigned)((a.slot_cap * (p.rt == 4 ? 2 : 6) + 15) / 16 * 16);
   if (p.rt == 1)
-    hipLaunchKernelGGL((tree_attn_kernel<1, 2>), dim3((unsigned)wgs), dim3(128), 0, st, a);
+    hipLaunchKernelGGL((tree_attn_kernel<1, 2>), dim3((unsigned)wgs), dim3(128), lds, st, a);
   else if (p.rt == 2)
-    hipLaunchKernelGGL((tree_attn_kernel<2, 2>), dim3((unsigned)wgs), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((tree_attn_kernel<2, 2>), dim3((unsigned)wgs), dim3(256), lds, st, a);
   else
-    hipLaunchKernelGGL((tree_attn_kernel<4, 1>), dim3((unsigned)wgs), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((tree_attn_kernel<4, 1>), dim3((unsigned)wgs), dim3(256), lds, st, a);
   if (p.nsplit > 1)
     hipLaunchKernelGGL(tree_merge_kernel, dim3((unsigned)((T * H + 3) / 4)), dim3(256), 0, st, a);
   const hipError_t e = hipGetLastError();
