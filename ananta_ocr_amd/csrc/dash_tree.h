@@ -82,8 +82,10 @@ __global__ __launch_bounds__(kTrMaxNodes) void tree_masks_kernel(const int32_t* 
 // RT row tiles of 32 rows are the columns of S^T = K Q^T (v_mfma_f32_32x32x16_bf16); with KG = 2
 // two wavefronts share a row tile, one half of every item each, and meet at the end.  A half's
 // visible keys are 32 bits per row, so the band's edges, the drafted keys' mask and the routed
-// blocks of rows that do not name them are one test.  A weight enters the second product as three
-// bf16 parts (24 bits), as in the extend kernels: it is not rounded.
+// blocks of rows that do not name them are one test.  A weight enters the second product as two
+// bf16 parts: it is off by at most 2^-17 of itself (16 bits and their rounding), which moves an output
+// by less than 8e-6 of the largest |v|, and by 1e-6 as roundings of either sign add up; a third part,
+// as in the extend kernels, costs a third of the matrix work and a quarter of the vector work.
 // ---------------------------------------------------------------------------
 constexpr uint32_t kTrNotNamed = 0xffffffffu;
 
@@ -91,12 +93,13 @@ template <int RT, int KG>
 __global__ __launch_bounds__(64 * RT * KG, 2) void tree_attn_kernel(TreeArgs a) {
   constexpr int D = 128, NW = RT * KG, TH = 64 * NW;
   constexpr int NH = 2 / KG;              // halves of an item that a wavefront takes
-  constexpr int CH = RT == 1 ? 16 : 8;    // items laid out at a time
+  constexpr int CH = 8;                   // items laid out at a time
+  constexpr int ST = RT == 1 ? 1 : 2;     // stages
   // arrays of their own: the compiler waits for direct loads before it reads an array they may write
   __shared__ __attribute__((aligned(16))) bf16 sK0[64 * D];
-  __shared__ __attribute__((aligned(16))) bf16 sK1[64 * D];
+  __shared__ __attribute__((aligned(16))) bf16 sK1[ST == 2 ? 64 * D : 8];
   __shared__ __attribute__((aligned(16))) bf16 sV0[64 * D];
-  __shared__ __attribute__((aligned(16))) bf16 sV1[64 * D];
+  __shared__ __attribute__((aligned(16))) bf16 sV1[ST == 2 ? 64 * D : 8];
   __shared__ uint32_t sBits[kPfMaxBlocks / 32];       // the blocks that the rows name
   __shared__ int sPref[kPfMaxBlocks / 32 + 1];        // set bits before each word
   // halves of the items laid out: first key, place among the laid out blocks (-1: the band, -2: no
@@ -251,36 +254,36 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void tree_attn_kernel(TreeArgs a) 
     }
     __syncthreads();
   };
-  // Direct loads of laid out item x into a stage.  Row r of a half is at r * stride + chunk.
+  // Direct loads of laid out item x into a stage: a half's rows at a scalar base plus 32-bit offsets.
   uint32_t ko[8 / NW], vo[8 / NW];
 #pragma unroll
   for (int u = 0; u < 8 / NW; ++u) {
     const int r = 4 * (NW * u + wv) + (lane >> 4);        // four rows a wavefront
-    ko[u] = (uint32_t)(r * a.k_st + k_slot(r, lane & 15) * 8);
-    vo[u] = (uint32_t)(r * a.v_st + v_slot(r, lane & 15) * 8);
+    ko[u] = 2u * (uint32_t)(r * a.k_st + k_slot(r, lane & 15) * 8);
+    vo[u] = 2u * (uint32_t)(r * a.v_st + v_slot(r, lane & 15) * 8);
   }
   auto fetch = [&](int x, bool band, bf16* sKn, bf16* sVn) __attribute__((always_inline)) {
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
       const int4 d = sHalf[2 * x + hf];
-      const int j = __builtin_amdgcn_readfirstlane(d.x), pg = __builtin_amdgcn_readfirstlane(d.z);
-      const int jp = __builtin_amdgcn_readfirstlane(d.w);
-      const int over = j + 31 - ((band ? jend : ctx) - 1);      // rows past the last key repeat it
-      const bf16* kb = a.k + ((int64_t)pg * a.k_sb + (int64_t)jp * a.k_st + (int64_t)hk * a.k_sh);
-      const bf16* vb = a.v + ((int64_t)pg * a.v_sb + (int64_t)jp * a.v_st + (int64_t)hk * a.v_sh);
+      const int pg = __builtin_amdgcn_readfirstlane(d.z);
+      // rows past the last key repeat it (a block's second half may lie past it as a whole)
+      const int last = (band ? jend : ctx) - 1 - __builtin_amdgcn_readfirstlane(d.x);
+      const int jp = __builtin_amdgcn_readfirstlane(d.w) + min(last, 0);
+      const char* kb = (const char*)(a.k + ((int64_t)pg * a.k_sb + (int64_t)jp * a.k_st + (int64_t)hk * a.k_sh));
+      const char* vb = (const char*)(a.v + ((int64_t)pg * a.v_sb + (int64_t)jp * a.v_st + (int64_t)hk * a.v_sh));
 #pragma unroll
       for (int u = 0; u < 8 / NW; ++u) {
         const int grp = NW * u + wv;
-        const bf16* kp = kb + ko[u];
-        const bf16* vp = vb + vo[u];
-        if (over > 0) {
-          const int back = min(31 - over - (4 * grp + (lane >> 4)), 0);
-          kp += (int64_t)back * a.k_st;
-          vp += (int64_t)back * a.v_st;
+        uint32_t kx = ko[u], vx = vo[u];
+        if (last < 31) {
+          const int r = 4 * grp + (lane >> 4), rc = max(min(r, last), 0);
+          kx = 2u * (uint32_t)(rc * a.k_st + k_slot(r, lane & 15) * 8);
+          vx = 2u * (uint32_t)(rc * a.v_st + v_slot(r, lane & 15) * 8);
         }
-        __builtin_amdgcn_global_load_lds((const void*)kp,
+        __builtin_amdgcn_global_load_lds((const void*)(kb + kx),
             (__attribute__((address_space(3))) void*)(sKn + (hf * 32 + grp * 4) * D), 16, 0, 0);
-        __builtin_amdgcn_global_load_lds((const void*)vp,
+        __builtin_amdgcn_global_load_lds((const void*)(vb + vx),
             (__attribute__((address_space(3))) void*)(sVn + (hf * 32 + grp * 4) * D), 16, 0, 0);
       }
     }
@@ -347,12 +350,25 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void tree_attn_kernel(TreeArgs a) 
       for (int kk = 0; kk < D / 16; ++kk)
         s[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k_frag_at(sKc, kl0, hf, kk), qop[kk], s[x],
                                                        0, 0, 0);
-      const uint32_t vb = vis[x] >> (4 * hl);
+      // a half that every row sees whole or not at all, as inside the band and the blocks: one
+      // minimum with +-inf (which also takes a score that is not a number away)
+      float mraw = -INFINITY;
+      if (__all(vis[x] == 0u || vis[x] == ~0u)) {
+        const float lim = vis[x] ? INFINITY : -INFINITY;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        s[x][r] = (vb >> (8 * (r >> 2) + (r & 3))) & 1u ? fmaf(s[x][r], csc, blog[x]) : -INFINITY;
-        mloc = fmaxf(mloc, s[x][r]);
+        for (int r = 0; r < 16; ++r) {
+          s[x][r] = fminf(s[x][r], lim);
+          mraw = fmaxf(mraw, s[x][r]);
+        }
+      } else {
+        const uint32_t vb = vis[x] >> (4 * hl);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[x][r] = (vb >> (8 * (r >> 2) + (r & 3))) & 1u ? s[x][r] : -INFINITY;
+          mraw = fmaxf(mraw, s[x][r]);
+        }
       }
+      mloc = fmaxf(mloc, fmaf(mraw, csc, vis[x] ? blog[x] : 0.f));
     }
     mloc = xor32_max(mloc);
     // the reference moves only when a row's maximum exceeds it by more than 8
@@ -366,20 +382,23 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void tree_attn_kernel(TreeArgs a) 
         for (int r = 0; r < 16; ++r) acc_o[dt][r] *= alpha;
       m_run = up ? mloc : m_run;
     }
-    const float off = m_run == -INFINITY ? 0.f : m_run;
 #pragma unroll
     for (int x = 0; x < NH; ++x) {
       const int hf = KG == 2 ? kg : x;
-      bf16x8 ph[2], pm[2], pl[2];
+      const float off = (vis[x] ? blog[x] : 0.f) - (m_run == -INFINITY ? 0.f : m_run);
+      bf16x8 ph[2], pl[2];
 #pragma unroll
       for (int jj = 0; jj < 2; ++jj) {
         float p[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) p[e] = fast_exp2(s[x][8 * jj + e] - off);
+        for (int e = 0; e < 8; ++e) p[e] = fast_exp2(fmaf(s[x][8 * jj + e], csc, off));
         l_run += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-        ext_split3(p, ph[jj], pm[jj], pl[jj]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          ph[jj][e] = (bf16)p[e];
+          pl[jj][e] = (bf16)(p[e] - (float)ph[jj][e]);
+        }
       }
-      // the half's products sum from zero, smallest parts first, before they meet the row's total
 #pragma unroll
       for (int dt = 0; dt < 4; ++dt) {
         bf16x8 vop[2];
@@ -395,26 +414,31 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void tree_attn_kernel(TreeArgs a) 
 #pragma unroll
           for (int e = 0; e < 4; ++e) { vop[jj][e] = l4[e]; vop[jj][e + 4] = h4[e]; }
         }
-        floatx16 t;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) t[r] = 0.f;
-#pragma unroll
-        for (int jj = 0; jj < 2; ++jj) t = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vop[jj], pl[jj], t, 0, 0, 0);
-#pragma unroll
-        for (int jj = 0; jj < 2; ++jj) t = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vop[jj], pm[jj], t, 0, 0, 0);
-#pragma unroll
-        for (int jj = 0; jj < 2; ++jj) t = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vop[jj], ph[jj], t, 0, 0, 0);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) acc_o[dt][r] += t[r];
+        for (int jj = 0; jj < 2; ++jj) {
+          acc_o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vop[jj], pl[jj], acc_o[dt], 0, 0, 0);
+          acc_o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vop[jj], ph[jj], acc_o[dt], 0, 0, 0);
+        }
       }
     }
   };
+
   reset();
   uint32_t vis[NH];
   for (int c0 = i_first; c0 < i_last; c0 += CH) {
     const int c1 = min(c0 + CH, i_last);
     if (c0 > i_first) __syncthreads();    // every wavefront left the items before
     lay_out(c0, c1);
+    if (ST == 1) {
+      for (int i = c0; i < c1; ++i) {
+        if (i > c0) __syncthreads();      // every wavefront left item i - 1
+        fetch(i - c0, i < n_wi, sK0, sV0);
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();                  // item i landed
+        item(i - c0, sK0, sV0, vis);
+      }
+      continue;
+    }
     fetch(0, c0 < n_wi, sK0, sV0);
     auto step = [&](int i, auto par) __attribute__((always_inline)) {
       constexpr int P = decltype(par)::value;
@@ -621,7 +645,7 @@ inline TreePlan tree_plan(int B, int H, int Hkv, int max_n, int K, int S, int bs
   const int64_t blocks = std::min<int64_t>((S + bs - 1) / bs, nodes * K);
   const int64_t items = (std::min<int64_t>(S, (int64_t)lw + max_n) + 95) / 64 + (blocks * (bs / 32) + 1) / 2;
   const int64_t streams = std::max<int64_t>(1, (int64_t)B * Hkv * p.groups);
-  p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({64, items, (kTrTarget + streams - 1) / streams}));
+  p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({64, items, kTrTarget / streams}));
   return p;
 }
 inline int64_t tree_workspace(const TreePlan& p, int64_t T, int H) {
