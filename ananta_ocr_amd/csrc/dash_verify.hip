@@ -42,7 +42,15 @@ struct VerifyArgs {
   int32_t* stop;                        // [B] the last accepted node
   double* gone;                         // [B] a at that node
   double2* sums;                        // [B, chunks] (what is left, the row itself)
+  int32_t* done;                        // [B] chunks that have arrived (the walk clears it)
   float* best_v; int32_t* best_i;       // [T, chunks] greedy partials
+};
+
+// Sixteen bytes of a row, at any element's boundary (global loads need no more).
+struct __attribute__((packed)) VfBytes { uint32_t x[4]; };
+template <typename T> struct VfVec {
+  static constexpr int kN = 16 / sizeof(T);
+  union { VfBytes b; T e[kN]; };
 };
 
 template <typename T> __device__ __forceinline__ float vf_load(const T* x) { return (float)*x; }
@@ -74,8 +82,9 @@ __device__ __forceinline__ double vf_block_sum(double v, double* sD) {
   return s;
 }
 
-// Greedy: the best token of a piece of a row; the lowest of equals, NaN never.
-template <typename T, bool VEC>
+// Greedy: the best token of a piece of a row; the lowest of equals, NaN never.  Bound by HBM (1,163
+// rows of 131,072 bf16 tokens in 54 us, 5.6 TB/s).
+template <typename T>
 __global__ __launch_bounds__(kVfThreads) void verify_best_kernel(VerifyArgs a) {
   __shared__ float sV[kVfThreads / kWave];
   __shared__ int sI[kVfThreads / kWave];
@@ -85,23 +94,19 @@ __global__ __launch_bounds__(kVfThreads) void verify_best_kernel(VerifyArgs a) {
   const T* p = (const T*)a.p + row * a.p_st;
   float best = -INFINITY;
   int at = INT32_MAX;
+  constexpr int E = VfVec<T>::kN, U = 4;
   int v = v0;
-  if (VEC) {
-    constexpr int E = 16 / sizeof(T), U = 4;
-    for (; v + kVfThreads * E * U <= v1; v += kVfThreads * E * U) {
-      uint4 x[U];
+  for (; v + kVfThreads * E * U <= v1; v += kVfThreads * E * U) {
+    VfVec<T> x[U];
 #pragma unroll
-      for (int k = 0; k < U; ++k) x[k] = *(const uint4*)(p + v + (k * kVfThreads + tid) * E);
+    for (int k = 0; k < U; ++k) x[k].b = *(const VfBytes*)(p + v + (k * kVfThreads + tid) * E);
 #pragma unroll
-      for (int k = 0; k < U; ++k) {
-        const T* e = (const T*)&x[k];
+    for (int k = 0; k < U; ++k)
 #pragma unroll
-        for (int j = 0; j < E; ++j) {
-          const float f = vf_load(e + j);
-          if (f > best) { best = f; at = v + (k * kVfThreads + tid) * E + j; }
-        }
+      for (int j = 0; j < E; ++j) {
+        const float f = vf_load(&x[k].e[j]);
+        if (f > best) { best = f; at = v + (k * kVfThreads + tid) * E + j; }
       }
-    }
   }
   for (int w = v + tid; w < v1; w += kVfThreads) {
     const float f = vf_load(p + w);
@@ -138,7 +143,7 @@ __global__ __launch_bounds__(THREADS) void verify_walk_kernel(VerifyArgs a) {
   const int n = min((int)(a.cu[b + 1] - r0), a.max_n);
   if (n <= 0) {
     for (int i = tid; i < a.max_n; i += THREADS) a.path[b * a.path_st + i] = -1;
-    if (tid == 0) { a.count[b] = 0; a.token[b] = -1; if (MODE) a.stop[b] = -1; }
+    if (tid == 0) { a.count[b] = 0; a.token[b] = -1; if (MODE != 0) a.stop[b] = -1; }
     return;
   }
   for (int i = tid; i < n; i += THREADS) {
@@ -198,17 +203,24 @@ __global__ __launch_bounds__(THREADS) void verify_walk_kernel(VerifyArgs a) {
           if (more) {
             const T* p = (const T*)a.p + (r0 + s) * a.p_st;
             const T* q = (const T*)a.q + (r0 + s) * a.q_st;
-            constexpr int U = 8;
+            // one work-group's reads in flight: 32 or 64 bytes a lane of each row, 64 or 128 KB
+            constexpr int E = VfVec<T>::kN, U = 4;
             double mine = 0.0;
-            int v = tid;
-            for (; v + (U - 1) * THREADS < a.V; v += U * THREADS) {
-              float x[U], y[U];
+            int v = 0;
+            for (; v + THREADS * E * U <= a.V; v += THREADS * E * U) {
+              VfVec<T> x[U], y[U];
 #pragma unroll
-              for (int k = 0; k < U; ++k) { x[k] = vf_load(p + v + k * THREADS); y[k] = vf_load(q + v + k * THREADS); }
+              for (int k = 0; k < U; ++k) {
+                x[k].b = *(const VfBytes*)(p + v + (k * THREADS + tid) * E);
+                y[k].b = *(const VfBytes*)(q + v + (k * THREADS + tid) * E);
+              }
 #pragma unroll
-              for (int k = 0; k < U; ++k) mine += vf_left(x[k], y[k], gone);
+              for (int k = 0; k < U; ++k)
+#pragma unroll
+                for (int j = 0; j < E; ++j) mine += vf_left(vf_load(&x[k].e[j]), vf_load(&y[k].e[j]), gone);
             }
-            for (; v < a.V; v += THREADS) mine += vf_left(vf_load(p + v), vf_load(q + v), gone);
+#pragma unroll 4
+            for (int w2 = v + tid; w2 < a.V; w2 += THREADS) mine += vf_left(vf_load(p + w2), vf_load(q + w2), gone);
             Z = vf_block_sum<THREADS>(mine, sD);
           }
         }
@@ -228,6 +240,7 @@ __global__ __launch_bounds__(THREADS) void verify_walk_kernel(VerifyArgs a) {
     } else {
       a.stop[b] = s;
       a.gone[b] = gone;
+      a.done[b] = 0;
     }
   }
 }
@@ -237,52 +250,59 @@ __global__ __launch_bounds__(THREADS) void verify_walk_kernel(VerifyArgs a) {
 __device__ __forceinline__ void vf_named(const VerifyArgs& a, int b, int s, int v0, uint32_t* sBits) {
   for (int i = threadIdx.x; i < kVfChunk / 32; i += kVfThreads) sBits[i] = 0u;
   __syncthreads();
-  if (!a.q) {
-    const int64_t r0 = a.cu[b];
-    const int n = min((int)(a.cu[b + 1] - r0), a.max_n);
-    for (int i = threadIdx.x + 1; i < n; i += kVfThreads) {
-      const int par = a.parents[r0 + i];
-      if (par != s || par >= i) continue;
-      const int64_t t = vf_token(a, r0 + i) - v0;
-      if (t >= 0 && t < kVfChunk) atomicOr(&sBits[t >> 5], 1u << (t & 31));
-    }
+  const int64_t r0 = a.cu[b];
+  const int n = min((int)(a.cu[b + 1] - r0), a.max_n);
+  for (int i = threadIdx.x + 1; i < n; i += kVfThreads) {
+    const int par = a.parents[r0 + i];
+    if (par != s || par >= i) continue;
+    const int64_t t = vf_token(a, r0 + i) - v0;
+    if (t >= 0 && t < kVfChunk) atomicOr(&sBits[t >> 5], 1u << (t & 31));
   }
   __syncthreads();
 }
 
-// (what is left, the row itself) of token v0 + e.
-template <typename T>
-__device__ __forceinline__ double2 vf_pair(const VerifyArgs& a, const T* p, const T* q, int v0, int e,
-                                           double gone, const uint32_t* sBits) {
-  const float x = vf_load(p + v0 + e);
-  const double whole = vf_left(x, 0.f, 0.0);
-  if (q) return make_double2(vf_left(x, vf_load(q + v0 + e), gone), whole);
-  return make_double2((sBits[e >> 5] >> (e & 31)) & 1u ? 0.0 : whole, whole);
-}
+constexpr int kVfPer = kVfChunk / kVfThreads;      // tokens of a thread, one after another
 
-template <typename T>
-__global__ __launch_bounds__(kVfThreads) void verify_sums_kernel(VerifyArgs a) {
-  __shared__ uint32_t sBits[kVfChunk / 32];
-  __shared__ double sD[kVfThreads / kWave];
-  const int b = blockIdx.y, v0 = blockIdx.x * kVfChunk;
-  const int s = a.stop[b];
-  if (s < 0) return;
-  const int64_t row = a.cu[b] + s;
-  const T* p = (const T*)a.p + row * a.p_st;
-  const T* q = a.q ? (const T*)a.q + row * a.q_st : nullptr;
-  const double gone = a.gone[b];
-  vf_named(a, b, s, v0, sBits);
-  const int m = min(kVfChunk, a.V - v0);
-  double left = 0.0, whole = 0.0;
-#pragma unroll 8
-  for (int e = threadIdx.x; e < m; e += kVfThreads) {
-    const double2 x = vf_pair<T>(a, p, q, v0, e, gone, sBits);
-    left += x.x;
-    whole += x.y;
+// This thread's tokens of chunk v0 of the last node's row: what is left of each, and their sum in
+// the row itself.
+template <typename T, bool DRAFT>
+__device__ __forceinline__ void vf_tokens(const VerifyArgs& a, int64_t row, int v0, double gone,
+                                          const uint32_t* sBits, double (&left)[kVfPer],
+                                          double (&whole)[kVfPer]) {
+  constexpr int E = VfVec<T>::kN, N = kVfPer / E;
+  const int e0 = threadIdx.x * kVfPer, m = min(a.V - v0 - e0, kVfPer);
+  const T* p = (const T*)a.p + row * a.p_st + v0 + e0;
+  const T* q = DRAFT ? (const T*)a.q + row * a.q_st + v0 + e0 : nullptr;
+  VfVec<T> x[N], y[N];
+  if (m == kVfPer) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      x[k].b = ((const VfBytes*)p)[k];
+      if (DRAFT) y[k].b = ((const VfBytes*)q)[k];
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      x[k].b = VfBytes{{0u, 0u, 0u, 0u}};
+      y[k].b = VfBytes{{0u, 0u, 0u, 0u}};
+#pragma unroll
+      for (int j = 0; j < E; ++j)
+        if (k * E + j < m) {
+          x[k].e[j] = p[k * E + j];
+          if (DRAFT) y[k].e[j] = q[k * E + j];
+        }
+    }
   }
-  left = vf_block_sum<kVfThreads>(left, sD);
-  whole = vf_block_sum<kVfThreads>(whole, sD);
-  if (threadIdx.x == 0) a.sums[(int64_t)b * a.chunks + blockIdx.x] = make_double2(left, whole);
+  const uint32_t named = DRAFT ? 0u : (sBits[e0 >> 5] >> (e0 & 31)) & ((1u << kVfPer) - 1u);
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      const int i = k * E + j;
+      const float f = vf_load(&x[k].e[j]);
+      whole[i] = vf_left(f, 0.f, 0.0);
+      left[i] = DRAFT ? vf_left(f, vf_load(&y[k].e[j]), gone) : (named >> i) & 1u ? 0.0 : whole[i];
+    }
 }
 
 // Sum over the work-group's earlier threads, and over all.
@@ -294,6 +314,8 @@ __device__ __forceinline__ double vf_before(double v, double* sD, double& total)
     const double y = __shfl_up(x, s, kWave);
     if (lane >= s) x += y;
   }
+  double own = __shfl_up(x, 1, kWave);
+  if (lane == 0) own = 0.0;
   __syncthreads();
   if (lane == kWave - 1) sD[wv] = x;
   __syncthreads();
@@ -304,28 +326,77 @@ __device__ __forceinline__ double vf_before(double v, double* sD, double& total)
     if (w < wv) before += sD[w];
     total += sD[w];
   }
-  return before + x - v;
+  return before + own;
 }
 
-// The chunk that the root's number falls into, then the token within it.
-template <typename T>
+// The smallest `first` and the largest `last` over the work-group.
+__device__ __forceinline__ void vf_ends(int& first, int& last, int2* sE) {
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) {
+    first = min(first, __shfl_xor(first, m, kWave));
+    last = max(last, __shfl_xor(last, m, kWave));
+  }
+  __syncthreads();
+  if (wave_lane() == 0) sE[threadIdx.x / kWave] = make_int2(first, last);
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kVfThreads / kWave; ++w) {
+    first = min(first, sE[w].x);
+    last = max(last, sE[w].y);
+  }
+}
+
+// The next token: every work-group sums a chunk of the last node's row, and the one that arrives
+// last finds the chunk that the root's number falls into, then the token within it.  Whichever that
+// is adds the same sums in the same order.  Bound by latency: a chunk's loads, the arrival, and the
+// chosen chunk again (a row is 0.26 to 0.8 MB, read by a tenth of the chip).
+template <typename T, bool DRAFT>
 __global__ __launch_bounds__(kVfThreads) void verify_draw_kernel(VerifyArgs a) {
   __shared__ uint32_t sBits[kVfChunk / 32];
   __shared__ double sD[kVfThreads / kWave];
-  __shared__ double sX[kVfChunk];
+  __shared__ int2 sE[kVfThreads / kWave];
   __shared__ double sBase;
-  __shared__ int sAt, sLast;
-  const int b = blockIdx.x, tid = threadIdx.x;
+  __shared__ int sTurn;
+  const int b = blockIdx.y, tid = threadIdx.x;
   const int s = a.stop[b];
   if (s < 0) return;
-  const double2* sums = a.sums + (int64_t)b * a.chunks;
+  const int64_t row = a.cu[b] + s;
+  const double gone = a.gone[b];
+  double2* sums = a.sums + (int64_t)b * a.chunks;
+  double left[kVfPer], whole[kVfPer];
+  {
+    const int v0 = blockIdx.x * kVfChunk;
+    if (!DRAFT) vf_named(a, b, s, v0, sBits);
+    vf_tokens<T, DRAFT>(a, row, v0, gone, sBits, left, whole);
+    double x = 0.0, y = 0.0;
+#pragma unroll
+    for (int k = 0; k < kVfPer; ++k) { x += left[k]; y += whole[k]; }
+    x = vf_block_sum<kVfThreads>(x, sD);
+    y = vf_block_sum<kVfThreads>(y, sD);
+    if (tid == 0) {
+      // agent scope: the work-group that adds them up may run on another XCD
+      __hip_atomic_store(&sums[blockIdx.x].x, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __hip_atomic_store(&sums[blockIdx.x].y, y, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      sTurn = __hip_atomic_fetch_add(&a.done[b], 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (sTurn != a.chunks - 1) return;
+  }
   // each thread's run of chunks
   const int per = (a.chunks + kVfThreads - 1) / kVfThreads;
   const int c0 = min(tid * per, a.chunks), c1 = min(c0 + per, a.chunks);
-  double left = 0.0, whole = 0.0, total, total_w;
-  for (int c = c0; c < c1; ++c) { left += sums[c].x; whole += sums[c].y; }
-  double before = vf_before(left, sD, total);
-  const double before_w = vf_before(whole, sD, total_w);
+  auto sum_of = [&](int c) {
+    return make_double2(__hip_atomic_load(&sums[c].x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT),
+                        __hip_atomic_load(&sums[c].y, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+  };
+  double mine = 0.0, mine_w = 0.0, total, total_w;
+  for (int c = c0; c < c1; ++c) {
+    const double2 x = sum_of(c);
+    mine += x.x;
+    mine_w += x.y;
+  }
+  double before = vf_before(mine, sD, total);
+  const double before_w = vf_before(mine_w, sD, total_w);
   const bool rest = total > 0.0;            // nothing left by rounding: the row itself
   if (!rest) { before = before_w; total = total_w; }
   if (!(total > 0.0)) {
@@ -333,51 +404,46 @@ __global__ __launch_bounds__(kVfThreads) void verify_draw_kernel(VerifyArgs a) {
     return;
   }
   const double want = (double)a.u[a.cu[b]] * total;
-  if (tid == 0) { sAt = INT32_MAX; sLast = -1; }
-  __syncthreads();
+  int first = INT32_MAX, last = -1;
   {
     double x = before;
     for (int c = c0; c < c1; ++c) {
-      const double y = rest ? sums[c].x : sums[c].y;
-      if (y > 0.0) atomicMax(&sLast, c);
-      if (x + y > want) { atomicMin(&sAt, c); break; }
+      const double2 z = sum_of(c);
+      const double y = rest ? z.x : z.y;
+      if (y > 0.0) last = c;
       x += y;
+      if (x > want) { first = c; break; }
     }
   }
-  __syncthreads();
-  const int at = sAt == INT32_MAX ? sLast : sAt;
+  vf_ends(first, last, sE);
+  const int at = first == INT32_MAX ? last : first;
   if (at >= c0 && at < c1) {
     double x = before;
-    for (int c = c0; c < at; ++c) x += rest ? sums[c].x : sums[c].y;
+    for (int c = c0; c < at; ++c) { const double2 z = sum_of(c); x += rest ? z.x : z.y; }
     sBase = x;
   }
+  const int v0 = at * kVfChunk;
+  if (!DRAFT) vf_named(a, b, s, v0, sBits);
   __syncthreads();
   const double base = sBase;
-  const int v0 = at * kVfChunk, m = min(kVfChunk, a.V - v0);
-  const int64_t row = a.cu[b] + s;
-  const T* p = (const T*)a.p + row * a.p_st;
-  const T* q = a.q ? (const T*)a.q + row * a.q_st : nullptr;
-  const double gone = a.gone[b];
-  vf_named(a, b, s, v0, sBits);
-  for (int e = tid; e < kVfChunk; e += kVfThreads) {
-    double2 x = make_double2(0.0, 0.0);
-    if (e < m) x = vf_pair<T>(a, p, q, v0, e, gone, sBits);
-    sX[e] = rest ? x.x : x.y;
-  }
-  if (tid == 0) { sAt = INT32_MAX; sLast = -1; }
-  __syncthreads();
-  constexpr int kPer = kVfChunk / kVfThreads;
+  vf_tokens<T, DRAFT>(a, row, v0, gone, sBits, left, whole);
   double run = 0.0;
-  for (int k = 0; k < kPer; ++k) run += sX[tid * kPer + k];
+#pragma unroll
+  for (int k = 0; k < kVfPer; ++k) run += rest ? left[k] : whole[k];
   double x = base + vf_before(run, sD, total);
-  for (int k = 0; k < kPer; ++k) {
-    const double y = sX[tid * kPer + k];
-    if (y > 0.0) atomicMax(&sLast, tid * kPer + k);
+  first = INT32_MAX;
+  last = -1;
+#pragma unroll
+  for (int k = 0; k < kVfPer; ++k) {
+    const double y = rest ? left[k] : whole[k];
     x += y;
-    if (x > want && y > 0.0) { atomicMin(&sAt, tid * kPer + k); break; }
+    if (y > 0.0) {
+      last = tid * kVfPer + k;
+      if (x > want && first == INT32_MAX) first = last;
+    }
   }
-  __syncthreads();
-  if (tid == 0) a.token[b] = v0 + (sAt == INT32_MAX ? sLast : sAt);
+  vf_ends(first, last, sE);
+  if (tid == 0) a.token[b] = v0 + (first == INT32_MAX ? last : first);
 }
 
 static int verify_chunks(int64_t T, int V, bool greedy, int& chunk) {
@@ -391,13 +457,14 @@ static int verify_chunks(int64_t T, int V, bool greedy, int& chunk) {
   return (V + chunk - 1) / chunk;
 }
 
-struct VerifyLayout { int64_t stop, gone, sums, best_v, best_i, total; int chunks, chunk; };
+struct VerifyLayout { int64_t stop, done, gone, sums, best_v, best_i, total; int chunks, chunk; };
 static VerifyLayout verify_layout(int B, int64_t T, int V, bool greedy) {
   VerifyLayout L;
   L.chunks = verify_chunks(T, V, greedy, L.chunk);
   auto align = [](int64_t x) { return (x + 255) / 256 * 256; };
   int64_t o = 0;
   L.stop = o; o = align(o + (int64_t)B * 4);
+  L.done = o; o = align(o + (int64_t)B * 4);
   L.gone = o; o = align(o + (int64_t)B * 8);
   L.sums = o; if (!greedy) o = align(o + (int64_t)B * L.chunks * 16);
   L.best_v = o; if (greedy) o = align(o + T * L.chunks * 4);
@@ -409,19 +476,19 @@ static VerifyLayout verify_layout(int B, int64_t T, int V, bool greedy) {
 template <typename T>
 static void verify_launch(const VerifyArgs& a, hipStream_t st) {
   if (!a.u) {
-    const bool vec = (uintptr_t)a.p % 16 == 0 && a.p_st * sizeof(T) % 16 == 0 && a.chunk % 64 == 0;
-    auto kern = vec ? verify_best_kernel<T, true> : verify_best_kernel<T, false>;
     if (a.T > 0)
-      hipLaunchKernelGGL(kern, dim3((unsigned)(a.T * a.chunks)), dim3(kVfThreads), 0, st, a);
+      hipLaunchKernelGGL(verify_best_kernel<T>, dim3((unsigned)(a.T * a.chunks)), dim3(kVfThreads), 0, st, a);
     hipLaunchKernelGGL((verify_walk_kernel<T, 0, 256>), dim3(a.B), dim3(256), 0, st, a);
     return;
   }
-  if (a.q)
+  const dim3 grid(a.chunks, a.B);
+  if (a.q) {
     hipLaunchKernelGGL((verify_walk_kernel<T, 2, 1024>), dim3(a.B), dim3(1024), 0, st, a);
-  else
+    hipLaunchKernelGGL((verify_draw_kernel<T, true>), grid, dim3(kVfThreads), 0, st, a);
+  } else {
     hipLaunchKernelGGL((verify_walk_kernel<T, 1, 256>), dim3(a.B), dim3(256), 0, st, a);
-  hipLaunchKernelGGL(verify_sums_kernel<T>, dim3(a.chunks, a.B), dim3(kVfThreads), 0, st, a);
-  hipLaunchKernelGGL(verify_draw_kernel<T>, dim3(a.B), dim3(kVfThreads), 0, st, a);
+    hipLaunchKernelGGL((verify_draw_kernel<T, false>), grid, dim3(kVfThreads), 0, st, a);
+  }
 }
 
 }  // namespace dash
@@ -457,7 +524,7 @@ extern "C" int dash_verify_tree(const void* target, int64_t target_stride, const
   a.tok = tokens; a.tok64 = tokens_int64; a.parents = parents; a.cu = cu_seqlens_q; a.u = uniforms;
   a.B = B; a.V = V; a.max_n = max_query_len; a.chunks = L.chunks; a.chunk = L.chunk; a.T = T;
   a.count = count; a.path = path; a.path_st = path_stride; a.token = next_token;
-  a.stop = (int32_t*)(w + L.stop); a.gone = (double*)(w + L.gone); a.sums = (double2*)(w + L.sums);
+  a.stop = (int32_t*)(w + L.stop); a.done = (int32_t*)(w + L.done); a.gone = (double*)(w + L.gone); a.sums = (double2*)(w + L.sums);
   a.best_v = (float*)(w + L.best_v); a.best_i = (int32_t*)(w + L.best_i);
   hipStream_t st = (hipStream_t)stream;
   if (dtype == 0) verify_launch<float>(a, st);
