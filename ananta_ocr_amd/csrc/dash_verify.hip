@@ -203,8 +203,8 @@ __global__ __launch_bounds__(THREADS) void verify_walk_kernel(VerifyArgs a) {
           if (more) {
             const T* p = (const T*)a.p + (r0 + s) * a.p_st;
             const T* q = (const T*)a.q + (r0 + s) * a.q_st;
-            // one work-group's reads in flight: 32 or 64 bytes a lane of each row, 64 or 128 KB
-            constexpr int E = VfVec<T>::kN, U = 4;
+            // one work-group's reads in flight: 32 tokens a lane of each row, 128 or 256 KB
+            constexpr int E = VfVec<T>::kN, U = 32 / E;
             double mine = 0.0;
             int v = 0;
             for (; v + THREADS * E * U <= a.V; v += THREADS * E * U) {
@@ -245,64 +245,69 @@ __global__ __launch_bounds__(THREADS) void verify_walk_kernel(VerifyArgs a) {
   }
 }
 
-// The tokens of a chunk that the children of the last accepted node named (certain proposals):
-// a bit each.
-__device__ __forceinline__ void vf_named(const VerifyArgs& a, int b, int s, int v0, uint32_t* sBits) {
+// The token of this thread's node where it is a child of node s, -1 else (certain proposals).
+__device__ __forceinline__ int64_t vf_child(const VerifyArgs& a, int64_t r0, int n, int s) {
+  static_assert(kVfMaxNodes <= kVfThreads, "a thread per node");
+  const int i = threadIdx.x;
+  if (i < 1 || i >= n) return -1;
+  const int par = a.parents[r0 + i];
+  const int64_t t = vf_token(a, r0 + i);
+  return par == s && par < i ? t : -1;
+}
+
+// The children's tokens that lie in chunk v0, a bit each.
+__device__ __forceinline__ void vf_named(int64_t child, int v0, uint32_t* sBits) {
   for (int i = threadIdx.x; i < kVfChunk / 32; i += kVfThreads) sBits[i] = 0u;
   __syncthreads();
-  const int64_t r0 = a.cu[b];
-  const int n = min((int)(a.cu[b + 1] - r0), a.max_n);
-  for (int i = threadIdx.x + 1; i < n; i += kVfThreads) {
-    const int par = a.parents[r0 + i];
-    if (par != s || par >= i) continue;
-    const int64_t t = vf_token(a, r0 + i) - v0;
-    if (t >= 0 && t < kVfChunk) atomicOr(&sBits[t >> 5], 1u << (t & 31));
-  }
+  const int64_t t = child - v0;
+  if (child >= 0 && t >= 0 && t < kVfChunk) atomicOr(&sBits[t >> 5], 1u << (t & 31));
   __syncthreads();
 }
 
 constexpr int kVfPer = kVfChunk / kVfThreads;      // tokens of a thread, one after another
 
-// This thread's tokens of chunk v0 of the last node's row: what is left of each, and their sum in
-// the row itself.
+// This thread's tokens of chunk v0 of the last node's row (zeros past the row's end) ...
 template <typename T, bool DRAFT>
-__device__ __forceinline__ void vf_tokens(const VerifyArgs& a, int64_t row, int v0, double gone,
-                                          const uint32_t* sBits, double (&left)[kVfPer],
-                                          double (&whole)[kVfPer]) {
-  constexpr int E = VfVec<T>::kN, N = kVfPer / E;
-  const int e0 = threadIdx.x * kVfPer, m = min(a.V - v0 - e0, kVfPer);
-  const T* p = (const T*)a.p + row * a.p_st + v0 + e0;
-  const T* q = DRAFT ? (const T*)a.q + row * a.q_st + v0 + e0 : nullptr;
-  VfVec<T> x[N], y[N];
-  if (m == kVfPer) {
+struct VfTokens {
+  static constexpr int E = VfVec<T>::kN, N = kVfPer / E;
+  VfVec<T> x[N], y[DRAFT ? N : 1];
+  __device__ __forceinline__ void load(const VerifyArgs& a, int64_t row, int v0) {
+    const int e0 = threadIdx.x * kVfPer, m = min(a.V - v0 - e0, kVfPer);
+    const T* p = (const T*)a.p + row * a.p_st + v0 + e0;
+    const T* q = DRAFT ? (const T*)a.q + row * a.q_st + v0 + e0 : nullptr;
+    if (m == kVfPer) {
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
-      x[k].b = ((const VfBytes*)p)[k];
-      if (DRAFT) y[k].b = ((const VfBytes*)q)[k];
-    }
-  } else {
+      for (int k = 0; k < N; ++k) {
+        x[k].b = ((const VfBytes*)p)[k];
+        if (DRAFT) y[k].b = ((const VfBytes*)q)[k];
+      }
+    } else {
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
-      x[k].b = VfBytes{{0u, 0u, 0u, 0u}};
-      y[k].b = VfBytes{{0u, 0u, 0u, 0u}};
+      for (int k = 0; k < N; ++k) {
+        x[k].b = VfBytes{{0u, 0u, 0u, 0u}};
+        if (DRAFT) y[k].b = VfBytes{{0u, 0u, 0u, 0u}};
 #pragma unroll
-      for (int j = 0; j < E; ++j)
-        if (k * E + j < m) {
-          x[k].e[j] = p[k * E + j];
-          if (DRAFT) y[k].e[j] = q[k * E + j];
-        }
+        for (int j = 0; j < E; ++j)
+          if (k * E + j < m) {
+            x[k].e[j] = p[k * E + j];
+            if (DRAFT) y[k].e[j] = q[k * E + j];
+          }
+      }
     }
   }
-  const uint32_t named = DRAFT ? 0u : (sBits[e0 >> 5] >> (e0 & 31)) & ((1u << kVfPer) - 1u);
-#pragma unroll
-  for (int k = 0; k < N; ++k)
-#pragma unroll
-    for (int j = 0; j < E; ++j) {
-      const int i = k * E + j;
-      const float f = vf_load(&x[k].e[j]);
-      whole[i] = vf_left(f, 0.f, 0.0);
-      left[i] = DRAFT ? vf_left(f, vf_load(&y[k].e[j]), gone) : (named >> i) & 1u ? 0.0 : whole[i];
-    }
+  // ... what is left of token i, and the row itself.
+  __device__ __forceinline__ double2 at(int i, double gone, uint32_t named) const {
+    const float f = vf_load(&x[i / E].e[i % E]);
+    const double whole = vf_left(f, 0.f, 0.0);
+    if (DRAFT) return make_double2(vf_left(f, vf_load(&y[i / E].e[i % E]), gone), whole);
+    return make_double2((named >> i) & 1u ? 0.0 : whole, whole);
+  }
+};
+
+// The bits of this thread's tokens.
+__device__ __forceinline__ uint32_t vf_bits(const uint32_t* sBits) {
+  const int e0 = threadIdx.x * kVfPer;
+  return (sBits[e0 >> 5] >> (e0 & 31)) & ((1u << kVfPer) - 1u);
 }
 
 // Sum over the work-group's earlier threads, and over all.
@@ -358,19 +363,31 @@ __global__ __launch_bounds__(kVfThreads) void verify_draw_kernel(VerifyArgs a) {
   __shared__ double sBase;
   __shared__ int sTurn;
   const int b = blockIdx.y, tid = threadIdx.x;
+  const int64_t r0 = a.cu[b];
+  const int n = min((int)(a.cu[b + 1] - r0), a.max_n);
   const int s = a.stop[b];
   if (s < 0) return;
-  const int64_t row = a.cu[b] + s;
+  const int64_t row = r0 + s;
   const double gone = a.gone[b];
+  const double u = (double)a.u[r0];
+  const int64_t child = DRAFT ? -1 : vf_child(a, r0, n, s);
   double2* sums = a.sums + (int64_t)b * a.chunks;
-  double left[kVfPer], whole[kVfPer];
+  VfTokens<T, DRAFT> tk;
+  uint32_t named = 0u;
   {
     const int v0 = blockIdx.x * kVfChunk;
-    if (!DRAFT) vf_named(a, b, s, v0, sBits);
-    vf_tokens<T, DRAFT>(a, row, v0, gone, sBits, left, whole);
+    tk.load(a, row, v0);
+    if (!DRAFT) {
+      vf_named(child, v0, sBits);
+      named = vf_bits(sBits);
+    }
     double x = 0.0, y = 0.0;
 #pragma unroll
-    for (int k = 0; k < kVfPer; ++k) { x += left[k]; y += whole[k]; }
+    for (int k = 0; k < kVfPer; ++k) {
+      const double2 z = tk.at(k, gone, named);
+      x += z.x;
+      y += z.y;
+    }
     x = vf_block_sum<kVfThreads>(x, sD);
     y = vf_block_sum<kVfThreads>(y, sD);
     if (tid == 0) {
@@ -382,13 +399,15 @@ __global__ __launch_bounds__(kVfThreads) void verify_draw_kernel(VerifyArgs a) {
     __syncthreads();
     if (sTurn != a.chunks - 1) return;
   }
-  // each thread's run of chunks
+  // each thread's run of chunks, the first of them in registers
   const int per = (a.chunks + kVfThreads - 1) / kVfThreads;
   const int c0 = min(tid * per, a.chunks), c1 = min(c0 + per, a.chunks);
-  auto sum_of = [&](int c) {
+  auto read = [&](int c) {
     return make_double2(__hip_atomic_load(&sums[c].x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT),
                         __hip_atomic_load(&sums[c].y, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
   };
+  const double2 sum0 = c0 < c1 ? read(c0) : make_double2(0.0, 0.0);
+  auto sum_of = [&](int c) { return c == c0 ? sum0 : read(c); };
   double mine = 0.0, mine_w = 0.0, total, total_w;
   for (int c = c0; c < c1; ++c) {
     const double2 x = sum_of(c);
@@ -403,7 +422,7 @@ __global__ __launch_bounds__(kVfThreads) void verify_draw_kernel(VerifyArgs a) {
     if (tid == 0) a.token[b] = -1;
     return;
   }
-  const double want = (double)a.u[a.cu[b]] * total;
+  const double want = u * total;
   int first = INT32_MAX, last = -1;
   {
     double x = before;
@@ -417,25 +436,31 @@ __global__ __launch_bounds__(kVfThreads) void verify_draw_kernel(VerifyArgs a) {
   }
   vf_ends(first, last, sE);
   const int at = first == INT32_MAX ? last : first;
+  const int v0 = at * kVfChunk;
+  tk.load(a, row, v0);
   if (at >= c0 && at < c1) {
     double x = before;
     for (int c = c0; c < at; ++c) { const double2 z = sum_of(c); x += rest ? z.x : z.y; }
     sBase = x;
   }
-  const int v0 = at * kVfChunk;
-  if (!DRAFT) vf_named(a, b, s, v0, sBits);
-  __syncthreads();
-  const double base = sBase;
-  vf_tokens<T, DRAFT>(a, row, v0, gone, sBits, left, whole);
+  if (!DRAFT) {
+    vf_named(child, v0, sBits);
+    named = vf_bits(sBits);
+  }
   double run = 0.0;
 #pragma unroll
-  for (int k = 0; k < kVfPer; ++k) run += rest ? left[k] : whole[k];
-  double x = base + vf_before(run, sD, total);
+  for (int k = 0; k < kVfPer; ++k) {
+    const double2 z = tk.at(k, gone, named);
+    run += rest ? z.x : z.y;
+  }
+  double x = vf_before(run, sD, total);     // (its barriers order sBase)
+  x += sBase;
   first = INT32_MAX;
   last = -1;
 #pragma unroll
   for (int k = 0; k < kVfPer; ++k) {
-    const double y = rest ? left[k] : whole[k];
+    const double2 z = tk.at(k, gone, named);
+    const double y = rest ? z.x : z.y;
     x += y;
     if (y > 0.0) {
       last = tid * kVfPer + k;
