@@ -212,6 +212,29 @@ __device__ __forceinline__ int kv_prefix(int n, int* want, int* sW, Value value)
   return base;
 }
 
+// take(i, k, tokens, page) for every entry k of the rows src[i] (entries past a row's tokens too), four
+// of a thread's loads in flight: one row after another took 20 us for 16 rows.
+template <typename Take>
+__device__ __forceinline__ void kv_entries(const int32_t* table, int64_t table_st, int P,
+                                           const int32_t* src, const int32_t* lens, int n, Take take) {
+  const int64_t all = (int64_t)n * P;
+  for (int64_t e0 = threadIdx.x; e0 < all; e0 += 4 * kKvThreads) {
+    int i[4], k[4], len[4], p[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int64_t e = min(e0 + u * kKvThreads, all - 1);
+      i[u] = (int)(e / P);
+      k[u] = (int)(e - (int64_t)i[u] * P);
+      const int s = src[i[u]];
+      len[u] = lens[s];
+      p[u] = table[(int64_t)s * table_st + k[u]];
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (e0 + u * kKvThreads < all) take(i[u], k[u], len[u], p[u]);
+  }
+}
+
 // Row dst[i] becomes row src[i]: its whole pages shared, its last, partly filled one a page of
 // its own, to be copied (frm[i] -> to[i]; -1 where there is none).  All pairs or none: ok is 0
 // and nothing changes where a row is out of range or named wrongly (a filled or repeated target, a
@@ -244,13 +267,9 @@ __global__ __launch_bounds__(kKvThreads) void fork_pages_kernel(
     return;
   }
   // every entry that is shared or copied names a page
-  for (int i = 0; i < n; ++i) {
-    const int s = src[i], nb = kv_blocks(lens[s], page);
-    for (int k = tid; k < nb; k += kKvThreads) {
-      const int p = table[(int64_t)s * table_st + k];
-      bad |= p < 0 || p >= num_pages;
-    }
-  }
+  kv_entries(table, table_st, P, src, lens, n, [&](int, int k, int len, int p) {
+    if (k * (int64_t)page < len) bad |= p < 0 || p >= num_pages;
+  });
   const int total = kv_prefix(n, sWant, sW, [&](int i) { return lens[src[i]] % page != 0 ? 1 : 0; });
   const int n_free = kv_count_free(refs, num_pages, sW);
   if (__syncthreads_or(bad || total > n_free)) {
@@ -269,14 +288,11 @@ __global__ __launch_bounds__(kKvThreads) void fork_pages_kernel(
     table[(int64_t)dst[i] * table_st + lens[src[i]] / page] = p;
   });
   __syncthreads();
-  for (int i = 0; i < n; ++i) {
-    const int s = src[i], full = lens[s] / page;
-    for (int k = tid; k < full; k += kKvThreads) {
-      const int p = table[(int64_t)s * table_st + k];
-      table[(int64_t)dst[i] * table_st + k] = p;
-      atomicAdd(&refs[p], 1);
-    }
-  }
+  kv_entries(table, table_st, P, src, lens, n, [&](int i, int k, int len, int p) {
+    if ((k + 1) * (int64_t)page > len) return;
+    table[(int64_t)dst[i] * table_st + k] = p;
+    atomicAdd(&refs[p], 1);
+  });
   __syncthreads();
   for (int i = tid; i < n; i += kKvThreads) lens[dst[i]] = lens[src[i]];
   if (tid == 0) *ok = 1;

@@ -60,12 +60,12 @@ __device__ __forceinline__ int64_t vf_token(const VerifyArgs& a, int64_t row) {
   return a.tok64 ? ((const int64_t*)a.tok)[row] : ((const int32_t*)a.tok)[row];
 }
 
-// What is left of probability p where the draft's is q.
+// What is left of probability p where the draft's is q (maxima take what is no number to 0).
+__device__ __forceinline__ double vf_rest(float p, float q, double gone) {
+  return fmax(fma(-gone, (double)q, (double)fmaxf(p, 0.f)), 0.0);
+}
 __device__ __forceinline__ double vf_left(float p, float q, double gone) {
-  const double x = p > 0.f ? (double)p : 0.0;
-  if (gone == 0.0) return x;
-  const double r = x - gone * (double)q;
-  return r > 0.0 ? r : 0.0;
+  return gone == 0.0 ? (double)fmaxf(p, 0.f) : vf_rest(p, q, gone);
 }
 
 // Sum over the work-group, the same on every thread.
@@ -205,7 +205,7 @@ __global__ __launch_bounds__(THREADS) void verify_walk_kernel(VerifyArgs a) {
             const T* q = (const T*)a.q + (r0 + s) * a.q_st;
             // one work-group's reads in flight: 32 tokens a lane of each row, 128 or 256 KB
             constexpr int E = VfVec<T>::kN, U = 32 / E;
-            double mine = 0.0;
+            double mine = 0.0, odd = 0.0;
             int v = 0;
             for (; v + THREADS * E * U <= a.V; v += THREADS * E * U) {
               VfVec<T> x[U], y[U];
@@ -217,11 +217,14 @@ __global__ __launch_bounds__(THREADS) void verify_walk_kernel(VerifyArgs a) {
 #pragma unroll
               for (int k = 0; k < U; ++k)
 #pragma unroll
-                for (int j = 0; j < E; ++j) mine += vf_left(vf_load(&x[k].e[j]), vf_load(&y[k].e[j]), gone);
+                for (int j = 0; j < E; j += 2) {
+                  mine += vf_rest(vf_load(&x[k].e[j]), vf_load(&y[k].e[j]), gone);
+                  odd += vf_rest(vf_load(&x[k].e[j + 1]), vf_load(&y[k].e[j + 1]), gone);
+                }
             }
 #pragma unroll 4
-            for (int w2 = v + tid; w2 < a.V; w2 += THREADS) mine += vf_left(vf_load(p + w2), vf_load(q + w2), gone);
-            Z = vf_block_sum<THREADS>(mine, sD);
+            for (int w2 = v + tid; w2 < a.V; w2 += THREADS) mine += vf_rest(vf_load(p + w2), vf_load(q + w2), gone);
+            Z = vf_block_sum<THREADS>(mine + odd, sD);
           }
         }
       }

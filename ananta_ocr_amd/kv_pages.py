@@ -68,6 +68,14 @@ class PageCaches:
         desc = (ctypes.c_int64 * max(8 * n, 1))()
         for i, (t, at) in enumerate(tensors):
             size, stride, es = t.shape, t.stride(), t.element_size()
+            rows = at == ax + 2
+            if t.is_contiguous():            # a page, or a row, in one piece
+                base[i] = t.data_ptr()
+                seg = es * (stride[at] * size[at] if at < t.dim() else 1)
+                desc[8 * i:8 * i + 8] = [size[0] if ax else 1, stride[0] * es if ax else 0,
+                                         stride[ax] * es, 1, stride[ax + 1] * es if rows else 0,
+                                         1, 0, seg]
+                continue
             seg, dims = 1, []                # by stride: source and target share the order
             for a in sorted(range(at, t.dim()), key=lambda a: stride[a]):
                 if size[a] == 1:
@@ -86,7 +94,6 @@ class PageCaches:
             for a in range(at):
                 if size[a] > 1 and stride[a] <= 0:
                     raise ValueError("a cache with overlapping pages")
-            rows = at == ax + 2
             if len(dims) > (1 if rows else 2):
                 raise NotImplementedError(
                     f"cache of shape {tuple(size)} and strides {tuple(stride)}: its pages lie in "
@@ -107,7 +114,7 @@ def copy_pages(caches, from_pages, to_pages):
     target, or the target of two pairs."""
     _shape(to_pages, from_pages.shape, "to_pages")
     with _device(caches.tensors[0], from_pages, to_pages):
-        f, t = _i32(from_pages.reshape(-1)), _i32(to_pages.reshape(-1))
+        f, t = _i32(from_pages), _i32(to_pages)
         n, base, desc = caches._copy
         _lib.check(_lib.load().dash_copy_pages(n, base, desc, _ptr(f), _ptr(t), f.numel(),
                                                caches.num_pages, _stream()), "dash_copy_pages")
@@ -148,8 +155,8 @@ def _in_place(**ts):
 
 
 def _moves(n, device):
-    m = torch.empty(2, n, dtype=torch.int32, device=device)
-    return torch.empty(1, dtype=torch.int32, device=device), m[0], m[1]
+    return (torch.empty(1, dtype=torch.int32, device=device),
+            *torch.empty(2, n, dtype=torch.int32, device=device).unbind(0))
 
 
 def fork_pages(refs, table, lens, src, dst, page_size):
@@ -164,7 +171,7 @@ def fork_pages(refs, table, lens, src, dst, page_size):
     if n > MAX_ROWS:
         raise NotImplementedError(f"at most {MAX_ROWS} forks a call")
     with _device(refs, table, lens, src, dst):
-        s, d = _i32(src.reshape(-1)), _i32(dst.reshape(-1))
+        s, d = _i32(src), _i32(dst)
         ok, frm, to = _moves(n, refs.device)
         R, P = table.shape
         _lib.check(_lib.load().dash_fork_pages(
@@ -222,13 +229,13 @@ def compact_pages(refs, table, lens, page_size):
         R, P = t.shape
         new_refs = torch.empty_like(r)
         new_table = torch.empty(R, P, dtype=torch.int32, device=r.device)
-        moves = torch.empty(2, max(n // 2, 1), dtype=torch.int32, device=r.device)
+        frm, to = torch.empty(2, max(n // 2, 1), dtype=torch.int32, device=r.device).unbind(0)
         place = torch.empty(n, dtype=torch.int32, device=r.device)
         _lib.check(_lib.load().dash_compact_pages(
             _ptr(r), n, _ptr(t), t.stride(0), R, P, _ptr(ln), int(page_size), _ptr(new_refs),
-            _ptr(new_table), _ptr(moves[0]), _ptr(moves[1]), _ptr(place), _stream()),
+            _ptr(new_table), _ptr(frm), _ptr(to), _ptr(place), _stream()),
             "dash_compact_pages")
-    return new_refs, new_table, moves[0, :n // 2], moves[1, :n // 2]
+    return (new_refs, new_table, frm, to) if n > 1 else (new_refs, new_table, frm[:0], to[:0])
 
 
 class PagePool:

@@ -13,6 +13,7 @@ C entry point on the current stream, and synchronise nothing.
 
 import contextlib
 import ctypes
+import functools
 
 import torch
 
@@ -22,20 +23,23 @@ from .ops import _bf16_rows, _i32, _need_gpu, _ptr, _stream, _u8
 MAX_NODES = 256                          # nodes of a sequence
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _device(*ts):
     """A context in which the tensors' device is the current one (they must share it)."""
-    _need_gpu(*ts)
-    ts = [t for t in ts if t is not None]
-    dev = ts[0].device
+    index = ts[0].get_device()
     for t in ts:
-        if t.device != dev:
-            raise ValueError(f"tensors on {dev} and {t.device}")
-    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() \
-        else torch.cuda.device(dev)
+        if t is not None and t.get_device() != index:
+            _need_gpu(*ts)
+            raise ValueError(f"tensors on {ts[0].device} and {t.device}")
+    if index < 0:
+        _need_gpu(*ts)
+    return _HERE if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
 
 
 def _shape(t, shape, what):
-    if t is not None and tuple(t.shape) != tuple(shape):
+    if t is not None and t.shape != shape:
         raise ValueError(f"{what}: {tuple(t.shape)} given, {tuple(shape)} needed")
 
 
@@ -147,11 +151,8 @@ def attn_tree(q, k, v, idx, bias, valid, mask, depth, context_lens, cu_seqlens_q
             else:
                 S, pages = k.shape[2], 0
                 kh, kt, vh, vt = k.stride(1), k.stride(2), v.stride(1), v.stride(2)
-            nbytes = ctypes.c_int64(0)
-            _lib.check(lib.dash_attn_tree_workspace_size(B, H, Hkv, T, n, K, S, int(block_size),
-                                                         int(local_window), nbytes), "workspace")
-            ws = torch.empty(nbytes.value, dtype=torch.uint8, device=q.device) \
-                if nbytes.value else None
+            nbytes = _attn_workspace(B, H, Hkv, T, n, K, S, int(block_size), int(local_window))
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
             _lib.check(lib.dash_attn_tree(
                 _ptr(q), q.stride(0), q.stride(1), _ptr(k), k.stride(0), kh, kt, _ptr(v),
                 v.stride(0), vh, vt, _ptr(bt), 0 if bt is None else bt.stride(0),
@@ -159,9 +160,23 @@ def attn_tree(q, k, v, idx, bias, valid, mask, depth, context_lens, cu_seqlens_q
                 _ptr(bias_c), K, _ptr(mask), mask.shape[1], _ptr(dep), _ptr(out),
                 int(out_dtype == torch.bfloat16), out.stride(0), out.stride(1), _ptr(lse),
                 0 if lse is None else lse.stride(0), 1, B, H, Hkv, T, n, S, D, int(block_size),
-                int(local_window), float(scale), _ptr(ws), nbytes.value, _stream()),
+                int(local_window), float(scale), _ptr(ws), nbytes, _stream()),
                 "dash_attn_tree")
     return (out, lse) if return_lse else out
+
+
+@functools.lru_cache(maxsize=256)
+def _attn_workspace(*sizes):
+    nbytes = ctypes.c_int64(0)
+    _lib.check(_lib.load().dash_attn_tree_workspace_size(*sizes, nbytes), "workspace")
+    return nbytes.value
+
+
+@functools.lru_cache(maxsize=256)
+def _verify_workspace(*sizes):
+    nbytes = ctypes.c_int64(0)
+    _lib.check(_lib.load().dash_verify_tree_workspace_size(*sizes, nbytes), "workspace")
+    return max(nbytes.value, 256)
 
 
 _VERIFY_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
@@ -209,10 +224,7 @@ def verify_tree(target, tokens, parents, cu_seqlens_q, max_query_len, uniforms=N
         count = torch.empty(B, dtype=torch.int32, device=dev)
         path = torch.empty(B, n, dtype=torch.int32, device=dev)
         token = torch.empty(B, dtype=torch.int64, device=dev)
-        nbytes = ctypes.c_int64(0)
-        _lib.check(lib.dash_verify_tree_workspace_size(B, T, V, int(u is None), nbytes),
-                   "workspace")
-        ws = torch.empty(max(nbytes.value, 256), dtype=torch.uint8, device=dev)
+        ws = torch.empty(_verify_workspace(B, T, V, int(u is None)), dtype=torch.uint8, device=dev)
         _lib.check(lib.dash_verify_tree(
             _ptr(target), target.stride(0), _ptr(draft), 0 if draft is None else draft.stride(0),
             _VERIFY_TYPES[target.dtype], _ptr(tok), int(tok.dtype == torch.int64), _ptr(par),
