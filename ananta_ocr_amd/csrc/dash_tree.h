@@ -103,8 +103,9 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void tree_attn_kernel(TreeArgs a) 
   __shared__ uint32_t sBits[kPfMaxBlocks / 32];       // the blocks that the rows name
   __shared__ int sPref[kPfMaxBlocks / 32 + 1];        // set bits before each word
   // halves of the items laid out: first key, place among the laid out blocks (-1: the band, -2: no
-  // keys), page and the first key's row in it
+  // keys), last row to load (later ones repeat it); the offsets of row 0 in K and V
   __shared__ int4 sHalf[2 * CH];
+  __shared__ longlong2 sOff[2 * CH];
   // (block, node): the bits of the log2 bias; kTrNotNamed where the node does not name the block
   __shared__ uint32_t sBias[2 * CH][32 * RT];
   __shared__ uint32_t sBad[NW];
@@ -114,7 +115,8 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void tree_attn_kernel(TreeArgs a) 
   extern __shared__ float dyn[];
   float* const sSlotBias = dyn;
   int16_t* const slots = (int16_t*)(dyn + (RT == 4 ? 0 : a.slot_cap));
-  const int tid = threadIdx.x, lane = wave_lane(), wv = tid / kWave;
+  const int tid = threadIdx.x, lane = wave_lane();
+  const int wv = __builtin_amdgcn_readfirstlane(tid / kWave);   // scalar: so are the stages' addresses
   const int rt = wv % RT, kg = wv / RT;
   int id = blockIdx.x;
   const int hk = id % a.Hkv; id /= a.Hkv;
@@ -140,6 +142,15 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void tree_attn_kernel(TreeArgs a) 
   const int w_row = ctx + a.depth[row] - a.lw + 1;
   const int top = min(w_row, ctx);
   const uint64_t mask0 = a.mask[row * a.words];
+  // over the wavefront's rows: the last window to start, the first end of the keys below one
+  int w_last = rvalid ? w_row : INT32_MIN, top_first = rvalid ? top : INT32_MAX;
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) {
+    w_last = max(w_last, __shfl_xor(w_last, m, kWave));
+    top_first = min(top_first, __shfl_xor(top_first, m, kWave));
+  }
+  w_last = __builtin_amdgcn_readfirstlane(w_last);
+  top_first = __builtin_amdgcn_readfirstlane(top_first);
   bf16x8 qop[D / 16];
   {
     const bf16* qb = a.q + row * a.q_st + (int64_t)h * a.q_sh;
@@ -227,9 +238,13 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void tree_attn_kernel(TreeArgs a) 
         j = (32 * lo + (int)__builtin_ctz(w)) * a.bs + x % hpb * 32;
         at = none ? -2 : l - l0;
       }
-      sHalf[tid] = a.table ? make_int4(j, at, tree_page(a, a.table[(int64_t)b * a.table_stride + j / a.page]),
-                                       j % a.page)
-                           : make_int4(j, at, b, j);
+      const int pg = a.table ? tree_page(a, a.table[(int64_t)b * a.table_stride + j / a.page]) : b;
+      // (a block's second half may lie past the last key as a whole)
+      const int last = (i < n_wi ? jend : ctx) - 1 - j;
+      const int jp = (a.table ? j % a.page : j) + min(last, 0);
+      sHalf[tid] = make_int4(j, at, min(max(last, 0), 31), 0);
+      sOff[tid] = make_longlong2((int64_t)pg * a.k_sb + (int64_t)jp * a.k_st + (int64_t)hk * a.k_sh,
+                                 (int64_t)pg * a.v_sb + (int64_t)jp * a.v_st + (int64_t)hk * a.v_sh);
     }
     if (l1 > l0) {
       // a block's first slot in a row wins: the smallest slot first, then its bias in its place (a
@@ -262,25 +277,27 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void tree_attn_kernel(TreeArgs a) 
     ko[u] = 2u * (uint32_t)(r * a.k_st + k_slot(r, lane & 15) * 8);
     vo[u] = 2u * (uint32_t)(r * a.v_st + v_slot(r, lane & 15) * 8);
   }
-  auto fetch = [&](int x, bool band, bf16* sKn, bf16* sVn) __attribute__((always_inline)) {
+  auto fetch = [&](int x, bf16* sKn, bf16* sVn) __attribute__((always_inline)) {
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
-      const int4 d = sHalf[2 * x + hf];
-      const int pg = __builtin_amdgcn_readfirstlane(d.z);
-      // rows past the last key repeat it (a block's second half may lie past it as a whole)
-      const int last = (band ? jend : ctx) - 1 - __builtin_amdgcn_readfirstlane(d.x);
-      const int jp = __builtin_amdgcn_readfirstlane(d.w) + min(last, 0);
-      const char* kb = (const char*)(a.k + ((int64_t)pg * a.k_sb + (int64_t)jp * a.k_st + (int64_t)hk * a.k_sh));
-      const char* vb = (const char*)(a.v + ((int64_t)pg * a.v_sb + (int64_t)jp * a.v_st + (int64_t)hk * a.v_sh));
+      const int4 o = *(const int4*)&sOff[2 * x + hf];
+      const int last = __builtin_amdgcn_readfirstlane(sHalf[2 * x + hf].z);
+      auto wide = [](int lo, int hi) {
+        return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane(lo) |
+                         (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane(hi) << 32);
+      };
+      const char* kb = (const char*)(a.k + wide(o.x, o.y));
+      const char* vb = (const char*)(a.v + wide(o.z, o.w));
 #pragma unroll
       for (int u = 0; u < 8 / NW; ++u) {
         const int grp = NW * u + wv;
         uint32_t kx = ko[u], vx = vo[u];
         if (last < 31) {
-          const int r = 4 * grp + (lane >> 4), rc = max(min(r, last), 0);
+          const int r = 4 * grp + (lane >> 4), rc = min(r, last);
           kx = 2u * (uint32_t)(rc * a.k_st + k_slot(r, lane & 15) * 8);
           vx = 2u * (uint32_t)(rc * a.v_st + v_slot(r, lane & 15) * 8);
         }
+        asm volatile("" : "+v"(kx), "+v"(vx));    // one load for both: a scalar base, a 32-bit offset
         __builtin_amdgcn_global_load_lds((const void*)(kb + kx),
             (__attribute__((address_space(3))) void*)(sKn + (hf * 32 + grp * 4) * D), 16, 0, 0);
         __builtin_amdgcn_global_load_lds((const void*)(vb + vx),
@@ -291,29 +308,33 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void tree_attn_kernel(TreeArgs a) 
   // the keys of half hf of laid out item x that this lane's row sees, a bit each, and their log2 bias
   auto visible = [&](int x, int hf, float& blog) -> uint32_t {
     const int2 d = *(const int2*)&sHalf[2 * x + hf];
-    const int j = d.x, at = d.y;
+    const int j = __builtin_amdgcn_readfirstlane(d.x), at = __builtin_amdgcn_readfirstlane(d.y);
     blog = 0.f;
-    if (at == -2 || !rvalid) return 0u;
+    if (at == -2) return 0u;
     auto below = [](int y) -> uint32_t { return y >= 32 ? ~0u : y <= 0 ? 0u : (1u << y) - 1u; };
-    if (at == -1) {
-      uint32_t v = below(ctx - j) & ~below(w_row - j);
-      const int m0 = j - ctx;
-      if (m0 > -32) {
-        uint64_t m;
-        if (m0 < 0) {
-          m = mask0 << -m0;
-        } else {
-          const int wd = m0 >> 6, sh = m0 & 63;
-          m = (wd ? a.mask[row * a.words + wd] : mask0) >> sh;
-          if (sh > 32 && wd + 1 < a.words) m |= a.mask[row * a.words + wd + 1] << (64 - sh);
-        }
-        v |= (uint32_t)m & below(jend - j) & ~below(ctx - j);
-      }
-      return v;
+    if (at == -1 && j >= w_last && j + 32 <= ctx) return rvalid ? ~0u : 0u;   // inside every window
+    if (at >= 0) {
+      const uint32_t bits = sBias[at][node - node0];
+      const bool sees = rvalid && bits != kTrNotNamed;
+      blog = sees ? __uint_as_float(bits) : 0.f;
+      if (j + 32 <= top_first) return sees ? ~0u : 0u;
+      return sees ? below(top - j) : 0u;
     }
-    const uint32_t bits = sBias[at][node - node0];
-    blog = __uint_as_float(bits);
-    return bits == kTrNotNamed ? 0u : below(top - j);
+    if (!rvalid) return 0u;
+    uint32_t v = below(ctx - j) & ~below(w_row - j);
+    const int m0 = j - ctx;
+    if (m0 > -32) {
+      uint64_t m;
+      if (m0 < 0) {
+        m = mask0 << -m0;
+      } else {
+        const int wd = m0 >> 6, sh = m0 & 63;
+        m = (wd ? a.mask[row * a.words + wd] : mask0) >> sh;
+        if (sh > 32 && wd + 1 < a.words) m |= a.mask[row * a.words + wd + 1] << (64 - sh);
+      }
+      v |= (uint32_t)m & below(jend - j) & ~below(ctx - j);
+    }
+    return v;
   };
 
   floatx16 acc_o[D / 32];
@@ -344,31 +365,34 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void tree_attn_kernel(TreeArgs a) 
 #pragma unroll
     for (int x = 0; x < NH; ++x) {
       const int hf = KG == 2 ? kg : x;
+      bf16x8 kf[D / 16];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[x][r] = 0.f;
+      for (int kk = 0; kk < D / 16; ++kk) kf[kk] = k_frag_at(sKc, kl0, hf, kk);
+      // two chains: a product need not wait for the one before it
+      floatx16 t;
 #pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk)
-        s[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k_frag_at(sKc, kl0, hf, kk), qop[kk], s[x],
-                                                       0, 0, 0);
-      // a half that every row sees whole or not at all, as inside the band and the blocks: one
-      // minimum with +-inf (which also takes a score that is not a number away)
+      for (int r = 0; r < 16; ++r) { s[x][r] = 0.f; t[r] = 0.f; }
+#pragma unroll
+      for (int kk = 0; kk < D / 16; kk += 2) {
+        s[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kk], qop[kk], s[x], 0, 0, 0);
+        t = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kk + 1], qop[kk + 1], t, 0, 0, 0);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[x][r] += t[r];
       float mraw = -INFINITY;
+      // a half that every row sees whole or not at all, as inside the band and the blocks
       if (__all(vis[x] == 0u || vis[x] == ~0u)) {
-        const float lim = vis[x] ? INFINITY : -INFINITY;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          s[x][r] = fminf(s[x][r], lim);
-          mraw = fmaxf(mraw, s[x][r]);
-        }
+        for (int r = 0; r < 16; ++r) s[x][r] = vis[x] ? s[x][r] : -INFINITY;
       } else {
         const uint32_t vb = vis[x] >> (4 * hl);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
+        for (int r = 0; r < 16; ++r)
           s[x][r] = (vb >> (8 * (r >> 2) + (r & 3))) & 1u ? s[x][r] : -INFINITY;
-          mraw = fmaxf(mraw, s[x][r]);
-        }
       }
-      mloc = fmaxf(mloc, fmaf(mraw, csc, vis[x] ? blog[x] : 0.f));
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mraw = fmaxf(mraw, s[x][r]);
+      mloc = fmaxf(mloc, fmaf(mraw, csc, blog[x]));
     }
     mloc = xor32_max(mloc);
     // the reference moves only when a row's maximum exceeds it by more than 8
@@ -385,23 +409,10 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void tree_attn_kernel(TreeArgs a) 
 #pragma unroll
     for (int x = 0; x < NH; ++x) {
       const int hf = KG == 2 ? kg : x;
-      const float off = (vis[x] ? blog[x] : 0.f) - (m_run == -INFINITY ? 0.f : m_run);
-      bf16x8 ph[2], pl[2];
+      // V in registers before the weights are ready
+      bf16x8 vop[4][2];
 #pragma unroll
-      for (int jj = 0; jj < 2; ++jj) {
-        float p[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) p[e] = fast_exp2(fmaf(s[x][8 * jj + e], csc, off));
-        l_run += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          ph[jj][e] = (bf16)p[e];
-          pl[jj][e] = (bf16)(p[e] - (float)ph[jj][e]);
-        }
-      }
-#pragma unroll
-      for (int dt = 0; dt < 4; ++dt) {
-        bf16x8 vop[2];
+      for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
         for (int jj = 0; jj < 2; ++jj) {
           const char* vp = (const char*)sVc + (32 * hf + 16 * jj) * 256 + (vl0 ^ (uint32_t)(dt << 6));
@@ -412,13 +423,39 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void tree_attn_kernel(TreeArgs a) 
           const bf16x4 l4 = __builtin_bit_cast(bf16x4, lo);
           const bf16x4 h4 = __builtin_bit_cast(bf16x4, hi);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) { vop[jj][e] = l4[e]; vop[jj][e + 4] = h4[e]; }
+          for (int e = 0; e < 4; ++e) { vop[dt][jj][e] = l4[e]; vop[dt][jj][e + 4] = h4[e]; }
         }
+      const float off = blog[x] - (m_run == -INFINITY ? 0.f : m_run);
+      uint32_t ph[2][4], pl[2][4];
 #pragma unroll
-        for (int jj = 0; jj < 2; ++jj) {
-          acc_o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vop[jj], pl[jj], acc_o[dt], 0, 0, 0);
-          acc_o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vop[jj], ph[jj], acc_o[dt], 0, 0, 0);
+      for (int jj = 0; jj < 2; ++jj) {
+        float p[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) p[e] = fast_exp2(fmaf(s[x][8 * jj + e], csc, off));
+        l_run += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+        auto pack = [](float u, float v) {
+          bf16x2 y;
+          y[0] = (bf16)u;
+          y[1] = (bf16)v;
+          return __builtin_bit_cast(uint32_t, y);
+        };
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          ph[jj][e] = pack(p[2 * e], p[2 * e + 1]);
+          pl[jj][e] = pack(p[2 * e] - __uint_as_float(ph[jj][e] << 16),
+                           p[2 * e + 1] - __uint_as_float(ph[jj][e] & 0xffff0000u));
         }
+      }
+#pragma unroll
+      for (int jj = 0; jj < 2; ++jj) {
+        const bf16x8 lo = __builtin_bit_cast(bf16x8, *(uint4*)pl[jj]);
+        const bf16x8 hi = __builtin_bit_cast(bf16x8, *(uint4*)ph[jj]);
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt)
+          acc_o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vop[dt][jj], lo, acc_o[dt], 0, 0, 0);
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt)
+          acc_o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vop[dt][jj], hi, acc_o[dt], 0, 0, 0);
       }
     }
   };
@@ -432,19 +469,19 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void tree_attn_kernel(TreeArgs a) 
     if (ST == 1) {
       for (int i = c0; i < c1; ++i) {
         if (i > c0) __syncthreads();      // every wavefront left item i - 1
-        fetch(i - c0, i < n_wi, sK0, sV0);
+        fetch(i - c0, sK0, sV0);
         __builtin_amdgcn_s_waitcnt(0);
         __syncthreads();                  // item i landed
         item(i - c0, sK0, sV0, vis);
       }
       continue;
     }
-    fetch(0, c0 < n_wi, sK0, sV0);
+    fetch(0, sK0, sV0);
     auto step = [&](int i, auto par) __attribute__((always_inline)) {
       constexpr int P = decltype(par)::value;
       __builtin_amdgcn_s_waitcnt(0);
       __syncthreads();                    // item i landed; every wavefront left item i - 1
-      if (i + 1 < c1) fetch(i + 1 - c0, i + 1 < n_wi, P ? sK0 : sK1, P ? sV0 : sV1);
+      if (i + 1 < c1) fetch(i + 1 - c0, P ? sK0 : sK1, P ? sV0 : sV1);
       item(i - c0, P ? sK1 : sK0, P ? sV1 : sV0, vis);
     };
     for (int i = c0; i < c1; i += 2) {
@@ -469,7 +506,7 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void tree_attn_kernel(TreeArgs a) 
         lay_out(i, min(i + CH, i_last));
       }
       __syncthreads();                    // every wavefront left the stage
-      fetch(x0, i < n_wi, sK0, sV0);
+      fetch(x0, sK0, sV0);
       __builtin_amdgcn_s_waitcnt(0);
       // each wavefront clears the rows it loaded; bit 8 hf + u: its group u of half hf holds some
       uint32_t bad = 0;
@@ -496,17 +533,15 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void tree_attn_kernel(TreeArgs a) 
 #pragma unroll
       for (int y = 0; y < NH; ++y) {
         const int hf = KG == 2 ? kg : y;
-        const int4 d = sHalf[2 * x0 + hf];
-        const int j = d.x;
-        const int last = (i < n_wi ? jend : ctx) - 1;
+        const int last = sHalf[2 * x0 + hf].z;
+        const bf16* vh = a.v + sOff[2 * x0 + hf].y + 4 * hl;
         for (int w = 0; w < NW; ++w)
           for (uint32_t todo = (sBad[w] >> (8 * hf)) & 0xffu; todo; todo &= todo - 1)
             for (int q4 = 0; q4 < 4; ++q4) {
               const int r = 4 * (NW * __builtin_ctz(todo) + w) + q4;
-              if (j + r > last) continue;          // a repeated row
+              if (r > last) continue;              // a repeated row
               const bool sees = (vis[y] >> r) & 1u;
-              const int64_t vr = (int64_t)d.z * a.v_sb + (int64_t)(d.w + r) * a.v_st;
-              const bf16* vp = a.v + vr + (int64_t)hk * a.v_sh + 4 * hl;
+              const bf16* vp = vh + (int64_t)r * a.v_st;
 #pragma unroll
               for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
