@@ -210,6 +210,11 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void tree_attn_kernel(TreeArgs a) 
   const int n_items = n_wi + (n_blocks * hpb + 1) / 2;
   const int i_first = (int)((int64_t)n_items * split / a.nsplit);
   const int i_last = (int)((int64_t)n_items * (split + 1) / a.nsplit);
+  if (i_first == i_last && a.nsplit > 1) {         // nothing for this split: no partial to read
+    if (kg == 0 && hl == 0 && rvalid)
+      a.part_ml[(row * a.H + h) * a.nsplit + split] = make_float2(-INFINITY, 0.f);
+    return;
+  }
 
   // Lays out items c0 .. c1 - 1 (at most CH): every wavefront has left the items before.
   auto lay_out = [&](int c0, int c1) {
@@ -677,7 +682,9 @@ inline TreePlan tree_plan(int B, int H, int Hkv, int max_n, int K, int S, int bs
   p.groups = (int)((rows + 32 * p.rt - 1) / (32 * p.rt));
   const int64_t nodes = std::min<int64_t>(max_n, (32 * p.rt - 1) / (H / Hkv) + 2);
   p.nodes = (int)nodes;                   // at most, of a row group
-  const int64_t blocks = std::min<int64_t>((S + bs - 1) / bs, nodes * K);
+  // the nodes of a tree name much the same blocks: splits for four times a row's (where they name
+  // more, a split takes more items)
+  const int64_t blocks = std::min<int64_t>({(S + bs - 1) / bs, nodes * K, 4 * K});
   const int64_t items = (std::min<int64_t>(S, (int64_t)lw + max_n) + 95) / 64 + (blocks * (bs / 32) + 1) / 2;
   const int64_t streams = std::max<int64_t>(1, (int64_t)B * Hkv * p.groups);
   p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({64, items, kTrTarget / streams}));

@@ -145,20 +145,21 @@ def attn_tree(q, k, v, idx, bias, valid, mask, depth, context_lens, cu_seqlens_q
         out = torch.empty(T, H, D, dtype=out_dtype, device=q.device)
         lse = torch.empty(T, H, dtype=torch.float32, device=q.device) if return_lse else None
         if T:
+            qs, os, (ks, k1, k2, _), (vs, v1, v2, _) = (x.stride() for x in (q, out, k, v))
             if paged:
                 S, pages = bt.shape[1] * k.shape[1], k.shape[0]
-                kh, kt, vh, vt = k.stride(2), k.stride(1), v.stride(2), v.stride(1)
+                kh, kt, vh, vt = k2, k1, v2, v1
             else:
                 S, pages = k.shape[2], 0
-                kh, kt, vh, vt = k.stride(1), k.stride(2), v.stride(1), v.stride(2)
+                kh, kt, vh, vt = k1, k2, v1, v2
             nbytes = _attn_workspace(B, H, Hkv, T, n, K, S, int(block_size), int(local_window))
             ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
             _lib.check(lib.dash_attn_tree(
-                _ptr(q), q.stride(0), q.stride(1), _ptr(k), k.stride(0), kh, kt, _ptr(v),
-                v.stride(0), vh, vt, _ptr(bt), 0 if bt is None else bt.stride(0),
-                int(page_size or 0), pages, _ptr(ctx), _ptr(cu), _ptr(idx_c), _ptr(valid_c),
-                _ptr(bias_c), K, _ptr(mask), mask.shape[1], _ptr(dep), _ptr(out),
-                int(out_dtype == torch.bfloat16), out.stride(0), out.stride(1), _ptr(lse),
+                q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks, kh, kt, v.data_ptr(), vs, vh, vt,
+                _ptr(bt), 0 if bt is None else bt.stride(0), int(page_size or 0), pages,
+                ctx.data_ptr(), cu.data_ptr(), _ptr(idx_c), _ptr(valid_c), _ptr(bias_c), K,
+                mask.data_ptr(), mask.shape[1], dep.data_ptr(), out.data_ptr(),
+                int(out_dtype == torch.bfloat16), os[0], os[1], _ptr(lse),
                 0 if lse is None else lse.stride(0), 1, B, H, Hkv, T, n, S, D, int(block_size),
                 int(local_window), float(scale), _ptr(ws), nbytes, _stream()),
                 "dash_attn_tree")
