@@ -21,63 +21,65 @@ constexpr int kKvMaxRows = 8192;      // rows of a table (prefix sums in LDS)
 constexpr int kKvMaxCaches = 32;      // caches per launch (kernel argument space)
 
 // One cache: page p of layer l starts at base + l * layer + p * page bytes; a page holds
-// n1 x n2 pieces of seg bytes at strides s1 and s2.  For rows, s1 is the stride of a token.
+// n1 x n2 pieces of seg bytes at strides s1 and s2.  For rows, s1 is the stride of a token and a row
+// holds n2 pieces.
 struct KvCache {
   char* base;
   int64_t layer, page, s1, s2;
-  int32_t layers, n1, n2, seg;
+  int64_t units;                      // of a layer's page (or row)
+  int32_t n2, segu;                   // segu: units of a piece (0: the page, or row, in one piece)
+  int32_t per;                        // tasks of a layer's page (or row)
+  int32_t task0;                      // first task of the cache
 };
 struct KvCaches {
   KvCache c[kKvMaxCaches];
-  int32_t task0[kKvMaxCaches + 1];    // first task of each cache
   int n;
 };
 
 // The cache that task t belongs to.
-__device__ __forceinline__ int kv_cache_of(const KvCaches& a, int t) {
+__device__ __forceinline__ const KvCache& kv_cache_of(const KvCaches& a, int t) {
   int i = 0;
-  while (i + 1 < a.n && t >= a.task0[i + 1]) ++i;
-  return i;
+  while (i + 1 < a.n && t >= a.c[i + 1].task0) ++i;
+  return a.c[i];
 }
 
+typedef uint32_t KvVec __attribute__((ext_vector_type(4)));   // 16 bytes
 constexpr int kCpThreads = 256, kCpUnroll = 4;
 
-// One work-group per (pair, task); a task is kCpThreads * kCpUnroll units of one layer's page.
+// One work-group per (pair, task); a task is kCpThreads * kCpUnroll units of one layer's page.  Bound
+// by HBM: 730 MB read and written in 137 us, 5.3 TB/s; 149 us where the loads and stores leave their
+// lines in the L2 (a page is not read again here), 225 with eight units a lane in flight instead of four.
 template <typename U>
 __global__ __launch_bounds__(kCpThreads) void copy_pages_kernel(KvCaches a, const int32_t* frm,
-                                                                const int32_t* to, int num_pages) {
-  const int tasks = a.task0[a.n];
+                                                                const int32_t* to, int num_pages,
+                                                                int tasks) {
   const int pair = blockIdx.x / tasks, t = blockIdx.x % tasks;
   const int f = frm[pair], d = to[pair];
   if (f < 0 || d < 0 || f >= num_pages || d >= num_pages || f == d) return;
-  const int i = kv_cache_of(a, t);
-  const KvCache& c = a.c[i];
-  const int per = (int)(((int64_t)c.n1 * c.n2 * c.seg / (int)sizeof(U) + kCpThreads * kCpUnroll - 1) /
-                        (kCpThreads * kCpUnroll));
-  const int rel = t - a.task0[i];
-  const int l = rel / per, ch = rel % per;
+  const KvCache& c = kv_cache_of(a, t);
+  const int rel = t - c.task0;
+  const int l = rel / c.per, ch = rel % c.per;
   char* const lb = c.base + l * c.layer;
   const char* const sp = lb + f * c.page;
   char* const dp = lb + d * c.page;
-  const int segu = c.seg / (int)sizeof(U);
-  const int64_t units = (int64_t)c.n1 * c.n2 * segu;
+  const int64_t units = c.units;
   const int64_t u0 = (int64_t)ch * (kCpThreads * kCpUnroll) + threadIdx.x;
   U x[kCpUnroll];
   int64_t off[kCpUnroll];
 #pragma unroll
   for (int k = 0; k < kCpUnroll; ++k) {
     const int64_t u = u0 + k * kCpThreads;
-    if (c.n1 == 1 && c.n2 == 1) {
+    if (c.segu == 0) {
       off[k] = u * (int)sizeof(U);
     } else {
-      const int64_t piece = u / segu;
-      off[k] = (piece / c.n2) * c.s1 + (piece % c.n2) * c.s2 + (u - piece * segu) * (int)sizeof(U);
+      const int64_t piece = u / c.segu;
+      off[k] = (piece / c.n2) * c.s1 + (piece % c.n2) * c.s2 + (u - piece * c.segu) * (int)sizeof(U);
     }
-    if (u < units) x[k] = *(const U*)(sp + off[k]);
+    if (u < units) x[k] = __builtin_nontemporal_load((const U*)(sp + off[k]));
   }
 #pragma unroll
   for (int k = 0; k < kCpUnroll; ++k)
-    if (u0 + k * kCpThreads < units) *(U*)(dp + off[k]) = x[k];
+    if (u0 + k * kCpThreads < units) __builtin_nontemporal_store(x[k], (U*)(dp + off[k]));
 }
 
 // Rows ctx + path[i] -> ctx + i, 1 <= i < count, of one sequence and one unit column of one
@@ -95,15 +97,13 @@ __global__ __launch_bounds__(kWave) void keep_rows_kernel(KvCaches a, const int3
   const int n = min(count[b], max_n);
   const int c0 = ctx[b];
   if (n <= 0 || c0 < 0) return;
-  const int i0 = kv_cache_of(a, blockIdx.x);
-  const KvCache& c = a.c[i0];
-  const int segu = c.seg / (int)sizeof(U);
-  const int units = c.n2 * segu;
-  const int per = (units + kWave - 1) / kWave;
-  const int rel = blockIdx.x - a.task0[i0];
-  const int l = rel / per, u = (rel % per) * kWave + lane;
+  const KvCache& c = kv_cache_of(a, blockIdx.x);
+  const int units = (int)c.units;
+  const int rel = blockIdx.x - c.task0;
+  const int l = rel / c.per, u = (rel % c.per) * kWave + lane;
   char* const lb = c.base + l * c.layer;
-  const int64_t col = (int64_t)(u / segu) * c.s2 + (int64_t)(u % segu) * (int)sizeof(U);
+  const int64_t col = c.segu == 0 ? (int64_t)u * (int)sizeof(U)
+                                  : (int64_t)(u / c.segu) * c.s2 + (int64_t)(u % c.segu) * (int)sizeof(U);
   const int32_t* tr = table + (int64_t)b * table_st;
   // byte offset of a slot's row in this layer, -1 where there is none
   auto row_of = [&](int64_t s) -> int64_t {
@@ -430,19 +430,6 @@ static int kv_status() {
   return e == hipSuccess ? kOk : (int)e;
 }
 
-// The kernel of the unit's size: 16 bytes where every address and size allows it, else the
-// largest that does.
-template <typename K16, typename K4, typename K2, typename K1, typename... Args>
-static int kv_launch(int unit, K16 k16, K4 k4, K2 k2, K1 k1, dim3 grid, dim3 block, void* stream,
-                     Args... args) {
-  hipStream_t st = (hipStream_t)stream;
-  if (unit == 16) hipLaunchKernelGGL(k16, grid, block, 0, st, args...);
-  else if (unit == 4) hipLaunchKernelGGL(k4, grid, block, 0, st, args...);
-  else if (unit == 2) hipLaunchKernelGGL(k2, grid, block, 0, st, args...);
-  else hipLaunchKernelGGL(k1, grid, block, 0, st, args...);
-  return kv_status();
-}
-
 // The caches of one launch: descriptors first .. first + n - 1 of desc [.., 8] (layers, layer
 // stride, page stride, n1, s1, n2, s2, seg; bytes), tasks of `task_units` units of a layer's page
 // (or row).  Returns the unit's bytes, 0 if a number does not fit.
@@ -462,18 +449,63 @@ static int kv_fill(KvCaches& a, void* const* base, const int64_t* desc, int n, b
     if (!base[i] || d[0] < 0 || d[3] < 1 || d[5] < 1 || d[7] < 1 || d[0] > INT32_MAX ||
         d[3] > INT32_MAX || d[5] > INT32_MAX || d[7] > INT32_MAX || d[1] < 0 || d[2] < 0)
       return 0;
-    a.c[i] = KvCache{(char*)base[i], d[1], d[2], d[4], d[6], (int)d[0], (int)d[3], (int)d[5],
-                     (int)d[7]};
-    a.task0[i] = (int)t;
-    const int64_t units = (rows ? 1 : d[3]) * d[5] * (d[7] / unit);
-    if (d[5] * (d[7] / unit) > INT32_MAX - 64) return 0;
-    t += d[0] * ((units + task_units - 1) / task_units);
+    const int64_t pieces = (rows ? 1 : d[3]) * d[5], segu = d[7] / unit, units = pieces * segu;
+    const int64_t per = (units + task_units - 1) / task_units;
+    if (d[5] * segu > INT32_MAX - 64 || per > INT32_MAX) return 0;
+    a.c[i] = KvCache{(char*)base[i], d[1], d[2], d[4], d[6], units, (int)d[5],
+                     pieces == 1 ? 0 : (int)segu, (int)per, (int)t};
+    t += d[0] * per;
     if (t > INT32_MAX) return 0;
   }
-  a.task0[n] = (int)t;
   *tasks = t;
   return unit;
 }
+
+// Launches Op over (tasks, count) of the caches, 32 at a time: units of 16 bytes where every address
+// and size allows it, else the largest that does.
+template <template <typename> class Op, typename... Args>
+static int kv_launches(void* const* base, const int64_t* desc, int num, int64_t count, void* stream,
+                       Args... args) {
+  hipStream_t st = (hipStream_t)stream;
+  for (int c0 = 0; c0 < num; c0 += kKvMaxCaches) {
+    KvCaches a;
+    int64_t tasks = 0;
+    const int unit = kv_fill(a, base + c0, desc + 8 * c0, std::min(kKvMaxCaches, num - c0), Op<KvVec>::kRows,
+                             Op<KvVec>::kTask, &tasks);
+    if (unit == 0) return kErrInvalid;
+    if (tasks == 0) continue;
+    if (tasks * count > INT32_MAX) return kErrUnsupported;
+    if (unit == 16) Op<KvVec>::launch(a, tasks, count, st, args...);
+    else if (unit == 4) Op<uint32_t>::launch(a, tasks, count, st, args...);
+    else if (unit == 2) Op<uint16_t>::launch(a, tasks, count, st, args...);
+    else Op<uint8_t>::launch(a, tasks, count, st, args...);
+    const int s = kv_status();
+    if (s != kOk) return s;
+  }
+  return kOk;
+}
+
+template <typename U>
+struct CopyOp {
+  static constexpr bool kRows = false;
+  static constexpr int kTask = kCpThreads * kCpUnroll;
+  static void launch(const KvCaches& a, int64_t tasks, int64_t pairs, hipStream_t st, const int32_t* frm,
+                     const int32_t* to, int num_pages) {
+    hipLaunchKernelGGL(copy_pages_kernel<U>, dim3((unsigned)(tasks * pairs)), dim3(kCpThreads), 0, st, a,
+                       frm, to, num_pages, (int)tasks);
+  }
+};
+template <typename U>
+struct KeepOp {
+  static constexpr bool kRows = true;
+  static constexpr int kTask = kWave;
+  static void launch(const KvCaches& a, int64_t tasks, int64_t B, hipStream_t st, const int32_t* path,
+                     int64_t path_st, const int32_t* count, const int32_t* ctx, const int32_t* table,
+                     int64_t table_st, int P, int page, int num_pages, int max_n) {
+    hipLaunchKernelGGL(keep_rows_kernel<U>, dim3((unsigned)tasks, (unsigned)B), dim3(kWave), 0, st, a,
+                       path, path_st, count, ctx, table, table_st, P, page, num_pages, max_n);
+  }
+};
 
 }  // namespace dash
 
@@ -484,21 +516,7 @@ extern "C" int dash_copy_pages(int num_caches, void* const* caches, const int64_
   if (num_caches < 0 || num_pairs < 0 || num_pages < 0) return kErrInvalid;
   if (num_caches == 0 || num_pairs == 0 || num_pages == 0) return kOk;
   if (!caches || !desc || !from_pages || !to_pages) return kErrInvalid;
-  for (int c0 = 0; c0 < num_caches; c0 += kKvMaxCaches) {
-    KvCaches a;
-    int64_t tasks = 0;
-    const int n = std::min(kKvMaxCaches, num_caches - c0);
-    const int unit = kv_fill(a, caches + c0, desc + 8 * c0, n, false, kCpThreads * kCpUnroll, &tasks);
-    if (unit == 0) return kErrInvalid;
-    if (tasks == 0) continue;
-    if (tasks * num_pairs > INT32_MAX) return kErrUnsupported;
-    const int s = kv_launch(unit, copy_pages_kernel<uint4>, copy_pages_kernel<uint32_t>,
-                            copy_pages_kernel<uint16_t>, copy_pages_kernel<uint8_t>,
-                            dim3((unsigned)(tasks * num_pairs)), dim3(kCpThreads), stream, a,
-                            from_pages, to_pages, num_pages);
-    if (s != kOk) return s;
-  }
-  return kOk;
+  return kv_launches<CopyOp>(caches, desc, num_caches, num_pairs, stream, from_pages, to_pages, num_pages);
 }
 
 extern "C" int dash_keep_rows(int num_caches, void* const* caches, const int64_t* desc,
@@ -512,21 +530,9 @@ extern "C" int dash_keep_rows(int num_caches, void* const* caches, const int64_t
   if (num_caches == 0 || B == 0 || P == 0 || num_pages == 0 || max_query_len == 0) return kOk;
   if (!caches || !desc || !path || !count || !context_lens || !block_table) return kErrInvalid;
   if (B > 65535) return kErrUnsupported;
-  for (int c0 = 0; c0 < num_caches; c0 += kKvMaxCaches) {
-    KvCaches a;
-    int64_t tasks = 0;
-    const int n = std::min(kKvMaxCaches, num_caches - c0);
-    const int unit = kv_fill(a, caches + c0, desc + 8 * c0, n, true, kWave, &tasks);
-    if (unit == 0) return kErrInvalid;
-    if (tasks == 0) continue;
-    const int s = kv_launch(unit, keep_rows_kernel<uint4>, keep_rows_kernel<uint32_t>,
-                            keep_rows_kernel<uint16_t>, keep_rows_kernel<uint8_t>,
-                            dim3((unsigned)tasks, B), dim3(kWave), stream, a, path, path_stride,
-                            count, context_lens, block_table, table_stride, P, page_size, num_pages,
-                            max_query_len);
-    if (s != kOk) return s;
-  }
-  return kOk;
+  return kv_launches<KeepOp>(caches, desc, num_caches, B, stream, path, path_stride, count,
+                             context_lens, block_table, table_stride, P, page_size, num_pages,
+                             max_query_len);
 }
 
 extern "C" int dash_fork_pages(int32_t* refs, int num_pages, int32_t* block_table,
