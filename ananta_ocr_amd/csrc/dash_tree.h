@@ -82,14 +82,16 @@ __global__ __launch_bounds__(kTrMaxNodes) void tree_masks_kernel(const int32_t* 
 // RT row tiles of 32 rows are the columns of S^T = K Q^T (v_mfma_f32_32x32x16_bf16); with KG = 2
 // two wavefronts share a row tile, one half of every item each, and meet at the end.  A half's
 // visible keys are 32 bits per row, so the band's edges, the drafted keys' mask and the routed
-// blocks of rows that do not name them are one test.  A weight enters the second product as two
-// bf16 parts: it is off by at most 2^-17 of itself (16 bits and their rounding), which moves an output
-// by less than 8e-6 of the largest |v|, and by 1e-6 as roundings of either sign add up; a third part,
-// as in the extend kernels, costs a third of the matrix work and a quarter of the vector work.
+// blocks of rows that do not name them are one test.  A weight enters the second product as three
+// bf16 parts (24 bits: it is not rounded) where the output is fp32, as in the extend kernels, and as
+// two where it is bf16: a weight is then off by at most 2^-17 of itself, an output by less than 8e-6 of
+// the largest |v|, against the 2^-8 of its own value that its type costs.  The third part is a third of
+// the matrix work and a quarter of the vector work, which an item's loads hide in all but the largest
+// batches (32 trees of 24 to 64 nodes over 27,300 tokens: 131 us with three parts, 124 with two).
 // ---------------------------------------------------------------------------
 constexpr uint32_t kTrNotNamed = 0xffffffffu;
 
-template <int RT, int KG>
+template <int RT, int KG, int PARTS>
 __global__ __launch_bounds__(64 * RT * KG, 2) void tree_attn_kernel(TreeArgs a) {
   constexpr int D = 128, NW = RT * KG, TH = 64 * NW;
   constexpr int NH = 2 / KG;              // halves of an item that a wavefront takes
@@ -282,6 +284,9 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void tree_attn_kernel(TreeArgs a) 
     ko[u] = 2u * (uint32_t)(r * a.k_st + k_slot(r, lane & 15) * 8);
     vo[u] = 2u * (uint32_t)(r * a.v_st + v_slot(r, lane & 15) * 8);
   }
+  // Up to 64 rows every key is read once: non-temporal (tree_b32_n64 131 -> 125 us); more rows are
+  // several work-groups, which share the lines in the L2.
+  constexpr int kAux = RT == 4 ? 0 : 2;
   auto fetch = [&](int x, bf16* sKn, bf16* sVn) __attribute__((always_inline)) {
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
@@ -304,9 +309,9 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void tree_attn_kernel(TreeArgs a) 
         }
         asm volatile("" : "+v"(kx), "+v"(vx));    // one load for both: a scalar base, a 32-bit offset
         __builtin_amdgcn_global_load_lds((const void*)(kb + kx),
-            (__attribute__((address_space(3))) void*)(sKn + (hf * 32 + grp * 4) * D), 16, 0, 0);
+            (__attribute__((address_space(3))) void*)(sKn + (hf * 32 + grp * 4) * D), 16, 0, kAux);
         __builtin_amdgcn_global_load_lds((const void*)(vb + vx),
-            (__attribute__((address_space(3))) void*)(sVn + (hf * 32 + grp * 4) * D), 16, 0, 0);
+            (__attribute__((address_space(3))) void*)(sVn + (hf * 32 + grp * 4) * D), 16, 0, kAux);
       }
     }
   };
@@ -431,37 +436,35 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void tree_attn_kernel(TreeArgs a) 
           for (int e = 0; e < 4; ++e) { vop[dt][jj][e] = l4[e]; vop[dt][jj][e + 4] = h4[e]; }
         }
       const float off = blog[x] - (m_run == -INFINITY ? 0.f : m_run);
-      uint32_t ph[2][4], pl[2][4];
+      uint32_t part[PARTS][2][4];
 #pragma unroll
       for (int jj = 0; jj < 2; ++jj) {
         float p[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) p[e] = fast_exp2(fmaf(s[x][8 * jj + e], csc, off));
         l_run += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-        auto pack = [](float u, float v) {
-          bf16x2 y;
-          y[0] = (bf16)u;
-          y[1] = (bf16)v;
-          return __builtin_bit_cast(uint32_t, y);
-        };
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          ph[jj][e] = pack(p[2 * e], p[2 * e + 1]);
-          pl[jj][e] = pack(p[2 * e] - __uint_as_float(ph[jj][e] << 16),
-                           p[2 * e + 1] - __uint_as_float(ph[jj][e] & 0xffff0000u));
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int i = 0; i < PARTS; ++i) {
+            bf16x2 y;
+            y[0] = (bf16)p[2 * e];
+            y[1] = (bf16)p[2 * e + 1];
+            const uint32_t w = __builtin_bit_cast(uint32_t, y);
+            part[i][jj][e] = w;
+            p[2 * e] -= __uint_as_float(w << 16);
+            p[2 * e + 1] -= __uint_as_float(w & 0xffff0000u);
+          }
+      }
+#pragma unroll
+      for (int jj = 0; jj < 2; ++jj)
+#pragma unroll
+        for (int i = PARTS - 1; i >= 0; --i) {       // smallest parts first
+          const bf16x8 w = __builtin_bit_cast(bf16x8, *(uint4*)part[i][jj]);
+#pragma unroll
+          for (int dt = 0; dt < 4; ++dt)
+            acc_o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vop[dt][jj], w, acc_o[dt], 0, 0, 0);
         }
-      }
-#pragma unroll
-      for (int jj = 0; jj < 2; ++jj) {
-        const bf16x8 lo = __builtin_bit_cast(bf16x8, *(uint4*)pl[jj]);
-        const bf16x8 hi = __builtin_bit_cast(bf16x8, *(uint4*)ph[jj]);
-#pragma unroll
-        for (int dt = 0; dt < 4; ++dt)
-          acc_o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vop[dt][jj], lo, acc_o[dt], 0, 0, 0);
-#pragma unroll
-        for (int dt = 0; dt < 4; ++dt)
-          acc_o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vop[dt][jj], hi, acc_o[dt], 0, 0, 0);
-      }
     }
   };
 
@@ -779,12 +782,17 @@ extern "C" int dash_attn_tree(
   hipStream_t st = (hipStream_t)stream;
   a.slot_cap = p.nodes * K;
   const unsigned lds = (unsigned)((a.slot_cap * (p.rt == 4 ? 2 : 6) + 15) / 16 * 16);
-  if (p.rt == 1)
-    hipLaunchKernelGGL((tree_attn_kernel<1, 2>), dim3((unsigned)wgs), dim3(128), lds, st, a);
-  else if (p.rt == 2)
-    hipLaunchKernelGGL((tree_attn_kernel<2, 2>), dim3((unsigned)wgs), dim3(256), lds, st, a);
-  else
-    hipLaunchKernelGGL((tree_attn_kernel<4, 1>), dim3((unsigned)wgs), dim3(256), lds, st, a);
+  const dim3 grid((unsigned)wgs);
+  if (p.rt == 1) {
+    auto kern = out_bf16 ? tree_attn_kernel<1, 2, 2> : tree_attn_kernel<1, 2, 3>;
+    hipLaunchKernelGGL(kern, grid, dim3(128), lds, st, a);
+  } else if (p.rt == 2) {
+    auto kern = out_bf16 ? tree_attn_kernel<2, 2, 2> : tree_attn_kernel<2, 2, 3>;
+    hipLaunchKernelGGL(kern, grid, dim3(256), lds, st, a);
+  } else {
+    auto kern = out_bf16 ? tree_attn_kernel<4, 1, 2> : tree_attn_kernel<4, 1, 3>;
+    hipLaunchKernelGGL(kern, grid, dim3(256), lds, st, a);
+  }
   if (p.nsplit > 1)
     hipLaunchKernelGGL(tree_merge_kernel, dim3((unsigned)((T * H + 3) / 4)), dim3(256), 0, st, a);
   const hipError_t e = hipGetLastError();
