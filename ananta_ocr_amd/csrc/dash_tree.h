@@ -45,13 +45,13 @@ __device__ __forceinline__ int tree_page(const TreeArgs& a, int p) {
 // The masks and depths of the trees: one work-group per sequence, one lane per node, which
 // climbs to the root (parents come before their children, so it ends).
 __global__ __launch_bounds__(kTrMaxNodes) void tree_masks_kernel(const int32_t* parents,
-                                                                 const int32_t* cu, int words,
-                                                                 int max_n, uint64_t* mask,
+                                                                 const int32_t* cu, int64_t T,
+                                                                 int words, int max_n, uint64_t* mask,
                                                                  int32_t* depth) {
   __shared__ int sPar[kTrMaxNodes];
   const int b = blockIdx.x, i = threadIdx.x;
-  const int64_t r0 = cu[b];
-  const int n = min((int)(cu[b + 1] - r0), max_n);
+  int64_t r0;
+  const int n = packed_rows(cu, b, T, max_n, r0);
   if (i < n) {
     const int p = parents[r0 + i];
     sPar[i] = p >= 0 && p < i ? p : -1;
@@ -125,9 +125,9 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void tree_attn_kernel(TreeArgs a) 
   const int split = id % a.nsplit; id /= a.nsplit;
   const int rg = id % a.groups, b = id / a.groups;
   const int G = a.H / a.Hkv;
-  const int64_t r0 = a.cu[b];
+  int64_t r0;
+  const int nn = packed_rows(a.cu, b, a.T, a.max_n, r0);  // nodes
   const int ctx = tree_ctx(a, b);
-  const int nn = min((int)(a.cu[b + 1] - r0), a.max_n);   // nodes
   const int n = min(nn, a.S - ctx);                       // with a slot in the cache
   const int R = nn * G, rb = rg * RT * 32;
   if (rb >= R) return;
@@ -708,7 +708,7 @@ extern "C" int dash_tree_masks(const int32_t* parents, const int32_t* cu_seqlens
   if (!parents || !cu_seqlens_q || !mask || !depth || max_query_len == 0) return kErrInvalid;
   if (max_query_len > kTrMaxNodes || words != (max_query_len + 63) / 64) return kErrUnsupported;
   hipLaunchKernelGGL(tree_masks_kernel, dim3(B), dim3(kTrMaxNodes), 0, (hipStream_t)stream, parents,
-                     cu_seqlens_q, words, max_query_len, (uint64_t*)mask, depth);
+                     cu_seqlens_q, T, words, max_query_len, (uint64_t*)mask, depth);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? kOk : (int)e;
 }

@@ -139,8 +139,8 @@ __global__ __launch_bounds__(THREADS) void verify_walk_kernel(VerifyArgs a) {
   __shared__ int sPath[kVfMaxNodes];
   __shared__ double sD[THREADS / kWave];
   const int b = blockIdx.x, tid = threadIdx.x, lane = wave_lane();
-  const int64_t r0 = a.cu[b];
-  const int n = min((int)(a.cu[b + 1] - r0), a.max_n);
+  int64_t r0;
+  const int n = packed_rows(a.cu, b, a.T, a.max_n, r0);
   if (n <= 0) {
     for (int i = tid; i < a.max_n; i += THREADS) a.path[b * a.path_st + i] = -1;
     if (tid == 0) { a.count[b] = 0; a.token[b] = -1; if (MODE != 0) a.stop[b] = -1; }
@@ -366,8 +366,8 @@ __global__ __launch_bounds__(kVfThreads) void verify_draw_kernel(VerifyArgs a) {
   __shared__ double sBase;
   __shared__ int sTurn;
   const int b = blockIdx.y, tid = threadIdx.x;
-  const int64_t r0 = a.cu[b];
-  const int n = min((int)(a.cu[b + 1] - r0), a.max_n);
+  int64_t r0;
+  const int n = packed_rows(a.cu, b, a.T, a.max_n, r0);
   const int s = a.stop[b];
   if (s < 0) return;
   const int64_t row = r0 + s;
@@ -542,7 +542,7 @@ extern "C" int dash_verify_tree(const void* target, int64_t target_stride, const
   if (T > 0 && (!target || !tokens || !parents)) return kErrInvalid;
   if (max_query_len > 0 && !path) return kErrInvalid;
   if (draft && !uniforms) return kErrInvalid;
-  if (max_query_len > kVfMaxNodes || B > 65535) return kErrUnsupported;
+  if (max_query_len > kVfMaxNodes || B > 65535 || V > (1 << 30)) return kErrUnsupported;
   const VerifyLayout L = verify_layout(B, T, V, !uniforms);
   if (T * L.chunks > INT32_MAX) return kErrUnsupported;
   if (!workspace || workspace_bytes < L.total || (uintptr_t)workspace % 256 != 0) return kErrWorkspace;

@@ -5,7 +5,9 @@ The nodes of the sequences are packed: rows cu_seqlens_q[b] .. cu_seqlens_q[b + 
 nodes of sequence b, node 0 its root (the newest sampled token, whose key and value are not
 committed yet), and ``parents`` holds each node's parent within its sequence, an earlier node.
 The key and value of node i are written to the cache at slot context_len + i before the
-attention.  ``pipeline.tree_step`` and ``pipeline.commit_tree`` are the whole step.
+attention.  max_query_len is at least the largest tree; rows that no tree has (a batch padded to a
+fixed size) come out with nothing in particular.  ``pipeline.tree_step`` and
+``pipeline.commit_tree`` are the whole step.
 
 Like the other wrappers these take tensors of one GPU, allocate their outputs with torch, call one
 C entry point on the current stream, and synchronise nothing.
@@ -152,7 +154,8 @@ def attn_tree(q, k, v, idx, bias, valid, mask, depth, context_lens, cu_seqlens_q
             else:
                 S, pages = k.shape[2], 0
                 kh, kt, vh, vt = k1, k2, v1, v2
-            nbytes = _attn_workspace(B, H, Hkv, T, n, K, S, int(block_size), int(local_window))
+            lw = min(int(local_window), 1 << 30)      # (past every position it is the same window)
+            nbytes = _attn_workspace(B, H, Hkv, T, n, K, S, int(block_size), lw)
             ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
             _lib.check(lib.dash_attn_tree(
                 q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks, kh, kt, v.data_ptr(), vs, vh, vt,
@@ -161,7 +164,7 @@ def attn_tree(q, k, v, idx, bias, valid, mask, depth, context_lens, cu_seqlens_q
                 mask.data_ptr(), mask.shape[1], dep.data_ptr(), out.data_ptr(),
                 int(out_dtype == torch.bfloat16), os[0], os[1], _ptr(lse),
                 0 if lse is None else lse.stride(0), 1, B, H, Hkv, T, n, S, D, int(block_size),
-                int(local_window), float(scale), _ptr(ws), nbytes, _stream()),
+                lw, float(scale), _ptr(ws), nbytes, _stream()),
                 "dash_attn_tree")
     return (out, lse) if return_lse else out
 

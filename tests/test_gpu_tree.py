@@ -323,3 +323,42 @@ def test_graph_streams_and_repeats():
             got = call(other)
         torch.cuda.synchronize()
         assert torch.equal(out, want[i % 2]) and torch.equal(got, want[2])
+
+
+def test_batches_padded_to_a_fixed_size():
+    """Rows past the last tree, and prefix sums past the rows: the trees' rows as without them."""
+    c = _case([300, 65], [9, 6], 4, 2, 64, 2, 4, seed=13)
+    ref = _reference(c)
+    d = {x: c[x].to(DEV) for x in ("q", "k", "v", "idx", "bias", "valid", "table", "ctx", "cu")}
+    par = torch.tensor(sum(c["par"], []), dtype=torch.int32, device=DEV)
+    pad = {x: torch.cat([d[x], torch.ones_like(d[x][:7])]) for x in ("q", "idx", "bias", "valid")}
+    par_p = torch.cat([par, torch.full_like(par[:7], 3)])
+    table = torch.cat([d["table"], torch.full_like(d["table"], -5)])
+    ctx = torch.cat([d["ctx"], torch.tensor([10 ** 6, -7], dtype=torch.int32, device=DEV)])
+    cu = torch.cat([d["cu"], torch.tensor([15, 15], dtype=torch.int32, device=DEV)])
+    mask, depth = tree.tree_masks(par_p, cu, 32)
+    out, lse = tree.attn_tree(pad["q"], d["k"], d["v"], pad["idx"], pad["bias"], pad["valid"], mask, depth,
+                              ctx, cu, 32, 64, 128, SCALE, block_table=table, page_size=64,
+                              return_lse=True)
+    assert out.shape[0] == 22
+    _close(out[:15], lse[:15], *ref, 5.0)
+    # a third and a fourth request that claim rows there are not
+    cu[3:] = torch.tensor([10 ** 6], device=DEV)
+    mask, depth = tree.tree_masks(par_p[:15], cu, 32)
+    out, lse = tree.attn_tree(d["q"], d["k"], d["v"], d["idx"], d["bias"], d["valid"], mask, depth, ctx, cu,
+                              32, 64, 1 << 40, SCALE, block_table=table, page_size=64, return_lse=True)
+    wide = dict(c, lw=1 << 20)
+    _close(out, lse, *_reference(wide), 5.0)
+
+
+def test_contexts_past_the_cache_are_cut_to_it():
+    """More context than the table holds: its last keys, and no drafted ones."""
+    c = _case([128], [4], 2, 2, 64, 8, 2, seed=14, bad=False)
+    c["idx"][:] = -1
+    long = dict(c, ctx=torch.tensor([5000], dtype=torch.int32))
+    out = _run(long)
+    d = c["table"][0, :3].long()
+    k, v = (c[x][d].reshape(-1, 2, 128) for x in "kv")
+    depth = [len(ancestors(c["par"][0], i)) - 1 for i in range(4)]
+    ref, _ = attend(c["q"], k, v, None, None, None, [[]] * 4, depth, 192, 64, 512, SCALE)
+    assert float((out.cpu().double() - ref).abs().max()) <= 1e-4

@@ -192,3 +192,37 @@ def test_forked_requests_decode_apart():
     pool.free(torch.tensor([n0, 0, 0], device=DEV))
     assert pool.refs.max() == 1 and int((pool.refs > 0).sum()) == -(-n0 // bs)
     assert float((step([0], [toks[0]]) - all3[:4]).abs().max()) <= 1e-4
+
+
+def test_index_keys_of_another_width_and_requests_without_context():
+    """Index queries of 64 dims (the general scores), and a request whose tree is all there is: a chain
+    gives extend_prefill's rows, a row without committed blocks routes nowhere."""
+    bs, H, d = 64, 2, 64
+    g = torch.Generator().manual_seed(5)
+    ctx, n = [bs * 6 + 9, 0], [5, 4]
+    pages = [-(-(c + m) // bs) for c, m in zip(ctx, n)]
+    table = torch.zeros(2, max(pages), dtype=torch.int32)
+    perm = torch.randperm(12, generator=g)
+    table[0, :pages[0]], table[1, 0] = perm[:pages[0]].int(), perm[-1].int()
+    k, v = (torch.randn(12, bs, H, 128, generator=g).bfloat16().to(DEV) for _ in range(2))
+    for width in (d, 128):
+        ik = torch.randn(12, bs, width, generator=g).to(DEV)
+        hc = torch.randn(width, generator=g).to(DEV) * 0.2
+        q = torch.randn(9, H, 128, generator=g).bfloat16().to(DEV)
+        iq = torch.randn(9, width, generator=g).to(DEV)
+        t, c = table.to(DEV), torch.tensor(ctx, device=DEV)
+        cu = torch.tensor([0, 5, 9], device=DEV)
+        args = (bs, 2, IDX, 1e-4, 1.0, 3, 4)
+        state = pipeline.KBarPageCache(12, width, DEV)
+        state.put_sequences(ik, hc, bs, t, c)
+        par = torch.tensor([-1, 0, 1, 2, 3, -1, 0, 1, 2], device=DEV)
+        out, (idx, bias, valid), pos = pipeline.tree_step(
+            state, q, k, v, iq, *args, t, c, cu, par, 5, out_dtype=torch.float32, return_routing=True)
+        assert pos.tolist() == [393, 394, 395, 396, 397, 0, 1, 2, 3]
+        assert bool(valid[:5].any()) and not bool(valid[5:].any())
+        ref, (idx2, _, valid2), _ = pipeline.extend_prefill(
+            state, q, k, v, iq, ik, hc, *args, t, c + torch.tensor(n, device=DEV), c, cu,
+            max_query_len=5, out_dtype=torch.float32, return_routing=True)
+        assert torch.equal(valid[:5].bool(), valid2[:5])
+        assert torch.equal(torch.where(valid2[:5], idx[:5], -1), torch.where(valid2[:5], idx2[:5], -1))
+        assert float((out - ref).abs().max()) <= 1e-4

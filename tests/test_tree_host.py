@@ -164,3 +164,38 @@ def test_oracle_by_hand():
     assert a.refs == [2, 1, 1, 0] and a.table[2][:2] == [0, 2]
     a.free([0, 0, 9])
     assert a.refs == [1, 0, 1, 0] and a.compact() == ([2], [1]) and a.table[2][:2] == [0, 1]
+
+
+def _addresses(desc, i, rows):
+    """Byte offsets of a layer's page (or row) of cache i, as the kernels walk its descriptor."""
+    _, _, _, n1, s1, n2, s2, seg = desc[8 * i:8 * i + 8]
+    return sorted(a * s1 + b * s2 + x for a in range(1 if rows else n1) for b in range(n2)
+                  for x in range(seg))
+
+
+@pytest.mark.parametrize("make", [
+    lambda: torch.zeros(2, 5, 4, 3, 8), lambda: torch.zeros(2, 5, 3, 4, 8).transpose(2, 3),
+    lambda: torch.zeros(2, 5, 2, 4, 3, 8)[:, :, 1], lambda: torch.zeros(2, 5, 4, 3, 10)[..., 1:9],
+    lambda: torch.zeros(2, 5, 4, 8, 3).transpose(3, 4), lambda: torch.zeros(2, 5, 4, 1, 8),
+    lambda: torch.zeros(5, 2, 4, 3, 8).transpose(0, 1), lambda: torch.zeros(2, 5, 4),
+    lambda: torch.zeros(2, 5, 4, 3, 8, dtype=torch.int8)])
+def test_descriptors_cover_a_page_and_a_row(make):
+    t = make()
+    es = t.element_size()
+    offs = torch.zeros(t.shape[1:], dtype=torch.int64)
+    for a, (n, st) in enumerate(zip(t.shape[1:], t.stride()[1:])):
+        offs += (torch.arange(n) * st).view(*[-1 if b == a else 1 for b in range(offs.dim())])
+    n, base, desc = kv_pages.PageCaches._describe([(t, 2)], 1)
+    page = [x * es + y for x in offs[0].flatten().tolist() for y in range(es)]
+    assert n == 1 and base[0] == t.data_ptr() and _addresses(desc, 0, False) == sorted(page)
+    assert list(desc[0:3]) == [2, t.stride(0) * es, t.stride(1) * es]
+    _, _, desc = kv_pages.PageCaches._describe([(t, 3)], 1)
+    row = [x * es + y for x in offs[0, 0].flatten().tolist() for y in range(es)]
+    assert _addresses(desc, 0, True) == sorted(row) and desc[4] == t.stride(2) * es
+
+
+def test_descriptors_refuse_overlaps():
+    for t in (torch.zeros(4, 1, 8).expand(4, 6, 8), torch.zeros(1, 6, 8).expand(4, 6, 8),
+              torch.zeros(200).as_strided((4, 6, 8), (48, 5, 1))):
+        with pytest.raises(ValueError, match="overlap"):
+            kv_pages.PageCaches._describe([(t, 1)], 0)
