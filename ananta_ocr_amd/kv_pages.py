@@ -13,6 +13,7 @@ parts.  ``PageCaches`` describes the tensors that the pages lie in, once for man
 """
 
 import ctypes
+import functools
 
 import torch
 
@@ -37,27 +38,33 @@ class PageCaches:
         if not tokens:
             raise ValueError("a pool needs a cache with a row per token")
         ax = 1 if layered else 0
-        self.device = self.tensors[0].device
         _device(*self.tensors)
-        for t in self.tensors:
+        first = self.tensors[0]
+        self.device = first.device
+        if first.dim() < ax + 2:
+            raise ValueError("a cache of [num_pages, page_size, ...] is needed")
+        self.num_pages, self.page_size = first.shape[ax:ax + 2]
+        head = (self.num_pages, self.page_size)
+        if 0 in head:
+            raise ValueError(f"caches of {head} pages and tokens")
+        for i, t in enumerate(self.tensors):
             if t.requires_grad:
                 raise ValueError("a cache that requires grad cannot be written in place")
-            if t.dim() <= ax:
-                raise ValueError(f"cache of shape {tuple(t.shape)}")
-        if any(t.dim() < ax + 2 for t in tokens):
-            raise ValueError("a cache of [num_pages, page_size, ...] is needed")
-        self.num_pages = self.tensors[0].shape[ax]
-        self.page_size = tokens[0].shape[ax + 1]
-        for t in self.tensors:
-            if t.shape[ax] != self.num_pages:
-                raise ValueError(f"caches of {self.num_pages} and {t.shape[ax]} pages")
-        for t in tokens:
-            if t.shape[ax + 1] != self.page_size:
-                raise ValueError(f"pages of {self.page_size} and {t.shape[ax + 1]} tokens")
-        live = [t for t in self.tensors if t.numel()]
-        self._copy = self._describe([(t, ax + 1) for t in live], ax)
-        live = [t for t in tokens if t.numel()]
-        self._rows = self._describe([(t, ax + 2) for t in live], ax)
+            n = 2 if i < len(tokens) else 1
+            if t.shape[ax:ax + n] != head[:n]:
+                raise ValueError(f"caches of {head} pages and tokens, and of shape {tuple(t.shape)}")
+        self._ax, self._tokens = ax, len(tokens)
+        if not all(t.is_contiguous() for t in self.tensors):
+            self._copy, self._rows           # refuse layouts here
+
+    @functools.cached_property
+    def _copy(self):
+        return self._describe([(t, self._ax + 1) for t in self.tensors if t.numel()], self._ax)
+
+    @functools.cached_property
+    def _rows(self):
+        return self._describe([(t, self._ax + 2) for t in self.tensors[:self._tokens] if t.numel()],
+                              self._ax)
 
     @staticmethod
     def _describe(tensors, ax):
