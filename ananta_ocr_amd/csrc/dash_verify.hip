@@ -27,6 +27,7 @@ namespace dash {
 constexpr int kVfMaxNodes = 256;      // nodes of a sequence
 constexpr int kVfChunk = 4096;        // tokens per work-group of the sums
 constexpr int kVfThreads = 256;
+constexpr uint64_t kVfUnset = ~0ull;  // of a sum that is not there yet (no sum has these bits: a NaN)
 
 struct VerifyArgs {
   const void* p; int64_t p_st;
@@ -41,7 +42,7 @@ struct VerifyArgs {
   // workspace
   int32_t* stop;                        // [B] the last accepted node
   double* gone;                         // [B] a at that node
-  double2* sums;                        // [B, chunks] (what is left, the row itself)
+  uint64_t* sums;                       // [B, chunks, 2] bits of (what is left, the row itself)
   int32_t* done;                        // [B] chunks that have arrived (the walk clears it)
   float* best_v; int32_t* best_i;       // [T, chunks] greedy partials
 };
@@ -237,6 +238,8 @@ __global__ __launch_bounds__(THREADS) void verify_walk_kernel(VerifyArgs a) {
   }
   __syncthreads();
   for (int i = tid; i < a.max_n; i += THREADS) a.path[b * a.path_st + i] = i < cnt ? sPath[i] : -1;
+  if (MODE != 0)
+    for (int i = tid; i < 2 * a.chunks; i += THREADS) a.sums[(int64_t)b * 2 * a.chunks + i] = kVfUnset;
   if (tid == 0) {
     a.count[b] = cnt;
     if (MODE == 0) {
@@ -375,7 +378,7 @@ __global__ __launch_bounds__(kVfThreads) void verify_draw_kernel(VerifyArgs a) {
   const double gone = a.gone[b];
   const double u = (double)a.u[r0];
   const int64_t child = DRAFT ? -1 : vf_child(a, r0, n, s);
-  double2* sums = a.sums + (int64_t)b * a.chunks;
+  uint64_t* sums = a.sums + (int64_t)b * 2 * a.chunks;
   VfTokens<T, DRAFT> tk;
   uint32_t named = 0u;
   {
@@ -395,10 +398,14 @@ __global__ __launch_bounds__(kVfThreads) void verify_draw_kernel(VerifyArgs a) {
     x = vf_block_sum<kVfThreads>(x, sD);
     y = vf_block_sum<kVfThreads>(y, sD);
     if (tid == 0) {
-      // agent scope: the work-group that adds them up may run on another XCD
-      __hip_atomic_store(&sums[blockIdx.x].x, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      __hip_atomic_store(&sums[blockIdx.x].y, y, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      sTurn = __hip_atomic_fetch_add(&a.done[b], 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+      // agent scope: the work-group that adds them up may run on another XCD.  No release, which
+      // would write the whole L2 back (2 us of a call's 12): a sum tells by its bits that it is there
+      __hip_atomic_store(&sums[2 * blockIdx.x], __builtin_bit_cast(uint64_t, x), __ATOMIC_RELAXED,
+                         __HIP_MEMORY_SCOPE_AGENT);
+      __hip_atomic_store(&sums[2 * blockIdx.x + 1], __builtin_bit_cast(uint64_t, y), __ATOMIC_RELAXED,
+                         __HIP_MEMORY_SCOPE_AGENT);
+      __builtin_amdgcn_s_waitcnt(0);
+      sTurn = __hip_atomic_fetch_add(&a.done[b], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
     if (sTurn != a.chunks - 1) return;
@@ -406,10 +413,14 @@ __global__ __launch_bounds__(kVfThreads) void verify_draw_kernel(VerifyArgs a) {
   // each thread's run of chunks, the first of them in registers
   const int per = (a.chunks + kVfThreads - 1) / kVfThreads;
   const int c0 = min(tid * per, a.chunks), c1 = min(c0 + per, a.chunks);
-  auto read = [&](int c) {
-    return make_double2(__hip_atomic_load(&sums[c].x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT),
-                        __hip_atomic_load(&sums[c].y, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+  // (every sum was stored before its work-group counted itself in: none stays unset)
+  auto one = [&](int i) {
+    uint64_t w;
+    do w = __hip_atomic_load(&sums[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    while (w == kVfUnset);
+    return __builtin_bit_cast(double, w);
   };
+  auto read = [&](int c) { return make_double2(one(2 * c), one(2 * c + 1)); };
   const double2 sum0 = c0 < c1 ? read(c0) : make_double2(0.0, 0.0);
   auto sum_of = [&](int c) { return c == c0 ? sum0 : read(c); };
   double mine = 0.0, mine_w = 0.0, total, total_w;
@@ -554,7 +565,7 @@ extern "C" int dash_verify_tree(const void* target, int64_t target_stride, const
   a.tok = tokens; a.tok64 = tokens_int64; a.parents = parents; a.cu = cu_seqlens_q; a.u = uniforms;
   a.B = B; a.V = V; a.max_n = max_query_len; a.chunks = L.chunks; a.chunk = L.chunk; a.T = T;
   a.count = count; a.path = path; a.path_st = path_stride; a.token = next_token;
-  a.stop = (int32_t*)(w + L.stop); a.done = (int32_t*)(w + L.done); a.gone = (double*)(w + L.gone); a.sums = (double2*)(w + L.sums);
+  a.stop = (int32_t*)(w + L.stop); a.done = (int32_t*)(w + L.done); a.gone = (double*)(w + L.gone); a.sums = (uint64_t*)(w + L.sums);
   a.best_v = (float*)(w + L.best_v); a.best_i = (int32_t*)(w + L.best_i);
   hipStream_t st = (hipStream_t)stream;
   if (dtype == 0) verify_launch<float>(a, st);
