@@ -163,7 +163,8 @@ __device__ __forceinline__ int block_exclusive(int v, int* sW, int& total) {
   return before + x - v;
 }
 
-__device__ __forceinline__ int kv_blocks(int len, int page) { return (len + page - 1) / page; }
+// (no sum that could pass 32 bits: a length that is no length must not look short)
+__device__ __forceinline__ int kv_blocks(int len, int page) { return len / page + (len % page > 0); }
 
 __device__ __forceinline__ int kv_count_free(const int32_t* refs, int num_pages, int* sW) {
   int mine = 0, total;
@@ -467,9 +468,16 @@ template <template <typename> class Op, typename... Args>
 static int kv_launches(void* const* base, const int64_t* desc, int num, int64_t count, void* stream,
                        Args... args) {
   hipStream_t st = (hipStream_t)stream;
+  KvCaches a;
+  int64_t tasks = 0;
+  if (num > kKvMaxCaches)                  // all of them or none
+    for (int c0 = 0; c0 < num; c0 += kKvMaxCaches) {
+      if (!kv_fill(a, base + c0, desc + 8 * c0, std::min(kKvMaxCaches, num - c0), Op<KvVec>::kRows,
+                   Op<KvVec>::kTask, &tasks))
+        return kErrInvalid;
+      if (tasks * count > INT32_MAX) return kErrUnsupported;
+    }
   for (int c0 = 0; c0 < num; c0 += kKvMaxCaches) {
-    KvCaches a;
-    int64_t tasks = 0;
     const int unit = kv_fill(a, base + c0, desc + 8 * c0, std::min(kKvMaxCaches, num - c0), Op<KvVec>::kRows,
                              Op<KvVec>::kTask, &tasks);
     if (unit == 0) return kErrInvalid;

@@ -14,6 +14,7 @@ parts.  ``PageCaches`` describes the tensors that the pages lie in, once for man
 
 import ctypes
 import functools
+import math
 
 import torch
 
@@ -29,7 +30,8 @@ class PageCaches:
     values, index keys: a row per token) and ``pages`` of [num_pages, ...] (block summaries: a
     row per page); with ``layered`` every tensor has a leading layer axis.  Any types and strides
     whose innermost piece is contiguous and that do not overlap; every tensor on one GPU and of the
-    same number of pages."""
+    same number of pages.  Addresses are noted once: the tensors keep their memory (no resize_ or
+    set_) while the object is in use."""
 
     def __init__(self, tokens, pages=(), layered=False):
         self.tensors = [*tokens, *pages]
@@ -78,7 +80,7 @@ class PageCaches:
             rows = at == ax + 2
             if t.is_contiguous():            # a page, or a row, in one piece
                 base[i] = t.data_ptr()
-                seg = es * (stride[at] * size[at] if at < t.dim() else 1)
+                seg = es * math.prod(size[at:])    # (an axis of one may have any stride)
                 desc[8 * i:8 * i + 8] = [size[0] if ax else 1, stride[0] * es if ax else 0,
                                          stride[ax] * es, 1, stride[ax + 1] * es if rows else 0,
                                          1, 0, seg]

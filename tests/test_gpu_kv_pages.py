@@ -175,6 +175,19 @@ def test_refused_forks_change_nothing():
     assert int(ok) == 0 and pool.lens.tolist() == lists.lens
 
 
+def test_lengths_that_are_none():
+    """A length past the table is refused, one past any sum of 32 bits too."""
+    for length in (2 ** 31 - 1, 2 ** 31 - 8, 10 ** 9, -1):
+        pool, _, _ = _pool()
+        pool.lens[0] = length
+        for f, rows in ((kv_pages.fork_pages, (_i32([0]), _i32([3]))),
+                        (kv_pages.reserve_pages, (_i32([1] * 6),))):
+            before = pool.table.clone(), pool.refs.clone(), pool.lens.clone()
+            ok, frm, to = f(pool.refs, pool.table, pool.lens, *rows, 8)
+            assert int(ok) == 0 and frm.tolist() == to.tolist() == [-1] * frm.numel()
+            assert all(torch.equal(x, y) for x, y in zip(before, (pool.table, pool.refs, pool.lens)))
+
+
 @pytest.mark.parametrize("dtype,inner", [
     (torch.bfloat16, (10, 128)), (torch.float32, (128,)), (torch.float32, (3,)),
     (torch.bfloat16, (5, 7)), (torch.int8, (9,)), (torch.float16, (1, 3)), (torch.float64, ()),
@@ -187,6 +200,18 @@ def test_copies_of_every_unit(dtype, inner):
     want[:, [7, 1]] = want[:, [4, 18]]
     kv_pages.copy_pages(kv_pages.PageCaches([x], layered=True), _i32(frm), _i32(to))
     assert torch.equal(x, want)
+
+
+def test_copies_of_pages_of_one_token():
+    """An axis of one token, of any stride, and more caches than one launch takes."""
+    base = torch.arange(40 * 9 * 16, dtype=torch.float32, device=DEV).view(40, 1, 9, 16)
+    keep = base.clone()
+    views = [base[i].transpose(0, 1) for i in range(40)]         # [9, 1, 16], strides (16, 144, 1)
+    assert views[0].stride() == (16, 144, 1) and views[0].is_contiguous()
+    caches = kv_pages.PageCaches(views)
+    kv_pages.copy_pages(caches, _i32([2, 8]), _i32([5, 0]))
+    keep[:, 0, 5], keep[:, 0, 0] = keep[:, 0, 2].clone(), keep[:, 0, 8].clone()
+    assert torch.equal(base, keep)
 
 
 def test_copies_of_strided_caches():
