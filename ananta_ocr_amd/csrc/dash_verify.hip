@@ -16,7 +16,7 @@
 // different order of a sum moves a border by 1e-16 of the row's mass, not by the 1e-7 that would
 // change a drawn token in every few thousandth row of 131,072 tokens.
 //
-// Probabilities that are not above 0 (NaN too) count as 0.
+// Probabilities that are not above 0 (NaN too) count as 0, and so do random numbers below it.
 
 #include <hip/hip_fp16.h>
 
@@ -61,9 +61,10 @@ __device__ __forceinline__ int64_t vf_token(const VerifyArgs& a, int64_t row) {
   return a.tok64 ? ((const int64_t*)a.tok)[row] : ((const int32_t*)a.tok)[row];
 }
 
-// What is left of probability p where the draft's is q (maxima take what is no number to 0).
+// What is left of probability p where the draft's is q (maxima take what is no number to 0; with q and
+// gone at least 0, a p below 0 ends there too).
 __device__ __forceinline__ double vf_rest(float p, float q, double gone) {
-  return fmax(fma(-gone, (double)q, (double)fmaxf(p, 0.f)), 0.0);
+  return fmax(fma(-gone, (double)fmaxf(q, 0.f), (double)p), 0.0);
 }
 __device__ __forceinline__ double vf_left(float p, float q, double gone) {
   return gone == 0.0 ? (double)fmaxf(p, 0.f) : vf_rest(p, q, gone);
@@ -157,8 +158,8 @@ __global__ __launch_bounds__(THREADS) void verify_walk_kernel(VerifyArgs a) {
     if (MODE != 0) {
       const bool in = par >= 0 && t >= 0 && t < a.V;
       sP[i] = in ? vf_load((const T*)a.p + (r0 + par) * a.p_st + t) : 0.f;
-      sQ[i] = MODE == 2 && in ? vf_load((const T*)a.q + (r0 + par) * a.q_st + t) : 1.f;
-      sU[i] = a.u[r0 + i];
+      sQ[i] = MODE == 2 && in ? fmaxf(vf_load((const T*)a.q + (r0 + par) * a.q_st + t), 0.f) : 1.f;
+      sU[i] = fmaxf(a.u[r0 + i], 0.f);
     }
   }
   if (MODE == 0) {
@@ -205,8 +206,9 @@ __global__ __launch_bounds__(THREADS) void verify_walk_kernel(VerifyArgs a) {
           if (more) {
             const T* p = (const T*)a.p + (r0 + s) * a.p_st;
             const T* q = (const T*)a.q + (r0 + s) * a.q_st;
-            // one work-group's reads in flight: 32 tokens a lane of each row, 128 or 256 KB
-            constexpr int E = VfVec<T>::kN, U = 32 / E;
+            // one work-group's reads in flight: 16 tokens a lane of each row, 64 or 128 KB (32 tokens:
+            // 36 us for the passes of 16 trees, 16: 34.5; the next 8 loaded while 8 are added up: 40)
+            constexpr int E = VfVec<T>::kN, U = 16 / E;
             double mine = 0.0, odd = 0.0;
             int v = 0;
             for (; v + THREADS * E * U <= a.V; v += THREADS * E * U) {
@@ -376,7 +378,7 @@ __global__ __launch_bounds__(kVfThreads) void verify_draw_kernel(VerifyArgs a) {
   if (s < 0) return;
   const int64_t row = r0 + s;
   const double gone = a.gone[b];
-  const double u = (double)a.u[r0];
+  const double u = (double)fmaxf(a.u[r0], 0.f);
   const int64_t child = DRAFT ? -1 : vf_child(a, r0, n, s);
   uint64_t* sums = a.sums + (int64_t)b * 2 * a.chunks;
   VfTokens<T, DRAFT> tk;

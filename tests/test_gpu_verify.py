@@ -124,6 +124,27 @@ def test_what_is_left_of_a_row():
     _check(p, [0, 5, 1], one, torch.tensor([0.3, 0.5, 0.5]), q, [3])
 
 
+def test_draft_values_and_numbers_that_count_as_0():
+    """NaN and negative draft probabilities neither hold mass back nor add any, and a number below
+    0 draws like 0."""
+    one = [[-1, 0, 0]]
+    p, q = torch.zeros(3, 6), torch.zeros(3, 6)
+    p[0] = torch.tensor([0.1, 0.4, 0.1, 0.2, 0.2, 0.0])
+    q[0] = torch.tensor([math.nan, 0.8, -0.5, math.nan, 0.2, math.nan])
+    for last in (0.0, 0.2, 0.45, 0.75, 0.999):
+        # left after token 1: (0.1, 0, 0.1, 0.2, 0, 0); token 0 is then rejected by its number 1
+        _check(p, [0, 1, 0], one, torch.tensor([last, 0.9, 1.0]), q, [3])
+    _check(p, [0, 5, 3], one, torch.tensor([0.3, 0.0, 0.5]), q, [3])
+    below = [[-1, 0]]
+    _check(p[:2], [0, 5], below, torch.tensor([0.0, 0.0]), None, [2])
+    c = [tree.verify_tree(p[:2].to(DEV), torch.tensor([0, 5], device=DEV),
+                          torch.tensor([-1, 0], dtype=torch.int32, device=DEV),
+                          torch.tensor([0, 2], dtype=torch.int32, device=DEV), 2,
+                          uniforms=torch.tensor([u, u], device=DEV)) for u in (0.0, -0.5, math.nan)]
+    for x in c[1:]:
+        assert all(torch.equal(s, t) for s, t in zip(c[0], x))
+
+
 def test_greedy_ties_and_odd_rows():
     V = 20000
     p = torch.zeros(4, V)

@@ -66,7 +66,7 @@ def verify(target, tokens, parents, u=None, draft=None):
             path.append(at)
             continue
         row = torch.where(target[at].double() > 0, target[at].double(), 0.0)
-        q = None if draft is None else draft[at].double()
+        q = None if draft is None else torch.where(draft[at].double() > 0, draft[at].double(), 0.0)
         rest, mass, found = row.clone(), 1.0, None
         for i in kids:
             x = tokens[i]
