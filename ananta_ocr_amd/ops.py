@@ -1012,7 +1012,8 @@ def extend_scores(idx_q, idx_k, head_cls, cu_seqlens_q, context_lens, seq_lens, 
 def kbar_pages_ok(idx_k, pool, block_size):
     """Whether kbar_pages takes these paged index keys and this k_bar pool."""
     return (idx_k.dim() == 3 and idx_k.shape[1] == block_size and idx_k.shape[2] == 128
-            and pool.shape[-1] == 128 and 0 < block_size <= 64 and pool.shape[0] > 0
+            and pool.dim() == 2 and pool.shape[1] == 128 and 0 < block_size <= 64
+            and 0 < pool.shape[0] <= idx_k.shape[0]
             and pool.dtype == torch.float32 and pool.is_contiguous() and pool.data_ptr() % 16 == 0
             and idx_k.dtype == torch.float32 and idx_k.stride(-1) == 1
             and idx_k.data_ptr() % 16 == 0 and all(s % 4 == 0 for s in idx_k.stride()[:-1]))
@@ -1022,8 +1023,14 @@ def kbar_pages(idx_k, head_cls, first_tokens, seq_lens, block_table, pool, block
     """The summaries of blocks first_tokens[b] // block_size .. of every sequence of seq_lens[b]
     tokens, written to their pages' rows of the k_bar pool [pages, 128] in one launch
     (KBarPageCache.refresh_from in its one-block pages)."""
-    _need_gpu(idx_k, head_cls, first_tokens, seq_lens, block_table, pool)
+    if not kbar_pages_ok(idx_k, pool, block_size):
+        raise NotImplementedError("kbar_pages takes fp32 index keys [pages, block_size, 128] and a "
+                                  "contiguous pool [pages, 128], block_size at most 64")
     B, P = block_table.shape
+    for t, n in ((first_tokens, B), (seq_lens, B), (head_cls, idx_k.shape[2])):
+        if t.numel() != n:
+            raise ValueError(f"kbar_pages: {n} values needed, {t.numel()} given")
+    _need_gpu(idx_k, head_cls, first_tokens, seq_lens, block_table, pool)
     first, lens, bt = (_i32(x) for x in (first_tokens, seq_lens, block_table))
     hc = _aligned(head_cls.float())
     _lib.check(_lib.load().dash_kbar_pages(

@@ -210,7 +210,8 @@ def tree_step(state, q, k_cache, v_cache, idx_q, block_size, local_blocks, idx_s
     mask, depth = tree.tree_masks(parents, cu, max_query_len)
     idx_q = idx_q.reshape(T, -1)
     pool = state.kbar
-    if idx_q.shape[1] == 128 and pool.shape[1] == 128 and pool.data_ptr() % 16 == 0:
+    if idx_q.shape[1] == pool.shape[1] == 128 and pool.dtype == torch.float32 \
+            and pool.is_contiguous() and pool.data_ptr() % 16 == 0:
         idx_q = idx_q if idx_q.dtype == torch.float32 else idx_q.float()
         z, q_pos, row_nblk = tree.tree_scores(ops._f4_rows(idx_q), cu, ctx, depth, table, pool,
                                               block_size, local_blocks, max_query_len)

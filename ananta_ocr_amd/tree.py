@@ -76,11 +76,16 @@ def tree_scores(idx_q, cu_seqlens_q, context_lens, depth, block_table, pool, blo
     [T, 128] fp32 against the k_bar pool's summaries of their sequences' committed blocks, the
     rows' positions (context_len + depth) and block counts [T] int32."""
     B, n = _nodes(cu_seqlens_q, max_query_len)
+    T, d = idx_q.shape
+    _shape(depth, (T,), "depth")
+    _shape(context_lens, (B,), "context_lens")
+    P = block_table.shape[1]
+    _shape(block_table, (B, P), "block_table")
+    _shape(pool, (pool.shape[0], d), "pool")
+    if idx_q.dtype != torch.float32 or idx_q.stride(1) != 1 or pool.dtype != torch.float32 \
+            or not pool.is_contiguous():
+        raise ValueError("idx_q and the k_bar pool: contiguous fp32 rows are needed")
     with _device(idx_q, cu_seqlens_q, context_lens, depth, block_table, pool):
-        T, d = idx_q.shape
-        _shape(depth, (T,), "depth")
-        _shape(context_lens, (B,), "context_lens")
-        P = block_table.shape[1]
         cu, ctx, dep, bt = (_i32(x) for x in (cu_seqlens_q, context_lens, depth, block_table))
         zs = max(32, (P + 31) // 32 * 32)
         z = torch.empty(T, zs, dtype=torch.float32, device=idx_q.device)
@@ -104,7 +109,8 @@ def attn_tree(q, k, v, idx, bias, valid, mask, depth, context_lens, cu_seqlens_q
       slot), with the bias of the slot;
     * the drafted keys (slot context_lens[b] + m) whose bit m is set in mask [T, words].
 
-    idx, bias and valid may be None (no routed blocks).  Returns out [T,H,128] (fp32 or bf16) and
+    idx, bias and valid may be None (no routed blocks).  block_size is 32 or a multiple of 64, at
+    most 2,048 blocks a sequence and 64 slots a row.  Returns out [T,H,128] (fp32 or bf16) and
     with return_lse the log-sum-exp [T,H] fp32; a row that sees no key gives 0 and -inf."""
     lib = _lib.load()
     B, n = _nodes(cu_seqlens_q, max_query_len)
@@ -200,7 +206,8 @@ def verify_tree(target, tokens, parents, cu_seqlens_q, max_query_len, uniforms=N
       a += Z and Z = sum(max(p - a q, 0)).
 
     The uniform of the root draws next_token from what is left at the last accepted node: the first
-    id whose running sum exceeds it times the whole.  path holds the accepted nodes, the root
+    id whose running sum exceeds it times the whole.  Uniforms lie in [0, 1); probabilities and
+    uniforms that are not above 0 (NaN too) count as 0.  path holds the accepted nodes, the root
     first, then -1; a sequence without nodes has count 0 and next_token -1."""
     lib = _lib.load()
     B, n = _nodes(cu_seqlens_q, max_query_len)

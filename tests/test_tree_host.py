@@ -6,7 +6,7 @@ import os
 import pytest
 import torch
 
-from ananta_ocr_amd import _lib, kv_pages, pipeline, tree
+from ananta_ocr_amd import _lib, kv_pages, ops, pipeline, tree
 from test_capi import ERR_INVALID, ERR_UNSUPPORTED, _call
 from tree_oracle import Pages, ancestors, verify
 
@@ -65,6 +65,28 @@ def test_verify_refuses(kw):
     with pytest.raises(ValueError) as e:
         tree.verify_tree(**{**a, **kw})
     assert "GPU" not in str(e.value)
+
+
+def test_scores_and_summaries_refuse():
+    a = dict(idx_q=torch.zeros(5, 128), cu_seqlens_q=torch.tensor([0, 5]), context_lens=torch.zeros(1, dtype=I32),
+             depth=torch.zeros(5, dtype=I32), block_table=torch.zeros(1, 2, dtype=I32),
+             pool=torch.zeros(3, 128), block_size=64, local_blocks=2, max_query_len=5)
+    b = dict(idx_k=torch.zeros(3, 64, 128), head_cls=torch.zeros(128), first_tokens=torch.zeros(1, dtype=I32),
+             seq_lens=torch.zeros(1, dtype=I32), block_table=torch.zeros(1, 2, dtype=I32),
+             pool=torch.zeros(3, 128), block_size=64)
+    for f, good, bad in (
+            (tree.tree_scores, a, [dict(idx_q=a["idx_q"].half()), dict(pool=a["pool"].half()),
+                                   dict(pool=torch.zeros(3, 64)), dict(pool=torch.zeros(3, 256)[:, :128]),
+                                   dict(block_table=torch.zeros(2, 2, dtype=I32)), dict(depth=torch.zeros(4))]),
+            (ops.kbar_pages, b, [dict(idx_k=torch.zeros(2, 64, 128)), dict(pool=torch.zeros(3, 64)),
+                                 dict(idx_k=torch.zeros(3, 64, 128).half()), dict(head_cls=torch.zeros(64)),
+                                 dict(seq_lens=torch.zeros(2)), dict(block_size=32)])):
+        with pytest.raises(ValueError, match="GPU"):
+            f(**good)
+        for kw in bad:
+            with pytest.raises((ValueError, NotImplementedError)) as e:
+                f(**{**good, **kw})
+            assert "GPU" not in str(e.value)
 
 
 def test_page_calls_refuse():
@@ -178,7 +200,8 @@ def _addresses(desc, i, rows):
     lambda: torch.zeros(2, 5, 2, 4, 3, 8)[:, :, 1], lambda: torch.zeros(2, 5, 4, 3, 10)[..., 1:9],
     lambda: torch.zeros(2, 5, 4, 8, 3).transpose(3, 4), lambda: torch.zeros(2, 5, 4, 1, 8),
     lambda: torch.zeros(5, 2, 4, 3, 8).transpose(0, 1), lambda: torch.zeros(2, 5, 4),
-    lambda: torch.zeros(2, 5, 4, 3, 8, dtype=torch.int8)])
+    lambda: torch.zeros(2, 5, 4, 3, 8, dtype=torch.int8),
+    lambda: torch.zeros(2, 1, 5, 8).transpose(1, 2), lambda: torch.zeros(2, 5, 1, 4, 8).transpose(2, 3)])
 def test_descriptors_cover_a_page_and_a_row(make):
     t = make()
     es = t.element_size()
