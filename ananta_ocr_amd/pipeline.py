@@ -245,11 +245,13 @@ def commit_tree(pool, path, count, context_lens, layers=()):
     kept = pool.keep(path, count, ctx)
     new = torch.where(count > 0, kept, ctx)
     bs = pool.page_size
+    # (a request that stays may share its last page with a longer one, whose summary that page holds)
+    lens = torch.where(count > 0, kept, 0) if layers else None
     for state, idx_k, head_cls in layers:
         if ops.kbar_pages_ok(idx_k, state.kbar, bs):
-            ops.kbar_pages(idx_k, head_cls, ctx, new, pool.table, state.kbar, bs)
+            ops.kbar_pages(idx_k, head_cls, ctx, lens, pool.table, state.kbar, bs)
         else:
-            state.refresh_from(idx_k, head_cls, bs, pool.table, new, ctx // bs)
+            state.refresh_from(idx_k, head_cls, bs, pool.table, lens, ctx // bs)
     return new
 
 

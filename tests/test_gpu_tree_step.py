@@ -194,6 +194,35 @@ def test_forked_requests_decode_apart():
     assert float((step([0], [toks[0]]) - all3[:4]).abs().max()) <= 1e-4
 
 
+@pytest.mark.parametrize("width", [128, 64])
+def test_requests_that_stay_leave_shared_pages_alone(width):
+    """Row 1 shares its pages with row 0 and is cut inside one; while row 0 takes a step, row 1's
+    summaries are not recomputed, and the pages that both name keep theirs."""
+    bs = 64
+    g = torch.Generator().manual_seed(8)
+    ik = torch.randn(9, bs, width, generator=g).to(DEV)
+    kv = torch.randn(9, bs, 1, 128, generator=g).bfloat16().to(DEV)
+    hc = torch.randn(width, generator=g).to(DEV)
+    state = pipeline.KBarPageCache(9, width, DEV)
+    pool = kv_pages.PagePool(kv_pages.PageCaches([kv, ik], pages=[state.kbar]), 2, 5)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    assert int(pool.reserve(i32([3 * bs, 0]))) == 1
+    state.put_sequences(ik, hc, bs, pool.table[:1], pool.lens[:1])
+    assert int(pool.fork(i32([0]), i32([1]))) == 1
+    pool.free(i32([3 * bs, bs + 7]))
+    assert int(pool.reserve(i32([3 * bs + 3, 0]))) == 1
+    before = state.kbar.clone()
+    new = pipeline.commit_tree(pool, i32([[0, 2, -1], [-1, -1, -1]]), i32([2, 0]), i32([3 * bs, bs + 7]),
+                               [(state, ik, hc)])
+    assert new.tolist() == pool.lens.tolist() == [3 * bs + 2, bs + 7]
+    grown = int(pool.table[0, 3])
+    keep = [p for p in range(9) if p != grown]
+    assert torch.equal(state.kbar[keep], before[keep])
+    want = pipeline.KBarPageCache(9, width, DEV)
+    want.put_sequences(ik, hc, bs, pool.table[:1], pool.lens[:1])
+    assert float((state.kbar[grown] - want.kbar[grown]).abs().max()) <= 1e-5
+
+
 def test_index_keys_of_another_width_and_requests_without_context():
     """Index queries of 64 dims (the general scores), and a request whose tree is all there is: a chain
     gives extend_prefill's rows, a row without committed blocks routes nowhere."""
