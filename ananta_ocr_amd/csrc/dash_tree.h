@@ -43,7 +43,8 @@ __device__ __forceinline__ int tree_page(const TreeArgs& a, int p) {
 }
 
 // The masks and depths of the trees: one work-group per sequence, one lane per node, which
-// climbs to the root (parents come before their children, so it ends).
+// climbs to the root (parents come before their children, so it ends).  Latency: the launch and a
+// step in LDS per level (a tree of 8 nodes 1.6 us, 32 of up to 64 nodes 4.8).
 __global__ __launch_bounds__(kTrMaxNodes) void tree_masks_kernel(const int32_t* parents,
                                                                  const int32_t* cu, int64_t T,
                                                                  int words, int max_n, uint64_t* mask,
@@ -87,7 +88,12 @@ __global__ __launch_bounds__(kTrMaxNodes) void tree_masks_kernel(const int32_t* 
 // two where it is bf16: a weight is then off by at most 2^-17 of itself, an output by less than 8e-6 of
 // the largest |v|, against the 2^-8 of its own value that its type costs.  The third part is a third of
 // the matrix work and a quarter of the vector work, which an item's loads hide in all but the largest
-// batches (32 trees of 24 to 64 nodes over 27,300 tokens: 131 us with three parts, 124 with two).
+// batches (32 trees of 24 to 64 nodes over 2,730 to 27,300 tokens: 131 us with three parts, 124 with two).
+//
+// Bound by HBM where there are many trees: those 32 read 517 MB of keys and values in 113 to 115 us,
+// 4.5 TB/s, where a large copy moves 4.7; eight trees over 27,300 tokens read 128 MB in 35 to 38 us.  One
+// tree of eight nodes takes 12 us for 8 MB: the rows, their slots, the page table, the keys and the
+// partials are trips to memory that wait for each other.
 // ---------------------------------------------------------------------------
 constexpr uint32_t kTrNotNamed = 0xffffffffu;
 
@@ -284,7 +290,7 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void tree_attn_kernel(TreeArgs a) 
     ko[u] = 2u * (uint32_t)(r * a.k_st + k_slot(r, lane & 15) * 8);
     vo[u] = 2u * (uint32_t)(r * a.v_st + v_slot(r, lane & 15) * 8);
   }
-  // Up to 64 rows every key is read once: non-temporal (tree_b32_n64 131 -> 125 us); more rows are
+  // Up to 64 rows every key is read once: non-temporal (the 32 trees 131 -> 125 us); more rows are
   // several work-groups, which share the lines in the L2.
   constexpr int kAux = RT == 4 ? 0 : 2;
   auto fetch = [&](int x, bf16* sKn, bf16* sVn) __attribute__((always_inline)) {
@@ -625,8 +631,8 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void tree_attn_kernel(TreeArgs a) 
         none ? -INFINITY : (m_run + log2f(l_tot)) * 0.6931471805599453f;
 }
 
-// One wavefront per (row, head), two dims a lane; lane s holds the weight of split s (at most 64).
-// A split that saw no key wrote m = -inf and is not read.
+// One wavefront per (row, head), two dims a lane; lane s holds the weight of split s (at most 64),
+// and eight partials are in flight (13,480 rows and heads of 3 splits: 7 us; 80 of 41: 4).  A split that saw no key wrote m = -inf and is not read.
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
   constexpr int D = 128;
   const int64_t rh = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
@@ -676,7 +682,8 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
 }
 
 // Rows of a work-group, row groups and splits of a call: 32 rows per wavefront pair up to 64, then
-// 128 rows; splits until the grid is about two rounds of two work-groups per CU.
+// 128 rows; splits until the grid is about two rounds of two work-groups per CU (640, 768, 1,536 or 2,048
+// work-groups instead of 1,024: slower by 3 to 20 % on one side or the other).
 struct TreePlan { int rt, groups, nsplit, nodes; };
 inline TreePlan tree_plan(int B, int H, int Hkv, int max_n, int K, int S, int bs, int lw) {
   TreePlan p;
