@@ -150,6 +150,74 @@ def test_loop_equals_chunks(Hkv, bs, lb, K, topm):
     assert grew > 4
 
 
+@pytest.mark.parametrize("width", [128, 64])
+def test_a_captured_step(width):
+    """Reserve, attention, verification and commit in one graph: every replay gives what the same
+    calls give outside of it, on other inputs and after other work."""
+    bs, H, V, B = 64, 2, 3000, 3
+    g = torch.Generator().manual_seed(width)
+    k, v = (torch.randn(30, bs, H, 128, generator=g).bfloat16().to(DEV) for _ in range(2))
+    ik, hc = torch.randn(30, bs, width, generator=g).to(DEV), torch.randn(width, generator=g).to(DEV)
+    state = pipeline.KBarPageCache(30, width, DEV)
+    pool = kv_pages.PagePool(kv_pages.PageCaches([k, v, ik], pages=[state.kbar]), B, 9)
+    start = torch.tensor([5 * bs + 60, 3 * bs, 0], dtype=torch.int32, device=DEV)
+    assert int(pool.reserve(start)) == 1
+    state.put_sequences(ik, hc, bs, pool.table.clamp(min=0), start)
+    nodes = [7, 5, 1]
+    T = sum(nodes)
+    cu = torch.tensor([0] + nodes).cumsum(0).to(torch.int32).to(DEV)
+    room = start + cu[1:] - cu[:-1]
+    held = [pool.refs, pool.table, pool.lens, k, v, ik, state.kbar]
+    before = [x.clone() for x in held]
+    q = torch.zeros(T, H, 128, dtype=torch.bfloat16, device=DEV)
+    iq, u = torch.zeros(T, width, device=DEV), torch.zeros(T, device=DEV)
+    probs, draft = torch.full((T, V), 1.0 / V, device=DEV), torch.full((T, V), 1.0 / V, device=DEV)
+    tokens, parents = (torch.zeros(T, dtype=torch.int32, device=DEV) for _ in range(2))
+
+    def fill(seed):
+        g = torch.Generator().manual_seed(seed)
+        logits = torch.randn(T, V, generator=g) * 3
+        p, d = logits.softmax(-1), (logits + torch.randn(T, V, generator=g) * 0.3).softmax(-1)
+        par = [x for n in nodes for x in [-1] + [int(torch.randint(0, i, (1,), generator=g)) for i in range(1, n)]]
+        first = [c for c, n in zip(cu.tolist(), nodes) for _ in range(n)]
+        at = torch.tensor([f + max(x, 0) for f, x in zip(first, par)])
+        for x, y in ((q, torch.randn(T, H, 128, generator=g)), (iq, torch.randn(T, width, generator=g)),
+                     (u, torch.rand(T, generator=g)), (probs, p), (draft, d),
+                     (parents, torch.tensor(par)),
+                     (tokens, torch.multinomial(d[at], 1, generator=g)[:, 0])):
+            x.copy_(y)
+        for x, y in zip(held, before):
+            x.copy_(y)
+
+    def step():
+        ok = pool.reserve(room)
+        out = pipeline.tree_step(state, q, k, v, iq, bs, 2, IDX, 1e-4, 1.0, 3, 4, pool.table, start, cu,
+                                 parents, 7)
+        found = tree.verify_tree(probs, tokens, parents, cu, 7, uniforms=u, draft=draft)
+        new = pipeline.commit_tree(pool, found[1], found[0], start, [(state, ik, hc)])
+        return [ok, out, *found, new]
+    fill(0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kept = step()
+    counts = set()
+    for seed in range(1, 7):
+        fill(seed)
+        want = [x.clone() for x in (*step(), *held)]
+        (q.float() @ q.float().transpose(1, 2)).sum()         # other work between
+        fill(seed)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(want, (*kept, *held)))
+        counts.add(tuple(want[2].tolist()))
+    assert len(counts) > 1
+
+
 def test_forked_requests_decode_apart():
     """A request forked to two rows, each grown by a tree of its own: both read the shared pages and
     their own copy of the last one, and the first row's outputs are what they were."""
