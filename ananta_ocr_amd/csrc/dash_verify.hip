@@ -417,11 +417,12 @@ __global__ __launch_bounds__(kVfThreads) void verify_draw_kernel(VerifyArgs a) {
   // each thread's run of chunks, the first of them in registers
   const int per = (a.chunks + kVfThreads - 1) / kVfThreads;
   const int c0 = min(tid * per, a.chunks), c1 = min(c0 + per, a.chunks);
-  // (every sum was stored before its work-group counted itself in: none stays unset)
+  // every sum was stored before its work-group counted itself in: none stays unset (two calls at once on
+  // one workspace, which is no use of it, could clear one for good: the wait ends all the same)
   auto one = [&](int i) {
-    uint64_t w;
-    do w = __hip_atomic_load(&sums[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    while (w == kVfUnset);
+    uint64_t w = kVfUnset;
+    for (int k = 0; k < 65536 && w == kVfUnset; ++k)
+      w = __hip_atomic_load(&sums[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     return __builtin_bit_cast(double, w);
   };
   auto read = [&](int c) { return make_double2(one(2 * c), one(2 * c + 1)); };
