@@ -198,38 +198,47 @@ def tree_step(state, q, k_cache, v_cache, idx_q, block_size, local_blocks, idx_s
     A chain gives extend_prefill's rows: no drafted key is remote while the tree is not deeper than
     the window.  q [T,H,D] bf16, k_cache / v_cache [pages, block_size, Hkv, D] bf16 (H a multiple
     of Hkv), idx_q [T,d] fp32, block_table [B,P] int32, context_lens [B], cu_seqlens_q [B+1],
-    max_query_len the largest tree.  Returns out [T,H,D] (out_dtype)."""
+    max_query_len at least the largest tree, block_cand [T,P] the blocks a row may route to (None: any).
+    Rows past cu_seqlens_q's last (a batch padded to a fixed size) come out with nothing in particular.
+    Returns out [T,H,D] (out_dtype)."""
     if not getattr(state, "paged", False):
         raise NotImplementedError("tree_step takes a k_bar page pool (KBarPageCache)")
     T, H, D = q.shape
     if scale is None:
         scale = 1.0 / math.sqrt(D)
-    ctx, cu, table = (x.to(device=q.device, dtype=torch.int32).contiguous()
-                      for x in (context_lens, cu_seqlens_q, block_table))
-    B, P = table.shape
-    mask, depth = tree.tree_masks(parents, cu, max_query_len)
-    idx_q = idx_q.reshape(T, -1)
-    pool = state.kbar
-    if idx_q.shape[1] == pool.shape[1] == 128 and pool.dtype == torch.float32 \
-            and pool.is_contiguous() and pool.data_ptr() % 16 == 0:
-        idx_q = idx_q if idx_q.dtype == torch.float32 else idx_q.float()
-        z, q_pos, row_nblk = tree.tree_scores(ops._f4_rows(idx_q), cu, ctx, depth, table, pool,
-                                              block_size, local_blocks, max_query_len)
-    else:
-        kb_seq = pool.index_select(0, table.to(torch.int64).clamp(0, pool.shape[0] - 1)
-                                   .reshape(-1)).view(B, P, -1)
-        row_seq = _row_seq(cu, B, T)
-        q_pos = ctx.index_select(0, row_seq) + depth
-        z = ops.block_scores(idx_q.reshape(1, T, -1), kb_seq, block_size, local_blocks,
-                             q_pos=q_pos, cu_seqlens=cu, max_seqlen=max_query_len, key_lens=ctx,
-                             S=P * block_size)
-        row_nblk = ((ctx + block_size - 1) // block_size).index_select(0, row_seq)
     width = max(1, min(int(K), int(topm))) if int(topm) > 0 else max(1, int(K))
-    idx, bias, valid = ops.route(z, block_cand, idx_scale, floor, sigma, K, topm,
-                                 row_nblk=row_nblk, width=width)
-    out = tree.attn_tree(q, k_cache, v_cache, idx, bias, valid, mask, depth, ctx, cu,
-                         max_query_len, block_size, local_blocks * block_size, scale,
-                         block_table=table, page_size=block_size, out_dtype=out_dtype)
+    if T == 0:                                   # no request has a node
+        out = torch.empty(0, H, D, dtype=out_dtype, device=q.device)
+        none = torch.empty(0, width, dtype=torch.int32, device=q.device)
+        return (out, (none, none.float(), none.bool()), none[:, 0]) if return_routing else out
+    with tree._device(q, k_cache, v_cache, idx_q, parents):
+        ctx, cu, table = (x.to(device=q.device, dtype=torch.int32).contiguous()
+                          for x in (context_lens, cu_seqlens_q, block_table))
+        B, P = table.shape
+        mask, depth = tree.tree_masks(parents, cu, max_query_len)
+        idx_q = idx_q.reshape(T, -1)
+        pool = state.kbar
+        if idx_q.shape[1] == pool.shape[1] == 128 and pool.dtype == torch.float32 \
+                and pool.is_contiguous() and pool.data_ptr() % 16 == 0:
+            idx_q = idx_q if idx_q.dtype == torch.float32 else idx_q.float()
+            z, q_pos, row_nblk = tree.tree_scores(ops._f4_rows(idx_q), cu, ctx, depth, table, pool,
+                                                  block_size, local_blocks, max_query_len)
+        else:
+            kb_seq = pool.index_select(0, table.to(torch.int64).clamp(0, pool.shape[0] - 1)
+                                       .reshape(-1)).view(B, P, -1)
+            # (rows of no tree, in a padded batch, count as the last one's)
+            row_seq = torch.searchsorted(cu[1:], torch.arange(T, dtype=torch.int32, device=q.device),
+                                         right=True).clamp_(max=B - 1)
+            q_pos = ctx.index_select(0, row_seq) + depth
+            z = ops.block_scores(idx_q.reshape(1, T, -1), kb_seq, block_size, local_blocks,
+                                 q_pos=q_pos, cu_seqlens=cu, max_seqlen=max_query_len, key_lens=ctx,
+                                 S=P * block_size)
+            row_nblk = ((ctx + block_size - 1) // block_size).index_select(0, row_seq)
+        idx, bias, valid = ops.route(z, block_cand, idx_scale, floor, sigma, K, topm,
+                                     row_nblk=row_nblk, width=width)
+        out = tree.attn_tree(q, k_cache, v_cache, idx, bias, valid, mask, depth, ctx, cu,
+                             max_query_len, block_size, local_blocks * block_size, scale,
+                             block_table=table, page_size=block_size, out_dtype=out_dtype)
     if return_routing:
         return out, (idx, bias, valid), q_pos
     return out
@@ -241,17 +250,18 @@ def commit_tree(pool, path, count, context_lens, layers=()):
     given back with their pages, and for every (state, idx_k, head_cls) of ``layers`` (its
     KBarPageCache and paged index keys) the block summaries are recomputed from the step's first
     block on.  Returns the new context lengths [B] int32 (requests without nodes keep theirs)."""
-    ctx = context_lens.to(device=pool.lens.device, dtype=torch.int32)
-    kept = pool.keep(path, count, ctx)
-    new = torch.where(count > 0, kept, ctx)
-    bs = pool.page_size
-    # (a request that stays may share its last page with a longer one, whose summary that page holds)
-    lens = torch.where(count > 0, kept, 0) if layers else None
-    for state, idx_k, head_cls in layers:
-        if ops.kbar_pages_ok(idx_k, state.kbar, bs):
-            ops.kbar_pages(idx_k, head_cls, ctx, lens, pool.table, state.kbar, bs)
-        else:
-            state.refresh_from(idx_k, head_cls, bs, pool.table, lens, ctx // bs)
+    with tree._device(pool.lens, path, count):
+        ctx = context_lens.to(device=pool.lens.device, dtype=torch.int32)
+        kept = pool.keep(path, count, ctx)
+        new = torch.where(count > 0, kept, ctx)
+        bs = pool.page_size
+        # (a request that stays may share its last page with a longer one, whose summary it holds)
+        lens = torch.where(count > 0, kept, 0) if layers else None
+        for state, idx_k, head_cls in layers:
+            if ops.kbar_pages_ok(idx_k, state.kbar, bs):
+                ops.kbar_pages(idx_k, head_cls, ctx, lens, pool.table, state.kbar, bs)
+            else:
+                state.refresh_from(idx_k, head_cls, bs, pool.table, lens, ctx // bs)
     return new
 
 

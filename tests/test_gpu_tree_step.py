@@ -263,6 +263,30 @@ def test_forked_requests_decode_apart():
 
 
 @pytest.mark.parametrize("width", [128, 64])
+def test_padded_and_empty_batches(width):
+    """Rows past the last tree, as a batch of fixed size has them, change nothing; nor do no rows at
+    all fail."""
+    bs, H = 64, 2
+    g = torch.Generator().manual_seed(11)
+    k, v = (torch.randn(12, bs, H, 128, generator=g).bfloat16().to(DEV) for _ in range(2))
+    ik, hc = torch.randn(12, bs, width, generator=g).to(DEV), torch.randn(width, generator=g).to(DEV)
+    table = torch.randperm(12, generator=g).to(torch.int32).view(2, 6).to(DEV)
+    ctx = torch.tensor([5 * bs + 3, 4 * bs], dtype=torch.int32, device=DEV)
+    state = pipeline.KBarPageCache(12, width, DEV)
+    state.put_sequences(ik, hc, bs, table, ctx)
+    q, iq = torch.randn(40, H, 128, generator=g).bfloat16().to(DEV), torch.randn(40, width, generator=g).to(DEV)
+    par = torch.randint(-3, 40, (40,), generator=g).to(torch.int32).to(DEV)
+    cu = torch.tensor([0, 6, 10], dtype=torch.int32, device=DEV)
+    call = lambda n, cu, most: pipeline.tree_step(state, q[:n], k, v, iq[:n], bs, 1, IDX, 1e-4, 1.0, 3, 4, table,
+                                                  ctx, cu, par[:n], most, out_dtype=torch.float32)
+    want = call(10, cu, 6)
+    for _ in range(3):
+        torch.full((4096,), -1, dtype=torch.int32, device=DEV)          # memory that held something
+        assert torch.equal(call(40, cu, 6)[:10], want)
+    assert call(0, torch.zeros_like(cu), 0).shape == (0, H, 128)
+
+
+@pytest.mark.parametrize("width", [128, 64])
 def test_requests_that_stay_leave_shared_pages_alone(width):
     """Row 1 shares its pages with row 0 and is cut inside one; while row 0 takes a step, row 1's
     summaries are not recomputed, and the pages that both name keep theirs."""
