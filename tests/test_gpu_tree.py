@@ -130,6 +130,16 @@ def test_rows_match_64_bits(case, paged):
     _close(b16, lse, ref, ref_lse, 5.0, str(case))
 
 
+@pytest.mark.parametrize("case", [
+    ([5000], [32], 2, 2, 32, 2, 64), ([5000, 900], [64, 33], 2, 2, 32, 2, 64),
+    ([5000], [128], 2, 1, 32, 2, 64), ([64 * 90], [50], 4, 2, 64, 1, 64)])
+def test_the_most_slots(case):
+    """64 slots a row in every height of the row tiles: the largest tables of slots beside the stages."""
+    c = _case(*case)
+    out, lse = _run(c, return_lse=True)
+    _close(out, lse, *_reference(c), 5.0, str(case))
+
+
 @pytest.mark.parametrize("bs,page", [(64, 128), (32, 96), (128, 128), (32, 64)])
 def test_pages_of_several_blocks(bs, page):
     c = _case([777, 130], [9, 20], 4, 2, bs, 2, 6, page=page)
