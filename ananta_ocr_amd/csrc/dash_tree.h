@@ -367,7 +367,8 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void tree_attn_kernel(TreeArgs a) 
   const float csc = a.scale_log2e;
 
   // this wavefront's halves of laid out item i
-  auto item = [&](int i, const bf16* sKc, const bf16* sVc, uint32_t (&vis)[NH]) __attribute__((always_inline)) {
+  auto item = [&](int i, const bf16* sKc, const bf16* sVc,
+                  uint32_t (&vis)[NH]) __attribute__((always_inline)) {
     float blog[NH];
     bool any = false;
 #pragma unroll
@@ -632,7 +633,8 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void tree_attn_kernel(TreeArgs a) 
 }
 
 // One wavefront per (row, head), two dims a lane; lane s holds the weight of split s (at most 64),
-// and eight partials are in flight (13,480 rows and heads of 3 splits: 7 us; 80 of 41: 4).  A split that saw no key wrote m = -inf and is not read.
+// and eight partials are in flight (13,480 rows and heads of 3 splits: 7 us; 80 of 41: 4).  A split that
+// saw no key wrote m = -inf and is not read.
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
   constexpr int D = 128;
   const int64_t rh = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;

@@ -193,7 +193,8 @@ __global__ __launch_bounds__(THREADS) void verify_walk_kernel(VerifyArgs a) {
           // a token that an earlier sibling named is no longer in p
           bool again = false;
           for (int k = 0; k <= w; k += kWave)
-            again |= __any(k + lane < i && sPar[min(k + lane, n - 1)] == s && sTok[min(k + lane, n - 1)] == sTok[i]);
+            again |= __any(k + lane < i && sPar[min(k + lane, n - 1)] == s &&
+                           sTok[min(k + lane, n - 1)] == sTok[i]);
           const double e = again ? 0.0 : vf_left(sP[i], 0.f, 0.0);
           if ((double)sU[i] * Z < e) { found = i; break; }
           Z -= e;
@@ -228,7 +229,8 @@ __global__ __launch_bounds__(THREADS) void verify_walk_kernel(VerifyArgs a) {
                 }
             }
 #pragma unroll 4
-            for (int w2 = v + tid; w2 < a.V; w2 += THREADS) mine += vf_rest(vf_load(p + w2), vf_load(q + w2), gone);
+            for (int w2 = v + tid; w2 < a.V; w2 += THREADS)
+              mine += vf_rest(vf_load(p + w2), vf_load(q + w2), gone);
             Z = vf_block_sum<THREADS>(mine + odd, sD);
           }
         }
@@ -498,7 +500,8 @@ static int verify_chunks(int64_t T, int V, bool greedy, int& chunk) {
   }
   // work-groups for two rounds of eight on every CU, a piece of a row of 8,192 tokens at least (1,156 rows
   // whole: 53 us, in four pieces: 51)
-  const int64_t pieces = std::max<int64_t>(1, std::min<int64_t>((4096 + T - 1) / std::max<int64_t>(T, 1), (V + 8191) / 8192));
+  const int64_t per_row = (4096 + T - 1) / std::max<int64_t>(T, 1);
+  const int64_t pieces = std::max<int64_t>(1, std::min<int64_t>(per_row, (V + 8191) / 8192));
   chunk = (int)(((V + pieces - 1) / pieces + 63) / 64 * 64);
   return (V + chunk - 1) / chunk;
 }
@@ -570,7 +573,8 @@ extern "C" int dash_verify_tree(const void* target, int64_t target_stride, const
   a.tok = tokens; a.tok64 = tokens_int64; a.parents = parents; a.cu = cu_seqlens_q; a.u = uniforms;
   a.B = B; a.V = V; a.max_n = max_query_len; a.chunks = L.chunks; a.chunk = L.chunk; a.T = T;
   a.count = count; a.path = path; a.path_st = path_stride; a.token = next_token;
-  a.stop = (int32_t*)(w + L.stop); a.done = (int32_t*)(w + L.done); a.gone = (double*)(w + L.gone); a.sums = (uint64_t*)(w + L.sums);
+  a.stop = (int32_t*)(w + L.stop); a.done = (int32_t*)(w + L.done);
+  a.gone = (double*)(w + L.gone); a.sums = (uint64_t*)(w + L.sums);
   a.best_v = (float*)(w + L.best_v); a.best_i = (int32_t*)(w + L.best_i);
   hipStream_t st = (hipStream_t)stream;
   if (dtype == 0) verify_launch<float>(a, st);
