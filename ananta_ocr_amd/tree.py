@@ -86,7 +86,7 @@ def tree_scores(idx_q, cu_seqlens_q, context_lens, depth, block_table, pool, blo
             or not pool.is_contiguous():
         raise ValueError("idx_q and the k_bar pool: contiguous fp32 rows are needed")
     with _device(idx_q, cu_seqlens_q, context_lens, depth, block_table, pool):
-        cu, ctx, dep, bt = (_i32(x) for x in (cu_seqlens_q, context_lens, depth, block_table))
+        cu, ctx, dep, bt = _i32(cu_seqlens_q), _i32(context_lens), _i32(depth), _i32(block_table)
         zs = max(32, (P + 31) // 32 * 32)
         z = torch.empty(T, zs, dtype=torch.float32, device=idx_q.device)
         rows = torch.empty(2, T, dtype=torch.int32, device=idx_q.device)
@@ -114,21 +114,23 @@ def attn_tree(q, k, v, idx, bias, valid, mask, depth, context_lens, cu_seqlens_q
     with return_lse the log-sum-exp [T,H] fp32; a row that sees no key gives 0 and -inf."""
     lib = _lib.load()
     B, n = _nodes(cu_seqlens_q, max_query_len)
-    if q.dim() != 3 or k.dim() != 4 or k.shape != v.shape:
+    q_shape, k_shape = q.shape, k.shape           # (a tensor's shape costs the host 0.2 us)
+    if len(q_shape) != 3 or len(k_shape) != 4 or k_shape != v.shape:
         raise ValueError("q [T,H,D] and k, v of one shape [.., .., .., D] are needed")
     if out_dtype not in (torch.float32, torch.bfloat16):
         raise NotImplementedError("attn_tree writes fp32 or bf16")
-    T, H, D = q.shape
+    T, H, D = q_shape
     paged = block_table is not None
-    Hkv = k.shape[2] if paged else k.shape[1]
-    if k.shape[3] != D or Hkv == 0 or H % Hkv:
-        raise ValueError(f"{H} query heads of {D} over {Hkv} key heads of {k.shape[3]}")
+    Hkv = k_shape[2] if paged else k_shape[1]
+    if k_shape[3] != D or Hkv == 0 or H % Hkv:
+        raise ValueError(f"{H} query heads of {D} over {Hkv} key heads of {k_shape[3]}")
     K = 0 if idx is None else idx.shape[-1]
-    if K and bias is None:
-        raise ValueError("routed blocks need their bias")
-    for t, what in ((idx, "idx"), (bias, "bias"), (valid, "valid")):
-        if K:
-            _shape(t, (T, K), what)
+    if K:
+        if bias is None:
+            raise ValueError("routed blocks need their bias")
+        _shape(idx, (T, K), "idx")
+        _shape(bias, (T, K), "bias")
+        _shape(valid, (T, K), "valid")
     _shape(depth, (T,), "depth")
     _shape(context_lens, (B,), "context_lens")
     _shape(mask, (T, (n + 63) // 64), "mask")
@@ -137,13 +139,13 @@ def attn_tree(q, k, v, idx, bias, valid, mask, depth, context_lens, cu_seqlens_q
     if paged:
         if block_table.dim() != 2 or block_table.shape[0] != B:
             raise ValueError(f"block_table: {B} rows needed")
-        if int(page_size or 0) != k.shape[1]:
-            raise ValueError(f"page_size {page_size}: the pages hold {k.shape[1]} tokens")
-    elif k.shape[0] != B:
-        raise ValueError(f"cache of {k.shape[0]} sequences, {B} trees")
+        if int(page_size or 0) != k_shape[1]:
+            raise ValueError(f"page_size {page_size}: the pages hold {k_shape[1]} tokens")
+    elif k_shape[0] != B:
+        raise ValueError(f"cache of {k_shape[0]} sequences, {B} trees")
     with _device(q, k, v, idx, bias, valid, mask, depth, context_lens, cu_seqlens_q, block_table):
         q, k, v = _bf16_rows(q), _bf16_rows(k), _bf16_rows(v)
-        cu, ctx, dep, bt = (_i32(x) for x in (cu_seqlens_q, context_lens, depth, block_table))
+        cu, ctx, dep, bt = _i32(cu_seqlens_q), _i32(context_lens), _i32(depth), _i32(block_table)
         mask = mask.contiguous()
         idx_c = bias_c = valid_c = None
         if K:
@@ -153,23 +155,23 @@ def attn_tree(q, k, v, idx, bias, valid, mask, depth, context_lens, cu_seqlens_q
         out = torch.empty(T, H, D, dtype=out_dtype, device=q.device)
         lse = torch.empty(T, H, dtype=torch.float32, device=q.device) if return_lse else None
         if T:
-            qs, os, (ks, k1, k2, _), (vs, v1, v2, _) = (x.stride() for x in (q, out, k, v))
+            qs, (ks, k1, k2, _), (vs, v1, v2, _) = q.stride(), k.stride(), v.stride()
             if paged:
-                S, pages = bt.shape[1] * k.shape[1], k.shape[0]
+                S, pages, bt_stride = bt.shape[1] * k_shape[1], k_shape[0], bt.stride(0)
                 kh, kt, vh, vt = k2, k1, v2, v1
             else:
-                S, pages = k.shape[2], 0
+                S, pages, bt_stride = k_shape[2], 0, 0
                 kh, kt, vh, vt = k1, k2, v1, v2
             lw = min(int(local_window), 1 << 30)      # (past every position it is the same window)
             nbytes = _attn_workspace(B, H, Hkv, T, n, K, S, int(block_size), lw)
             ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
             _lib.check(lib.dash_attn_tree(
                 q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks, kh, kt, v.data_ptr(), vs, vh, vt,
-                _ptr(bt), 0 if bt is None else bt.stride(0), int(page_size or 0), pages,
+                _ptr(bt), bt_stride, int(page_size or 0), pages,
                 ctx.data_ptr(), cu.data_ptr(), _ptr(idx_c), _ptr(valid_c), _ptr(bias_c), K,
-                mask.data_ptr(), mask.shape[1], dep.data_ptr(), out.data_ptr(),
-                int(out_dtype == torch.bfloat16), os[0], os[1], _ptr(lse),
-                0 if lse is None else lse.stride(0), 1, B, H, Hkv, T, n, S, D, int(block_size),
+                mask.data_ptr(), (n + 63) // 64, dep.data_ptr(), out.data_ptr(),
+                int(out_dtype == torch.bfloat16), H * D, D, _ptr(lse),
+                0 if lse is None else H, 1, B, H, Hkv, T, n, S, D, int(block_size),
                 lw, float(scale), _ptr(ws), nbytes, _stream()),
                 "dash_attn_tree")
     return (out, lse) if return_lse else out
