@@ -84,11 +84,11 @@ __global__ __launch_bounds__(kTrMaxNodes) void tree_masks_kernel(const int32_t* 
 // two wavefronts share a row tile, one half of every item each, and meet at the end.  A half's
 // visible keys are 32 bits per row, so the band's edges, the drafted keys' mask and the routed
 // blocks of rows that do not name them are one test.  A weight enters the second product as three
-// bf16 parts (24 bits: it is not rounded) where the output is fp32, as in the extend kernels, and as
-// two where it is bf16: a weight is then off by at most 2^-17 of itself, an output by less than 8e-6 of
-// the largest |v|, against the 2^-8 of its own value that its type costs.  The third part is a third of
-// the matrix work and a quarter of the vector work, which an item's loads hide in all but the largest
-// batches (32 trees of 24 to 64 nodes over 2,730 to 27,300 tokens: 131 us with three parts, 124 with two).
+// bf16 parts (24 bits: it is not rounded), as in the extend kernels, whatever the output's type: a bf16
+// output is the fp32 one rounded once.  Two parts (17 bits) changed the last bit of one bf16 output in
+// 400; the third is a third of the matrix work and a quarter of the vector work, which an item's loads
+// hide in all but the largest batches (8 trees of 16 to 32 nodes: 42.8 and 43.3 us, 32 trees of 24 to 64
+// over 2,730 to 27,300 tokens: 119 and 124).
 //
 // Bound by HBM where there are many trees: those 32 read 517 MB of keys and values in 113 to 115 us,
 // 4.5 TB/s, where a large copy moves 4.7; eight trees over 27,300 tokens read 128 MB in 35 to 38 us.  One
@@ -97,10 +97,11 @@ __global__ __launch_bounds__(kTrMaxNodes) void tree_masks_kernel(const int32_t* 
 // ---------------------------------------------------------------------------
 constexpr uint32_t kTrNotNamed = 0xffffffffu;
 
-template <int RT, int KG, int PARTS>
+template <int RT, int KG>
 __global__ __launch_bounds__(64 * RT * KG, 2) void tree_attn_kernel(TreeArgs a) {
   constexpr int D = 128, NW = RT * KG, TH = 64 * NW;
   constexpr int NH = 2 / KG;              // halves of an item that a wavefront takes
+  constexpr int PARTS = 3;                // of a weight
   constexpr int CH = 8;                   // items laid out at a time
   constexpr int ST = RT == 1 ? 1 : 2;     // stages
   // arrays of their own: the compiler waits for direct loads before it reads an array they may write
@@ -793,14 +794,11 @@ extern "C" int dash_attn_tree(
   const unsigned lds = (unsigned)((a.slot_cap * (p.rt == 4 ? 2 : 6) + 15) / 16 * 16);
   const dim3 grid((unsigned)wgs);
   if (p.rt == 1) {
-    auto kern = out_bf16 ? tree_attn_kernel<1, 2, 2> : tree_attn_kernel<1, 2, 3>;
-    hipLaunchKernelGGL(kern, grid, dim3(128), lds, st, a);
+    hipLaunchKernelGGL((tree_attn_kernel<1, 2>), grid, dim3(128), lds, st, a);
   } else if (p.rt == 2) {
-    auto kern = out_bf16 ? tree_attn_kernel<2, 2, 2> : tree_attn_kernel<2, 2, 3>;
-    hipLaunchKernelGGL(kern, grid, dim3(256), lds, st, a);
+    hipLaunchKernelGGL((tree_attn_kernel<2, 2>), grid, dim3(256), lds, st, a);
   } else {
-    auto kern = out_bf16 ? tree_attn_kernel<4, 1, 2> : tree_attn_kernel<4, 1, 3>;
-    hipLaunchKernelGGL(kern, grid, dim3(256), lds, st, a);
+    hipLaunchKernelGGL((tree_attn_kernel<4, 1>), grid, dim3(256), lds, st, a);
   }
   if (p.nsplit > 1)
     hipLaunchKernelGGL(tree_merge_kernel, dim3((unsigned)((T * H + 3) / 4)), dim3(256), 0, st, a);
