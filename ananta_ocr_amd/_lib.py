@@ -113,6 +113,7 @@ SIGNATURES = {
                               _p, _l, _p]),
     "dash_copy_pages": (_i, [_i, _p, _p, _p, _p, _i, _i, _p]),
     "dash_keep_rows": (_i, [_i, _p, _p, _p, _l, _p, _p, _p, _l, _i, _i, _i, _i, _i, _p]),
+    "dash_keep_lens": (_i, [_p, _l, _p, _p, _p, _i, _i, _p, _p, _p, _p, _p]),
     "dash_fork_pages": (_i, [_p, _i, _p, _l, _i, _i, _p, _p, _p, _i, _i, _p, _p, _p, _p]),
     "dash_reserve_pages": (_i, [_p, _i, _p, _l, _i, _i, _p, _p, _i, _p, _p, _p, _p]),
     "dash_free_pages": (_i, [_p, _i, _p, _l, _i, _i, _p, _p, _i, _p]),

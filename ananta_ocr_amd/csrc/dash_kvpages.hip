@@ -142,6 +142,29 @@ __global__ __launch_bounds__(kWave) void keep_rows_kernel(KvCaches a, const int3
   }
 }
 
+// What a step leaves of every row: its accepted nodes stand where the row holds the slot of the last of
+// them, which is the highest (path is strictly increasing), and none does where it does not, as after a
+// reserve that was refused.  stand: how many stand; kept: the row's tokens; context: its context;
+// summed: the tokens whose block summaries changed (0: none).  One lane a row, three dependent loads.
+__global__ __launch_bounds__(256) void keep_lens_kernel(const int32_t* path, int64_t path_st,
+                                                        const int32_t* count, const int32_t* ctx,
+                                                        const int32_t* lens, int B, int max_n,
+                                                        int32_t* stand, int32_t* kept,
+                                                        int32_t* context, int32_t* summed) {
+  const int b = blockIdx.x * 256 + threadIdx.x;
+  if (b >= B) return;
+  const int n = min(count[b], max_n), c = ctx[b], len = lens[b];
+  bool ok = false;
+  if (n > 0 && c >= 0) {
+    const int p = path[b * path_st + n - 1];
+    ok = p >= n - 1 && (int64_t)c + p < len;
+  }
+  stand[b] = ok ? n : 0;
+  kept[b] = ok ? c + n : len;
+  context[b] = ok ? c + n : c;
+  summed[b] = ok ? c + n : 0;
+}
+
 // Sum of v over the work-group's earlier threads; `total` gets the sum over all.
 __device__ __forceinline__ int block_exclusive(int v, int* sW, int& total) {
   const int lane = wave_lane(), wv = threadIdx.x / kWave;
@@ -542,6 +565,22 @@ extern "C" int dash_keep_rows(int num_caches, void* const* caches, const int64_t
   return kv_launches<KeepOp>(caches, desc, num_caches, B, stream, path, path_stride, count,
                              context_lens, block_table, table_stride, P, page_size, num_pages,
                              max_query_len);
+}
+
+extern "C" int dash_keep_lens(const int32_t* path, int64_t path_stride, const int32_t* count,
+                              const int32_t* context_lens, const int32_t* lens, int B,
+                              int max_query_len, int32_t* stand, int32_t* kept,
+                              int32_t* new_context, int32_t* summed, void* stream) {
+  using namespace dash;
+  if (B < 0 || max_query_len < 0) return kErrInvalid;
+  if (B == 0) return kOk;
+  if ((max_query_len > 0 && !path) || !count || !context_lens || !lens || !stand || !kept ||
+      !new_context || !summed)
+    return kErrInvalid;
+  hipLaunchKernelGGL(keep_lens_kernel, dim3(B / 256 + 1), dim3(256), 0, (hipStream_t)stream, path,
+                     path_stride, count, context_lens, lens, B, max_query_len, stand, kept,
+                     new_context, summed);
+  return kv_status();
 }
 
 extern "C" int dash_fork_pages(int32_t* refs, int num_pages, int32_t* block_table,

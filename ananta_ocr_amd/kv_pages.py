@@ -144,6 +144,20 @@ def keep_rows(caches, path, count, context_lens, table):
             caches.page_size, caches.num_pages, n, _stream()), "dash_keep_rows")
 
 
+def _keep_lens(path, count, context_lens, lens):
+    """(stand, kept, new_context, summed) of a verified step's rows, int32 [B] each
+    (dash_keep_lens)."""
+    B, n = path.shape
+    for x, what in ((count, "count"), (context_lens, "context_lens"), (lens, "lens")):
+        _shape(x, (B,), what)
+    with _device(lens, path, count, context_lens):
+        p, c, ctx, ln = (_i32(x) for x in (path, count, context_lens, lens))
+        out = _ints(lens.device, B, B, B, B)
+        _lib.check(_lib.load().dash_keep_lens(_ptr(p), n, _ptr(c), _ptr(ctx), _ptr(ln), B, n,
+                                              *(_ptr(x) for x in out), _stream()), "dash_keep_lens")
+    return out
+
+
 def _state(refs, table, lens, page_size):
     if refs.dim() != 1 or refs.numel() == 0 or table.dim() != 2:
         raise ValueError("refs [num_pages] and table [R, P] are needed")
@@ -193,7 +207,7 @@ def reserve_pages(refs, table, lens, new_lens, page_size):
     page of its own for the partly filled last page of a growing row that another row shares.
     refs, table and lens in place.  Returns (ok, from_pages [R], to_pages [R]) with the pages to
     copy.  ok is 0, and nothing changed, where a length does not fit the table or pages do not
-    suffice."""
+    suffice; the new tokens then have no pages of their own to be written to."""
     _state(refs, table, lens, page_size)
     _in_place(refs=refs, table=table, lens=lens)
     _shape(new_lens, lens.shape, "new_lens")
@@ -279,11 +293,16 @@ class PagePool:
 
     def keep(self, path, count, context_lens):
         """After a verification of the rows' trees (path and count of tree.verify_tree; a row
-        without nodes has count 0 and stays): the accepted rows moved up, the rest given back."""
-        keep_rows(self.caches, path, count, context_lens, self.table)
-        kept = torch.where(count > 0, (context_lens + count).to(torch.int32), self.lens)
-        self.free(kept)
-        return kept
+        without nodes has count 0 and stays): the accepted rows moved up, the rest given back.
+        A row that does not hold the slots of its accepted nodes, as after a reserve that was
+        refused, stays as it is: none of them stands.  Returns the rows' tokens [rows] int32."""
+        return self._keep(path, count, context_lens)[1]
+
+    def _keep(self, path, count, context_lens):
+        step = _keep_lens(path, count, context_lens, self.lens)
+        keep_rows(self.caches, path, step[0], context_lens, self.table)
+        self.free(step[1])
+        return step
 
     def compact(self):
         """The pages in use moved to the lowest numbers, in the caches too."""

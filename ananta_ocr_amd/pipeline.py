@@ -249,14 +249,13 @@ def commit_tree(pool, path, count, context_lens, layers=()):
     moved up in the caches of ``pool`` (kv_pages.PagePool, whose row b is request b), the others
     given back with their pages, and for every (state, idx_k, head_cls) of ``layers`` (its
     KBarPageCache and paged index keys) the block summaries are recomputed from the step's first
-    block on.  Returns the new context lengths [B] int32 (requests without nodes keep theirs)."""
+    block on.  Returns the new context lengths [B] int32 (requests without nodes keep theirs, and so
+    do those whose room pool.reserve refused: nothing of their step stands, its next token neither)."""
     with tree._device(pool.lens, path, count):
         ctx = context_lens.to(device=pool.lens.device, dtype=torch.int32)
-        kept = pool.keep(path, count, ctx)
-        new = torch.where(count > 0, kept, ctx)
-        bs = pool.page_size
         # (a request that stays may share its last page with a longer one, whose summary it holds)
-        lens = torch.where(count > 0, kept, 0) if layers else None
+        _, _, new, lens = pool._keep(path, count, ctx)
+        bs = pool.page_size
         for state, idx_k, head_cls in layers:
             if ops.kbar_pages_ok(idx_k, state.kbar, bs):
                 ops.kbar_pages(idx_k, head_cls, ctx, lens, pool.table, state.kbar, bs)

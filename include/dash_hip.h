@@ -753,6 +753,15 @@ int dash_keep_rows(int num_caches, void* const* caches, const int64_t* desc, con
                    const int32_t* block_table, int64_t table_stride, int B, int P, int page_size,
                    int num_pages, int max_query_len, void* stream);
 
+/* What a verified step leaves of rows of lens[b] tokens (path and count as above): where row b holds
+ * slot context_lens[b] + path[b][count[b] - 1], stand = count and kept = new_context = summed =
+ * context_lens + count; else (its reserve was refused, or it has no nodes) stand = summed = 0,
+ * kept = lens and new_context = context_lens.  Each [B]. */
+int dash_keep_lens(const int32_t* path, int64_t path_stride, const int32_t* count,
+                   const int32_t* context_lens, const int32_t* lens, int B, int max_query_len,
+                   int32_t* stand, int32_t* kept, int32_t* new_context, int32_t* summed,
+                   void* stream);
+
 /* Row dst_rows[i] (empty) becomes row src_rows[i]: its filled pages shared, a partly filled last one
  * replaced by a page of its own, whose content is to be copied from_pages[i] -> to_pages[i] (-1: none).
  * ok = 1; or ok = 0 and nothing changed, where a row is out of range, a target filled, repeated or a
