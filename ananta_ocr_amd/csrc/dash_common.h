@@ -138,9 +138,12 @@ __device__ __forceinline__ int seq_length(const int32_t* cu, const int32_t* lens
 
 // Rows r0 .. r0 + n - 1 of sequence b of a packed batch of T rows, at most `most` (trees of drafted
 // tokens): prefix sums that do not fit the rows are cut to them, so that no row past T is touched.
-__device__ __forceinline__ int packed_rows(const int32_t* cu, int b, int64_t T, int most, int64_t& r0) {
-  r0 = min(max((int64_t)cu[b], (int64_t)0), T);
-  return (int)max(min(min((int64_t)cu[b + 1], T) - r0, (int64_t)most), (int64_t)0);
+__host__ __device__ __forceinline__ int packed_rows(const int32_t* cu, int b, int64_t T, int most,
+                                                    int64_t& r0) {
+  const int64_t c0 = cu[b], c1 = cu[b + 1];
+  r0 = c0 < 0 ? 0 : c0 < T ? c0 : T;
+  const int64_t n = (c1 < T ? c1 : T) - r0;
+  return (int)(n < 0 ? 0 : n < most ? n : most);
 }
 
 // Flat row index of (sequence b, token t) for per-token outputs such as the

@@ -307,7 +307,7 @@ __device__ __forceinline__ void split3(float x, __bf16& h, __bf16& m, __bf16& l)
 }
 
 __global__ __launch_bounds__(256) void scores_mfma_kernel(
-    const float* __restrict__ idx_q, SeqLayout lay_q, const int32_t* __restrict__ cu_q, int Lq,
+    const float* __restrict__ idx_q, SeqLayout lay_q, const int32_t* __restrict__ cu_q, int64_t T, int Lq,
     const int32_t* __restrict__ q_pos, const float* __restrict__ kbar, int64_t kb_sb,
     const int32_t* __restrict__ cu_k, const int32_t* __restrict__ lens_k, int S, int bs,
     int local_blocks, int nblk_cap, float inv_sqrt_d, float* __restrict__ z, int64_t z_stride,
@@ -315,7 +315,9 @@ __global__ __launch_bounds__(256) void scores_mfma_kernel(
   __shared__ __attribute__((aligned(16))) bf16 sK[3][kSmBlk * 128];
   __shared__ int sLim[kSmRows];
   const int b = blockIdx.z;
-  const int nq = cu_q ? (cu_q[b + 1] - cu_q[b]) : Lq;
+  // the sequence's rows q0 .. q0 + nq - 1 of the T packed ones (or of the B Lq others)
+  int64_t q0 = (int64_t)b * Lq;
+  const int nq = cu_q ? packed_rows(cu_q, b, T, INT_MAX, q0) : Lq;
   const int r0 = blockIdx.x * kSmRows;
   const int c0 = blockIdx.y * kSmBlk;
   if (r0 >= nq) return;
@@ -327,7 +329,7 @@ __global__ __launch_bounds__(256) void scores_mfma_kernel(
     const int r = r0 + tid;
     int lim = INT_MIN;
     if (r < nq) {
-      const int pos = q_pos ? q_pos[token_row(cu_q, b, r, Lq)] : r;
+      const int pos = q_pos ? q_pos[q0 + r] : r;
       lim = (pos >= 0 ? pos / bs : -((-pos + bs - 1) / bs)) - local_blocks;
     }
     sLim[tid] = lim;
@@ -336,7 +338,7 @@ __global__ __launch_bounds__(256) void scores_mfma_kernel(
   if (!__syncthreads_or(c0 <= my_max && c0 < nblk_b)) {
     for (int e = tid; e < kSmRows * kSmBlk; e += 256) {
       const int r = r0 + e / kSmBlk, c = c0 + e % kSmBlk;
-      if (r < nq && c < nblk_cap) z[token_row(cu_q, b, r, Lq) * z_stride + c] = kScoreNeg;
+      if (r < nq && c < nblk_cap) z[(q0 + r) * z_stride + c] = kScoreNeg;
     }
     return;
   }
@@ -344,7 +346,7 @@ __global__ __launch_bounds__(256) void scores_mfma_kernel(
   // its 64 dims are loaded now, in flight during the k_bar split
   const int mrow = lane & 31, half = lane >> 5;
   const int rq = min(r0 + wv * 32 + mrow, nq - 1);
-  const float* qr = idx_q + lay_q.row(b, rq) + 8 * half;
+  const float* qr = idx_q + (cu_q ? (q0 + rq) * lay_q.stride_t : lay_q.row(b, rq)) + 8 * half;
   float4 qv[16];
 #pragma unroll
   for (int kk = 0; kk < 8; ++kk) {
@@ -447,7 +449,7 @@ __global__ __launch_bounds__(256) void scores_mfma_kernel(
     const int r = r0 + wv * 32 + rr;
     const float4 v = *(const float4*)(so + rr * kSmBlk + cq);
     if (r < nq) {
-      float* zr = z + token_row(cu_q, b, r, Lq) * z_stride + c0 + cq;
+      float* zr = z + (q0 + r) * z_stride + c0 + cq;
       if (c0 + cq + 3 < nblk_cap && ((uintptr_t)zr & 15) == 0) {
         *(float4*)zr = v;
       } else {
@@ -1308,8 +1310,8 @@ extern "C" int dash_block_scores(const float* idx_q, int64_t iq_sb, int64_t iq_s
   if (vec && d == 128) {
     dim3 g2((Lq + kSmRows - 1) / kSmRows, (nblk_cap + kSmBlk - 1) / kSmBlk, B);
     hipLaunchKernelGGL(scores_mfma_kernel, g2, dim3(256), 0, (hipStream_t)stream, idx_q, lay, cu_q,
-                       Lq, q_pos, kbar, kb_sb, cu_k, lens_k, S, block_size, local_blocks, nblk_cap,
-                       (float)(1.0 / sqrt((double)d)), z, z_stride, (const int32_t*)nullptr,
+                       INT64_MAX, Lq, q_pos, kbar, kb_sb, cu_k, lens_k, S, block_size, local_blocks,
+                       nblk_cap, (float)(1.0 / sqrt((double)d)), z, z_stride, (const int32_t*)nullptr,
                        (int64_t)0, 0);
     return launch_status();
   }
@@ -1386,7 +1388,7 @@ extern "C" int dash_extend_scores(const float* idx_q, int64_t iq_st, const float
   const SeqLayout lq{cu_seqlens_q, nullptr, 0, 0, 0, iq_st, 1};
   dim3 grid((max_query_len + kSmRows - 1) / kSmRows, (nblk + kSmBlk - 1) / kSmBlk, B);
   hipLaunchKernelGGL(scores_mfma_kernel, grid, dim3(256), 0, st, idx_q, lq, cu_seqlens_q,
-                     max_query_len, q_pos, pool, (int64_t)0, (const int32_t*)nullptr, seq_lens,
+                     (int64_t)T, max_query_len, q_pos, pool, (int64_t)0, (const int32_t*)nullptr, seq_lens,
                      nblk * block_size, block_size, local_blocks, nblk, inv, z, z_stride, block_table,
                      table_stride, pool_rows);
   return launch_status();
@@ -1434,7 +1436,7 @@ extern "C" int dash_tree_scores(const float* idx_q, int64_t iq_st, const int32_t
   const SeqLayout lq{cu_seqlens_q, nullptr, 0, 0, 0, iq_st, 1};
   dim3 grid((max_query_len + kSmRows - 1) / kSmRows, (nblk + kSmBlk - 1) / kSmBlk, B);
   hipLaunchKernelGGL(scores_mfma_kernel, grid, dim3(256), 0, st, idx_q, lq, cu_seqlens_q,
-                     max_query_len, q_pos, pool, (int64_t)0, (const int32_t*)nullptr, context_lens,
+                     (int64_t)T, max_query_len, q_pos, pool, (int64_t)0, (const int32_t*)nullptr, context_lens,
                      nblk * block_size, block_size, local_blocks, nblk,
                      (float)(1.0 / sqrt((double)d)), z, z_stride, block_table, table_stride, pool_rows);
   return launch_status();

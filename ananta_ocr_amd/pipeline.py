@@ -199,7 +199,8 @@ def tree_step(state, q, k_cache, v_cache, idx_q, block_size, local_blocks, idx_s
     the window.  q [T,H,D] bf16, k_cache / v_cache [pages, block_size, Hkv, D] bf16 (H a multiple
     of Hkv), idx_q [T,d] fp32, block_table [B,P] int32, context_lens [B], cu_seqlens_q [B+1],
     max_query_len at least the largest tree, block_cand [T,P] the blocks a row may route to (None: any).
-    Rows past cu_seqlens_q's last (a batch padded to a fixed size) come out with nothing in particular.
+    Rows past cu_seqlens_q's last (a batch padded to a fixed size) come out with nothing in particular;
+    prefix sums past the T rows are cut to them.
     Returns out [T,H,D] (out_dtype)."""
     if not getattr(state, "paged", False):
         raise NotImplementedError("tree_step takes a k_bar page pool (KBarPageCache)")
@@ -231,8 +232,8 @@ def tree_step(state, q, k_cache, v_cache, idx_q, block_size, local_blocks, idx_s
                                          right=True).clamp_(max=B - 1)
             q_pos = ctx.index_select(0, row_seq) + depth
             z = ops.block_scores(idx_q.reshape(1, T, -1), kb_seq, block_size, local_blocks,
-                                 q_pos=q_pos, cu_seqlens=cu, max_seqlen=max_query_len, key_lens=ctx,
-                                 S=P * block_size)
+                                 q_pos=q_pos, cu_seqlens=cu.clamp(0, T), max_seqlen=max_query_len,
+                                 key_lens=ctx, S=P * block_size)
             row_nblk = ((ctx + block_size - 1) // block_size).index_select(0, row_seq)
         idx, bias, valid = ops.route(z, block_cand, idx_scale, floor, sigma, K, topm,
                                      row_nblk=row_nblk, width=width)

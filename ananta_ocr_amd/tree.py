@@ -6,7 +6,7 @@ nodes of sequence b, node 0 its root (the newest sampled token, whose key and va
 committed yet), and ``parents`` holds each node's parent within its sequence, an earlier node.
 The key and value of node i are written to the cache at slot context_len + i before the
 attention.  max_query_len is at least the largest tree; rows that no tree has (a batch padded to a
-fixed size) come out with nothing in particular.  ``pipeline.tree_step`` and
+fixed size) come out with nothing in particular, and prefix sums past the rows are cut to them.  ``pipeline.tree_step`` and
 ``pipeline.commit_tree`` are the whole step.
 
 Like the other wrappers these take tensors of one GPU, allocate their outputs with torch, call one

@@ -643,7 +643,8 @@ int64_t dash_decode_step_scratch_bytes(void);
  * Trees of drafted tokens.  Row cu_seqlens_q[b] + i (cu_seqlens_q [B + 1], T rows in all, at most
  * max_query_len <= 256 a sequence) is node i of sequence b, node 0 its root; parents [T] holds
  * each node's parent within its sequence, an earlier node (anything else: none).  The key and
- * value of node i lie in the cache at slot context_lens[b] + i.
+ * value of node i lie in the cache at slot context_lens[b] + i.  Prefix sums that do not fit the T rows
+ * are cut to them.
  */
 
 /* mask [T, words] (words = ceil(max_query_len / 64)): bit m of row (b, i) is set where node m is
