@@ -444,16 +444,19 @@ __global__ __launch_bounds__(kVfThreads) void verify_draw_kernel(VerifyArgs a) {
     if (tid == 0) a.token[b] = -1;
     return;
   }
-  const double want = u * total;
+  // a number of 1 is exceeded by no running sum, however its additions were grouped
+  const double want = u < 1.0 ? u * total : (double)INFINITY;
   int first = INT32_MAX, last = -1;
   {
     double x = before;
     for (int c = c0; c < c1; ++c) {
       const double2 z = sum_of(c);
       const double y = rest ? z.x : z.y;
-      if (y > 0.0) last = c;
       x += y;
-      if (x > want) { first = c; break; }
+      if (y > 0.0) {                          // (a chunk without anything holds no token to draw)
+        last = c;
+        if (x > want) { first = c; break; }
+      }
     }
   }
   vf_ends(first, last, sE);

@@ -718,7 +718,8 @@ int dash_verify_tree_workspace_size(int B, int64_t T, int V, int greedy, int64_t
  * node's best token (0 for a row with nothing above -inf), else drawn by uniforms[root] from what is
  * left at the last node: the first id whose running sum exceeds uniforms[root] times the whole (the
  * row itself where nothing is left, -1 where that holds nothing above 0 either).  Probabilities that
- * are not above 0 count as 0; a token outside [0, V) is rejected.  Sums in 64 bits.
+ * are not above 0 count as 0, a uniform of 1 or more draws the last id left; a token outside [0, V) is
+ * rejected.  Sums in 64 bits.
  */
 int dash_verify_tree(const void* target, int64_t target_stride, const void* draft,
                      int64_t draft_stride, int dtype, const void* tokens, int tokens_int64,
