@@ -262,7 +262,8 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void tree_attn_kernel(TreeArgs a) 
     }
     if (l1 > l0) {
       // a block's first slot in a row wins: the smallest slot first, then its bias in its place (a
-      // bias whose bits could be a slot's number counts as 0)
+      // bias whose bits could be a slot's number counts as 0, and a NaN is one whose bits are not
+      // kTrNotNamed)
       auto place_of = [&](int c) {
         return c < 0 ? -1 : sPref[c >> 5] + __popc(sBits[c >> 5] & ((1u << (c & 31)) - 1u)) - l0;
       };
@@ -278,7 +279,7 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void tree_attn_kernel(TreeArgs a) 
         uint32_t& to = sBias[l][i / a.K];
         if (to != (uint32_t)(i % a.K)) continue;
         const float x = (RT == 4 ? a.bias[s0 + i] : sSlotBias[i]) * 1.4426950408889634f;
-        to = __float_as_uint(fabsf(x) < 1e-30f ? 0.f : x);
+        to = x != x ? 0x7fc00000u : __float_as_uint(fabsf(x) < 1e-30f ? 0.f : x);
       }
     }
     __syncthreads();
