@@ -136,6 +136,10 @@ __device__ __forceinline__ int seq_length(const int32_t* cu, const int32_t* lens
   return S;
 }
 
+// Whether a launch may have `groups` work-groups of `threads` in a dimension: its work-items are counted
+// in 32 bits.
+inline bool fits_grid(int64_t groups, int threads) { return groups <= (int64_t)UINT32_MAX / threads; }
+
 // Rows r0 .. r0 + n - 1 of sequence b of a packed batch of T rows, at most `most` (trees of drafted
 // tokens): prefix sums that do not fit the rows are cut to them, so that no row past T is touched.
 __host__ __device__ __forceinline__ int packed_rows(const int32_t* cu, int b, int64_t T, int most,

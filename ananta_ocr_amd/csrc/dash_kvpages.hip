@@ -46,41 +46,43 @@ __device__ __forceinline__ const KvCache& kv_cache_of(const KvCaches& a, int t) 
 
 typedef uint32_t KvVec __attribute__((ext_vector_type(4)));   // 16 bytes
 constexpr int kCpThreads = 256, kCpUnroll = 4;
+constexpr int kCpPairs = 65535;       // of a launch's grid
 
-// One work-group per (pair, task); a task is kCpThreads * kCpUnroll units of one layer's page.  Bound
-// by HBM: 730 MB read and written in 137 us, 5.3 TB/s; 149 us where the loads and stores leave their
+// One work-group per (task, pair), pairs past the grid's kCpPairs in a loop; a task is kCpThreads *
+// kCpUnroll units of one layer's page.  Bound by HBM: 730 MB read and written in 137 us, 5.3 TB/s; 149 us where the loads and stores leave their
 // lines in the L2 (a page is not read again here), 225 with eight units a lane in flight instead of four.
 template <typename U>
 __global__ __launch_bounds__(kCpThreads) void copy_pages_kernel(KvCaches a, const int32_t* frm,
-                                                                const int32_t* to, int num_pages,
-                                                                int tasks) {
-  const int pair = blockIdx.x / tasks, t = blockIdx.x % tasks;
-  const int f = frm[pair], d = to[pair];
-  if (f < 0 || d < 0 || f >= num_pages || d >= num_pages || f == d) return;
-  const KvCache& c = kv_cache_of(a, t);
-  const int rel = t - c.task0;
-  const int l = rel / c.per, ch = rel % c.per;
-  char* const lb = c.base + l * c.layer;
-  const char* const sp = lb + f * c.page;
-  char* const dp = lb + d * c.page;
-  const int64_t units = c.units;
-  const int64_t u0 = (int64_t)ch * (kCpThreads * kCpUnroll) + threadIdx.x;
-  U x[kCpUnroll];
-  int64_t off[kCpUnroll];
+                                                                const int32_t* to, int pairs,
+                                                                int num_pages) {
+  for (int64_t pair = blockIdx.y; pair < pairs; pair += gridDim.y) {
+    const int f = frm[pair], d = to[pair];
+    if (f < 0 || d < 0 || f >= num_pages || d >= num_pages || f == d) continue;
+    const KvCache& c = kv_cache_of(a, blockIdx.x);
+    const int rel = blockIdx.x - c.task0;
+    const int l = rel / c.per, ch = rel % c.per;
+    char* const lb = c.base + l * c.layer;
+    const char* const sp = lb + f * c.page;
+    char* const dp = lb + d * c.page;
+    const int64_t units = c.units;
+    const int64_t u0 = (int64_t)ch * (kCpThreads * kCpUnroll) + threadIdx.x;
+    U x[kCpUnroll];
+    int64_t off[kCpUnroll];
 #pragma unroll
-  for (int k = 0; k < kCpUnroll; ++k) {
-    const int64_t u = u0 + k * kCpThreads;
-    if (c.segu == 0) {
-      off[k] = u * (int)sizeof(U);
-    } else {
-      const int64_t piece = u / c.segu;
-      off[k] = (piece / c.n2) * c.s1 + (piece % c.n2) * c.s2 + (u - piece * c.segu) * (int)sizeof(U);
+    for (int k = 0; k < kCpUnroll; ++k) {
+      const int64_t u = u0 + k * kCpThreads;
+      if (c.segu == 0) {
+        off[k] = u * (int)sizeof(U);
+      } else {
+        const int64_t piece = u / c.segu;
+        off[k] = (piece / c.n2) * c.s1 + (piece % c.n2) * c.s2 + (u - piece * c.segu) * (int)sizeof(U);
+      }
+      if (u < units) x[k] = __builtin_nontemporal_load((const U*)(sp + off[k]));
     }
-    if (u < units) x[k] = __builtin_nontemporal_load((const U*)(sp + off[k]));
-  }
 #pragma unroll
-  for (int k = 0; k < kCpUnroll; ++k)
-    if (u0 + k * kCpThreads < units) __builtin_nontemporal_store(x[k], (U*)(dp + off[k]));
+    for (int k = 0; k < kCpUnroll; ++k)
+      if (u0 + k * kCpThreads < units) __builtin_nontemporal_store(x[k], (U*)(dp + off[k]));
+  }
 }
 
 // Rows ctx + path[i] -> ctx + i, 1 <= i < count, of one sequence and one unit column of one
@@ -499,14 +501,14 @@ static int kv_launches(void* const* base, const int64_t* desc, int num, int64_t 
       if (!kv_fill(a, base + c0, desc + 8 * c0, std::min(kKvMaxCaches, num - c0), Op<KvVec>::kRows,
                    Op<KvVec>::kTask, &tasks))
         return kErrInvalid;
-      if (tasks * count > INT32_MAX) return kErrUnsupported;
+      if (!fits_grid(tasks, Op<KvVec>::kThreads)) return kErrUnsupported;
     }
   for (int c0 = 0; c0 < num; c0 += kKvMaxCaches) {
     const int unit = kv_fill(a, base + c0, desc + 8 * c0, std::min(kKvMaxCaches, num - c0), Op<KvVec>::kRows,
                              Op<KvVec>::kTask, &tasks);
     if (unit == 0) return kErrInvalid;
     if (tasks == 0) continue;
-    if (tasks * count > INT32_MAX) return kErrUnsupported;
+    if (!fits_grid(tasks, Op<KvVec>::kThreads)) return kErrUnsupported;
     if (unit == 16) Op<KvVec>::launch(a, tasks, count, st, args...);
     else if (unit == 4) Op<uint32_t>::launch(a, tasks, count, st, args...);
     else if (unit == 2) Op<uint16_t>::launch(a, tasks, count, st, args...);
@@ -520,17 +522,18 @@ static int kv_launches(void* const* base, const int64_t* desc, int num, int64_t 
 template <typename U>
 struct CopyOp {
   static constexpr bool kRows = false;
-  static constexpr int kTask = kCpThreads * kCpUnroll;
+  static constexpr int kThreads = kCpThreads, kTask = kCpThreads * kCpUnroll;
   static void launch(const KvCaches& a, int64_t tasks, int64_t pairs, hipStream_t st, const int32_t* frm,
                      const int32_t* to, int num_pages) {
-    hipLaunchKernelGGL(copy_pages_kernel<U>, dim3((unsigned)(tasks * pairs)), dim3(kCpThreads), 0, st, a,
-                       frm, to, num_pages, (int)tasks);
+    hipLaunchKernelGGL(copy_pages_kernel<U>,
+                       dim3((unsigned)tasks, (unsigned)std::min<int64_t>(pairs, kCpPairs)),
+                       dim3(kCpThreads), 0, st, a, frm, to, (int)pairs, num_pages);
   }
 };
 template <typename U>
 struct KeepOp {
   static constexpr bool kRows = true;
-  static constexpr int kTask = kWave;
+  static constexpr int kThreads = kWave, kTask = kWave;
   static void launch(const KvCaches& a, int64_t tasks, int64_t B, hipStream_t st, const int32_t* path,
                      int64_t path_st, const int32_t* count, const int32_t* ctx, const int32_t* table,
                      int64_t table_st, int P, int page, int num_pages, int max_n) {
