@@ -625,6 +625,7 @@ extern "C" int dash_free_pages(int32_t* refs, int num_pages, int32_t* block_tabl
   if (!refs || !block_table || !lens || !keep_lens || num_pages < 0 || R < 0 || P < 0 ||
       page_size <= 0)
     return kErrInvalid;
+  if (R > kKvMaxRows) return kErrUnsupported;
   if (R == 0) return kOk;
   hipLaunchKernelGGL(free_pages_kernel, dim3(R), dim3(256), 0, (hipStream_t)stream, refs, num_pages,
                      block_table, table_stride, P, lens, keep_lens, page_size);
@@ -642,7 +643,7 @@ extern "C" int dash_compact_pages(const int32_t* refs, int num_pages, const int3
   const int64_t entries = (int64_t)R * P;
   if (entries > 0 && (!block_table || !lens || !new_table || (num_pages > 0 && !place)))
     return kErrInvalid;
-  if ((entries + 255) / 256 > INT32_MAX) return kErrUnsupported;
+  if (R > kKvMaxRows || !fits_grid((entries + 255) / 256, 256)) return kErrUnsupported;
   hipStream_t st = (hipStream_t)stream;
   if (num_pages > 0)
     hipLaunchKernelGGL(compact_plan_kernel, dim3(1), dim3(kKvThreads), 0, st, refs, num_pages,

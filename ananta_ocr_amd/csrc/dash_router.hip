@@ -1405,7 +1405,7 @@ extern "C" int dash_kbar_pages(const float* idx_k, int64_t ik_st, int64_t ik_sp,
   if (!idx_k || !head_cls || !first_tokens || !seq_lens || !block_table || !pool) return kErrInvalid;
   if (d != kKbD || block_size <= 0 || block_size > kKbMaxBs || ik_st % 4 != 0 || ik_sp % 4 != 0 ||
       (uintptr_t)idx_k % 16 != 0 || (uintptr_t)head_cls % 16 != 0 || (uintptr_t)pool % 16 != 0 ||
-      B > 65535)
+      B > 65535 || !fits_grid(nblk, 256) || (int64_t)nblk * block_size > INT32_MAX)
     return kErrUnsupported;
   const SeqLayout lk{nullptr, block_table, table_stride, 0, ik_sp, ik_st, block_size};
   hipLaunchKernelGGL(kbar128_kernel, dim3(nblk, B), dim3(256), 0, (hipStream_t)stream, idx_k, lk,
@@ -1428,7 +1428,8 @@ extern "C" int dash_tree_scores(const float* idx_q, int64_t iq_st, const int32_t
       !row_nblk || !z)
     return kErrInvalid;
   if (d != kKbD || block_size <= 0 || iq_st % 4 != 0 || (uintptr_t)idx_q % 16 != 0 ||
-      (uintptr_t)pool % 16 != 0 || B > 65535)
+      (uintptr_t)pool % 16 != 0 || B > 65535 || max_query_len > 256 || nblk > 65535 * kSmBlk ||
+      T > INT32_MAX - 255)
     return kErrUnsupported;
   hipStream_t st = (hipStream_t)stream;
   hipLaunchKernelGGL(extend_rows_kernel, dim3((T + 255) / 256), dim3(256), 0, st, cu_seqlens_q,

@@ -717,7 +717,8 @@ extern "C" int dash_tree_masks(const int32_t* parents, const int32_t* cu_seqlens
   if (B < 0 || T < 0 || max_query_len < 0) return kErrInvalid;
   if (B == 0 || T == 0) return kOk;
   if (!parents || !cu_seqlens_q || !mask || !depth || max_query_len == 0) return kErrInvalid;
-  if (max_query_len > kTrMaxNodes || words != (max_query_len + 63) / 64) return kErrUnsupported;
+  if (max_query_len > kTrMaxNodes || words != (max_query_len + 63) / 64 || !fits_grid(B, kTrMaxNodes))
+    return kErrUnsupported;
   hipLaunchKernelGGL(tree_masks_kernel, dim3(B), dim3(kTrMaxNodes), 0, (hipStream_t)stream, parents,
                      cu_seqlens_q, T, words, max_query_len, (uint64_t*)mask, depth);
   const hipError_t e = hipGetLastError();
@@ -783,7 +784,9 @@ extern "C" int dash_attn_tree(
   const TreePlan p = tree_plan(B, H, Hkv, max_query_len, K, S, block_size, local_window);
   a.groups = p.groups; a.nsplit = p.nsplit;
   const int64_t wgs = (int64_t)B * Hkv * p.groups * p.nsplit;
-  if (wgs > INT32_MAX || T * H > INT32_MAX) return kErrUnsupported;
+  if (T > INT32_MAX || !fits_grid(wgs, 64 * (p.rt == 1 ? 2 : 4)) || T * H > INT32_MAX ||
+      (p.nsplit > 1 && !fits_grid((T * H + 3) / 4, 256)))
+    return kErrUnsupported;
   if (p.nsplit > 1) {
     if (!workspace || workspace_bytes < tree_workspace(p, T, H) || (uintptr_t)workspace % 16 != 0)
       return kErrWorkspace;

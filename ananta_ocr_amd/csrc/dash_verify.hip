@@ -568,7 +568,7 @@ extern "C" int dash_verify_tree(const void* target, int64_t target_stride, const
   if (draft && !uniforms) return kErrInvalid;
   if (max_query_len > kVfMaxNodes || B > 65535 || V > (1 << 30)) return kErrUnsupported;
   const VerifyLayout L = verify_layout(B, T, V, !uniforms);
-  if (T * L.chunks > INT32_MAX) return kErrUnsupported;
+  if (!uniforms && (T > INT32_MAX || !fits_grid(T * L.chunks, kVfThreads))) return kErrUnsupported;
   if (!workspace || workspace_bytes < L.total || (uintptr_t)workspace % 256 != 0) return kErrWorkspace;
   char* w = (char*)workspace;
   VerifyArgs a = {};
