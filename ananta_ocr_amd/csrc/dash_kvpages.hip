@@ -611,7 +611,8 @@ extern "C" int dash_reserve_pages(int32_t* refs, int num_pages, int32_t* block_t
   if (!refs || !block_table || !lens || !new_lens || !ok || !from_pages || !to_pages ||
       num_pages < 0 || R < 0 || P < 0 || page_size <= 0)
     return kErrInvalid;
-  if (R > kKvMaxRows) return kErrUnsupported;
+  // (the pages that all rows want, at most R * P, are added up in 32 bits)
+  if (R > kKvMaxRows || (int64_t)R * P > INT32_MAX) return kErrUnsupported;
   hipLaunchKernelGGL(reserve_pages_kernel, dim3(1), dim3(kKvThreads), 0, (hipStream_t)stream, refs,
                      num_pages, block_table, table_stride, R, P, lens, new_lens, page_size, ok,
                      from_pages, to_pages);

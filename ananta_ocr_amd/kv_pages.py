@@ -207,7 +207,8 @@ def reserve_pages(refs, table, lens, new_lens, page_size):
     page of its own for the partly filled last page of a growing row that another row shares.
     refs, table and lens in place.  Returns (ok, from_pages [R], to_pages [R]) with the pages to
     copy.  ok is 0, and nothing changed, where a length does not fit the table or pages do not
-    suffice; the new tokens then have no pages of their own to be written to."""
+    suffice; the new tokens then have no pages of their own to be written to.  Tables of at most
+    2^31 - 1 entries."""
     _state(refs, table, lens, page_size)
     _in_place(refs=refs, table=table, lens=lens)
     _shape(new_lens, lens.shape, "new_lens")

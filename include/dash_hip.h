@@ -775,7 +775,8 @@ int dash_fork_pages(int32_t* refs, int num_pages, int32_t* block_table, int64_t 
 /* Rows grow to new_lens [R] (shorter ones stay): pages for the blocks they lack, and a page of its
  * own for the partly filled last page of a growing row that another row shares, to be copied
  * from_pages[r] -> to_pages[r] (-1: none).  ok = 1, or 0 and nothing changed, where a length does not
- * fit the table, such a last entry names no page, or the free pages do not suffice. */
+ * fit the table, such a last entry names no page, or the free pages do not suffice.  R * P below
+ * 2^31. */
 int dash_reserve_pages(int32_t* refs, int num_pages, int32_t* block_table, int64_t table_stride, int R,
                        int P, int32_t* lens, const int32_t* new_lens, int page_size, int32_t* ok,
                        int32_t* from_pages, int32_t* to_pages, void* stream);

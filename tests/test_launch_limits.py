@@ -65,3 +65,10 @@ def test_launches_of_too_many_work_groups():
                 stream=None)
     for kw in (dict(nblk=16777216, block_size=1), dict(nblk=2 ** 26), dict(B=65536)):
         assert _call("dash_kbar_pages", **{**kbar, **kw}) == ERR_UNSUPPORTED, kw
+
+
+def test_tables_whose_wanted_pages_pass_32_bits():
+    """8,192 rows that each want 262,144 pages or more would add up to a number below 0."""
+    state = dict(num_pages=9, table_stride=1 << 18, R=8192, page_size=8, stream=None)
+    assert _call("dash_reserve_pages", **{**state, "P": 1 << 18}) == ERR_UNSUPPORTED
+    assert _call("dash_reserve_pages", **{**state, "R": 3, "P": 2 ** 31 - 1}) == ERR_UNSUPPORTED
