@@ -208,10 +208,11 @@ def tree_step(state, q, k_cache, v_cache, idx_q, block_size, local_blocks, idx_s
     if scale is None:
         scale = 1.0 / math.sqrt(D)
     width = max(1, min(int(K), int(topm))) if int(topm) > 0 else max(1, int(K))
-    if T == 0:                                   # no request has a node
-        out = torch.empty(0, H, D, dtype=out_dtype, device=q.device)
-        none = torch.empty(0, width, dtype=torch.int32, device=q.device)
-        return (out, (none, none.float(), none.bool()), none[:, 0]) if return_routing else out
+    if T == 0 or len(block_table) == 0:          # no request has a node
+        out = torch.empty(T, H, D, dtype=out_dtype, device=q.device)
+        none = torch.full((T, width), -1, dtype=torch.int32, device=q.device)
+        return (out, (none, torch.zeros_like(none, dtype=torch.float32), none >= 0), none[:, 0]) \
+            if return_routing else out
     with tree._device(q, k_cache, v_cache, idx_q, parents):
         ctx, cu, table = (x.to(device=q.device, dtype=torch.int32).contiguous()
                           for x in (context_lens, cu_seqlens_q, block_table))
