@@ -169,10 +169,12 @@ def _state(refs, table, lens, page_size):
 
 
 def _in_place(**ts):
-    """Tensors that a call writes: int32, with contiguous rows."""
+    """Tensors that a call writes: int32, with contiguous rows that do not overlap."""
     for name, t in ts.items():
-        if t.dtype != torch.int32 or (t.numel() > 1 and t.stride(-1) != 1):
+        if t.dtype != torch.int32 or (t.shape[-1] > 1 and t.stride(-1) != 1):
             raise ValueError(f"{name}: contiguous int32 rows are needed (written in place)")
+        if t.dim() > 1 and t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+            raise ValueError(f"{name}: rows that overlap (written in place)")
 
 
 def _ints(device, *sizes):

@@ -22,3 +22,21 @@ def test_steps_without_requests(width, rows):
     assert out.shape == (rows, 2, 128) and out.dtype == torch.bfloat16
     assert idx.shape == bias.shape == valid.shape == (rows, 3) and pos.shape == (rows,)
     assert not valid.any()
+
+
+def test_page_calls_refuse_rows_that_overlap():
+    """One row for all, or rows that share entries, cannot be written in place; a column of a wider
+    table, or a table of one row of any stride, can."""
+    refs, lens = torch.zeros(9, dtype=I32), torch.zeros(3, dtype=I32)
+    for table in (torch.zeros(1, 4, dtype=I32).expand(3, 4),
+                  torch.zeros(20, dtype=I32).as_strided((3, 4), (3, 1))):
+        for f, more in ((kv_pages.fork_pages, (lens[:1], lens[:1])), (kv_pages.reserve_pages, (lens,)),
+                        (kv_pages.free_pages, (lens,))):
+            with pytest.raises(ValueError, match="overlap"):
+                f(refs, table, lens, *more, 8)
+    for table in (torch.zeros(3, 7, dtype=I32)[:, 2:6], torch.zeros(3, 5, dtype=I32)[:, 1:2],
+                  torch.zeros(3, 4, dtype=I32)):
+        with pytest.raises(ValueError, match="GPU"):
+            kv_pages.reserve_pages(refs, table, lens, lens, 8)
+    with pytest.raises(ValueError, match="GPU"):
+        kv_pages.reserve_pages(refs, torch.zeros(1, 4, dtype=I32).expand(1, 4), lens[:1], lens[:1], 8)
