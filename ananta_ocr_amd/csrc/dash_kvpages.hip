@@ -8,10 +8,14 @@
 // in order, so that a result does not depend on how a launch ran: what is added up by atomics
 // is whole numbers.
 //
-// The table kernels run as one work-group: their data (a few kilobytes) lives in one L2, and
-// what bounds them is the latency of three or four dependent passes, not bandwidth: a fork of four
-// rows to sixteen 10 us, their growth 4.5, freeing them 3.2, the plan of a compaction 3 to 5.  The
-// copies are bound by HBM: 16 bytes a lane, several loads in flight before the first store.
+// Fork, reserve and the plan of a compaction run as one work-group, pass after pass with a barrier between
+// them.  For the tables of a serving batch (a few kilobytes) the latency of these passes bounds them: a fork
+// of four rows to sixteen 10 us (targets, sources, the entries' check, a prefix sum, the free pages' count,
+// the moves, the hand-out, the entries' sharing, the lengths), its growth 4.5, the plan 3 to 5.  Their time
+// grows with the entries and the pages, 1,024 lanes at a time: rows of 100 pages forked, 16 of them 11 us,
+// 128 44, 1,024 302, 4,096 1,198; grown, 16 rows 6 us, 1,024 (of a pool of 110,656 pages) 62, 4,096 (of
+// 442,432) 255.  Freeing takes a work-group a row, 3.1 us for twenty.  The copies are bound by HBM: 16 bytes a
+// lane, several loads in flight before the first store.
 
 #include "dash_common.h"
 
@@ -49,8 +53,10 @@ constexpr int kCpThreads = 256, kCpUnroll = 4;
 constexpr int kCpPairs = 65535;       // of a launch's grid
 
 // One work-group per (task, pair), pairs past the grid's kCpPairs in a loop; a task is kCpThreads *
-// kCpUnroll units of one layer's page.  Bound by HBM: 730 MB read and written in 137 us, 5.3 TB/s; 149 us where the loads and stores leave their
-// lines in the L2 (a page is not read again here), 225 with eight units a lane in flight instead of four.
+// kCpUnroll units of one layer's page.  Bound by HBM: 730 MB read and written in 138 to 145 us, 5.0 to 5.3
+// TB/s; 149 us where the loads and stores leave their lines in the L2 (a page is not read again here), 225
+// with eight units a lane in flight instead of four.  A pair without pages costs its work-groups' launch:
+// 5,280 of them 3.1 us.
 template <typename U>
 __global__ __launch_bounds__(kCpThreads) void copy_pages_kernel(KvCaches a, const int32_t* frm,
                                                                 const int32_t* to, int pairs,
@@ -147,7 +153,7 @@ __global__ __launch_bounds__(kWave) void keep_rows_kernel(KvCaches a, const int3
 // What a step leaves of every row: its accepted nodes stand where the row holds the slot of the last of
 // them, which is the highest (path is strictly increasing), and none does where it does not, as after a
 // reserve that was refused.  stand: how many stand; kept: the row's tokens; context: its context;
-// summed: the tokens whose block summaries changed (0: none).  One lane a row, three dependent loads.
+// summed: the tokens whose block summaries changed (0: none).  One lane a row; 1.7 us, two trips to memory.
 __global__ __launch_bounds__(256) void keep_lens_kernel(const int32_t* path, int64_t path_st,
                                                         const int32_t* count, const int32_t* ctx,
                                                         const int32_t* lens, int B, int max_n,

@@ -43,8 +43,10 @@ __device__ __forceinline__ int tree_page(const TreeArgs& a, int p) {
 }
 
 // The masks and depths of the trees: one work-group per sequence, one lane per node, which
-// climbs to the root (parents come before their children, so it ends).  Latency: the launch and a
-// step in LDS per level (a tree of 8 nodes 1.6 us, 32 of up to 64 nodes 4.8).
+// climbs to the root (parents come before their children, so it ends).  Latency: two trips to memory
+// (the prefix sums, then the parents: 1.4 us where the L2 of the work-group's XCD holds them, 2 to 3 more
+// where it does not, as for 8 trees of up to 32 nodes, 3.7, and 32 of up to 64, 4.8) and 65 ns in LDS per
+// level of the deepest node (a chain of 32 nodes 3.5 us, of 256 18).
 __global__ __launch_bounds__(kTrMaxNodes) void tree_masks_kernel(const int32_t* parents,
                                                                  const int32_t* cu, int64_t T,
                                                                  int words, int max_n, uint64_t* mask,
@@ -90,10 +92,13 @@ __global__ __launch_bounds__(kTrMaxNodes) void tree_masks_kernel(const int32_t* 
 // hide in all but the largest batches (8 trees of 16 to 32 nodes: 42.8 and 43.3 us, 32 trees of 24 to 64
 // over 2,730 to 27,300 tokens: 119 and 124).
 //
-// Bound by HBM where there are many trees: those 32 read 517 MB of keys and values in 113 to 115 us,
-// 4.5 TB/s, where a large copy moves 4.7; eight trees over 27,300 tokens read 128 MB in 35 to 38 us.  One
-// tree of eight nodes takes 12 us for 8 MB: the rows, their slots, the page table, the keys and the
-// partials are trips to memory that wait for each other.
+// Bound by HBM and the work on the weights together where there are many trees: those 32 fetch 500 MB
+// (counted; every key once) and write 22 MB of partials in 119 to 123 us, 4.3 TB/s, where a read alone
+// reaches 5.9.  Eight trees over 27,300 tokens fetch 127 MB in 37 us.  One tree of eight nodes takes 12 us for
+// 8 MB: the rows, their slots, the page table, the keys and the partials are trips to memory that wait for
+// each other.  More than 64 rows a key head, over 27,300 tokens: 64 nodes of 10 heads on one key head, one
+// tree 19 us, eight 44 (16 MB of keys, which the five groups of rows fetch as 74, and 70 MB of partials);
+// 256 nodes of 10 heads of their own, one tree 54 and eight 133 (293 MB fetched for 147: two groups of rows).
 // ---------------------------------------------------------------------------
 constexpr uint32_t kTrNotNamed = 0xffffffffu;
 

@@ -8,6 +8,8 @@ row, whose first ceil(lens / page_size) entries are in use.  Free pages are hand
 first, to the rows in order.  Nothing synchronises: calls that can fail return ``ok`` (int32 [1]
 on the GPU; where it is 0 nothing was changed).
 
+The outputs of a call are views of one allocation (some KB); clone what is kept for long or saved.
+
 ``PagePool`` holds the state and the caches and keeps them consistent; the functions are its
 parts.  ``PageCaches`` describes the tensors that the pages lie in, once for many calls.
 """
@@ -285,7 +287,8 @@ class PagePool:
         return ok
 
     def fork(self, src, dst):
-        """The empty rows dst become the rows src (fork_pages), their last pages copied."""
+        """The empty rows dst become the rows src (fork_pages), their last pages copied.  Rows are
+        forked between steps: what reserve() gave a row for a step counts as its tokens until keep()."""
         ok, frm, to = fork_pages(self.refs, self.table, self.lens, src, dst, self.page_size)
         copy_pages(self.caches, frm, to)
         return ok

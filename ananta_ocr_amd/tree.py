@@ -210,7 +210,9 @@ def verify_tree(target, tokens, parents, cu_seqlens_q, max_query_len, uniforms=N
     The uniform of the root draws next_token from what is left at the last accepted node: the first
     id whose running sum exceeds it times the whole.  Uniforms lie in [0, 1); probabilities and
     uniforms that are not above 0 (NaN too) count as 0.  path holds the accepted nodes, the root
-    first, then -1; a sequence without nodes has count 0 and next_token -1."""
+    first, then -1; a sequence without nodes has count 0 and next_token -1.  The three are views of one
+    allocation with the call's workspace (some KB; greedy 8 B a row and piece of it): clone what is
+    kept for long or saved."""
     lib = _lib.load()
     B, n = _nodes(cu_seqlens_q, max_query_len)
     if target.dim() != 2 or target.shape[1] == 0:
