@@ -141,6 +141,8 @@ def attn_tree(q, k, v, idx, bias, valid, mask, depth, context_lens, cu_seqlens_q
             raise ValueError(f"block_table: {B} rows needed")
         if int(page_size or 0) != k_shape[1]:
             raise ValueError(f"page_size {page_size}: the pages hold {k_shape[1]} tokens")
+        if block_table.shape[1] * k_shape[1] > 2 ** 31 - 1:
+            raise NotImplementedError("a block_table of at most 2^31 - 1 tokens a sequence")
     elif k_shape[0] != B:
         raise ValueError(f"cache of {k_shape[0]} sequences, {B} trees")
     with _device(q, k, v, idx, bias, valid, mask, depth, context_lens, cu_seqlens_q, block_table):

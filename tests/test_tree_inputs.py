@@ -4,7 +4,7 @@ calls."""
 import pytest
 import torch
 
-from ananta_ocr_amd import kv_pages, pipeline
+from ananta_ocr_amd import kv_pages, pipeline, tree
 
 I32 = torch.int32
 
@@ -40,3 +40,16 @@ def test_page_calls_refuse_rows_that_overlap():
             kv_pages.reserve_pages(refs, table, lens, lens, 8)
     with pytest.raises(ValueError, match="GPU"):
         kv_pages.reserve_pages(refs, torch.zeros(1, 4, dtype=I32).expand(1, 4), lens[:1], lens[:1], 8)
+
+
+def test_attention_refuses_tables_of_more_tokens_than_32_bits():
+    """A row of the table for 2^32 tokens and a few more would be taken for the few."""
+    a = dict(q=torch.zeros(5, 4, 128), k=torch.zeros(3, 64, 2, 128), v=torch.zeros(3, 64, 2, 128), idx=None,
+             bias=None, valid=None, mask=torch.zeros(5, 1, dtype=torch.int64), depth=torch.zeros(5, dtype=I32),
+             context_lens=torch.zeros(2, dtype=I32), cu_seqlens_q=torch.tensor([0, 1, 5]), max_query_len=4,
+             block_size=64, local_window=128, scale=0.1, page_size=64)
+    for pages in (2 ** 26 + 16, 2 ** 25):
+        with pytest.raises(NotImplementedError):
+            tree.attn_tree(**a, block_table=torch.zeros(1, 1, dtype=I32).expand(2, pages))
+    with pytest.raises(ValueError, match="GPU"):
+        tree.attn_tree(**a, block_table=torch.zeros(1, 1, dtype=I32).expand(2, 2 ** 25 - 1))
