@@ -126,3 +126,25 @@ def test_rows_that_hold_some_of_their_nodes():
     again = pool.keep(torch.tensor([[0, 7]] * 5, device=DEV), torch.ones(5, dtype=torch.int32, device=DEV),
                       torch.tensor([7, 8, 6, 0, -3], device=DEV))
     assert again.tolist() == [8, 9, 6, 0, 8]
+
+
+@pytest.mark.parametrize("rows,n", [(1, 1), (255, 3), (256, 4), (1500, 9), (8192, 2)])
+def test_what_a_step_leaves_of_many_rows(rows, n):
+    """Lengths, contexts and counts of any number of rows against lists; counts past the path and below
+    0, contexts below 0, lengths that reach 2^31 - 1."""
+    g = torch.Generator().manual_seed(rows)
+    rnd = lambda lo, hi: torch.randint(lo, hi, (rows,), generator=g)
+    big = 2 ** 31 - 1
+    ctx = torch.where(rnd(0, 9) == 0, rnd(-3, 2), rnd(0, 40))
+    ctx = torch.where(rnd(0, 9) == 0, big - rnd(0, 4), ctx)
+    lens = (ctx + rnd(-2, 2 * n)).clamp(0, big)
+    count = rnd(-1, n + 3)
+    path = torch.stack([torch.arange(n)] * rows) + torch.randint(0, 2, (rows, n), generator=g).cumsum(1)
+    path[:, 0] = 0
+    got = kv_pages._keep_lens(path.to(DEV), count.to(DEV), ctx.to(DEV), lens.to(torch.int32).to(DEV))
+    want = []
+    for p, c, x, m in zip(path.tolist(), count.tolist(), ctx.tolist(), lens.tolist()):
+        k = min(c, n)
+        ok = k > 0 and x >= 0 and x + p[k - 1] < m
+        want.append((k if ok else 0, x + k if ok else m, x + k if ok else x, x + k if ok else 0))
+    assert list(zip(*(t.tolist() for t in got))) == want
