@@ -114,10 +114,15 @@ SIGNATURES = {
     "dash_copy_pages": (_i, [_i, _p, _p, _p, _p, _i, _i, _p]),
     "dash_keep_rows": (_i, [_i, _p, _p, _p, _l, _p, _p, _p, _l, _i, _i, _i, _i, _i, _p]),
     "dash_keep_lens": (_i, [_p, _l, _p, _p, _p, _i, _i, _p, _p, _p, _p, _p]),
+    "dash_step_rows": (_i, [_p, _p, _p, _p, _l, _i, _i, _i, _i, _i, _p, _p, _p, _p, _p]),
     "dash_fork_pages": (_i, [_p, _i, _p, _l, _i, _i, _p, _p, _p, _i, _i, _p, _p, _p, _p]),
     "dash_reserve_pages": (_i, [_p, _i, _p, _l, _i, _i, _p, _p, _i, _p, _p, _p, _p]),
     "dash_free_pages": (_i, [_p, _i, _p, _l, _i, _i, _p, _p, _i, _p]),
     "dash_compact_pages": (_i, [_p, _i, _p, _l, _i, _i, _p, _i, _p, _p, _p, _p, _p, _p]),
+    "dash_rope": (_i, [_p, _l, _l, _l, _i, _p, _l, _l, _l, _p, _l, _l, _l, _i, _p, _l, _l, _l, _i, _p, _i, _l,
+                       _l, _p, _i, _i, _i, _i, _f, _i, _i, _i, _p]),
+    "dash_rope_append": (_i, [_p, _l, _l, _i, _p, _l, _l, _p, _l, _l, _p, _l, _l, _i, _i, _p, _i, _p, _p, _l, _l,
+                              _l, _p, _l, _l, _l, _i, _i, _p, _i, _i, _i, _f, _i, _i, _p]),
     "dash_page_rope_advance": (_i, [_p, _l, _i, _l, _p, _p, _p, _l, _p, _p, _p, _p]),
 }
 

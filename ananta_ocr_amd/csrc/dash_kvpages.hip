@@ -1,6 +1,6 @@
 // Pages of a paged cache on gfx950: copied, shared between sequences (fork), handed out
-// (reserve), given back (free) and moved together (compact), and the rows of accepted drafted
-// tokens moved up in the last pages (keep).
+// (reserve), given back (free) and moved together (compact), the rows of accepted drafted
+// tokens moved up in the last pages (keep), and the slots of a step's new tokens (step rows).
 //
 // The state is three int32 arrays: refs [num_pages], how many block-table entries name a page
 // (0: free); table [R, P], the pages of every sequence row; lens [R], its tokens.  Entry i of a
@@ -171,6 +171,69 @@ __global__ __launch_bounds__(256) void keep_lens_kernel(const int32_t* path, int
   kept[b] = ok ? c + n : len;
   context[b] = ok ? c + n : c;
   summed[b] = ok ? c + n : 0;
+}
+
+// Where the rows of a step go: request b has n[b] new tokens after ctx[b], packed in order; row r is token
+// i = r - cu[b] of its request, at position ctx[b] + i and in slot table[position / page] * page + position %
+// page.  Every work-group adds the requests up by itself (32 KB of lengths at most), so that no launch comes
+// before, and finds its rows' requests by bisection in LDS.  Sums are taken in 64 bits and cut to the rows.
+constexpr int kRowsThreads = 256;
+__global__ __launch_bounds__(kRowsThreads) void step_rows_kernel(
+    const int32_t* n, const int32_t* ctx, const int32_t* lens, const int32_t* table, int64_t table_st, int B,
+    int P, int page, int num_pages, int rows, int32_t* cu, int32_t* seq, int32_t* pos, int64_t* slot) {
+  __shared__ int sCu[kKvMaxRows + 1];
+  __shared__ int64_t sW[kRowsThreads / kWave];
+  const int tid = threadIdx.x, lane = wave_lane(), wv = tid / kWave;
+  const int per = (B + kRowsThreads - 1) / kRowsThreads;
+  const int b0 = min(tid * per, B), b1 = min(b0 + per, B);
+  int64_t mine = 0;
+  for (int b = b0; b < b1; ++b) {
+    const int x = max(n[b], 0);
+    sCu[b] = x;
+    mine += x;
+  }
+  int64_t x = mine;
+#pragma unroll
+  for (int s = 1; s < kWave; s <<= 1) {
+    const int64_t y = __shfl_up(x, s, kWave);
+    if (lane >= s) x += y;
+  }
+  if (lane == kWave - 1) sW[wv] = x;
+  __syncthreads();
+  x -= mine;
+  for (int w = 0; w < wv; ++w) x += sW[w];
+  for (int b = b0; b < b1; ++b) {
+    const int y = sCu[b];
+    sCu[b] = (int)min(x, (int64_t)rows);
+    x += y;
+  }
+  if (tid == kRowsThreads - 1) sCu[B] = (int)min(x, (int64_t)rows);
+  __syncthreads();
+  if (blockIdx.x == 0)
+    for (int b = tid; b <= B; b += kRowsThreads) cu[b] = sCu[b];
+  const int64_t r = (int64_t)blockIdx.x * kRowsThreads + tid;
+  if (r >= rows) return;
+  if (r >= sCu[B]) {                       // of no request
+    seq[r] = pos[r] = -1;
+    slot[r] = -1;
+    return;
+  }
+  int lo = 0, hi = B;                      // sCu[lo] <= r < sCu[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (sCu[mid] <= r) lo = mid; else hi = mid;
+  }
+  const int64_t t = (int64_t)ctx[lo] + (r - sCu[lo]);
+  const bool in = t >= 0 && t <= INT32_MAX;
+  int64_t at = -1;
+  if (in && t < (int64_t)P * page && (!lens || t < lens[lo])) {
+    const int i = (int)t / page;
+    const int p = table[(int64_t)lo * table_st + i];
+    if (p >= 0 && p < num_pages) at = (int64_t)p * page + ((int)t - i * page);
+  }
+  seq[r] = lo;
+  pos[r] = in ? (int)t : -1;
+  slot[r] = at;
 }
 
 // Sum of v over the work-group's earlier threads; `total` gets the sum over all.
@@ -589,6 +652,23 @@ extern "C" int dash_keep_lens(const int32_t* path, int64_t path_stride, const in
   hipLaunchKernelGGL(keep_lens_kernel, dim3(B / 256 + 1), dim3(256), 0, (hipStream_t)stream, path,
                      path_stride, count, context_lens, lens, B, max_query_len, stand, kept,
                      new_context, summed);
+  return kv_status();
+}
+
+extern "C" int dash_step_rows(const int32_t* query_lens, const int32_t* context_lens, const int32_t* lens,
+                              const int32_t* block_table, int64_t table_stride, int B, int P,
+                              int page_size, int num_pages, int rows, int32_t* cu_seqlens_q,
+                              int32_t* seq, int32_t* positions, int64_t* slots, void* stream) {
+  using namespace dash;
+  if (B < 0 || P < 0 || rows < 0 || page_size <= 0 || num_pages < 0 || !cu_seqlens_q) return kErrInvalid;
+  if (B > 0 && (!query_lens || !context_lens)) return kErrInvalid;
+  if (B > 0 && P > 0 && !block_table) return kErrInvalid;
+  if (rows > 0 && (!seq || !positions || !slots)) return kErrInvalid;
+  const int64_t groups = std::max<int64_t>(1, ((int64_t)rows + kRowsThreads - 1) / kRowsThreads);
+  if (B > kKvMaxRows) return kErrUnsupported;
+  hipLaunchKernelGGL(step_rows_kernel, dim3((unsigned)groups), dim3(kRowsThreads), 0, (hipStream_t)stream,
+                     query_lens, context_lens, lens, block_table, table_stride, B, P, page_size, num_pages,
+                     rows, cu_seqlens_q, seq, positions, slots);
   return kv_status();
 }
 

@@ -1,6 +1,6 @@
 """Pages of a paged cache on the HIP kernels (csrc/dash_kvpages.hip): copied, shared between
-sequences (fork), handed out (reserve), given back (free) and moved together (compact), and the
-rows of accepted drafted tokens moved up (keep).
+sequences (fork), handed out (reserve), given back (free) and moved together (compact), the rows of accepted drafted tokens
+moved up (keep), and the slots of a step's new tokens (step_rows).
 
 The state is three int32 tensors on the GPU: ``refs`` [num_pages], how many table entries name a
 page (0: free); ``table`` [R, P], the pages of every sequence row; ``lens`` [R], the tokens of a
@@ -184,6 +184,36 @@ def _ints(device, *sizes):
     return torch.empty(sum(sizes), dtype=torch.int32, device=device).split_with_sizes(sizes)
 
 
+def step_rows(table, context_lens, query_lens, page_size, num_pages, rows, lens=None):
+    """Where the new tokens of a step go: request b brings query_lens[b] of them (a number below 0
+    counts as 0) after its context_lens[b], packed in order into a batch of `rows` rows.  Returns
+    (cu_seqlens_q int32 [B + 1], seq int32 [rows], positions int32 [rows], slots int64 [rows]): the
+    prefix sums, cut to the rows, and every row's request, position (context + its place among the
+    new ones) and slot in the pool, table[seq, position // page_size] * page_size + position %
+    page_size.  Rows of no request hold -1, and a row's slot is -1 where the table [B, P] has no page
+    for it (an entry that is none of num_pages) or, with lens [B] given, where its position is not
+    below lens: after a reserve_pages that was refused a last page may be another row's too.
+    At most 8,192 requests."""
+    if table.dim() != 2:
+        raise ValueError("table [B, P] is needed")
+    B, P = table.shape
+    for x, what in ((context_lens, "context_lens"), (query_lens, "query_lens"), (lens, "lens")):
+        _shape(x, (B,), what)
+    rows = int(rows)
+    if int(page_size) < 1 or int(num_pages) < 0 or not 0 <= rows < 2 ** 31:
+        raise ValueError(f"page_size {page_size}, {num_pages} pages, {rows} rows")
+    if B > MAX_ROWS:
+        raise NotImplementedError(f"tables of at most {MAX_ROWS} rows")
+    with _device(table, context_lens, query_lens, lens):
+        bt, ctx, n, ln = _i32(table), _i32(context_lens), _i32(query_lens), _i32(lens)
+        slots, cu, seq, pos = _ints(bt.device, 2 * rows, B + 1, rows, rows)
+        _lib.check(_lib.load().dash_step_rows(
+            _ptr(n), _ptr(ctx), _ptr(ln), _ptr(bt), bt.stride(0), B, P, int(page_size),
+            int(num_pages), rows, _ptr(cu), _ptr(seq), _ptr(pos), _ptr(slots), _stream()),
+            "dash_step_rows")
+    return cu, seq, pos, slots.view(torch.int64)
+
+
 def fork_pages(refs, table, lens, src, dst, page_size):
     """Row dst[i], which is empty, becomes row src[i]: its filled pages are shared, a partly filled
     last one gets a page of its own.  refs, table and lens in place.  Returns (ok, from_pages,
@@ -309,6 +339,12 @@ class PagePool:
         keep_rows(self.caches, path, step[0], context_lens, self.table)
         self.free(step[1])
         return step
+
+    def step_rows(self, context_lens, query_lens, rows):
+        """(cu_seqlens_q, seq, positions, slots) of a step's new tokens (step_rows), once reserve()
+        has made room for them: rows that hold no slot for a token get -1 for it."""
+        return step_rows(self.table, context_lens, query_lens, self.page_size,
+                         self.caches.num_pages, rows, self.lens)
 
     def compact(self):
         """The pages in use moved to the lowest numbers, in the caches too."""

@@ -764,6 +764,17 @@ int dash_keep_lens(const int32_t* path, int64_t path_stride, const int32_t* coun
                    int32_t* stand, int32_t* kept, int32_t* new_context, int32_t* summed,
                    void* stream);
 
+/* The rows of a step: request b brings query_lens[b] new tokens (below 0: none) after its context_lens[b],
+ * packed in order.  cu_seqlens_q [B + 1] gets their prefix sums, cut to `rows`; row r = cu_seqlens_q[b] + i
+ * gets seq = b, positions = context_lens[b] + i (-1 outside 0 .. 2^31 - 1) and slots = the token's place in
+ * the pool, page * page_size + offset (int64; -1 where the table has no such entry, the entry names no page,
+ * or, with lens given, the position is not below lens[b]).  Rows past the last request's: -1 each.
+ * B <= 8,192. */
+int dash_step_rows(const int32_t* query_lens, const int32_t* context_lens, const int32_t* lens,
+                   const int32_t* block_table, int64_t table_stride, int B, int P, int page_size,
+                   int num_pages, int rows, int32_t* cu_seqlens_q, int32_t* seq, int32_t* positions,
+                   int64_t* slots, void* stream);
+
 /* Row dst_rows[i] (empty) becomes row src_rows[i]: its filled pages shared, a partly filled last one
  * replaced by a page of its own, whose content is to be copied from_pages[i] -> to_pages[i] (-1: none).
  * ok = 1; or ok = 0 and nothing changed, where a row is out of range, a target filled, repeated or a
@@ -794,6 +805,30 @@ int dash_compact_pages(const int32_t* refs, int num_pages, const int32_t* block_
                        int64_t table_stride, int R, int P, const int32_t* lens, int page_size,
                        int32_t* new_refs, int32_t* new_table, int32_t* from_pages,
                        int32_t* to_pages, int32_t* place, void* stream);
+
+/*
+ * Rotary positions.  The part [start, start + 2 pairs) of every head row of q [B, S, H, D] and k [B, S, Hkv, D]
+ * (fp32, bf16, fp16: dtype 0, 1, 2; any strides) is turned into q_out and k_out, the rest copied: pair j, elements
+ * (j, j + pairs) of the part, or (2 j, 2 j + 1) with interleaved, by the angle p * inv_freq[j] (64 bits) of its
+ * token's position p (int32 or int64, strides pos_sb, pos_st), times factor:
+ *   (x, y) -> factor (x cos - y sin, y cos + x sin).
+ * back: by the negative angle (the gradient).  Either of H and Hkv may be 0.  D even, pairs <= 256.
+ */
+int dash_rope(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, int H, void* q_out, int64_t qo_sb,
+              int64_t qo_st, int64_t qo_sh, const void* k, int64_t k_sb, int64_t k_st, int64_t k_sh, int Hkv,
+              void* k_out, int64_t ko_sb, int64_t ko_st, int64_t ko_sh, int dtype, const void* positions,
+              int positions_int64, int64_t pos_sb, int64_t pos_st, const double* inv_freq, int pairs, int start,
+              int interleaved, int back, float factor, int B, int S, int D, void* stream);
+
+/* The same of T tokens' q [T, H, D] into q_out, with k [T, Hkv, D] turned and v copied into the rows `slots` of
+ * caches [num_pages, page_size, Hkv, D] (strides of page, token and head; slot = page * page_size + offset; a slot
+ * that is none: the token's rows are not written).  Slots are distinct; positions contiguous. */
+int dash_rope_append(const void* q, int64_t q_st, int64_t q_sh, int H, void* q_out, int64_t qo_st, int64_t qo_sh,
+                     const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, int Hkv,
+                     int dtype, const void* positions, int positions_int64, const int64_t* slots, void* k_cache,
+                     int64_t kc_sp, int64_t kc_st, int64_t kc_sh, void* v_cache, int64_t vc_sp, int64_t vc_st,
+                     int64_t vc_sh, int page_size, int num_pages, const double* inv_freq, int pairs, int start,
+                     int interleaved, float factor, int T, int D, void* stream);
 
 #ifdef __cplusplus
 }
