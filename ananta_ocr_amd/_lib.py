@@ -123,6 +123,9 @@ SIGNATURES = {
                        _l, _p, _i, _i, _i, _i, _f, _i, _i, _i, _p]),
     "dash_rope_append": (_i, [_p, _l, _l, _i, _p, _l, _l, _p, _l, _l, _p, _l, _l, _i, _i, _p, _i, _p, _p, _l, _l,
                               _l, _p, _l, _l, _l, _i, _i, _p, _i, _i, _i, _f, _i, _i, _p]),
+    "dash_attn_shared_workspace_size": (_i, [_i, _i, _i, _i, _l, ctypes.POINTER(_l)]),
+    "dash_attn_shared": (_i, [_p, _l, _l, _p, _l, _l, _l, _p, _l, _l, _l, _p, _l, _i, _i, _i, _p, _p, _p,
+                              _p, _p, _i, _l, _l, _p, _l, _l, _i, _i, _i, _i, _l, _i, _f, _p, _l, _p]),
     "dash_page_rope_advance": (_i, [_p, _l, _i, _l, _p, _p, _p, _l, _p, _p, _p, _p]),
 }
 

@@ -1747,6 +1747,7 @@ inline PlanLayout plan_layout(int B, int H, int S_max, int64_t rows, int K, int 
 #include "dash_prefill_bwd.h"
 #include "dash_extend.h"
 #include "dash_tree.h"
+#include "dash_shared.h"
 
 namespace dash {
 // Workspace of the backward: the plan (as the forward's, every routed pair

@@ -1,0 +1,653 @@
+// Full attention of a batch whose sequences share prompts, over a paged cache.  Included by
+// dash_prefill.hip, whose tile helpers it uses.
+//
+// Row r = cu[b] + i is new token i of sequence b, at position t = ctx[b] + i, and sees the keys j <= t.
+// The keys below prefix[g] of the sequences of group g (cu_groups[g] <= b < cu_groups[g + 1]) are read
+// through the block-table row of the group's first sequence, once for all rows of the group; the
+// others through the sequence's own row.  So there are G + B segments: rows of a group with the keys [0, prefix),
+// and rows of a sequence with the keys [prefix, ctx + n).  A row's result is the sum of two segments'.
+//
+// The lengths lie on the device, and a launch's grid cannot depend on them: the plan kernel adds up the
+// segments' work in units of 64 keys of one key head and one tile of rows, and every one of the W
+// work-groups of the attention takes the same number of units, one after another, over as many segments
+// as that reaches.  Each run of units within a (segment, key head, row tile) leaves an unnormalised
+// fp32 partial per row, and the merge kernel adds a row's partials up.
+#pragma once
+
+namespace dash {
+
+constexpr int kShMaxSeqs = 8192;
+constexpr int kShThreads = 1024;          // of the plan kernel
+
+struct SharedSeg {
+  int32_t r0, rows;                       // first packed row; rows times query heads of a key head
+  int32_t k0, k1;                         // keys
+  int32_t table_row, group;               // group: of a sequence's segment, -1 none
+  int32_t base, tiles;                    // partial rows of the segments before; row tiles
+};
+
+struct SharedArgs {
+  const bf16* q; int64_t q_st, q_sh;
+  const bf16* k; int64_t k_sp, k_st, k_sh;
+  const bf16* v; int64_t v_sp, v_st, v_sh;
+  const int32_t* table; int64_t table_stride; int page, num_pages;
+  const int32_t* ctx; const int32_t* cu;
+  const int32_t* cu_groups; const int32_t* prefix;
+  void* out; int out_bf16; int64_t o_st, o_sh;
+  float* lse; int64_t lse_st, lse_sh;
+  int B, G, H, Hkv, S, W, tile_rows;
+  int64_t T;
+  float scale_log2e;
+  // workspace
+  int64_t* head;                          // units in all, units of a work-group
+  int64_t* starts;                        // [G + B] units of the segments before
+  SharedSeg* seg;                         // [G + B]
+  int32_t* row_seq; int32_t* row_pos;     // [T]
+  float2* part_ml;                        // base-2 reference and weight sum
+  float* part_o;                          // [.., 128]
+};
+
+__device__ __forceinline__ int sh_cu(const SharedArgs& a, int b) {
+  return (int)min(max((int64_t)a.cu[b], (int64_t)0), a.T);
+}
+
+// Sum over the work-group's earlier threads, and over all.
+__device__ __forceinline__ int64_t sh_before(int64_t v, int64_t* sW, int64_t& total) {
+  const int lane = wave_lane(), wv = threadIdx.x / kWave;
+  int64_t x = v;
+#pragma unroll
+  for (int s = 1; s < kWave; s <<= 1) {
+    const int64_t y = __shfl_up(x, s, kWave);
+    if (lane >= s) x += y;
+  }
+  __syncthreads();
+  if (lane == kWave - 1) sW[wv] = x;
+  __syncthreads();
+  int64_t before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kShThreads / kWave; ++w) {
+    if (w < wv) before += sW[w];
+    total += sW[w];
+  }
+  return before + x - v;
+}
+
+// Work-group 0: the segments and their units.  The others: the sequence and position of every row.
+__global__ __launch_bounds__(kShThreads) void shared_plan_kernel(SharedArgs a) {
+  __shared__ int sCu[kShMaxSeqs + 1];
+  __shared__ int64_t sW[kShThreads / kWave];
+  const int tid = threadIdx.x, Gq = a.H / a.Hkv;
+  if (blockIdx.x > 0) {
+    for (int b = tid; b <= a.B; b += kShThreads) sCu[b] = sh_cu(a, b);
+    __syncthreads();
+    const int64_t r = (int64_t)(blockIdx.x - 1) * kShThreads + tid;
+    if (r >= a.T) return;
+    int seq = -1, pos = -1;
+    if (r >= sCu[0] && r < sCu[a.B]) {
+      int lo = 0, hi = a.B;               // sCu[lo] <= r < sCu[hi]
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (sCu[mid] <= r) lo = mid; else hi = mid;
+      }
+      seq = lo;
+      pos = (int)min((int64_t)min(max(a.ctx[lo], 0), a.S) + (r - sCu[lo]), (int64_t)INT32_MAX - 1);
+    }
+    a.row_seq[r] = seq;
+    a.row_pos[r] = pos;
+    return;
+  }
+  int64_t units_before = 0, rows_before = 0, own_before = 0;
+  const int ns = a.G + a.B;
+  for (int s0 = 0; s0 < ns; s0 += kShThreads) {
+    const int s = s0 + tid;
+    SharedSeg g = {0, 0, 0, 0, 0, -1, 0, 0};
+    const bool group = s < a.G;
+    if (group) {
+      const int b0 = min(max(a.cu_groups[s], 0), a.B), b1 = min(max(a.cu_groups[s + 1], b0), a.B);
+      g.r0 = sh_cu(a, b0);
+      g.rows = b1 > b0 ? max(sh_cu(a, b1) - g.r0, 0) * Gq : 0;
+      g.k1 = min(max(a.prefix[s], 0), a.S);
+      g.table_row = min(b0, a.B - 1);
+    } else if (s < ns) {
+      const int b = s - a.G;
+      g.r0 = sh_cu(a, b);
+      const int n = max(sh_cu(a, b + 1) - g.r0, 0);
+      g.rows = n * Gq;
+      int lo = -1, hi = a.G;              // the last group that starts at or before b
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a.cu_groups[mid] <= b) lo = mid; else hi = mid;
+      }
+      if (lo >= 0 && b < a.cu_groups[lo + 1]) {
+        g.group = lo;
+        g.k0 = min(max(a.prefix[lo], 0), a.S);
+      }
+      g.k1 = (int)min((int64_t)min(max(a.ctx[b], 0), a.S) + n, (int64_t)a.S);
+      g.table_row = b;
+    }
+    int64_t total;
+    int64_t before = sh_before(g.rows, sW, total);
+    // (groups, or sequences, whose prefix sums are none could have more rows than the workspace holds)
+    const int64_t mine = group ? 0 : g.rows, room = a.T * Gq;
+    int64_t own_total;
+    const int64_t own = sh_before(mine, sW, own_total) + own_before;
+    before += rows_before;               // (groups come first: of a group's thread, rows of groups)
+    if ((group ? before : own) + g.rows > room) g.rows = 0;
+    rows_before += total;
+    own_before += own_total;
+    g.base = (int)(min(group ? before : room + own, 2 * room) * a.Hkv);
+    g.tiles = (g.rows + a.tile_rows - 1) / a.tile_rows;
+    const int64_t units = (int64_t)g.tiles * a.Hkv * ((max(g.k1 - g.k0, 0) + 63) / 64);
+    before = sh_before(units, sW, total);
+    if (s < ns) {
+      a.starts[s] = units_before + before;
+      a.seg[s] = g;
+    }
+    units_before += total;
+  }
+  if (tid == 0) {
+    a.head[0] = units_before;
+    a.head[1] = max((units_before + a.W - 1) / a.W, (int64_t)1);
+  }
+}
+
+// The last segment that starts at or before unit u, over the wavefront.
+__device__ __forceinline__ int sh_find(const SharedArgs& a, int64_t u) {
+  const int lane = wave_lane();
+  int lo = 0, n = a.G + a.B;
+  while (n > 1) {
+    const int step = (n + kWave - 1) / kWave;
+    const int i = lane * step;
+    const bool at = i < n && a.starts[lo + i] <= u;
+    const int c = max(__popcll(__ballot(at)) - 1, 0) * step;
+    lo += c;
+    n = min(step, n - c);
+  }
+  return __builtin_amdgcn_readfirstlane(lo);
+}
+
+// RT row tiles of 32 rows are the columns of S^T = K Q^T (v_mfma_f32_32x32x16_bf16); with KG = 2 two
+// wavefronts share a row tile, one half of 64 keys each, and meet at the end of a run.  Weights enter
+// the second product as three bf16 parts (24 bits), so that a bf16 output is the fp32 one rounded once.
+template <int RT, int KG>
+__global__ __launch_bounds__(64 * RT * KG, 2) void shared_attn_kernel(SharedArgs a) {
+  constexpr int D = 128, NW = RT * KG, TH = 64 * NW, TR = 32 * RT;
+  constexpr int NH = 2 / KG;              // halves of 64 keys that a wavefront takes
+  constexpr int PARTS = 3;                // of a weight
+  constexpr int CH = RT == 1 ? 4 : 8;     // units whose rows' offsets are laid out at a time
+  constexpr int ST = RT == 1 ? 1 : 2;     // stages
+  constexpr int NG = 16 / NW;             // groups of four key rows that a wavefront loads
+  __shared__ __attribute__((aligned(16))) bf16 sK0[64 * D];
+  __shared__ __attribute__((aligned(16))) bf16 sK1[ST == 2 ? 64 * D : 8];
+  __shared__ __attribute__((aligned(16))) bf16 sV0[64 * D];
+  __shared__ __attribute__((aligned(16))) bf16 sV1[ST == 2 ? 64 * D : 8];
+  __shared__ longlong2 sOff[64 * CH];     // offsets of a key row in K and V
+  __shared__ uint32_t sBad[2][NW];
+  __shared__ int sEnd[NW];
+  __shared__ float2 sMl[32 * RT];
+  const int tid = threadIdx.x, lane = wave_lane();
+  const int wv = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int rt = wv % RT, kg = wv / RT;
+  const int hl = lane >> 5, col = lane & 31;
+  const int Gq = a.H / a.Hkv;
+  const int64_t per = a.head[1];
+  int64_t u = blockIdx.x * per;
+  const int64_t u_end = min(u + per, a.head[0]);
+  const uint32_t kl0 = k_lane_off(col, hl), vl0 = v_lane_off(lane);
+  const float csc = a.scale_log2e;
+
+  while (u < u_end) {
+    const int s = sh_find(a, u);
+    const SharedSeg g = a.seg[s];
+    const int items = (g.k1 - g.k0 + 63) / 64;
+    const int64_t rel = u - a.starts[s], stream = rel / items;
+    const int i_first = (int)(rel - stream * items);
+    const int i_last = (int)min((int64_t)items, i_first + (u_end - u));
+    u += i_last - i_first;
+    const int hk = (int)(stream / g.tiles), rb = (int)(stream - (int64_t)hk * g.tiles) * TR;
+
+    // this lane's row
+    const int rr = min(rb + rt * 32 + col, g.rows - 1);
+    const bool rvalid = rb + rt * 32 + col < g.rows;
+    const int64_t row = g.r0 + rr / Gq;
+    const int h = hk * Gq + rr % Gq;
+    const int end = min(a.row_pos[row] + 1, g.k1);         // the keys below it are seen
+    int e_min = rvalid ? end : INT32_MAX;
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) e_min = min(e_min, __shfl_xor(e_min, m, kWave));
+    e_min = __builtin_amdgcn_readfirstlane(e_min);
+    __syncthreads();                      // every wavefront left the run before
+    if (lane == 0) sEnd[wv] = e_min;
+    bf16x8 qop[D / 16];
+    {
+      const bf16* qb = a.q + row * a.q_st + (int64_t)h * a.q_sh;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) qop[kk] = *(const bf16x8*)(qb + kk * 16 + hl * 8);
+    }
+
+    auto lay_out = [&](int c0, int c1) {
+      for (int x = tid; x < 64 * (c1 - c0); x += TH) {
+        const int j = min(g.k0 + 64 * c0 + x, g.k1 - 1);
+        const int i = j / a.page;
+        const int p = min(max(a.table[(int64_t)g.table_row * a.table_stride + i], 0), a.num_pages - 1);
+        const int jp = j - i * a.page;
+        sOff[x] = make_longlong2((int64_t)p * a.k_sp + (int64_t)jp * a.k_st + (int64_t)hk * a.k_sh,
+                                 (int64_t)p * a.v_sp + (int64_t)jp * a.v_st + (int64_t)hk * a.v_sh);
+      }
+      __syncthreads();
+    };
+    auto fetch = [&](int x, bf16* sKn, bf16* sVn) __attribute__((always_inline)) {
+#pragma unroll
+      for (int n = 0; n < NG; ++n) {
+        const int grp = NW * n + wv, r = 4 * grp + (lane >> 4);
+        const longlong2 o = sOff[64 * x + r];
+        __builtin_amdgcn_global_load_lds((const void*)(a.k + o.x + k_slot(r, lane & 15) * 8),
+            (__attribute__((address_space(3))) void*)(sKn + grp * 4 * D), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((const void*)(a.v + o.y + v_slot(r, lane & 15) * 8),
+            (__attribute__((address_space(3))) void*)(sVn + grp * 4 * D), 16, 0, 0);
+      }
+    };
+
+    floatx16 acc_o[D / 32];
+    float m_run = -INFINITY, l_run = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc_o[dt][r] = 0.f;
+    int e_all = INT32_MAX;                // keys below it are seen by every row of the tile
+
+    // V values that are not finite would reach, through weights of 0, rows that do not see their keys.
+    // Where some row does not see every key, each wavefront clears them in the rows it loaded, and notes
+    // their groups: item() adds them to the rows that see them.
+    auto clear = [&](int i, bf16* sVn, uint32_t* bad_of) __attribute__((always_inline)) {
+      uint32_t bad = 0;
+      if (g.k0 + 64 * (i + 1) > e_all) {
+#pragma unroll
+        for (int n = 0; n < NG; ++n) {
+          uint4* p = (uint4*)(sVn + (NW * n + wv) * 4 * D) + lane;
+          uint4 x = *p;
+          bool is = false;
+          auto fix = [&](uint32_t& w) {
+            if ((w & 0x7f80u) == 0x7f80u) { w &= 0xffff0000u; is = true; }
+            if ((w & 0x7f800000u) == 0x7f800000u) { w &= 0xffffu; is = true; }
+          };
+          fix(x.x); fix(x.y); fix(x.z); fix(x.w);
+          if (is) *p = x;
+          if (__any(is)) bad |= 1u << n;
+        }
+      }
+      if (lane == 0) bad_of[wv] = bad;
+    };
+    // unit i of the run, laid out at x: this wavefront's halves
+    auto item = [&](int i, int x0, const bf16* sKc, const bf16* sVc,
+                    const uint32_t* bad_of) __attribute__((always_inline)) {
+      const int j0 = g.k0 + 64 * i;
+      uint32_t vis[NH];
+      bool any = false;
+      auto below = [](int y) -> uint32_t { return y >= 32 ? ~0u : y <= 0 ? 0u : (1u << y) - 1u; };
+#pragma unroll
+      for (int x = 0; x < NH; ++x) {
+        const int j = j0 + 32 * (KG == 2 ? kg : x);
+        vis[x] = rvalid ? (j + 32 <= e_min ? ~0u : below(end - j)) : 0u;
+        any = any || vis[x] != 0u;
+      }
+      if (!__any(any)) return;
+      floatx16 sc[NH];
+      float mloc = -INFINITY;
+#pragma unroll
+      for (int x = 0; x < NH; ++x) {
+        const int hf = KG == 2 ? kg : x;
+        bf16x8 kf[D / 16];
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) kf[kk] = k_frag_at(sKc, kl0, hf, kk);
+        floatx16 t;                       // two chains: a product need not wait for the one before it
+#pragma unroll
+        for (int r = 0; r < 16; ++r) { sc[x][r] = 0.f; t[r] = 0.f; }
+#pragma unroll
+        for (int kk = 0; kk < D / 16; kk += 2) {
+          sc[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kk], qop[kk], sc[x], 0, 0, 0);
+          t = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kk + 1], qop[kk + 1], t, 0, 0, 0);
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sc[x][r] += t[r];
+        if (__all(vis[x] == 0u || vis[x] == ~0u)) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) sc[x][r] = vis[x] ? sc[x][r] : -INFINITY;
+        } else {
+          const uint32_t vb = vis[x] >> (4 * hl);
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            sc[x][r] = (vb >> (8 * (r >> 2) + (r & 3))) & 1u ? sc[x][r] : -INFINITY;
+        }
+        float mraw = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mraw = fmaxf(mraw, sc[x][r]);
+        mloc = fmaxf(mloc, mraw * csc);
+      }
+      mloc = xor32_max(mloc);
+      // the reference moves only when a row's maximum exceeds it by more than 8
+      const bool up = mloc > m_run + 8.f;
+      if (__any(up)) {
+        const float alpha = up ? fast_exp2(m_run - mloc) : 1.f;
+        l_run *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc_o[dt][r] *= alpha;
+        m_run = up ? mloc : m_run;
+      }
+      const float off = m_run == -INFINITY ? 0.f : -m_run;
+#pragma unroll
+      for (int x = 0; x < NH; ++x) {
+        const int hf = KG == 2 ? kg : x;
+        bf16x8 vop[4][2];                 // V in registers before the weights are ready
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+          for (int jj = 0; jj < 2; ++jj) {
+            const char* vp = (const char*)sVc + (32 * hf + 16 * jj) * 256 + (vl0 ^ (uint32_t)(dt << 6));
+            const bf16x4 l4 = __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (lds_short4*)(__attribute__((address_space(3))) void*)vp));
+            const bf16x4 h4 = __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (lds_short4*)(__attribute__((address_space(3))) void*)(vp + 2048)));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { vop[dt][jj][e] = l4[e]; vop[dt][jj][e + 4] = h4[e]; }
+          }
+        uint32_t part[PARTS][2][4];
+#pragma unroll
+        for (int jj = 0; jj < 2; ++jj) {
+          float p[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) p[e] = fast_exp2(fmaf(sc[x][8 * jj + e], csc, off));
+          l_run += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int n = 0; n < PARTS; ++n) {
+              bf16x2 y;
+              y[0] = (bf16)p[2 * e];
+              y[1] = (bf16)p[2 * e + 1];
+              const uint32_t w = __builtin_bit_cast(uint32_t, y);
+              part[n][jj][e] = w;
+              p[2 * e] -= __uint_as_float(w << 16);
+              p[2 * e + 1] -= __uint_as_float(w & 0xffff0000u);
+            }
+        }
+#pragma unroll
+        for (int jj = 0; jj < 2; ++jj)
+#pragma unroll
+          for (int n = PARTS - 1; n >= 0; --n) {       // smallest parts first
+            const bf16x8 w = __builtin_bit_cast(bf16x8, *(uint4*)part[n][jj]);
+#pragma unroll
+            for (int dt = 0; dt < 4; ++dt)
+              acc_o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vop[dt][jj], w, acc_o[dt], 0, 0, 0);
+          }
+      }
+      if (j0 + 64 <= e_all) return;
+      for (int w = 0; w < NW; ++w)
+        for (uint32_t todo = bad_of[w]; todo; todo &= todo - 1)
+          for (int q4 = 0; q4 < 4; ++q4) {
+            const int r = 4 * (NW * __builtin_ctz(todo) + w) + q4;
+            if (j0 + r >= g.k1 || (KG == 2 && r / 32 != kg)) continue;   // a repeated row
+            const bool sees = (vis[KG == 2 ? 0 : r / 32] >> (r & 31)) & 1u;
+            const bf16* vp = a.v + sOff[64 * x0 + r].y + 4 * hl;
+#pragma unroll
+            for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+              for (int n = 0; n < 4; ++n) {
+                const bf16x4 y = *(const bf16x4*)(vp + 32 * dt + 8 * n);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const float f = (float)y[e];
+                  if (sees && !(fabsf(f) <= 3.402823466e38f)) acc_o[dt][4 * n + e] += f;
+                }
+              }
+          }
+    };
+
+    for (int c0 = i_first; c0 < i_last; c0 += CH) {
+      const int c1 = min(c0 + CH, i_last);
+      if (c0 > i_first) __syncthreads();  // every wavefront left the units before
+      lay_out(c0, c1);
+      if (c0 == i_first) {
+#pragma unroll
+        for (int w = 0; w < NW; ++w) e_all = min(e_all, sEnd[w]);
+      }
+      if (ST == 1) {
+        for (int i = c0; i < c1; ++i) {
+          if (i > c0) __syncthreads();    // every wavefront left unit i - 1
+          fetch(i - c0, sK0, sV0);
+          __builtin_amdgcn_s_waitcnt(0);
+          clear(i, sV0, sBad[0]);
+          __syncthreads();                // unit i landed
+          item(i, i - c0, sK0, sV0, sBad[0]);
+        }
+        continue;
+      }
+      fetch(0, sK0, sV0);
+      auto step = [&](int i, auto par) __attribute__((always_inline)) {
+        constexpr int P = decltype(par)::value;
+        __builtin_amdgcn_s_waitcnt(0);
+        clear(i, P ? sV1 : sV0, sBad[P]);
+        __syncthreads();                  // unit i landed; every wavefront left unit i - 1
+        if (i + 1 < c1) fetch(i + 1 - c0, P ? sK0 : sK1, P ? sV0 : sV1);
+        item(i, i - c0, P ? sK1 : sK0, P ? sV1 : sV0, sBad[P]);
+      };
+      for (int i = c0; i < c1; i += 2) {
+        step(i, std::integral_constant<int, 0>{});
+        if (i + 1 < c1) step(i + 1, std::integral_constant<int, 1>{});
+      }
+    }
+
+    float l_tot = xor32_sum(l_run);
+    if (KG == 2) {
+      // the second half's wavefronts hand their sums to the first's
+      __syncthreads();
+      float* so = (float*)(rt ? sK1 : sK0);
+      if (kg == 1) {
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) so[(16 * dt + r) * 64 + lane] = acc_o[dt][r];
+        if (hl == 0) sMl[rt * 32 + col] = make_float2(m_run, l_tot);
+      }
+      __syncthreads();
+      if (kg == 0) {
+        const float2 ml = sMl[rt * 32 + col];
+        const float mn = fmaxf(m_run, ml.x), mu = mn == -INFINITY ? 0.f : mn;
+        const float al = fast_exp2(m_run - mu), be = fast_exp2(ml.x - mu);
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc_o[dt][r] = acc_o[dt][r] * al + so[(16 * dt + r) * 64 + lane] * be;
+        l_tot = l_tot * al + ml.y * be;
+        m_run = mn;
+      }
+    }
+    if (kg == 0 && rvalid) {
+      const int64_t at = (int64_t)g.base + (int64_t)hk * g.rows + rr + (int64_t)blockIdx.x * TR;
+      float* po = a.part_o + at * D + 4 * hl;
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+          *(float4*)(po + dt * 32 + 8 * n) = make_float4(acc_o[dt][4 * n], acc_o[dt][4 * n + 1],
+                                                         acc_o[dt][4 * n + 2], acc_o[dt][4 * n + 3]);
+      if (hl == 0) a.part_ml[at] = make_float2(m_run, l_tot);
+    }
+  }
+}
+
+// One wavefront per (row, head), two dims a lane: the partials of the row's two segments, a lane for the
+// (maximum, sum) of each, 64 at a time, eight partials' loads in flight.
+__global__ __launch_bounds__(256) void shared_merge_kernel(SharedArgs a) {
+  constexpr int D = 128;
+  const int64_t rh = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
+  if (rh >= a.T * a.H) return;
+  const int lane = wave_lane(), Gq = a.H / a.Hkv;
+  const int64_t row = rh / a.H;
+  const int h = (int)(rh - row * a.H), hk = h / Gq;
+  const int b = a.row_seq[row];
+  // runs [first, first + n) of work-groups, and the row's place in the first one's partials
+  int64_t first[2] = {0, 0}, at[2] = {0, 0};
+  int n[2] = {0, 0};
+  if (b >= 0) {
+    const int64_t per = a.head[1];
+    int s = a.G + b;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const SharedSeg g = a.seg[s];
+      const int items = (max(g.k1 - g.k0, 0) + 63) / 64;
+      const int64_t rr = (row - g.r0) * Gq + h % Gq;
+      if (items > 0 && rr >= 0 && rr < g.rows) {
+        const int64_t u0 = a.starts[s] + ((int64_t)hk * g.tiles + rr / a.tile_rows) * items;
+        first[x] = u0 / per;
+        n[x] = (int)((u0 + items - 1) / per - first[x]) + 1;
+        at[x] = g.base + (int64_t)hk * g.rows + rr + first[x] * a.tile_rows;
+      }
+      if (g.group < 0) break;
+      s = g.group;
+    }
+  }
+  float M = -INFINITY, L = 0.f;
+  float2 acc = make_float2(0.f, 0.f);
+  bool any = false;
+  for (int e0 = 0; e0 < n[0] + n[1]; e0 += kWave) {
+    const int e = e0 + lane;
+    const bool in = e < n[0] + n[1];
+    const int64_t p = e < n[0] ? at[0] + (int64_t)e * a.tile_rows
+                               : at[1] + (int64_t)(e - n[0]) * a.tile_rows;
+    const float2 ml = in ? a.part_ml[p] : make_float2(-INFINITY, 0.f);
+    // NaN in a score leaves the maximum and comes in through the sums
+    const bool seen = in && !(ml.x == -INFINITY && ml.y == 0.f);
+    const float Mn = fmaxf(M, wave_max(ml.x)), Mu = Mn == -INFINITY ? 0.f : Mn;
+    const float al = fast_exp2(M - Mu), w = seen ? fast_exp2(ml.x - Mu) : 0.f;
+    M = Mn;
+    L = L * al + wave_sum(seen ? ml.y * w : 0.f);
+    acc.x *= al;
+    acc.y *= al;
+    uint64_t todo = __ballot(seen);
+    any = any || todo != 0;
+    while (todo) {
+      float2 x[8];
+      float f[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int l = todo ? __builtin_ctzll(todo) : 0;
+        f[i] = todo ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), l)) : 0.f;
+        const int64_t pl = __shfl(p, l, kWave);
+        x[i] = make_float2(0.f, 0.f);
+        if (todo) x[i] = *(const float2*)(a.part_o + pl * D + 2 * lane);
+        todo &= todo - 1;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        acc.x = fmaf(f[i], x[i].x, acc.x);
+        acc.y = fmaf(f[i], x[i].y, acc.y);
+      }
+    }
+  }
+  const float inv = any ? 1.f / L : 0.f;
+  const int64_t to = row * a.o_st + (int64_t)h * a.o_sh + 2 * lane;
+  if (a.out_bf16) {
+    bf16x2 r;
+    r[0] = (bf16)(acc.x * inv);
+    r[1] = (bf16)(acc.y * inv);
+    *(bf16x2*)((bf16*)a.out + to) = r;
+  } else {
+    *(float2*)((float*)a.out + to) = make_float2(acc.x * inv, acc.y * inv);
+  }
+  if (a.lse && lane == 0)
+    a.lse[row * a.lse_st + (int64_t)h * a.lse_sh] = any ? (M + log2f(L)) * 0.6931471805599453f : -INFINITY;
+}
+
+// Row tiles of a work-group by the rows that share a key head (a group's on average), and its work-groups:
+// four a CU of the one-stage kernel, two of the others.
+struct SharedPlan { int rt, W; int64_t head, starts, seg, rows, ml, o, total; };
+inline SharedPlan shared_plan(int B, int G, int H, int Hkv, int64_t T) {
+  SharedPlan p;
+  const int64_t rows = T * (H / Hkv) / std::max(1, G > 0 ? G : B);
+  p.rt = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
+  p.W = p.rt == 1 ? 1024 : 512;
+  const int64_t parts = 2 * T * H + (int64_t)p.W * 32 * p.rt;
+  auto align = [](int64_t x) { return (x + 255) / 256 * 256; };
+  int64_t o = 0;
+  p.head = o; o += 256;
+  p.starts = o; o = align(o + ((int64_t)G + B) * 8);
+  p.seg = o; o = align(o + ((int64_t)G + B) * (int64_t)sizeof(SharedSeg));
+  p.rows = o; o = align(o + 2 * T * 4);
+  p.ml = o; o = align(o + parts * 8);
+  p.o = o; o = align(o + parts * 128 * 4);
+  p.total = o;
+  return p;
+}
+
+}  // namespace dash
+
+extern "C" int dash_attn_shared_workspace_size(int B, int G, int H, int Hkv, int64_t T, int64_t* bytes) {
+  using namespace dash;
+  if (!bytes || B < 0 || G < 0 || H <= 0 || Hkv <= 0 || T < 0) return kErrInvalid;
+  if (H % Hkv != 0) return kErrUnsupported;
+  *bytes = shared_plan(B, G, H, Hkv, T).total;
+  return kOk;
+}
+
+extern "C" int dash_attn_shared(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_sp,
+                                int64_t k_st, int64_t k_sh, const void* v, int64_t v_sp, int64_t v_st,
+                                int64_t v_sh, const int32_t* block_table, int64_t table_stride, int P,
+                                int page_size, int num_pages, const int32_t* context_lens,
+                                const int32_t* cu_seqlens_q, const int32_t* cu_groups,
+                                const int32_t* prefix_lens, void* out, int out_bf16, int64_t o_st,
+                                int64_t o_sh, float* lse, int64_t lse_st, int64_t lse_sh, int B, int G, int H,
+                                int Hkv, int64_t T, int D, float scale, void* workspace,
+                                int64_t workspace_bytes, void* stream) {
+  using namespace dash;
+  if (B < 0 || G < 0 || H <= 0 || Hkv <= 0 || T < 0 || P < 0 || page_size <= 0 || num_pages < 0)
+    return kErrInvalid;
+  if (T == 0) return kOk;
+  if (!q || !out || !cu_seqlens_q || (B > 0 && !context_lens) || (G > 0 && (!cu_groups || !prefix_lens)))
+    return kErrInvalid;
+  if (B > 0 && P > 0 && !block_table) return kErrInvalid;
+  if (num_pages > 0 && (!k || !v)) return kErrInvalid;
+  if (D != 128 || H % Hkv != 0 || B > kShMaxSeqs || G > kShMaxSeqs || !(scale > 0.f) ||
+      (int64_t)P * page_size > INT32_MAX)
+    return kErrUnsupported;
+  const int64_t strides[] = {q_st, q_sh, k_sp, k_st, k_sh, v_sp, v_st, v_sh};
+  for (int64_t s : strides)
+    if (s % 8 != 0) return kErrUnsupported;
+  const void* ptrs[] = {q, k, v};
+  for (const void* x : ptrs)
+    if ((uintptr_t)x % 16 != 0) return kErrUnsupported;
+  if (T > INT32_MAX - kShThreads || 2 * T * H > INT32_MAX || !fits_grid((T * H + 3) / 4, 256))
+    return kErrUnsupported;
+  const SharedPlan p = shared_plan(B, G, H, Hkv, T);
+  if (!workspace || workspace_bytes < p.total || (uintptr_t)workspace % 256 != 0) return kErrWorkspace;
+  char* w = (char*)workspace;
+  SharedArgs a = {};
+  a.q = (const bf16*)q; a.q_st = q_st; a.q_sh = q_sh;
+  a.k = (const bf16*)k; a.k_sp = k_sp; a.k_st = k_st; a.k_sh = k_sh;
+  a.v = (const bf16*)v; a.v_sp = v_sp; a.v_st = v_st; a.v_sh = v_sh;
+  a.table = block_table; a.table_stride = table_stride; a.page = page_size; a.num_pages = num_pages;
+  a.ctx = context_lens; a.cu = cu_seqlens_q; a.cu_groups = cu_groups; a.prefix = prefix_lens;
+  a.out = out; a.out_bf16 = out_bf16; a.o_st = o_st; a.o_sh = o_sh;
+  a.lse = lse; a.lse_st = lse_st; a.lse_sh = lse_sh;
+  a.B = B; a.G = B > 0 ? G : 0; a.H = H; a.Hkv = Hkv; a.T = T;
+  a.S = num_pages > 0 ? P * page_size : 0;
+  a.W = p.W; a.tile_rows = 32 * p.rt; a.scale_log2e = scale * 1.4426950408889634f;
+  a.head = (int64_t*)(w + p.head); a.starts = (int64_t*)(w + p.starts);
+  a.seg = (SharedSeg*)(w + p.seg); a.row_seq = (int32_t*)(w + p.rows); a.row_pos = a.row_seq + T;
+  a.part_ml = (float2*)(w + p.ml); a.part_o = (float*)(w + p.o);
+  hipStream_t st = (hipStream_t)stream;
+  hipLaunchKernelGGL(shared_plan_kernel, dim3((unsigned)(1 + (T + kShThreads - 1) / kShThreads)),
+                     dim3(kShThreads), 0, st, a);
+  if (a.S > 0) {
+    const dim3 grid(p.W);
+    if (p.rt == 1) hipLaunchKernelGGL((shared_attn_kernel<1, 2>), grid, dim3(128), 0, st, a);
+    else if (p.rt == 2) hipLaunchKernelGGL((shared_attn_kernel<2, 2>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((shared_attn_kernel<4, 1>), grid, dim3(256), 0, st, a);
+  }
+  hipLaunchKernelGGL(shared_merge_kernel, dim3((unsigned)((T * H + 3) / 4)), dim3(256), 0, st, a);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? kOk : (int)e;
+}

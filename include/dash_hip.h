@@ -830,6 +830,27 @@ int dash_rope_append(const void* q, int64_t q_st, int64_t q_sh, int H, void* q_o
                      int64_t vc_sh, int page_size, int num_pages, const double* inv_freq, int pairs, int start,
                      int interleaved, float factor, int T, int D, void* stream);
 
+/* Workspace bytes dash_attn_shared needs. */
+int dash_attn_shared_workspace_size(int B, int G, int H, int Hkv, int64_t T, int64_t* bytes);
+
+/*
+ * Full attention of new tokens q [T, H, 128] bf16 over pages [num_pages, page_size, Hkv, 128] (strides of page,
+ * token and head; H a multiple of Hkv) through block_table [B, P].  Row cu_seqlens_q[b] + i is at position
+ * context_lens[b] + i of sequence b and sees its keys up to itself, whose keys and values are written.  The
+ * sequences cu_groups[g] .. cu_groups[g + 1] - 1 (cu_groups [G + 1]) share the keys below prefix_lens[g]: those are
+ * read through the first one's table row, once for the group.  Sequences of no group share nothing.  Prefix sums
+ * that do not fit the rows or sequences are cut to them.  out [T, H, 128] fp32 (out_bf16 = 0) or bf16, lse [T, H]
+ * optional; a row that sees no key, and a row of no sequence, gives 0 and -inf.  B, G <= 8,192; any page size;
+ * P * page_size < 2^31.  workspace: dash_attn_shared_workspace_size bytes, 256-byte aligned, any contents.
+ */
+int dash_attn_shared(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_sp, int64_t k_st,
+                     int64_t k_sh, const void* v, int64_t v_sp, int64_t v_st, int64_t v_sh,
+                     const int32_t* block_table, int64_t table_stride, int P, int page_size, int num_pages,
+                     const int32_t* context_lens, const int32_t* cu_seqlens_q, const int32_t* cu_groups,
+                     const int32_t* prefix_lens, void* out, int out_bf16, int64_t o_st, int64_t o_sh, float* lse,
+                     int64_t lse_st, int64_t lse_sh, int B, int G, int H, int Hkv, int64_t T, int D, float scale,
+                     void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
