@@ -126,6 +126,8 @@ SIGNATURES = {
     "dash_attn_shared_workspace_size": (_i, [_i, _i, _i, _i, _l, ctypes.POINTER(_l)]),
     "dash_attn_shared": (_i, [_p, _l, _l, _p, _l, _l, _l, _p, _l, _l, _l, _p, _l, _i, _i, _i, _p, _p, _p,
                               _p, _p, _i, _l, _l, _p, _l, _l, _i, _i, _i, _i, _l, _i, _f, _p, _l, _p]),
+    "dash_sample_workspace_size": (_i, [_l, _i, ctypes.POINTER(_l)]),
+    "dash_sample": (_i, [_p, _l, _i, _p, _p, _f, _p, _i, _p, _f, _p, _f, _l, _i, _p, _p, _l, _i, _p, _l, _p]),
     "dash_page_rope_advance": (_i, [_p, _l, _i, _l, _p, _p, _p, _l, _p, _p, _p, _p]),
 }
 

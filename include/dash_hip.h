@@ -851,6 +851,25 @@ int dash_attn_shared(const void* q, int64_t q_st, int64_t q_sh, const void* k, i
                      int64_t lse_st, int64_t lse_sh, int B, int G, int H, int Hkv, int64_t T, int D, float scale,
                      void* workspace, int64_t workspace_bytes, void* stream);
 
+/* Workspace bytes dash_sample needs for R rows of V logits. */
+int dash_sample_workspace_size(int64_t R, int V, int64_t* bytes);
+
+/*
+ * The next token of every row of logits [R, V] (fp32, bf16, fp16: dtype 0, 1, 2; contiguous rows).  Weights
+ * exp((x - max) / temperature), in the order of falling logits (of equals the lower id first): the first top_k stay
+ * (<= 0: all); of those, the ones whose predecessors hold less than top_p of the weight of the first top_k (>= 1:
+ * all); of those, the ones of at least min_p times the best one's weight (<= 0: all); the first always does, and
+ * alone where the temperature is not above 0.  Each a device array [R], or where that is null the number beside it.
+ * tokens [R] gets the first id whose running sum of weights exceeds uniforms[r] times the whole (-1: every logit is
+ * -inf or NaN); both null: no draw.  probs (optional; probs_dtype as dtype, row stride probs_stride) gets the
+ * probabilities that are left.  V <= 2^20.  workspace: dash_sample_workspace_size bytes, 256-byte aligned, any
+ * contents.
+ */
+int dash_sample(const void* logits, int64_t row_stride, int dtype, const float* uniforms, const float* temperature,
+                float temperature0, const int32_t* top_k, int top_k0, const float* top_p, float top_p0,
+                const float* min_p, float min_p0, int64_t R, int V, int64_t* tokens, void* probs,
+                int64_t probs_stride, int probs_dtype, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
