@@ -12,38 +12,43 @@
 // atomics add them up, and a border lies where the 64-bit weights put it but for 2^-46 of the
 // best token's weight a token.  A token below half of 2^-s is never drawn and counts as none.
 //
-// A row is cut into S chunks of a work-group each; a chunk's tiles are 4,096 tokens, four in a row a thread:
-//   sample_max    the best token and the lowest logit of every chunk
-//   sample_bins   count and weight of a chunk's tokens in kSmBins bins of equal width in M - x, from M down
-//   sample_pick   the bins in which the k-th token and the border of p lie (every work-group by itself from
-//                 the chunks' sums), their tokens listed; the weight of what surely stays, tile by tile
-//   sample_draw   the borders within the listed tokens, by their (logit, id); the tile and then the token
-//                 that u falls into; the probabilities
-// Rows that need no border skip the bins.  A list that would be too long (many tokens of one logit) is
-// not made: its work-group reads the row again instead, as often as the border needs.
+// A short row, or one of many, is one work-group's (sample_row_kernel).  A long one is cut into S chunks of a
+// work-group each:
+//   sample_max     the best token and the lowest logit of every chunk
+//   sample_bins    count and weight of a chunk's tokens in kSmBins bins of equal width in M - x, from M down
+//   sample_select  the bins in which the k-th token, the border of p and the one of min_p lie: the bins before
+//                  them surely stay, those behind surely do not
+//   sample_pick    the tokens between, listed
+//   sample_draw    the borders within the list, by the tokens' (logit, id); the chunk, the tile and then the
+//                  token that u falls into; the probabilities
+// A list that would be too long (many tokens of one logit) is not made: its work-group reads the row again
+// instead, as often as the border needs.
 #include <hip/hip_fp16.h>
+
+#include <cfloat>
 
 #include "dash_common.h"
 
 namespace dash {
 
-constexpr int kSmThreads = 1024;
-constexpr int kSmTile = 4 * kSmThreads;   // tokens
+constexpr int kSmWide = 1024;             // threads of a row's work-group
+constexpr int kSmThreads = 256;           // of a chunk's
 constexpr int kSmBins = 512;
 constexpr int kSmMaxChunks = 16;
 constexpr int kSmList = 2048;             // tokens listed of a row
 constexpr int kSmMaxV = 1 << 20;
-constexpr int kSmTiles = kSmMaxV / kSmTile;
-constexpr int kSmRows = 2048;             // rows of a pass
-constexpr int kSmWaves = kSmThreads / kWave;
+constexpr int kSmTiles = 256;             // tiles of a row's work-group, or of a chunk's, at most
+constexpr int kSmShort = 32768;           // tokens of a row that one work-group takes
+constexpr int kSmMany = 256;              // rows that take a work-group each, however long
+constexpr int kSmCut = 256;               // threads, and steps a pass, of the search for a border
 
-struct SampleState {                      // of a row, from sample_pick
-  uint64_t k_mass, k_whole;               // weight of the bins before the k-th token's; of the first k if exact
+struct SampleState {                      // of a row, once its bins are known
+  uint64_t k_mass, k_whole;               // weight of the bins before the k-th token's; of the first k, 0 if unknown
   uint64_t p_mass;                        // weight of the bins before the border of p's
   int32_t k_count, k_bin;                 // tokens of the bins before; -1: no border of k
   int32_t p_lo, p_hi;                     // bins that may hold the border of p; p_lo -1: none
-  int32_t sure;                           // bins below it stay
-  int32_t listed;                         // tokens listed, -1: too many
+  int32_t sure, end;                      // bins below `sure` stay, bins from `end` on do not
+  int32_t listed;                         // tokens to be looked at, -1: too many to list
 };
 
 struct SampleArgs {
@@ -51,17 +56,17 @@ struct SampleArgs {
   const float* u;                         // null: no draw
   const float* t; const int32_t* k; const float* p; const float* m;    // null: the number below
   float t0; int32_t k0; float p0, m0;
-  int V, S, chunk, tiles;                 // tiles of a row
+  int V, S, chunk;
   int bits;                               // s
-  int64_t* token; void* probs; int64_t p_st;
+  int64_t* token; void* probs; int p_type; int64_t p_st;
   // workspace
   uint64_t* best;                         // [R, S] key and inverted id of a chunk's best token
-  uint32_t* low;                          // [R, S] lowest live key
+  float* low;                             // [R, S] lowest logit that is not masked
   uint32_t* cnt; uint64_t* mass;          // [R, S, kSmBins]
   SampleState* state;                     // [R]
   int32_t* n_list;                        // [R]
   uint64_t* list;                         // [R, kSmList]
-  uint64_t* tile;                         // [R, tiles] weight of what surely stays
+  uint64_t* sure;                         // [R, S] weight of a chunk's tokens that surely stay
 };
 
 __device__ __forceinline__ float sm_in(float x) { return x; }
@@ -71,24 +76,47 @@ __device__ __forceinline__ void sm_out(float x, float& y) { y = x; }
 __device__ __forceinline__ void sm_out(float x, bf16& y) { y = (bf16)x; }
 __device__ __forceinline__ void sm_out(float x, __half& y) { y = __float2half_rn(x); }
 
-// Four tokens from v on (masked, -inf, past v1).
+// A vector of kN tokens, 16 bytes at any element's boundary (global loads need no more); masked (-inf) past
+// the row's end.
 template <typename T>
-__device__ __forceinline__ void sm_load(const T* row, int v, int v1, float (&x)[4]) {
-  typedef uint32_t V __attribute__((ext_vector_type(sizeof(T)), aligned(2)));
-  if (v + 4 <= v1) {
-    union { V b; T e[4]; } y;
-    y.b = *(const V*)(row + v);
+struct SmVec {
+  static constexpr int kN = 16 / sizeof(T);
+  typedef uint32_t V __attribute__((ext_vector_type(4), aligned(2)));
+  V b;
+  __device__ __forceinline__ void load(const T* row, int v, int v1) {
+    if (v + kN <= v1) {
+      b = *(const V*)(row + v);
+    } else {
+      T e[kN];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = sm_in(y.e[j]);
-  } else {
+      for (int j = 0; j < kN; ++j) sm_out(-INFINITY, e[j]);
+      if (v < v1) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = v + j < v1 ? sm_in(row[v + j]) : -INFINITY;
+        for (int j = 0; j < kN; ++j)
+          if (v + j < v1) e[j] = row[v + j];
+      }
+      __builtin_memcpy(&b, e, 16);
+    }
   }
-}
+  // Logit j: NaN as masked, +inf as the largest number.
+  __device__ __forceinline__ float at(int j) const {
+    float x;
+    if (sizeof(T) == 4) {
+      x = __uint_as_float(b[j]);
+    } else {
+      const uint16_t h = (uint16_t)(b[j / 2] >> (16 * (j & 1)));
+      T e;
+      __builtin_memcpy(&e, &h, sizeof(T));
+      x = sm_in(e);
+    }
+    return x == x ? fminf(x, FLT_MAX) : -INFINITY;
+  }
+};
 
-// Keys order the logits; 0: masked (-inf) or no number.  -0 is 0.
+template <typename T, int NT> constexpr int kSmTile = SmVec<T>::kN * NT;     // tokens of NT threads
+
+// Keys order the logits; -0 is 0.
 __device__ __forceinline__ uint32_t sm_key(float x) {
-  if (!(x > -INFINITY)) return 0u;
   const uint32_t b = __float_as_uint(x + 0.f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
@@ -102,7 +130,7 @@ __device__ __forceinline__ uint64_t sm_place(uint32_t key, int v) {
 
 // What a row's tokens are measured by.
 struct SampleRow {
-  float top, bin_scale;
+  float top, t, bin_scale;
   double c, scale;                        // log2(e) / T; 2^s
   float min_p;
   int k; float p;
@@ -111,7 +139,7 @@ struct SampleRow {
 };
 
 template <typename A>
-__device__ __forceinline__ SampleRow sm_row(const A& a, int64_t r, uint64_t best, uint32_t low) {
+__device__ __forceinline__ SampleRow sm_row(const A& a, int64_t r, uint64_t best, float low) {
   SampleRow w;
   const float t = a.t ? a.t[r] : a.t0;
   w.k = a.k ? a.k[r] : a.k0;
@@ -123,58 +151,75 @@ __device__ __forceinline__ SampleRow sm_row(const A& a, int64_t r, uint64_t best
   w.best_id = (int)~(uint32_t)best;
   w.greedy = !(t > 0.f);
   w.top = sm_logit(key);
+  w.t = t;
   w.c = 1.4426950408889634 / (double)t;
   w.scale = __builtin_bit_cast(double, (uint64_t)(1023 + a.bits) << 52);
   if (w.k >= a.V) w.k = 0;
-  w.filter = w.any && !w.greedy && (w.k > 0 || w.p < 1.f);
+  w.filter = w.any && !w.greedy && (w.k > 0 || w.p < 1.f || w.min_p > 0.f);
   // past (s + 1) ln 2 T from the top a weight is none
-  const float range = fminf(w.top - sm_logit(low), (float)(a.bits + 1) * 0.6931472f * t);
-  w.bin_scale = range > 1e-30f ? (float)kSmBins / range : 0.f;
+  const float range = fminf(w.top - low, (float)(a.bits + 1) * 0.6931472f * t);
+  w.bin_scale = range > 1e-30f ? fmaxf((float)kSmBins / range, 1e-37f) : 1e-37f;
   return w;
 }
-// The best token of a row and its lowest logit, from its chunks.
+// The best token of a row and its lowest logit, from its chunks: a lane each.
 template <typename A>
 __device__ __forceinline__ SampleRow sm_row_of(const A& a, int64_t r) {
+  static_assert(kSmMaxChunks == 16, "four exchanges");
+  const int lane = wave_lane();
   uint64_t best = 0;
-  uint32_t low = ~0u;
-  for (int c = 0; c < a.S; ++c) {
-    best = max(best, a.best[r * a.S + c]);
-    low = min(low, a.low[r * a.S + c]);
+  float low = INFINITY;
+  if (lane < a.S) {
+    best = a.best[r * a.S + lane];
+    low = a.low[r * a.S + lane];
   }
-  return sm_row(a, r, best, low);
+#pragma unroll
+  for (int m = 8; m >= 1; m >>= 1) {
+    best = max(best, (uint64_t)__shfl_xor((unsigned long long)best, m, kWave));
+    low = fminf(low, __shfl_xor(low, m, kWave));
+  }
+  const uint32_t b0 = __builtin_amdgcn_readfirstlane((uint32_t)best);
+  const uint32_t b1 = __builtin_amdgcn_readfirstlane((uint32_t)(best >> 32));
+  return sm_row(a, r, (uint64_t)b1 << 32 | b0,
+                __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(low))));
 }
 
-// exp((x - top) / T).  2^y = 2^n 2^f with |f| <= 1/2, 2^f by the exponential's series up to the 12th power
-// of f ln 2, whose next term is below 1.7e-16.
+// exp((x - top) / T) = 2^y = 2^n 2^f with |f| <= 1/2, 2^f by the exponential's series up to the 11th power of
+// f ln 2: the next term is below 6.4e-15, less than the half of 2^-46 that whole numbers are rounded by.  Masked: 2^-60.
 __device__ __forceinline__ double sm_weight(const SampleRow& w, float x) {
-  if (x == w.top) return 1.0;
-  const double y = ((double)x - (double)w.top) * w.c;
-  if (!(y > -60.0)) return 0.0;
-  const double n = __builtin_rint(y), f = (y - n) * 0.6931471805599453;
-  double s = 1.0 / 479001600.0;
-  s = fma(s, f, 1.0 / 39916800.0);
-  s = fma(s, f, 1.0 / 3628800.0);
-  s = fma(s, f, 1.0 / 362880.0);
-  s = fma(s, f, 1.0 / 40320.0);
-  s = fma(s, f, 1.0 / 5040.0);
-  s = fma(s, f, 1.0 / 720.0);
-  s = fma(s, f, 1.0 / 120.0);
-  s = fma(s, f, 1.0 / 24.0);
-  s = fma(s, f, 1.0 / 6.0);
-  s = fma(s, f, 0.5);
+  const double y = fmax(((double)x - (double)w.top) * w.c, -60.0);
+  // y rounded to a whole number by adding 3 2^51, in whose last bits that then stands
+  const double near = y + 6755399441055744.0;
+  const double f = y - (near - 6755399441055744.0);
+  constexpr double L = 0.69314718055994530942;
+  constexpr double c2 = L * L / 2, c3 = c2 * L / 3, c4 = c3 * L / 4, c5 = c4 * L / 5, c6 = c5 * L / 6,
+                   c7 = c6 * L / 7, c8 = c7 * L / 8, c9 = c8 * L / 9, c10 = c9 * L / 10, c11 = c10 * L / 11;
+  double s = fma(c11, f, c10);
+  s = fma(s, f, c9);
+  s = fma(s, f, c8);
+  s = fma(s, f, c7);
+  s = fma(s, f, c6);
+  s = fma(s, f, c5);
+  s = fma(s, f, c4);
+  s = fma(s, f, c3);
+  s = fma(s, f, c2);
+  s = fma(s, f, L);
   s = fma(s, f, 1.0);
-  s = fma(s, f, 1.0);
-  return __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, s) + ((uint64_t)(int64_t)(int)n << 52));
+  const uint64_t bits = __builtin_bit_cast(uint64_t, s);
+  const uint32_t top = (uint32_t)(bits >> 32) + ((uint32_t)__builtin_bit_cast(uint64_t, near) << 20);
+  return __builtin_bit_cast(double, (uint64_t)top << 32 | (uint32_t)bits);
 }
 // The weight as a whole number of 2^-s, to the nearest: added to 2^52 it stands in the last bits.
 __device__ __forceinline__ uint64_t sm_whole(const SampleRow& w, double e) {
   return __builtin_bit_cast(uint64_t, fma(e, w.scale, 4503599627370496.0)) - 0x4330000000000000ull;
 }
+// How far a logit lies below the top, in bins.
+__device__ __forceinline__ float sm_below(const SampleRow& w, float x) { return (w.top - x) * w.bin_scale; }
 __device__ __forceinline__ int sm_bin(const SampleRow& w, float x) {
-  return x == w.top ? 0 : (int)fminf((w.top - x) * w.bin_scale, (float)(kSmBins - 1));
+  return (int)fminf(sm_below(w, x), (float)(kSmBins - 1));
 }
 
 // Sum over the work-group's earlier threads; total: over all.
+template <int NT>
 __device__ __forceinline__ uint64_t sm_before(uint64_t v, uint64_t* sW, uint64_t& total) {
   const int lane = wave_lane(), wv = threadIdx.x / kWave;
   uint64_t x = v;
@@ -189,50 +234,238 @@ __device__ __forceinline__ uint64_t sm_before(uint64_t v, uint64_t* sW, uint64_t
   uint64_t before = 0;
   total = 0;
 #pragma unroll
-  for (int w = 0; w < kSmWaves; ++w) {
+  for (int w = 0; w < NT / kWave; ++w) {
     if (w < wv) before += sW[w];
     total += sW[w];
   }
   return before + x - v;
 }
 
-template <typename T>
-__global__ __launch_bounds__(kSmThreads) void sample_max_kernel(SampleArgs a) {
-  __shared__ uint64_t sB[kSmWaves];
-  __shared__ uint32_t sL[kSmWaves];
-  const int64_t r = blockIdx.y;
-  const int c = blockIdx.x, tid = threadIdx.x;
-  const int v0 = c * a.chunk, v1 = min(a.V, v0 + a.chunk);
-  const T* row = (const T*)a.x + r * a.x_st;
-  uint64_t best = 0;
-  uint32_t low = ~0u;
-  for (int v = v0 + 4 * tid; v < v1; v += kSmTile) {
-    float x[4];
-    sm_load(row, v, v1, x);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t key = sm_key(x[j]);
-      if (key == 0) continue;
-      best = max(best, sm_place(key, v + j));
-      low = min(low, key);
-    }
-  }
+// The best token and the lowest logit of a work-group's tokens, on every thread.
+template <int NT>
+__device__ __forceinline__ void sm_ends(float x, int id, float& low, uint64_t& best, uint64_t* sB, float* sL) {
+  best = x > -INFINITY ? sm_place(sm_key(x), id) : 0;
 #pragma unroll
   for (int m = 32; m >= 1; m >>= 1) {
     best = max(best, (uint64_t)__shfl_xor((unsigned long long)best, m, kWave));
-    low = min(low, (uint32_t)__shfl_xor(low, m, kWave));
+    low = fminf(low, __shfl_xor(low, m, kWave));
   }
-  if (wave_lane() == 0) { sB[tid / kWave] = best; sL[tid / kWave] = low; }
+  if (wave_lane() == 0) { sB[threadIdx.x / kWave] = best; sL[threadIdx.x / kWave] = low; }
   __syncthreads();
-  if (tid == 0) {
 #pragma unroll
-    for (int w = 1; w < kSmWaves; ++w) {
-      best = max(best, sB[w]);
-      low = min(low, sL[w]);
+  for (int w = 0; w < NT / kWave; ++w) {
+    best = max(best, sB[w]);
+    low = fminf(low, sL[w]);
+  }
+}
+__device__ __forceinline__ void sm_see(float x, int v, float& best, int& id, float& low) {
+  if (x > best) { best = x; id = v; }
+  low = x > -INFINITY ? fminf(low, x) : low;
+}
+// A token into the bins.
+__device__ __forceinline__ void sm_count(const SampleRow& w, float x, uint32_t* sCnt, unsigned long long* sMass) {
+  const uint64_t e = sm_whole(w, sm_weight(w, x));
+  const int b = sm_bin(w, x);
+  if (e == 0) return;
+  atomicAdd(&sCnt[b], 1u);
+  atomicAdd(&sMass[b], (unsigned long long)e);
+}
+
+struct SampleShared {
+  uint64_t sW[kSmWide / kWave];
+  float sL[kSmWide / kWave];
+  uint32_t before[kSmBins + 1];           // tokens of the bins before
+  uint64_t k_bin_mass;
+  SampleState st;
+  int at[2];
+  int listed;
+  unsigned long long ends[2];
+  unsigned long long chunk[kSmMaxChunks];
+  unsigned long long tile[kSmTiles];
+  uint32_t cnt[kSmBins];
+  unsigned long long mass[kSmBins];
+  uint64_t list[kSmList];
+  uint64_t whole[kSmCut];                 // a token of every step
+};
+
+// The row's borders as far as its bins tell, from the counts and weights in s.cnt and s.mass.  A thread adds up
+// kSmBins / kSmSelect bins of its own, of the first kSmSelect threads.
+constexpr int kSmSelect = 256;
+template <int NT>
+__device__ __forceinline__ void sm_select(const SampleRow& w, SampleShared& s) {
+  constexpr int PER = kSmBins / kSmSelect;
+  const int tid = threadIdx.x;
+  if (tid == 0) s.st = SampleState{0, 0, 0, 0, -1, -1, -1, kSmBins, kSmBins, 0};
+  if (w.filter) {
+    uint32_t cnt[PER], c = 0;
+    uint64_t mass[PER], m = 0, live, all;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      cnt[i] = tid < kSmSelect ? s.cnt[PER * tid + i] : 0;
+      mass[i] = tid < kSmSelect ? s.mass[PER * tid + i] : 0;
+      c += cnt[i];
+      m += mass[i];
     }
+    uint64_t cb = sm_before<NT>(c, s.sW, live), mb = sm_before<NT>(m, s.sW, all);
+    const uint64_t mb0 = mb;
+    const bool k_on = w.k > 0 && (uint64_t)w.k < live;
+    if (tid == 0 && !k_on) s.st.k_whole = all;
+    if (tid <= kSmSelect) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        if (tid < kSmSelect || i == 0) s.before[PER * tid + i] = (uint32_t)cb;
+        if (k_on && cb < (uint64_t)w.k && cb + cnt[i] >= (uint64_t)w.k) {
+          s.st.k_bin = PER * tid + i;
+          s.st.k_count = (int)cb;
+          s.st.k_mass = mb;
+          s.k_bin_mass = mass[i];
+          // (0: the k-th token is not its bin's last)
+          s.st.k_whole = cb + cnt[i] == (uint64_t)w.k ? mb + mass[i] : 0;
+        }
+        cb += cnt[i];
+        mb += mass[i];
+      }
+    }
+    __syncthreads();
+    const int kb = s.st.k_bin;
+    const bool part = s.st.k_whole == 0;
+    if (w.p < 1.f && tid < kSmSelect) {
+      const double hi = (double)w.p * (double)(part ? s.st.k_mass + s.k_bin_mass : s.st.k_whole);
+      const double lo = part ? (double)w.p * (double)s.st.k_mass : hi;
+      mb = mb0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int b = PER * tid + i;
+        if (mass[i] > 0) {
+          // the bin in which the weight reaches p of the first k's, whatever that is between lo and hi
+          if ((lo <= 0.0 && b == 0) || ((double)mb < lo && (double)(mb + mass[i]) >= lo)) {
+            s.st.p_lo = b;
+            s.st.p_mass = mb;
+          }
+          if ((hi <= 0.0 && b == 0) || ((double)mb < hi && (double)(mb + mass[i]) >= hi)) s.st.p_hi = b;
+        }
+        mb += mass[i];
+      }
+    }
+    __syncthreads();
+    if (tid == 0) {
+      SampleState st = s.st;
+      if (kb >= 0) {
+        st.sure = part ? kb : kb + 1;
+        st.end = kb + 1;
+      }
+      if (st.p_lo >= 0) {
+        st.sure = min(st.sure, st.p_lo);
+        st.end = min(st.end, st.p_hi + 1);
+      }
+      if (w.min_p > 0.f) {
+        // where exp((x - M) / T) = min_p, and the bins beside it, for what the logarithm may be off by
+        const float d = fminf(-logf(w.min_p) * w.t * w.bin_scale, (float)(kSmBins - 1));
+        st.sure = min(st.sure, max((int)d - 1, 0));
+        st.end = min(st.end, (int)d + 2);
+      }
+      int n = s.before[st.end] - s.before[min(st.sure, st.end)];
+      if (part && kb >= st.end && st.p_lo >= 0 && st.p_lo < st.end) n += s.before[kb + 1] - s.before[kb];
+      st.listed = n <= kSmList ? n : -1;
+      s.st = st;
+    }
+  }
+  __syncthreads();
+}
+// The k-th token lies within a bin; and is to be looked for (for itself or for the border of p).
+__device__ __forceinline__ bool sm_seeks_k(const SampleState& st) {
+  return st.k_bin >= 0 && st.k_whole == 0 && (st.k_bin < st.end || (st.p_lo >= 0 && st.p_lo < st.end));
+}
+
+// The bins' borders as they compare with sm_below: a masked token (inf) lies in none.
+struct SampleGate { float sure, end, k0, k1; };
+__device__ __forceinline__ SampleGate sm_gate(const SampleState& st) {
+  auto edge = [](int b) { return b >= kSmBins ? INFINITY : (float)b; };
+  const bool k = sm_seeks_k(st);
+  return SampleGate{edge(st.sure), edge(st.end), k ? edge(st.k_bin) : INFINITY, k ? edge(st.k_bin + 1) : 0.f};
+}
+// A token into the list, if it is to be looked at.
+__device__ __forceinline__ void sm_take(const SampleRow& w, const SampleGate& g, float x, int v, uint64_t* list,
+                                        int* listed) {
+  const float t = sm_below(w, x);
+  if (!((t >= g.sure && t < g.end) || (t >= g.k0 && t < g.k1))) return;
+  if (sm_whole(w, sm_weight(w, x)) == 0) return;
+  const int at = atomicAdd(listed, 1);
+  if (at < kSmList) list[at] = sm_place(sm_key(x), v);
+}
+// Adds `sum` over the wavefront to another.
+__device__ __forceinline__ void sm_add(uint64_t sum, unsigned long long* to) {
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) sum += __shfl_xor((unsigned long long)sum, m, kWave);
+  if (wave_lane() == 0 && sum > 0) atomicAdd(to, (unsigned long long)sum);
+}
+
+// A row, in memory or (HELD) in LDS as well, a vector after the other.
+template <typename T, bool HELD>
+struct SmSrc {
+  const T* row;
+  const uint4* held;
+  __device__ __forceinline__ SmVec<T> at(int v, int v1) const {
+    SmVec<T> x;
+    if (HELD) {
+      x.b = __builtin_bit_cast(typename SmVec<T>::V, held[v / SmVec<T>::kN]);
+    } else {
+      x.load(row, v, v1);
+    }
+    return x;
+  }
+};
+// f(vector, first id) of this thread's vectors of v0 .. v1 - 1, two in flight from memory.
+template <int NT, typename T, bool HELD, typename F>
+__device__ __forceinline__ void sm_vectors(const SmSrc<T, HELD>& src, int v0, int v1, F f) {
+  constexpr int E = SmVec<T>::kN, tile = kSmTile<T, NT>;
+  if (HELD) {
+#pragma unroll 1
+    for (int v = v0 + E * threadIdx.x; v < v1; v += tile) f(src.at(v, v1), v);
+    return;
+  }
+  for (int v = v0 + E * threadIdx.x; v < v1; v += 2 * tile) {
+    const SmVec<T> x = src.at(v, v1), y = src.at(v + tile, v1);
+    f(x, v);
+    if (v + tile < v1) f(y, v + tile);
+  }
+}
+// f(logit, id) of the tokens.
+template <int NT, typename T, bool HELD, typename F>
+__device__ __forceinline__ void sm_tokens(const SmSrc<T, HELD>& src, int v0, int v1, F f) {
+  sm_vectors<NT>(src, v0, v1, [&](const SmVec<T>& x, int v) {
+#pragma unroll
+    for (int j = 0; j < SmVec<T>::kN; ++j) f(x.at(j), v + j);
+  });
+}
+
+// f(place, weight) of the row's tokens of bins b0 .. b1 - 1.
+template <int NT, typename T, bool HELD, typename F>
+__device__ __forceinline__ void sm_of_row(const SampleRow& w, const SmSrc<T, HELD>& row, int V, int b0, int b1, F f) {
+  sm_tokens<NT>(row, 0, V, [&](float x, int v) {
+    const int b = sm_bin(w, x);
+    if (b < b0 || b >= b1) return;
+    const uint64_t e = sm_whole(w, sm_weight(w, x));
+    if (e > 0) f(sm_place(sm_key(x), v), e);
+  });
+}
+
+template <typename T>
+__global__ __launch_bounds__(kSmThreads) void sample_max_kernel(SampleArgs a) {
+  __shared__ uint64_t sB[kSmThreads / kWave];
+  __shared__ float sL[kSmThreads / kWave];
+  const int64_t r = blockIdx.y;
+  const int c = blockIdx.x, tid = threadIdx.x;
+  const int v0 = c * a.chunk, v1 = min(a.V, v0 + a.chunk);
+  const SmSrc<T, false> row = {(const T*)a.x + r * a.x_st, nullptr};
+  uint64_t best;
+  float top = -INFINITY, low = INFINITY;
+  int id = 0;
+  sm_tokens<kSmThreads>(row, v0, v1, [&](float x, int v) { sm_see(x, v, top, id, low); });
+  sm_ends<kSmThreads>(top, id, low, best, sB, sL);
+  if (tid == 0) {
     a.best[r * a.S + c] = best;
     a.low[r * a.S + c] = low;
-    if (c == 0) a.n_list[r] = 0;
   }
 }
 
@@ -242,389 +475,514 @@ __global__ __launch_bounds__(kSmThreads) void sample_bins_kernel(SampleArgs a) {
   __shared__ unsigned long long sMass[kSmBins];
   const int64_t r = blockIdx.y;
   const SampleRow w = sm_row_of(a, r);
-  if (!w.filter) return;
+  if (!w.any || w.greedy) return;
   const int c = blockIdx.x, tid = threadIdx.x;
   const int v0 = c * a.chunk, v1 = min(a.V, v0 + a.chunk);
-  const T* row = (const T*)a.x + r * a.x_st;
-  if (tid < kSmBins) { sCnt[tid] = 0; sMass[tid] = 0; }
+  const SmSrc<T, false> row = {(const T*)a.x + r * a.x_st, nullptr};
+  for (int b = tid; b < kSmBins; b += kSmThreads) { sCnt[b] = 0; sMass[b] = 0; }
   __syncthreads();
-  for (int v = v0 + 4 * tid; v < v1; v += kSmTile) {
-    float x[4];
-    sm_load(row, v, v1, x);
+  uint64_t sum = 0;
+  if (w.filter)
+    sm_tokens<kSmThreads>(row, v0, v1, [&](float x, int) { sm_count(w, x, sCnt, sMass); });
+  else
+    sm_tokens<kSmThreads>(row, v0, v1, [&](float x, int) { sum += sm_whole(w, sm_weight(w, x)); });
+  if (!w.filter) sm_add(sum, &sMass[0]);
+  __syncthreads();
+  const int64_t at = (r * a.S + c) * kSmBins;
+  for (int b = tid; b < kSmBins; b += kSmThreads) {
+    a.cnt[at + b] = sCnt[b];
+    a.mass[at + b] = sMass[b];
+  }
+}
+
+__global__ __launch_bounds__(kSmBins) void sample_select_kernel(SampleArgs a) {
+  __shared__ SampleShared s;
+  const int64_t r = blockIdx.x;
+  const int tid = threadIdx.x;
+  const SampleRow w = sm_row_of(a, r);
+  if (!w.any || w.greedy) return;
+  const uint32_t* cnts = a.cnt + r * a.S * kSmBins + tid;
+  const uint64_t* masses = a.mass + r * a.S * kSmBins + tid;
+  uint32_t cnt = 0;
+  uint64_t mass = 0;
+  if (w.filter) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (sm_key(x[j]) == 0) continue;
-      const uint64_t e = sm_whole(w, sm_weight(w, x[j]));
-      if (e == 0) continue;
-      const int b = sm_bin(w, x[j]);
-      atomicAdd(&sCnt[b], 1u);
-      atomicAdd(&sMass[b], (unsigned long long)e);
+    for (int i = 0; i < kSmMaxChunks; ++i) {
+      if (i < a.S) {
+        cnt += cnts[i * kSmBins];
+        mass += masses[i * kSmBins];
+      }
     }
   }
+  s.cnt[tid] = cnt;
+  s.mass[tid] = mass;
   __syncthreads();
-  if (tid < kSmBins) {
-    const int64_t at = (r * a.S + c) * kSmBins + tid;
-    a.cnt[at] = sCnt[tid];
-    a.mass[at] = sMass[tid];
+  sm_select<kSmBins>(w, s);
+  if (tid == 0) {
+    a.state[r] = s.st;
+    a.n_list[r] = 0;
   }
 }
 
 template <typename T>
 __global__ __launch_bounds__(kSmThreads) void sample_pick_kernel(SampleArgs a) {
-  __shared__ uint64_t sW[kSmWaves];
-  __shared__ uint32_t sBefore[kSmBins + 1];         // tokens of the bins before
-  __shared__ SampleState sSt;
-  __shared__ uint64_t sKMass, sAll;
-  __shared__ unsigned long long sTile[kSmTiles];
+  __shared__ uint64_t sList[kSmList];
+  __shared__ int sN, sAt;
+  __shared__ unsigned long long sSum;
   const int64_t r = blockIdx.y;
   const SampleRow w = sm_row_of(a, r);
   if (!w.any || w.greedy) return;
+  const SampleState st = a.state[r];
   const int c = blockIdx.x, tid = threadIdx.x;
   const int v0 = c * a.chunk, v1 = min(a.V, v0 + a.chunk);
-  if (tid == 0) sSt = SampleState{0, 0, 0, 0, -1, -1, -1, kSmBins, 0};
-  if (w.filter) {
-    uint32_t cnt = 0;
-    uint64_t mass = 0;
-    if (tid < kSmBins)
-      for (int i = 0; i < a.S; ++i) {
-        cnt += a.cnt[(r * a.S + i) * kSmBins + tid];
-        mass += a.mass[(r * a.S + i) * kSmBins + tid];
-      }
-    uint64_t live, all;
-    const uint64_t cb = sm_before(cnt, sW, live), mb = sm_before(mass, sW, all);
-    if (tid <= kSmBins) sBefore[tid] = (uint32_t)cb;
-    if (tid == 0) sAll = all;
-    const bool k_on = w.k > 0 && (uint64_t)w.k < live;
-    if (k_on && cb < (uint64_t)w.k && cb + cnt >= (uint64_t)w.k) {
-      sSt.k_bin = tid;
-      sSt.k_count = (int)cb;
-      sSt.k_mass = mb;
-      sKMass = mass;
-      if (cb + cnt == (uint64_t)w.k) sSt.k_whole = mb + mass;
-    }
-    __syncthreads();
-    const int kb = sSt.k_bin;
-    const bool part = kb >= 0 && sSt.k_whole == 0;  // the k-th token is not its bin's last
-    if (w.p < 1.f) {
-      const double hi = (double)w.p * (double)(kb >= 0 ? sSt.k_mass + sKMass : all);
-      const double lo = part ? (double)w.p * (double)sSt.k_mass : hi;
-      if (mass > 0) {
-        // the bin in which the weight reaches p of the first k's, whatever that is between lo and hi
-        if ((lo <= 0.0 && tid == 0) || ((double)mb < lo && (double)(mb + mass) >= lo)) {
-          sSt.p_lo = tid;
-          sSt.p_mass = mb;
-        }
-        if ((hi <= 0.0 && tid == 0) || ((double)mb < hi && (double)(mb + mass) >= hi)) sSt.p_hi = tid;
-      }
-    }
-    __syncthreads();
-    if (tid == 0) {
-      SampleState st = sSt;
-      int n = part ? sBefore[kb + 1] - sBefore[kb] : 0;
-      st.sure = kb < 0 ? kSmBins : part ? kb : kb + 1;
-      if (st.p_lo >= 0) {
-        if (kb >= 0) st.p_hi = min(st.p_hi, kb);
-        st.sure = st.p_lo;
-        n += sBefore[st.p_hi + 1] - sBefore[st.p_lo];
-        if (part && kb >= st.p_lo && kb <= st.p_hi) n -= sBefore[kb + 1] - sBefore[kb];
-      }
-      st.listed = n <= kSmList ? n : -1;
-      sSt = st;
-    }
-  }
+  if (tid == 0) { sN = 0; sSum = 0; }
   __syncthreads();
-  const SampleState st = sSt;
-  const bool part = st.k_bin >= 0 && st.k_whole == 0;
-  if (c == 0 && tid == 0) a.state[r] = st;
-  const int t0 = v0 / kSmTile, nt = (v1 - v0 + kSmTile - 1) / kSmTile;
-  if (tid < nt) sTile[tid] = 0;
+  uint64_t sum = 0;
+  for (int b = tid; b < st.sure; b += kSmThreads) sum += a.mass[(r * a.S + c) * kSmBins + b];
+  sm_add(sum, &sSum);
+  const SampleGate g = sm_gate(st);
+  const SmSrc<T, false> row = {(const T*)a.x + r * a.x_st, nullptr};
+  if (st.listed > 0)
+    sm_tokens<kSmThreads>(row, v0, v1, [&](float x, int v) { sm_take(w, g, x, v, sList, &sN); });
   __syncthreads();
-  const T* row = (const T*)a.x + r * a.x_st;
-  for (int i = 0; i < nt; ++i) {
-    const int v = v0 + i * kSmTile + 4 * tid;
-    float x[4];
-    if (v < v1) {
-      sm_load(row, v, v1, x);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = -INFINITY;
-    }
-    uint64_t sum = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t key = sm_key(x[j]);
-      if (key == 0) continue;
-      const int b = sm_bin(w, x[j]);
-      const bool sure = b < st.sure;
-      const bool take = st.listed > 0 && ((part && b == st.k_bin) || (b >= st.p_lo && b <= st.p_hi && st.p_lo >= 0));
-      if (!sure && !take) continue;
-      const double e = sm_weight(w, x[j]);
-      const uint64_t whole = sm_whole(w, e);
-      if (sure && e >= (double)w.min_p) sum += whole;
-      if (take && whole > 0) {
-        const int at = atomicAdd(&a.n_list[r], 1);
-        if (at < kSmList) a.list[r * kSmList + at] = sm_place(key, v + j);
-      }
-    }
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) sum += __shfl_xor((unsigned long long)sum, m, kWave);
-    if (wave_lane() == 0 && sum > 0) atomicAdd(&sTile[i], (unsigned long long)sum);
-  }
+  if (tid == 0) a.sure[r * a.S + c] = sSum;
+  const int n = min(sN, kSmList);
+  if (n == 0) return;
+  if (tid == 0) sAt = atomicAdd(&a.n_list[r], n);
   __syncthreads();
-  if (tid < nt) a.tile[r * a.tiles + t0 + tid] = sTile[tid];
+  for (int i = tid; i < n; i += kSmThreads)
+    if (sAt + i < kSmList) a.list[r * kSmList + sAt + i] = sList[i];
 }
 
 // The last token (by its place) of those in [lo, hi] that the rule keeps: with `need` > 0 the need-th,
 // else the last whose predecessors' weight, `mass` of them outside, is below `target` (the first if none
-// is).  for_each(f) calls f(place, key) for the tokens of the source.  mass: with the token found added.
+// is).  for_each(f) calls f(place, weight) for the tokens of the source.  mass: with the token found added.
+// A pass cuts [lo, hi] into kSmCut steps, which one wavefront adds up; at most eight passes, two for a list of a
+// few hundred.
 struct SampleCut { uint64_t place, mass; };
 template <typename Each>
-__device__ SampleCut sm_cut(const SampleRow& w, Each for_each, int need, double target, uint64_t mass,
-                            uint64_t lo, uint64_t hi, uint32_t* sCnt, unsigned long long* sMass, uint64_t* sW,
-                            unsigned long long* sEnds, int* sAt) {
-  const int tid = threadIdx.x;
-  // the ends of what there is
-  __syncthreads();
-  if (tid == 0) { sEnds[0] = ~0ull; sEnds[1] = 0; }
-  __syncthreads();
-  {
-    uint64_t mn = ~0ull, mx = 0;
-    for_each([&](uint64_t place, float) {
-      if (place < lo || place > hi) return;
-      mn = min(mn, place);
-      mx = max(mx, place);
-    });
+__device__ SampleCut sm_cut(Each for_each, int need, double target, uint64_t mass, uint64_t lo, uint64_t hi,
+                            SampleShared& s) {
+  const int tid = threadIdx.x, lane = wave_lane();
+  constexpr int PER = kSmCut / kWave;
+  uint64_t found = 0;                     // the weight of the token found
+  for (;;) {
+    // the ends of what there is: logits of 16 bits leave most of a range of places empty
+    __syncthreads();
+    if (tid == 0) { s.ends[0] = ~0ull; s.ends[1] = 0; }
+    if (tid < kSmCut) { s.cnt[tid] = 0; s.mass[tid] = 0; }
+    __syncthreads();
+    {
+      uint64_t mn = ~0ull, mx = 0;
+      for_each([&](uint64_t place, uint64_t) {
+        if (place < lo || place > hi) return;
+        mn = min(mn, place);
+        mx = max(mx, place);
+      });
+      if (__any(mx > 0)) {
 #pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) {
-      mn = min(mn, (uint64_t)__shfl_xor((unsigned long long)mn, m, kWave));
-      mx = max(mx, (uint64_t)__shfl_xor((unsigned long long)mx, m, kWave));
+        for (int m = 32; m >= 1; m >>= 1) {
+          mn = min(mn, (uint64_t)__shfl_xor((unsigned long long)mn, m, kWave));
+          mx = max(mx, (uint64_t)__shfl_xor((unsigned long long)mx, m, kWave));
+        }
+        if (lane == 0) { atomicMin(&s.ends[0], (unsigned long long)mn); atomicMax(&s.ends[1], (unsigned long long)mx); }
+      }
     }
-    if (wave_lane() == 0 && mx > 0) { atomicMin(&sEnds[0], (unsigned long long)mn); atomicMax(&sEnds[1], (unsigned long long)mx); }
-  }
-  __syncthreads();
-  lo = sEnds[0];
-  hi = sEnds[1];
-  while (lo < hi) {                       // 256 steps a pass: at most eight passes
-    const int top = 64 - __clzll(hi - lo), shift = max(top - 8, 0);
     __syncthreads();
-    if (tid < 256) { sCnt[tid] = 0; sMass[tid] = 0; }
-    if (tid == 0) *sAt = 0;
-    __syncthreads();
-    for_each([&](uint64_t place, float x) {
+    lo = s.ends[0];
+    hi = s.ends[1];
+    const uint64_t span = hi - lo;
+    const int shift = span ? max(64 - (int)__clzll(span) - 8, 0) : 0;
+    for_each([&](uint64_t place, uint64_t e) {
       if (place < lo || place > hi) return;
       const int b = (int)((hi - place) >> shift);
-      atomicAdd(&sCnt[b], 1u);
-      atomicAdd(&sMass[b], (unsigned long long)sm_whole(w, sm_weight(w, x)));
+      atomicAdd(&s.cnt[b], 1u);
+      atomicAdd(&s.mass[b], (unsigned long long)e);
+      s.whole[b] = place;                 // (of a step of one token: that token)
     });
     __syncthreads();
-    const uint32_t cnt = tid < 256 ? sCnt[tid] : 0;
-    const uint64_t mine = tid < 256 ? sMass[tid] : 0;
-    uint64_t total;
-    const uint64_t cb = sm_before(cnt, sW, total), mb = mass + sm_before(mine, sW, total);
-    if (cnt > 0) {
-      if (need > 0 ? cb < (uint64_t)need : cb == 0 || (double)mb < target) atomicMax(sAt, tid);
+    if (tid < kWave) {
+      uint32_t cnt[PER], c = 0;
+      uint64_t m[PER], x = 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        cnt[i] = s.cnt[PER * lane + i];
+        m[i] = s.mass[PER * lane + i];
+        c += cnt[i];
+        x += m[i];
+      }
+      uint32_t cb = c;
+      uint64_t mb = x;
+#pragma unroll
+      for (int d = 1; d < kWave; d <<= 1) {
+        const uint32_t yc = __shfl_up(cb, d, kWave);
+        const uint64_t ym = __shfl_up((unsigned long long)mb, d, kWave);
+        if (lane >= d) { cb += yc; mb += ym; }
+      }
+      cb -= c;
+      mb += mass - x;
+      // the last step that has a kept token
+      int at = -1;
+      uint32_t at_c = 0;
+      uint64_t at_m = 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        if (cnt[i] > 0 && (need > 0 ? cb < (uint32_t)need : cb == 0 || (double)mb < target)) {
+          at = PER * lane + i;
+          at_c = cb;
+          at_m = mb;
+        }
+        cb += cnt[i];
+        mb += m[i];
+      }
+      const uint64_t some = __ballot(at >= 0);
+      if (some ? lane == 63 - (int)__clzll(some) : lane == 0) {
+        s.at[0] = max(at, 0);
+        s.at[1] = (int)at_c;
+        s.ends[0] = at_m;
+      }
     }
     __syncthreads();
-    const int b = *sAt;
-    if (tid == b) { sEnds[0] = cb; sEnds[1] = mb; }
-    __syncthreads();
-    if (need > 0) need -= (int)sEnds[0];
-    mass = sEnds[1];
+    const int b = s.at[0];
+    if (need > 0) need -= s.at[1];
+    mass = s.ends[0];
+    found = s.mass[b];
+    if (shift == 0 || s.cnt[b] <= 1) {    // one token
+      hi = s.cnt[b] == 1 ? s.whole[b] : hi - (uint64_t)b;
+      break;
+    }
     hi -= (uint64_t)b << shift;
     const uint64_t width = (1ull << shift) - 1;
     lo = hi - lo > width ? hi - width : lo;
-    if (sCnt[b] == 1 && shift > 0) {      // one token: where it is
-      __syncthreads();
-      for_each([&](uint64_t place, float) {
-        if (place >= lo && place <= hi) sEnds[0] = place;
-      });
-      __syncthreads();
-      lo = hi = sEnds[0];
-    }
   }
   __syncthreads();
-  return SampleCut{hi, mass + sm_whole(w, sm_weight(w, sm_logit((uint32_t)(hi >> 32))))};
+  return SampleCut{hi, mass + found};
 }
 
-template <typename T, typename P>
+// The last place that stays (0: every one of the bins before `end`) from the source's tokens.
+template <typename Each>
+__device__ __forceinline__ uint64_t sm_borders(const SampleRow& w, const SampleState& st, Each tokens,
+                                               SampleShared& s) {
+  uint64_t last = 0, k_mass = st.k_whole;
+  if (sm_seeks_k(st)) {
+    const SampleCut z = sm_cut([&](auto f) { tokens(st.k_bin, st.k_bin + 1, f); }, w.k - st.k_count, 0.0, st.k_mass,
+                               0, ~0ull, s);
+    last = z.place;
+    k_mass = z.mass;
+  }
+  if (st.p_lo >= 0 && st.p_lo < st.end)
+    last = max(last, sm_cut([&](auto f) { tokens(st.p_lo, st.end, f); }, 0, (double)w.p * (double)k_mass, st.p_mass,
+                            last, ~0ull, s).place);
+  return last;
+}
+
+// The first (u below 1) or last of `n` weights' sums that exceeds `want`; the sum of those before it.
+template <int NT>
+__device__ __forceinline__ int sm_find(uint64_t mine, uint64_t ahead, double want, SampleShared& s,
+                                       uint64_t& before) {
+  const int tid = threadIdx.x;
+  uint64_t total;
+  ahead += sm_before<NT>(mine, s.sW, total);
+  if (tid == 0) { s.at[0] = INT32_MAX; s.at[1] = 0; }
+  __syncthreads();
+  if (mine > 0) {
+    if ((double)(ahead + mine) > want) atomicMin(&s.at[0], tid);
+    atomicMax(&s.at[1], tid);
+  }
+  __syncthreads();
+  const int t = s.at[0] == INT32_MAX ? s.at[1] : s.at[0];
+  if (tid == t) s.ends[0] = ahead;
+  __syncthreads();
+  before = s.ends[0];
+  return t;
+}
+
+// The token of v0 .. v1 - 1 that `want` falls into; `ahead` lies before.  The tile first, then its thread.
+template <int NT, typename T, bool HELD, typename Stays>
+__device__ __forceinline__ int sm_draw(const SampleRow& w, const SmSrc<T, HELD>& row, double want, uint64_t ahead, int v0, int v1,
+                                       SampleShared& s, Stays stays) {
+  const int tid = threadIdx.x;
+  constexpr int E = SmVec<T>::kN;
+  const int nt = (v1 - v0 + kSmTile<T, NT> - 1) / kSmTile<T, NT>;
+  int t = 0;
+  if (nt > 1) {
+    for (int i = tid; i < nt; i += NT) s.tile[i] = 0;
+    __syncthreads();
+    sm_vectors<NT>(row, v0, v1, [&](const SmVec<T>& x, int v) {
+      uint64_t sum = 0;
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        double f;
+        if (stays(x.at(j), v + j, f)) sum += sm_whole(w, f);
+      }
+      if (sum > 0) atomicAdd(&s.tile[(v - v0) / kSmTile<T, NT>], (unsigned long long)sum);
+    });
+    __syncthreads();
+    uint64_t before;
+    t = sm_find<NT>(tid < nt ? s.tile[tid] : 0, ahead, want, s, before);
+    ahead = before;
+  }
+  const int v = v0 + t * kSmTile<T, NT> + E * tid;
+  SmVec<T> x;
+  if (v < v1) x = row.at(v, v1);
+  uint64_t e[E], sum = 0, before;
+#pragma unroll
+  for (int j = 0; j < E; ++j) {
+    double f;
+    e[j] = v < v1 && stays(x.at(j), v + j, f) ? sm_whole(w, f) : 0;
+    sum += e[j];
+  }
+  const int th = sm_find<NT>(sum, ahead, want, s, before);
+  if (tid == th) {
+    uint64_t run = before;
+    int first = -1, last = v;
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      run += e[j];
+      if (e[j] > 0) {
+        if (first < 0 && (double)run > want) first = v + j;
+        last = v + j;
+      }
+    }
+    s.at[1] = first < 0 ? last : first;
+  }
+  __syncthreads();
+  return s.at[1];
+}
+
+__device__ __forceinline__ void sm_put(void* probs, int type, int64_t at, float x) {
+  if (type == 0) ((float*)probs)[at] = x;
+  else if (type == 1) sm_out(x, ((bf16*)probs)[at]);
+  else sm_out(x, ((__half*)probs)[at]);
+}
+// kN probabilities from v on.
+template <typename T>
+__device__ __forceinline__ void sm_put_vec(const SampleArgs& a, int64_t r, int v, int v1, const float* x) {
+#pragma unroll
+  for (int j = 0; j < SmVec<T>::kN; ++j)
+    if (v + j < v1) sm_put(a.probs, a.p_type, r * a.p_st + v + j, x[j]);
+}
+
+// Whether a token stays, and its weight.
+__device__ __forceinline__ bool sm_stays(const SampleRow& w, const SampleGate& g, uint64_t last, float x, int v,
+                                         double& e) {
+  const float t = sm_below(w, x);
+  if (t >= g.end || (t >= g.sure && sm_place(sm_key(x), v) < last)) return false;
+  e = sm_weight(w, x);
+  return e >= (double)w.min_p;
+}
+// What a greedy row, or one without any token, gives.
+template <int NT>
+__device__ __forceinline__ void sm_one(const SampleArgs& a, const SampleRow& w, int64_t r, int c, int v0, int v1) {
+  if (c == 0 && threadIdx.x == 0 && a.token) a.token[r] = w.any ? w.best_id : -1;
+  if (a.probs)
+    for (int v = v0 + threadIdx.x; v < v1; v += NT)
+      sm_put(a.probs, a.p_type, r * a.p_st + v, w.any && v == w.best_id ? 1.f : 0.f);
+}
+// u times the whole.  A number of 1 is exceeded by no running sum: the last token that stays.
+__device__ __forceinline__ double sm_want(float u, uint64_t total) {
+  u = fmaxf(u, 0.f);
+  return u < 1.f ? (double)u * (double)total : (double)INFINITY;
+}
+// f(place, weight) of the listed tokens of bins b0 .. b1 - 1.
+template <typename F>
+__device__ __forceinline__ void sm_listed(const SampleRow& w, int n, int b0, int b1, const SampleShared& s, F f) {
+  if (threadIdx.x < kSmCut)
+    for (int i = threadIdx.x; i < n; i += kSmCut) {
+      const uint64_t place = s.list[i];
+      const float x = sm_logit((uint32_t)(place >> 32));
+      const int b = sm_bin(w, x);
+      if (b >= b0 && b < b1) f(place, sm_whole(w, sm_weight(w, x)));
+    }
+}
+
+// The probabilities of tokens v0 .. v1 - 1.
+template <int NT, typename T, bool HELD, typename Stays>
+__device__ __forceinline__ void sm_probs(const SampleArgs& a, const SampleRow& w, const SmSrc<T, HELD>& row,
+                                         int64_t r, int v0, int v1, uint64_t total, Stays stays) {
+  constexpr int E = SmVec<T>::kN;
+  const double inv = w.scale / (double)total;
+  sm_vectors<NT>(row, v0, v1, [&](const SmVec<T>& x, int v) {
+    float p[E];
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      double e;
+      p[j] = stays(x.at(j), v + j, e) && sm_whole(w, e) > 0 ? (float)(e * inv) : 0.f;
+    }
+    sm_put_vec<T>(a, r, v, v1, p);
+  });
+}
+
+template <typename T>
 __global__ __launch_bounds__(kSmThreads) void sample_draw_kernel(SampleArgs a) {
-  __shared__ uint64_t sList[kSmList];
-  __shared__ uint32_t sCnt[256];
-  __shared__ unsigned long long sMass[256];
-  __shared__ uint64_t sW[kSmWaves];
-  __shared__ unsigned long long sEnds[2];
-  __shared__ int sAt[2];
-  __shared__ unsigned long long sTile[kSmTiles];
+  __shared__ SampleShared s;
   const int64_t r = blockIdx.y;
   const int c = blockIdx.x, tid = threadIdx.x;
   const SampleRow w = sm_row_of(a, r);
   const int v0 = c * a.chunk, v1 = min(a.V, v0 + a.chunk);
-  P* const probs = a.probs ? (P*)a.probs + r * a.p_st : nullptr;
   if (!w.any || w.greedy) {
-    if (c == 0 && tid == 0 && a.token) a.token[r] = w.any ? w.best_id : -1;
-    if (probs)
-      for (int v = v0 + tid; v < v1; v += kSmThreads) sm_out(w.any && v == w.best_id ? 1.f : 0.f, probs[v]);
+    sm_one<kSmThreads>(a, w, r, c, v0, v1);
     return;
   }
-  const T* row = (const T*)a.x + r * a.x_st;
+  const SmSrc<T, false> row = {(const T*)a.x + r * a.x_st, nullptr};
   const SampleState st = a.state[r];
-  const bool part = st.k_bin >= 0 && st.k_whole == 0;
-  for (int i = tid; i < st.listed; i += kSmThreads) sList[i] = a.list[r * kSmList + i];
-  for (int i = tid; i < a.tiles; i += kSmThreads) sTile[i] = a.tile[r * a.tiles + i];
+  for (int i = tid; i < st.listed; i += kSmThreads) s.list[i] = a.list[r * kSmList + i];
+  if (tid < a.S) s.chunk[tid] = a.sure[r * a.S + tid];
   __syncthreads();
-  // the tokens of bins b0 .. b1
-  auto tokens = [&](int b0, int b1) {
-    return [&, b0, b1](auto f) {
-      if (st.listed >= 0) {
-        for (int i = tid; i < st.listed; i += kSmThreads) {
-          const float x = sm_logit((uint32_t)(sList[i] >> 32));
-          const int b = sm_bin(w, x);
-          if (b >= b0 && b <= b1) f(sList[i], x);
-        }
-        return;
-      }
-      for (int v = 4 * tid; v < a.V; v += kSmTile) {
-        float x[4];
-        sm_load(row, v, a.V, x);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t key = sm_key(x[j]);
-          if (key == 0) continue;
-          const int b = sm_bin(w, x[j]);
-          if (b >= b0 && b <= b1 && sm_whole(w, sm_weight(w, x[j])) > 0) f(sm_place(key, v + j), x[j] + 0.f);
-        }
-      }
-    };
-  };
-  uint64_t last = ~0ull;                  // the last place that stays past the sure bins
-  uint64_t k_place = 0, k_mass = st.k_whole;
-  if (part) {
-    const SampleCut z = sm_cut(w, tokens(st.k_bin, st.k_bin), w.k - st.k_count, 0.0, st.k_mass, 0, ~0ull, sCnt,
-                               sMass, sW, sEnds, sAt);
-    last = k_place = z.place;
-    k_mass = z.mass;
-  }
-  if (st.p_lo >= 0) {
-    if (st.k_bin < 0) {                   // of the whole row
-      uint64_t all = 0;
-      if (tid < kSmBins)
-        for (int i = 0; i < a.S; ++i) all += a.mass[(r * a.S + i) * kSmBins + tid];
-      sm_before(all, sW, k_mass);
-    }
-    last = sm_cut(w, tokens(st.p_lo, st.p_hi), 0, (double)w.p * (double)k_mass, st.p_mass, k_place, ~0ull, sCnt,
-                  sMass, sW, sEnds, sAt).place;
-  }
-  if (st.sure < kSmBins)
-    tokens(st.sure, kSmBins - 1)([&](uint64_t place, float x) {
-      if (place < last) return;
-      const double e = sm_weight(w, x);
-      if (e >= (double)w.min_p)
-        atomicAdd(&sTile[(int)~(uint32_t)place / kSmTile], (unsigned long long)sm_whole(w, e));
+  uint64_t last = 0;
+  auto finish = [&](auto tokens) {
+    last = sm_borders(w, st, tokens, s);
+    tokens(st.sure, st.end, [&](uint64_t place, uint64_t e) {
+      if (place >= last && sm_weight(w, sm_logit((uint32_t)(place >> 32))) >= (double)w.min_p)
+        atomicAdd(&s.chunk[(int)~(uint32_t)place / a.chunk], (unsigned long long)e);
     });
-  auto stays = [&](float x, int v, double& e) {
-    const uint32_t key = sm_key(x);
-    if (key == 0 || (sm_bin(w, x) >= st.sure && sm_place(key, v) < last)) return false;
-    e = sm_weight(w, x);
-    return e >= (double)w.min_p;
+    __syncthreads();
   };
-  // the tile that the number falls into
-  __syncthreads();
-  uint64_t total;
-  const uint64_t mine = tid < a.tiles ? sTile[tid] : 0;
-  const uint64_t before = sm_before(mine, sW, total);
+  if (st.listed > 0)
+    finish([&](int b0, int b1, auto f) { sm_listed(w, st.listed, b0, b1, s, f); });
+  else if (st.listed < 0)
+    finish([&](int b0, int b1, auto f) { sm_of_row<kSmThreads>(w, row, a.V, b0, b1, f); });
+  const SampleGate g = sm_gate(st);
+  auto stays = [&](float x, int v, double& e) { return sm_stays(w, g, last, x, v, e); };
+  uint64_t total = 0;
+  for (int i = 0; i < a.S; ++i) total += s.chunk[i];
   if (c == 0 && a.u) {
-    const float u = fmaxf(a.u[r], 0.f);
-    // a number of 1 is exceeded by no running sum: the last token that stays
-    const double want = u < 1.f ? (double)u * (double)total : (double)INFINITY;
-    if (tid == 0) { sAt[0] = INT32_MAX; sAt[1] = 0; }
-    __syncthreads();
-    if (mine > 0) {
-      if ((double)(before + mine) > want) atomicMin(&sAt[0], tid);
-      atomicMax(&sAt[1], tid);
-    }
-    __syncthreads();
-    const int t = sAt[0] == INT32_MAX ? sAt[1] : sAt[0];
-    if (tid == t) sEnds[0] = before;
-    __syncthreads();
-    if (tid == 0) { sAt[0] = INT32_MAX; sAt[1] = 0; }
-    const int v = t * kSmTile + 4 * tid;
-    float x[4];
-    if (v < a.V) {
-      sm_load(row, v, a.V, x);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = -INFINITY;
-    }
-    uint64_t e[4], sum = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      double f;
-      e[j] = stays(x[j], v + j, f) ? sm_whole(w, f) : 0;
-      sum += e[j];
-    }
-    uint64_t tile;
-    uint64_t run = sEnds[0] + sm_before(sum, sW, tile);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      run += e[j];
-      if (e[j] > 0) {
-        if ((double)run > want) atomicMin(&sAt[0], v + j);
-        atomicMax(&sAt[1], v + j);
+    const double want = sm_want(a.u[r], total);
+    int at = -1, any = 0;
+    uint64_t run = 0, ahead = 0, any_ahead = 0;
+    for (int i = 0; i < a.S; ++i) {
+      const uint64_t e = s.chunk[i];
+      if (e > 0) {
+        any = i;
+        any_ahead = run;
+        if (at < 0 && (double)(run + e) > want) {
+          at = i;
+          ahead = run;
+        }
       }
+      run += e;
     }
-    __syncthreads();
-    if (tid == 0) a.token[r] = sAt[0] == INT32_MAX ? sAt[1] : sAt[0];
-  }
-  if (!probs) return;
-  const double inv = w.scale / (double)total;
-  for (int v = v0 + 4 * tid; v < v1; v += kSmTile) {
-    float x[4];
-    sm_load(row, v, v1, x);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      double e;
-      const bool is = stays(x[j], v + j, e) && sm_whole(w, e) > 0;
-      if (v + j < v1) sm_out(is ? (float)(e * inv) : 0.f, probs[v + j]);
+    if (at < 0) {
+      at = any;
+      ahead = any_ahead;
     }
+    const int d0 = at * a.chunk, d1 = min(a.V, d0 + a.chunk);
+    const int token = sm_draw<kSmThreads>(w, row, want, ahead, d0, d1, s, stays);
+    if (tid == 0) a.token[r] = token;
   }
+  if (a.probs) sm_probs<kSmThreads>(a, w, row, r, v0, v1, total, stays);
 }
 
-// Chunks of a row: work-groups for two a CU in all, a tile each at least.
+// The same, a work-group a row.  A short row stays in LDS (HELD): one CU takes 5 us to read 128 KB, from the L2
+// too, and four of the five steps read the row.
+template <typename T, bool HELD>
+__global__ __launch_bounds__(kSmWide) void sample_row_kernel(SampleArgs a) {
+  constexpr int NT = kSmWide, E = SmVec<T>::kN, VECS = HELD ? kSmShort / E : 1;
+  __shared__ SampleShared s;
+  __shared__ uint4 sRow[VECS];
+  const int64_t r = blockIdx.x;
+  const int tid = threadIdx.x;
+  const SmSrc<T, HELD> row = {(const T*)a.x + r * a.x_st, sRow};
+  if constexpr (HELD) {
+    SmVec<T> x[VECS / NT];
+#pragma unroll
+    for (int n = 0; n < VECS / NT; ++n) x[n].load(row.row, E * (n * NT + tid), a.V);
+#pragma unroll
+    for (int n = 0; n < VECS / NT; ++n) sRow[n * NT + tid] = __builtin_bit_cast(uint4, x[n].b);
+  }
+  if (tid < kSmBins) { s.cnt[tid] = 0; s.mass[tid] = 0; }
+  if (tid == 0) { s.listed = 0; s.chunk[0] = 0; }
+  uint64_t best;
+  float top = -INFINITY, low = INFINITY;
+  int id = 0;
+  sm_tokens<NT>(row, 0, a.V, [&](float x, int v) { sm_see(x, v, top, id, low); });
+  sm_ends<NT>(top, id, low, best, s.sW, s.sL);
+  const SampleRow w = sm_row(a, r, best, low);
+  if (!w.any || w.greedy) {
+    sm_one<NT>(a, w, r, 0, 0, a.V);
+    return;
+  }
+  uint64_t sum = 0;
+  if (w.filter)
+    sm_tokens<NT>(row, 0, a.V, [&](float x, int) { sm_count(w, x, s.cnt, s.mass); });
+  else
+    sm_tokens<NT>(row, 0, a.V, [&](float x, int) { sum += sm_whole(w, sm_weight(w, x)); });
+  __syncthreads();
+  const uint64_t mass = tid < kSmBins ? s.mass[tid] : 0;
+  sm_select<NT>(w, s);
+  const SampleState st = s.st;
+  const SampleGate g = sm_gate(st);
+  sm_add(!w.filter ? sum : tid < st.sure ? mass : 0, &s.chunk[0]);
+  uint64_t last = 0;
+  auto finish = [&](auto tokens) {
+    last = sm_borders(w, st, tokens, s);
+    tokens(st.sure, st.end, [&](uint64_t place, uint64_t e) {
+      if (place >= last && sm_weight(w, sm_logit((uint32_t)(place >> 32))) >= (double)w.min_p)
+        atomicAdd(&s.chunk[0], (unsigned long long)e);
+    });
+  };
+  if (st.listed > 0) {
+    sm_tokens<NT>(row, 0, a.V, [&](float x, int v) { sm_take(w, g, x, v, s.list, &s.listed); });
+    __syncthreads();
+    finish([&](int b0, int b1, auto f) { sm_listed(w, st.listed, b0, b1, s, f); });
+  } else if (st.listed < 0) {
+    finish([&](int b0, int b1, auto f) { sm_of_row<NT>(w, row, a.V, b0, b1, f); });
+  }
+  __syncthreads();
+  const uint64_t total = s.chunk[0];
+  auto stays = [&](float l, int v, double& e) { return sm_stays(w, g, last, l, v, e); };
+  if (a.u) {
+    const int token = sm_draw<NT>(w, row, sm_want(a.u[r], total), 0, 0, a.V, s, stays);
+    if (tid == 0) a.token[r] = token;
+  }
+  if (a.probs) sm_probs<NT>(a, w, row, r, 0, a.V, total, stays);
+}
+
+// Rows of up to kSmShort tokens, and batches of kSmMany rows and more, take a work-group a row.
+static bool sample_whole(int64_t R, int V) { return V <= kSmShort || R >= kSmMany; }
+
+// Chunks of a row: work-groups for four a CU in all, a tile each at least.
 struct SampleLayout {
-  int S, chunk, tiles;
-  int64_t best, low, cnt, mass, state, n_list, list, tile, total;
+  int S, chunk;
+  int64_t best, low, cnt, mass, state, n_list, list, sure, total;
 };
-static SampleLayout sample_layout(int64_t R, int V) {
-  SampleLayout L;
-  const int64_t rows = std::max<int64_t>(1, std::min<int64_t>(R, kSmRows));
-  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(kSmMaxChunks, 512 / rows));
-  L.chunk = (int)(((V + want - 1) / want + kSmTile - 1) / kSmTile * kSmTile);
+static SampleLayout sample_layout(int64_t R, int V, int tile) {
+  SampleLayout L = {};
+  if (R == 0 || sample_whole(R, V)) return L;
+  const int64_t want = std::min<int64_t>(kSmMaxChunks, 1024 / R);
+  static_assert(kSmMaxV / (1024 / kSmMany) <= kSmTiles * kSmTile<float, kSmThreads> && kSmTiles <= kSmThreads,
+                "a chunk's tiles, a thread each");
+  L.chunk = (int)(((V + want - 1) / want + tile - 1) / tile * tile);
   L.S = (V + L.chunk - 1) / L.chunk;
-  L.tiles = (V + kSmTile - 1) / kSmTile;
   auto align = [](int64_t x) { return (x + 255) / 256 * 256; };
   int64_t o = 0;
-  L.best = o; o = align(o + rows * L.S * 8);
-  L.low = o; o = align(o + rows * L.S * 4);
-  L.cnt = o; o = align(o + rows * L.S * kSmBins * 4);
-  L.mass = o; o = align(o + rows * L.S * kSmBins * 8);
-  L.state = o; o = align(o + rows * (int64_t)sizeof(SampleState));
-  L.n_list = o; o = align(o + rows * 4);
-  L.list = o; o = align(o + rows * kSmList * 8);
-  L.tile = o; o = align(o + rows * L.tiles * 8);
+  L.best = o; o = align(o + R * L.S * 8);
+  L.low = o; o = align(o + R * L.S * 4);
+  L.cnt = o; o = align(o + R * L.S * kSmBins * 4);
+  L.mass = o; o = align(o + R * L.S * kSmBins * 8);
+  L.state = o; o = align(o + R * (int64_t)sizeof(SampleState));
+  L.n_list = o; o = align(o + R * 4);
+  L.list = o; o = align(o + R * kSmList * 8);
+  L.sure = o; o = align(o + R * L.S * 8);
   L.total = o;
   return L;
 }
 
 template <typename T>
-static void sample_launch(const SampleArgs& a, int rows, int p_dtype, bool filter, hipStream_t st) {
-  const dim3 grid(a.S, rows), block(kSmThreads);
+static void sample_launch(const SampleArgs& a, int64_t R, hipStream_t st) {
+  const dim3 block(kSmThreads);
+  if (sample_whole(R, a.V)) {
+    const dim3 grid((unsigned)R), wide(kSmWide);
+    if (a.V <= kSmShort) hipLaunchKernelGGL((sample_row_kernel<T, true>), grid, wide, 0, st, a);
+    else hipLaunchKernelGGL((sample_row_kernel<T, false>), grid, wide, 0, st, a);
+    return;
+  }
+  const dim3 grid(a.S, (unsigned)R);
   hipLaunchKernelGGL(sample_max_kernel<T>, grid, block, 0, st, a);
-  if (filter) hipLaunchKernelGGL(sample_bins_kernel<T>, grid, block, 0, st, a);
+  hipLaunchKernelGGL(sample_bins_kernel<T>, grid, block, 0, st, a);
+  hipLaunchKernelGGL(sample_select_kernel, dim3((unsigned)R), dim3(kSmBins), 0, st, a);
   hipLaunchKernelGGL(sample_pick_kernel<T>, grid, block, 0, st, a);
-  const dim3 draw(a.probs ? a.S : 1, rows);
-  if (p_dtype == 1) hipLaunchKernelGGL((sample_draw_kernel<T, bf16>), draw, block, 0, st, a);
-  else if (p_dtype == 2) hipLaunchKernelGGL((sample_draw_kernel<T, __half>), draw, block, 0, st, a);
-  else hipLaunchKernelGGL((sample_draw_kernel<T, float>), draw, block, 0, st, a);
+  hipLaunchKernelGGL(sample_draw_kernel<T>, dim3(a.probs ? a.S : 1, (unsigned)R), block, 0, st, a);
 }
 
 }  // namespace dash
@@ -633,7 +991,7 @@ extern "C" int dash_sample_workspace_size(int64_t R, int V, int64_t* bytes) {
   using namespace dash;
   if (!bytes || R < 0 || V <= 0) return kErrInvalid;
   if (V > kSmMaxV) return kErrUnsupported;
-  *bytes = sample_layout(R, V).total;
+  *bytes = std::max(sample_layout(R, V, kSmTile<float, kSmThreads>).total, sample_layout(R, V, kSmTile<bf16, kSmThreads>).total);
   return kOk;
 }
 
@@ -646,37 +1004,28 @@ extern "C" int dash_sample(const void* logits, int64_t row_stride, int dtype, co
   if (R < 0 || V <= 0 || dtype < 0 || dtype > 2 || probs_dtype < 0 || probs_dtype > 2) return kErrInvalid;
   if (R == 0) return kOk;
   if (!logits || (!uniforms != !tokens) || (!tokens && !probs)) return kErrInvalid;
-  if (V > kSmMaxV) return kErrUnsupported;
-  const SampleLayout L = sample_layout(R, V);
-  if (!workspace || workspace_bytes < L.total || (uintptr_t)workspace % 256 != 0) return kErrWorkspace;
+  if (V > kSmMaxV || !fits_grid(R, kSmWide)) return kErrUnsupported;
+  const SampleLayout L = sample_layout(R, V, dtype == 0 ? kSmTile<float, kSmThreads> : kSmTile<bf16, kSmThreads>);
+  if (L.total > 0 && (!workspace || workspace_bytes < L.total || (uintptr_t)workspace % 256 != 0))
+    return kErrWorkspace;
   char* ws = (char*)workspace;
   hipStream_t st = (hipStream_t)stream;
-  const int size = dtype == 0 ? 4 : 2, p_size = probs_dtype == 0 ? 4 : 2;
-  for (int64_t r0 = 0; r0 < R; r0 += kSmRows) {
-    const int rows = (int)std::min<int64_t>(R - r0, kSmRows);
-    SampleArgs a = {};
-    a.x = (const char*)logits + r0 * row_stride * size; a.x_st = row_stride;
-    a.u = uniforms ? uniforms + r0 : nullptr;
-    a.t = temperature ? temperature + r0 : nullptr; a.t0 = temperature0;
-    a.k = top_k ? top_k + r0 : nullptr; a.k0 = top_k0;
-    a.p = top_p ? top_p + r0 : nullptr; a.p0 = top_p0;
-    a.m = min_p ? min_p + r0 : nullptr; a.m0 = min_p0;
-    a.V = V; a.S = L.S; a.chunk = L.chunk; a.tiles = L.tiles;
-    int log = 0;
-    while ((1 << log) < V) ++log;
-    a.bits = std::min(51, 62 - log);
-    a.token = tokens ? tokens + r0 : nullptr;
-    a.probs = probs ? (char*)probs + r0 * probs_stride * p_size : nullptr; a.p_st = probs_stride;
-    a.best = (uint64_t*)(ws + L.best); a.low = (uint32_t*)(ws + L.low);
-    a.cnt = (uint32_t*)(ws + L.cnt); a.mass = (uint64_t*)(ws + L.mass);
-    a.state = (SampleState*)(ws + L.state); a.n_list = (int32_t*)(ws + L.n_list);
-    a.list = (uint64_t*)(ws + L.list); a.tile = (uint64_t*)(ws + L.tile);
-    const bool filter = top_k || top_p || top_k0 > 0 || top_p0 < 1.f;
-    if (dtype == 0) sample_launch<float>(a, rows, probs_dtype, filter, st);
-    else if (dtype == 1) sample_launch<bf16>(a, rows, probs_dtype, filter, st);
-    else sample_launch<__half>(a, rows, probs_dtype, filter, st);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return (int)e;
-  }
-  return kOk;
+  SampleArgs a = {};
+  a.x = logits; a.x_st = row_stride; a.u = uniforms;
+  a.t = temperature; a.t0 = temperature0; a.k = top_k; a.k0 = top_k0;
+  a.p = top_p; a.p0 = top_p0; a.m = min_p; a.m0 = min_p0;
+  a.V = V; a.S = L.S; a.chunk = L.chunk;
+  int log = 0;
+  while ((1 << log) < V) ++log;
+  a.bits = std::min(51, 62 - log);
+  a.token = tokens; a.probs = probs; a.p_type = probs_dtype; a.p_st = probs_stride;
+  a.best = (uint64_t*)(ws + L.best); a.low = (float*)(ws + L.low);
+  a.cnt = (uint32_t*)(ws + L.cnt); a.mass = (uint64_t*)(ws + L.mass);
+  a.state = (SampleState*)(ws + L.state); a.n_list = (int32_t*)(ws + L.n_list);
+  a.list = (uint64_t*)(ws + L.list); a.sure = (uint64_t*)(ws + L.sure);
+  if (dtype == 0) sample_launch<float>(a, R, st);
+  else if (dtype == 1) sample_launch<bf16>(a, R, st);
+  else sample_launch<__half>(a, R, st);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? kOk : (int)e;
 }
