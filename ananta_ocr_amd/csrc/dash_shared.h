@@ -8,10 +8,11 @@
 // and rows of a sequence with the keys [prefix, ctx + n).  A row's result is the sum of two segments'.
 //
 // The lengths lie on the device, and a launch's grid cannot depend on them: the plan kernel adds up the
-// segments' work in units of 64 keys of one key head and one tile of rows, and every one of the W
-// work-groups of the attention takes the same number of units, one after another, over as many segments
-// as that reaches.  Each run of units within a (segment, key head, row tile) leaves an unnormalised
-// fp32 partial per row, and the merge kernel adds a row's partials up.
+// segments' work in units of 64 keys and one tile of rows, the same for every key head, and each of the W
+// work-groups of a head takes the same number of units, one after another, over as many segments as that
+// reaches.  Each run of units within a (segment, row tile) leaves an unnormalised fp32 partial per row, and
+// the merge kernel adds a row's partials up.  Neighbouring work-groups take the heads of the same keys, whose
+// rows lie side by side in memory.
 #pragma once
 
 namespace dash {
@@ -23,7 +24,7 @@ struct SharedSeg {
   int32_t r0, rows;                       // first packed row; rows times query heads of a key head
   int32_t k0, k1;                         // keys
   int32_t table_row, group;               // group: of a sequence's segment, -1 none
-  int32_t base, tiles;                    // partial rows of the segments before; row tiles
+  int32_t base, tiles;                    // partial rows of a head of the segments before; row tiles
 };
 
 struct SharedArgs {
@@ -35,8 +36,9 @@ struct SharedArgs {
   const int32_t* cu_groups; const int32_t* prefix;
   void* out; int out_bf16; int64_t o_st, o_sh;
   float* lse; int64_t lse_st, lse_sh;
-  int B, G, H, Hkv, S, W, tile_rows;
-  int64_t T;
+  int B, G, H, Hkv, S, tile_rows;
+  int W;                                  // work-groups of a key head
+  int64_t T, parts;                       // partial rows of a key head
   float scale_log2e;
   // workspace
   int64_t* head;                          // units in all, units of a work-group
@@ -136,9 +138,9 @@ __global__ __launch_bounds__(kShThreads) void shared_plan_kernel(SharedArgs a) {
     if ((group ? before : own) + g.rows > room) g.rows = 0;
     rows_before += total;
     own_before += own_total;
-    g.base = (int)(min(group ? before : room + own, 2 * room) * a.Hkv);
+    g.base = (int)min(group ? before : room + own, 2 * room);
     g.tiles = (g.rows + a.tile_rows - 1) / a.tile_rows;
-    const int64_t units = (int64_t)g.tiles * a.Hkv * ((max(g.k1 - g.k0, 0) + 63) / 64);
+    const int64_t units = (int64_t)g.tiles * ((max(g.k1 - g.k0, 0) + 63) / 64);
     before = sh_before(units, sW, total);
     if (s < ns) {
       a.starts[s] = units_before + before;
@@ -192,7 +194,8 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void shared_attn_kernel(SharedArgs
   const int hl = lane >> 5, col = lane & 31;
   const int Gq = a.H / a.Hkv;
   const int64_t per = a.head[1];
-  int64_t u = blockIdx.x * per;
+  const int hk = blockIdx.x % a.Hkv, turn = blockIdx.x / a.Hkv;
+  int64_t u = turn * per;
   const int64_t u_end = min(u + per, a.head[0]);
   const uint32_t kl0 = k_lane_off(col, hl), vl0 = v_lane_off(lane);
   const float csc = a.scale_log2e;
@@ -201,11 +204,11 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void shared_attn_kernel(SharedArgs
     const int s = sh_find(a, u);
     const SharedSeg g = a.seg[s];
     const int items = (g.k1 - g.k0 + 63) / 64;
-    const int64_t rel = u - a.starts[s], stream = rel / items;
-    const int i_first = (int)(rel - stream * items);
+    const int64_t rel = u - a.starts[s];
+    const int tile = (int)(rel / items), i_first = (int)(rel - (int64_t)tile * items);
     const int i_last = (int)min((int64_t)items, i_first + (u_end - u));
     u += i_last - i_first;
-    const int hk = (int)(stream / g.tiles), rb = (int)(stream - (int64_t)hk * g.tiles) * TR;
+    const int rb = tile * TR;
 
     // this lane's row
     const int rr = min(rb + rt * 32 + col, g.rows - 1);
@@ -466,7 +469,7 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void shared_attn_kernel(SharedArgs
       }
     }
     if (kg == 0 && rvalid) {
-      const int64_t at = (int64_t)g.base + (int64_t)hk * g.rows + rr + (int64_t)blockIdx.x * TR;
+      const int64_t at = hk * a.parts + g.base + rr + (int64_t)turn * TR;
       float* po = a.part_o + at * D + 4 * hl;
 #pragma unroll
       for (int dt = 0; dt < D / 32; ++dt)
@@ -501,10 +504,10 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(SharedArgs a) {
       const int items = (max(g.k1 - g.k0, 0) + 63) / 64;
       const int64_t rr = (row - g.r0) * Gq + h % Gq;
       if (items > 0 && rr >= 0 && rr < g.rows) {
-        const int64_t u0 = a.starts[s] + ((int64_t)hk * g.tiles + rr / a.tile_rows) * items;
+        const int64_t u0 = a.starts[s] + rr / a.tile_rows * items;
         first[x] = u0 / per;
         n[x] = (int)((u0 + items - 1) / per - first[x]) + 1;
-        at[x] = g.base + (int64_t)hk * g.rows + rr + first[x] * a.tile_rows;
+        at[x] = hk * a.parts + g.base + rr + first[x] * a.tile_rows;
       }
       if (g.group < 0) break;
       s = g.group;
@@ -564,13 +567,14 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(SharedArgs a) {
 
 // Row tiles of a work-group by the rows that share a key head (a group's on average), and its work-groups:
 // four a CU of the one-stage kernel, two of the others.
-struct SharedPlan { int rt, W; int64_t head, starts, seg, rows, ml, o, total; };
+struct SharedPlan { int rt, W; int64_t parts, head, starts, seg, rows, ml, o, total; };
 inline SharedPlan shared_plan(int B, int G, int H, int Hkv, int64_t T) {
   SharedPlan p;
   const int64_t rows = T * (H / Hkv) / std::max(1, G > 0 ? G : B);
   p.rt = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
-  p.W = p.rt == 1 ? 1024 : 512;
-  const int64_t parts = 2 * T * H + (int64_t)p.W * 32 * p.rt;
+  p.W = std::max(1, (p.rt == 1 ? 1024 : 512) / Hkv);
+  p.parts = 2 * T * (H / Hkv) + (int64_t)p.W * 32 * p.rt;
+  const int64_t parts = p.parts * Hkv;
   auto align = [](int64_t x) { return (x + 255) / 256 * 256; };
   int64_t o = 0;
   p.head = o; o += 256;
@@ -634,7 +638,7 @@ extern "C" int dash_attn_shared(const void* q, int64_t q_st, int64_t q_sh, const
   a.lse = lse; a.lse_st = lse_st; a.lse_sh = lse_sh;
   a.B = B; a.G = B > 0 ? G : 0; a.H = H; a.Hkv = Hkv; a.T = T;
   a.S = num_pages > 0 ? P * page_size : 0;
-  a.W = p.W; a.tile_rows = 32 * p.rt; a.scale_log2e = scale * 1.4426950408889634f;
+  a.W = p.W; a.parts = p.parts; a.tile_rows = 32 * p.rt; a.scale_log2e = scale * 1.4426950408889634f;
   a.head = (int64_t*)(w + p.head); a.starts = (int64_t*)(w + p.starts);
   a.seg = (SharedSeg*)(w + p.seg); a.row_seq = (int32_t*)(w + p.rows); a.row_pos = a.row_seq + T;
   a.part_ml = (float2*)(w + p.ml); a.part_o = (float*)(w + p.o);
@@ -642,7 +646,7 @@ extern "C" int dash_attn_shared(const void* q, int64_t q_st, int64_t q_sh, const
   hipLaunchKernelGGL(shared_plan_kernel, dim3((unsigned)(1 + (T + kShThreads - 1) / kShThreads)),
                      dim3(kShThreads), 0, st, a);
   if (a.S > 0) {
-    const dim3 grid(p.W);
+    const dim3 grid((unsigned)(p.W * Hkv));
     if (p.rt == 1) hipLaunchKernelGGL((shared_attn_kernel<1, 2>), grid, dim3(128), 0, st, a);
     else if (p.rt == 2) hipLaunchKernelGGL((shared_attn_kernel<2, 2>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((shared_attn_kernel<4, 1>), grid, dim3(256), 0, st, a);
