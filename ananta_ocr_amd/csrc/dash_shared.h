@@ -18,7 +18,7 @@
 namespace dash {
 
 constexpr int kShMaxSeqs = 8192;
-constexpr int kShThreads = 1024;          // of the plan kernel
+constexpr int kShThreads = 256;           // of the plan kernel
 
 struct SharedSeg {
   int32_t r0, rows;                       // first packed row; rows times query heads of a key head
@@ -52,6 +52,10 @@ struct SharedArgs {
 __device__ __forceinline__ int sh_cu(const SharedArgs& a, int b) {
   return (int)min(max((int64_t)a.cu[b], (int64_t)0), a.T);
 }
+
+// a / b rounded down, of numbers of 53 bits at most (a product of the two is none: the quotient of the
+// doubles does not reach the next whole number).
+__device__ __forceinline__ int64_t sh_div(int64_t a, int64_t b) { return (int64_t)((double)a / (double)b); }
 
 // Sum over the work-group's earlier threads, and over all.
 __device__ __forceinline__ int64_t sh_before(int64_t v, int64_t* sW, int64_t& total) {
@@ -101,12 +105,14 @@ __global__ __launch_bounds__(kShThreads) void shared_plan_kernel(SharedArgs a) {
   }
   int64_t units_before = 0, rows_before = 0, own_before = 0;
   const int ns = a.G + a.B;
+  for (int g = tid; g <= a.G && a.G > 0; g += kShThreads) sCu[g] = a.cu_groups[g];
+  __syncthreads();
   for (int s0 = 0; s0 < ns; s0 += kShThreads) {
     const int s = s0 + tid;
     SharedSeg g = {0, 0, 0, 0, 0, -1, 0, 0};
     const bool group = s < a.G;
     if (group) {
-      const int b0 = min(max(a.cu_groups[s], 0), a.B), b1 = min(max(a.cu_groups[s + 1], b0), a.B);
+      const int b0 = min(max(sCu[s], 0), a.B), b1 = min(max(sCu[s + 1], b0), a.B);
       g.r0 = sh_cu(a, b0);
       g.rows = b1 > b0 ? max(sh_cu(a, b1) - g.r0, 0) * Gq : 0;
       g.k1 = min(max(a.prefix[s], 0), a.S);
@@ -119,9 +125,9 @@ __global__ __launch_bounds__(kShThreads) void shared_plan_kernel(SharedArgs a) {
       int lo = -1, hi = a.G;              // the last group that starts at or before b
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (a.cu_groups[mid] <= b) lo = mid; else hi = mid;
+        if (sCu[mid] <= b) lo = mid; else hi = mid;
       }
-      if (lo >= 0 && b < a.cu_groups[lo + 1]) {
+      if (lo >= 0 && b < sCu[lo + 1]) {
         g.group = lo;
         g.k0 = min(max(a.prefix[lo], 0), a.S);
       }
@@ -205,7 +211,7 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void shared_attn_kernel(SharedArgs
     const SharedSeg g = a.seg[s];
     const int items = (g.k1 - g.k0 + 63) / 64;
     const int64_t rel = u - a.starts[s];
-    const int tile = (int)(rel / items), i_first = (int)(rel - (int64_t)tile * items);
+    const int tile = (int)sh_div(rel, items), i_first = (int)(rel - (int64_t)tile * items);
     const int i_last = (int)min((int64_t)items, i_first + (u_end - u));
     u += i_last - i_first;
     const int rb = tile * TR;
@@ -482,18 +488,18 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void shared_attn_kernel(SharedArgs
   }
 }
 
-// One wavefront per (row, head), two dims a lane: the partials of the row's two segments, a lane for the
-// (maximum, sum) of each, 64 at a time, eight partials' loads in flight.
+// One wavefront per (row, head): the partials of the row's two segments, a lane for the (maximum, sum) of each,
+// 64 at a time; half a wavefront reads a partial, four dims a lane, and sixteen are in flight.
 __global__ __launch_bounds__(256) void shared_merge_kernel(SharedArgs a) {
-  constexpr int D = 128;
+  constexpr int D = 128, U = 8;
   const int64_t rh = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
   if (rh >= a.T * a.H) return;
-  const int lane = wave_lane(), Gq = a.H / a.Hkv;
+  const int lane = wave_lane(), hl = lane >> 5, Gq = a.H / a.Hkv;
   const int64_t row = rh / a.H;
   const int h = (int)(rh - row * a.H), hk = h / Gq;
   const int b = a.row_seq[row];
   // runs [first, first + n) of work-groups, and the row's place in the first one's partials
-  int64_t first[2] = {0, 0}, at[2] = {0, 0};
+  int64_t at[2] = {0, 0};
   int n[2] = {0, 0};
   if (b >= 0) {
     const int64_t per = a.head[1];
@@ -505,22 +511,23 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(SharedArgs a) {
       const int64_t rr = (row - g.r0) * Gq + h % Gq;
       if (items > 0 && rr >= 0 && rr < g.rows) {
         const int64_t u0 = a.starts[s] + rr / a.tile_rows * items;
-        first[x] = u0 / per;
-        n[x] = (int)((u0 + items - 1) / per - first[x]) + 1;
-        at[x] = hk * a.parts + g.base + rr + first[x] * a.tile_rows;
+        const int64_t first = sh_div(u0, per);
+        n[x] = (int)(sh_div(u0 + items - 1, per) - first) + 1;
+        at[x] = hk * a.parts + g.base + rr + first * a.tile_rows;
       }
       if (g.group < 0) break;
       s = g.group;
     }
   }
   float M = -INFINITY, L = 0.f;
-  float2 acc = make_float2(0.f, 0.f);
+  floatx4 acc = {0.f, 0.f, 0.f, 0.f};
   bool any = false;
-  for (int e0 = 0; e0 < n[0] + n[1]; e0 += kWave) {
+  const int all = n[0] + n[1];
+  for (int e0 = 0; e0 < all; e0 += kWave) {
     const int e = e0 + lane;
-    const bool in = e < n[0] + n[1];
+    const bool in = e < all;
     const int64_t p = e < n[0] ? at[0] + (int64_t)e * a.tile_rows
-                               : at[1] + (int64_t)(e - n[0]) * a.tile_rows;
+                               : at[1] + (int64_t)(in ? e - n[0] : 0) * a.tile_rows;
     const float2 ml = in ? a.part_ml[p] : make_float2(-INFINITY, 0.f);
     // NaN in a score leaves the maximum and comes in through the sums
     const bool seen = in && !(ml.x == -INFINITY && ml.y == 0.f);
@@ -528,38 +535,39 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(SharedArgs a) {
     const float al = fast_exp2(M - Mu), w = seen ? fast_exp2(ml.x - Mu) : 0.f;
     M = Mn;
     L = L * al + wave_sum(seen ? ml.y * w : 0.f);
-    acc.x *= al;
-    acc.y *= al;
-    uint64_t todo = __ballot(seen);
-    any = any || todo != 0;
-    while (todo) {
-      float2 x[8];
-      float f[8];
+    acc *= al;
+    any = any || __any(seen);
+    const int m = min(kWave, all - e0);
+    for (int i0 = 0; i0 < m; i0 += 2 * U) {
+      floatx4 x[U];
+      float f[U];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int l = todo ? __builtin_ctzll(todo) : 0;
-        f[i] = todo ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), l)) : 0.f;
-        const int64_t pl = __shfl(p, l, kWave);
-        x[i] = make_float2(0.f, 0.f);
-        if (todo) x[i] = *(const float2*)(a.part_o + pl * D + 2 * lane);
-        todo &= todo - 1;
+      for (int i = 0; i < U; ++i) {
+        const int l = i0 + 2 * i + hl;
+        const int64_t pl = __shfl(p, min(l, m - 1), kWave);
+        f[i] = __shfl(w, min(l, m - 1), kWave);
+        if (l >= m) f[i] = 0.f;
+        x[i] = *(const floatx4*)(a.part_o + pl * D + 4 * (lane & 31));
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        acc.x = fmaf(f[i], x[i].x, acc.x);
-        acc.y = fmaf(f[i], x[i].y, acc.y);
-      }
+      for (int i = 0; i < U; ++i)
+        if (f[i] != 0.f) acc += f[i] * x[i];      // (a weight of 0: of a run that saw no key, or none)
     }
   }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) acc[i] = xor32_sum(acc[i]);
   const float inv = any ? 1.f / L : 0.f;
-  const int64_t to = row * a.o_st + (int64_t)h * a.o_sh + 2 * lane;
-  if (a.out_bf16) {
-    bf16x2 r;
-    r[0] = (bf16)(acc.x * inv);
-    r[1] = (bf16)(acc.y * inv);
-    *(bf16x2*)((bf16*)a.out + to) = r;
-  } else {
-    *(float2*)((float*)a.out + to) = make_float2(acc.x * inv, acc.y * inv);
+  acc *= inv;
+  const int64_t to = row * a.o_st + (int64_t)h * a.o_sh + 4 * lane;
+  if (hl == 0) {
+    if (a.out_bf16) {
+      bf16x4 r;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r[i] = (bf16)acc[i];
+      *(bf16x4*)((bf16*)a.out + to) = r;
+    } else {
+      *(floatx4*)((float*)a.out + to) = acc;
+    }
   }
   if (a.lse && lane == 0)
     a.lse[row * a.lse_st + (int64_t)h * a.lse_sh] = any ? (M + log2f(L)) * 0.6931471805599453f : -INFINITY;
