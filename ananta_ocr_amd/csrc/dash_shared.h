@@ -25,6 +25,7 @@ struct SharedSeg {
   int32_t k0, k1;                         // keys
   int32_t table_row, group;               // group: of a sequence's segment, -1 none
   int32_t base, tiles;                    // partial rows of a head of the segments before; row tiles
+  int32_t lo, unused[3];                  // keys below it are seen by every row
 };
 
 struct SharedArgs {
@@ -81,7 +82,7 @@ __device__ __forceinline__ int64_t sh_before(int64_t v, int64_t* sW, int64_t& to
 
 // Work-group 0: the segments and their units.  The others: the sequence and position of every row.
 __global__ __launch_bounds__(kShThreads) void shared_plan_kernel(SharedArgs a) {
-  __shared__ int sCu[kShMaxSeqs + 1];
+  __shared__ int sCu[kShMaxSeqs + 1], sLo[kShMaxSeqs];
   __shared__ int64_t sW[kShThreads / kWave];
   const int tid = threadIdx.x, Gq = a.H / a.Hkv;
   if (blockIdx.x > 0) {
@@ -105,11 +106,14 @@ __global__ __launch_bounds__(kShThreads) void shared_plan_kernel(SharedArgs a) {
   }
   int64_t units_before = 0, rows_before = 0, own_before = 0;
   const int ns = a.G + a.B;
-  for (int g = tid; g <= a.G && a.G > 0; g += kShThreads) sCu[g] = a.cu_groups[g];
+  for (int g = tid; g <= a.G && a.G > 0; g += kShThreads) {
+    sCu[g] = a.cu_groups[g];
+    if (g < a.G) sLo[g] = INT32_MAX;
+  }
   __syncthreads();
   for (int s0 = 0; s0 < ns; s0 += kShThreads) {
     const int s = s0 + tid;
-    SharedSeg g = {0, 0, 0, 0, 0, -1, 0, 0};
+    SharedSeg g = {0, 0, 0, 0, 0, -1, 0, 0, 0, {0, 0, 0}};
     const bool group = s < a.G;
     if (group) {
       const int b0 = min(max(sCu[s], 0), a.B), b1 = min(max(sCu[s + 1], b0), a.B);
@@ -131,7 +135,10 @@ __global__ __launch_bounds__(kShThreads) void shared_plan_kernel(SharedArgs a) {
         g.group = lo;
         g.k0 = min(max(a.prefix[lo], 0), a.S);
       }
-      g.k1 = (int)min((int64_t)min(max(a.ctx[b], 0), a.S) + n, (int64_t)a.S);
+      const int ctx = min(max(a.ctx[b], 0), a.S);
+      g.k1 = (int)min((int64_t)ctx + n, (int64_t)a.S);
+      g.lo = ctx + 1;
+      if (g.group >= 0 && n > 0) atomicMin(&sLo[g.group], g.lo);
       g.table_row = b;
     }
     int64_t total;
@@ -158,6 +165,8 @@ __global__ __launch_bounds__(kShThreads) void shared_plan_kernel(SharedArgs a) {
     a.head[0] = units_before;
     a.head[1] = max((units_before + a.W - 1) / a.W, (int64_t)1);
   }
+  __syncthreads();
+  for (int g = tid; g < a.G; g += kShThreads) a.seg[g].lo = sLo[g];
 }
 
 // The last segment that starts at or before unit u, over the wavefront.
@@ -175,285 +184,298 @@ __device__ __forceinline__ int sh_find(const SharedArgs& a, int64_t u) {
   return __builtin_amdgcn_readfirstlane(lo);
 }
 
+// What a unit is: seg, first row, first key, end of the segment's keys; table row, end of the keys that every row of
+// the tile sees, whether its run starts or ends with it, rows of the segment; first packed row, partial rows before,
+// end of the keys that the first row sees.
+struct SharedUnit { int4 a, b, c; };
+constexpr int kShUnits = 64;              // made at a time, a lane each
+
+// Units u .. of the work-group's u0 .. u_end - 1, by one wavefront: the segments that begin among them are met one
+// after another.
+__device__ __forceinline__ void sh_units(const SharedArgs& a, int64_t u0, int64_t u, int64_t u_end, int tr,
+                                         SharedUnit* sU) {
+  const int lane = wave_lane(), ns = a.G + a.B, Gq = a.H / a.Hkv;
+  const int n = (int)min((int64_t)kShUnits, u_end - u);
+  const int64_t mine = u + min(lane, n - 1);
+  const int s0 = sh_find(a, u);
+  int s = s0;
+  for (int k0 = s0 + 1; k0 < ns; k0 += kWave) {
+    const int64_t next = k0 + lane < ns ? a.starts[k0 + lane] : INT64_MAX;
+    uint64_t some = __ballot(next < u + n);
+    const bool more = some == ~0ull;
+    for (; some; some &= some - 1) {
+      const int l = __builtin_ctzll(some);
+      if (__shfl((long long)next, l, kWave) <= mine) s = k0 + l;
+    }
+    if (!more) break;
+  }
+  const SharedSeg g = a.seg[s];
+  const int items = max((g.k1 - g.k0 + 63) / 64, 1);
+  const int64_t rel = mine - a.starts[s];
+  const int tile = (int)sh_div(rel, items), i = (int)(rel - (int64_t)tile * items), rb = tile * tr;
+  const int j0 = g.k0 + 64 * i;
+  const int seen = min(s >= a.G ? (int)min((int64_t)g.lo + rb / Gq, (int64_t)INT32_MAX) : g.lo, g.k1);
+  const int ends = (i == 0 || mine == u0 ? 1 : 0) | (i == items - 1 || mine == u_end - 1 ? 2 : 0);
+  if (lane < n) {
+    sU[lane].a = make_int4(s, rb, j0, g.k1);
+    sU[lane].b = make_int4(g.table_row, seen, ends, g.rows);
+    sU[lane].c = make_int4(g.r0, g.base, g.lo, 0);
+  }
+}
+
 // RT row tiles of 32 rows are the columns of S^T = K Q^T (v_mfma_f32_32x32x16_bf16); with KG = 2 two
 // wavefronts share a row tile, one half of 64 keys each, and meet at the end of a run.  Weights enter
 // the second product as three bf16 parts (24 bits), so that a bf16 output is the fp32 one rounded once.
+// A work-group's units form one pipeline whatever runs they belong to: the next unit's keys and values are on their
+// way to LDS (two stages) and the pages of the units after looked up while one is multiplied.
 template <int RT, int KG>
 __global__ __launch_bounds__(64 * RT * KG, 2) void shared_attn_kernel(SharedArgs a) {
   constexpr int D = 128, NW = RT * KG, TH = 64 * NW, TR = 32 * RT;
   constexpr int NH = 2 / KG;              // halves of 64 keys that a wavefront takes
   constexpr int PARTS = 3;                // of a weight
-  constexpr int CH = RT == 1 ? 4 : 8;     // units whose rows' offsets are laid out at a time
+  constexpr int CH = RT == 1 ? 2 : 4;     // units whose rows' offsets are laid out at a time
+  constexpr int PER = 64 * CH / TH;       // offsets of a thread
   constexpr int ST = RT == 1 ? 1 : 2;     // stages
   constexpr int NG = 16 / NW;             // groups of four key rows that a wavefront loads
   __shared__ __attribute__((aligned(16))) bf16 sK0[64 * D];
   __shared__ __attribute__((aligned(16))) bf16 sK1[ST == 2 ? 64 * D : 8];
   __shared__ __attribute__((aligned(16))) bf16 sV0[64 * D];
   __shared__ __attribute__((aligned(16))) bf16 sV1[ST == 2 ? 64 * D : 8];
-  __shared__ longlong2 sOff[64 * CH];     // offsets of a key row in K and V
+  __shared__ SharedUnit sU[kShUnits];
+  __shared__ longlong2 sOff[2][64 * CH];  // offsets of a key row in K and V
   __shared__ uint32_t sBad[2][NW];
-  __shared__ int sEnd[NW];
   __shared__ float2 sMl[32 * RT];
   const int tid = threadIdx.x, lane = wave_lane();
   const int wv = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int rt = wv % RT, kg = wv / RT;
   const int hl = lane >> 5, col = lane & 31;
   const int Gq = a.H / a.Hkv;
-  const int64_t per = a.head[1];
   const int hk = blockIdx.x % a.Hkv, turn = blockIdx.x / a.Hkv;
-  int64_t u = turn * per;
-  const int64_t u_end = min(u + per, a.head[0]);
+  const int64_t u0 = turn * a.head[1], u_end = min(u0 + a.head[1], a.head[0]);
+  if (u0 >= u_end) return;
   const uint32_t kl0 = k_lane_off(col, hl), vl0 = v_lane_off(lane);
   const float csc = a.scale_log2e;
+  const bf16* const kb = a.k + hk * a.k_sh;
+  const bf16* const vb = a.v + hk * a.v_sh;
 
-  while (u < u_end) {
-    const int s = sh_find(a, u);
-    const SharedSeg g = a.seg[s];
-    const int items = (g.k1 - g.k0 + 63) / 64;
-    const int64_t rel = u - a.starts[s];
-    const int tile = (int)sh_div(rel, items), i_first = (int)(rel - (int64_t)tile * items);
-    const int i_last = (int)min((int64_t)items, i_first + (u_end - u));
-    u += i_last - i_first;
-    const int rb = tile * TR;
+  // the run at hand
+  int rr = 0, end = 0, e_min = 0;         // this lane's row; keys below `end` are seen, below e_min by the wavefront's
+  bool rvalid = false;
+  bf16x8 qop[D / 16];
+  floatx16 acc_o[D / 32];
+  float m_run = -INFINITY, l_run = 0.f;
 
-    // this lane's row
-    const int rr = min(rb + rt * 32 + col, g.rows - 1);
-    const bool rvalid = rb + rt * 32 + col < g.rows;
-    const int64_t row = g.r0 + rr / Gq;
+  auto begin = [&](int x) __attribute__((always_inline)) {
+    const int4 ua = sU[x].a, ub = sU[x].b, uc = sU[x].c;
+    const int rows = ub.w, r = ua.y + rt * 32 + col;
+    rvalid = r < rows;
+    rr = min(r, rows - 1);
+    const int64_t row = uc.x + rr / Gq;
     const int h = hk * Gq + rr % Gq;
-    const int end = min(a.row_pos[row] + 1, g.k1);         // the keys below it are seen
-    int e_min = rvalid ? end : INT32_MAX;
+    end = ua.x >= a.G ? (int)min((int64_t)uc.z + rr / Gq, (int64_t)INT32_MAX) : a.row_pos[row] + 1;
+    const bf16* qb = a.q + row * a.q_st + (int64_t)h * a.q_sh;
 #pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) e_min = min(e_min, __shfl_xor(e_min, m, kWave));
-    e_min = __builtin_amdgcn_readfirstlane(e_min);
-    __syncthreads();                      // every wavefront left the run before
-    if (lane == 0) sEnd[wv] = e_min;
-    bf16x8 qop[D / 16];
-    {
-      const bf16* qb = a.q + row * a.q_st + (int64_t)h * a.q_sh;
+    for (int kk = 0; kk < D / 16; ++kk) qop[kk] = *(const bf16x8*)(qb + kk * 16 + hl * 8);
+    end = min(end, ua.w);
+    int e = rvalid ? end : INT32_MAX;
 #pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) qop[kk] = *(const bf16x8*)(qb + kk * 16 + hl * 8);
-    }
-
-    auto lay_out = [&](int c0, int c1) {
-      for (int x = tid; x < 64 * (c1 - c0); x += TH) {
-        const int j = min(g.k0 + 64 * c0 + x, g.k1 - 1);
-        const int i = j / a.page;
-        const int p = min(max(a.table[(int64_t)g.table_row * a.table_stride + i], 0), a.num_pages - 1);
-        const int jp = j - i * a.page;
-        sOff[x] = make_longlong2((int64_t)p * a.k_sp + (int64_t)jp * a.k_st + (int64_t)hk * a.k_sh,
-                                 (int64_t)p * a.v_sp + (int64_t)jp * a.v_st + (int64_t)hk * a.v_sh);
-      }
-      __syncthreads();
-    };
-    auto fetch = [&](int x, bf16* sKn, bf16* sVn) __attribute__((always_inline)) {
-#pragma unroll
-      for (int n = 0; n < NG; ++n) {
-        const int grp = NW * n + wv, r = 4 * grp + (lane >> 4);
-        const longlong2 o = sOff[64 * x + r];
-        __builtin_amdgcn_global_load_lds((const void*)(a.k + o.x + k_slot(r, lane & 15) * 8),
-            (__attribute__((address_space(3))) void*)(sKn + grp * 4 * D), 16, 0, 0);
-        __builtin_amdgcn_global_load_lds((const void*)(a.v + o.y + v_slot(r, lane & 15) * 8),
-            (__attribute__((address_space(3))) void*)(sVn + grp * 4 * D), 16, 0, 0);
-      }
-    };
-
-    floatx16 acc_o[D / 32];
-    float m_run = -INFINITY, l_run = 0.f;
+    for (int m = 32; m >= 1; m >>= 1) e = min(e, __shfl_xor(e, m, kWave));
+    e_min = __builtin_amdgcn_readfirstlane(e);
+    m_run = -INFINITY;
+    l_run = 0.f;
 #pragma unroll
     for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) acc_o[dt][r] = 0.f;
-    int e_all = INT32_MAX;                // keys below it are seen by every row of the tile
-
-    // V values that are not finite would reach, through weights of 0, rows that do not see their keys.
-    // Where some row does not see every key, each wavefront clears them in the rows it loaded, and notes
-    // their groups: item() adds them to the rows that see them.
-    auto clear = [&](int i, bf16* sVn, uint32_t* bad_of) __attribute__((always_inline)) {
-      uint32_t bad = 0;
-      if (g.k0 + 64 * (i + 1) > e_all) {
+      for (int n = 0; n < 16; ++n) acc_o[dt][n] = 0.f;
+  };
+  // The table entries of units CH c .. of the batch; their offsets, once they have come.
+  int page_of[PER];
+  auto key_of = [&](int y, int c, int nu) {
+    const int x = min(CH * c + y / 64, nu - 1);
+    return min(sU[x].a.z + (y & 63), sU[x].a.w - 1);
+  };
+  auto look_up = [&](int c, int nu) __attribute__((always_inline)) {
 #pragma unroll
-        for (int n = 0; n < NG; ++n) {
-          uint4* p = (uint4*)(sVn + (NW * n + wv) * 4 * D) + lane;
-          uint4 x = *p;
-          bool is = false;
-          auto fix = [&](uint32_t& w) {
-            if ((w & 0x7f80u) == 0x7f80u) { w &= 0xffff0000u; is = true; }
-            if ((w & 0x7f800000u) == 0x7f800000u) { w &= 0xffffu; is = true; }
-          };
-          fix(x.x); fix(x.y); fix(x.z); fix(x.w);
-          if (is) *p = x;
-          if (__any(is)) bad |= 1u << n;
-        }
-      }
-      if (lane == 0) bad_of[wv] = bad;
-    };
-    // unit i of the run, laid out at x: this wavefront's halves
-    auto item = [&](int i, int x0, const bf16* sKc, const bf16* sVc,
-                    const uint32_t* bad_of) __attribute__((always_inline)) {
-      const int j0 = g.k0 + 64 * i;
-      uint32_t vis[NH];
-      bool any = false;
-      auto below = [](int y) -> uint32_t { return y >= 32 ? ~0u : y <= 0 ? 0u : (1u << y) - 1u; };
+    for (int n = 0; n < PER; ++n) {
+      const int y = n * TH + tid, x = min(CH * c + y / 64, nu - 1);
+      page_of[n] = a.table[(int64_t)sU[x].b.x * a.table_stride + key_of(y, c, nu) / a.page];
+    }
+  };
+  auto put = [&](int c, int nu) __attribute__((always_inline)) {
 #pragma unroll
-      for (int x = 0; x < NH; ++x) {
-        const int j = j0 + 32 * (KG == 2 ? kg : x);
-        vis[x] = rvalid ? (j + 32 <= e_min ? ~0u : below(end - j)) : 0u;
-        any = any || vis[x] != 0u;
-      }
-      if (!__any(any)) return;
-      floatx16 sc[NH];
-      float mloc = -INFINITY;
+    for (int n = 0; n < PER; ++n) {
+      const int y = n * TH + tid, jp = key_of(y, c, nu) % a.page;
+      const int p = min(max(page_of[n], 0), a.num_pages - 1);
+      sOff[c & 1][y] = make_longlong2((int64_t)p * a.k_sp + (int64_t)jp * a.k_st,
+                                      (int64_t)p * a.v_sp + (int64_t)jp * a.v_st);
+    }
+  };
+  auto fetch = [&](int x, bf16* sKn, bf16* sVn) __attribute__((always_inline)) {
 #pragma unroll
-      for (int x = 0; x < NH; ++x) {
-        const int hf = KG == 2 ? kg : x;
-        bf16x8 kf[D / 16];
+    for (int n = 0; n < NG; ++n) {
+      const int grp = NW * n + wv, r = 4 * grp + (lane >> 4);
+      const longlong2 o = sOff[x / CH & 1][64 * (x % CH) + r];
+      __builtin_amdgcn_global_load_lds((const void*)(kb + o.x + k_slot(r, lane & 15) * 8),
+          (__attribute__((address_space(3))) void*)(sKn + grp * 4 * D), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((const void*)(vb + o.y + v_slot(r, lane & 15) * 8),
+          (__attribute__((address_space(3))) void*)(sVn + grp * 4 * D), 16, 0, 0);
+    }
+  };
+  // V values that are not finite would reach, through weights of 0, rows that do not see their keys.
+  // Where some row does not see every key, each wavefront clears them in the rows it loaded, and notes
+  // their groups: item() adds them to the rows that see them.
+  auto clear = [&](int x, bf16* sVn, uint32_t* bad_of) __attribute__((always_inline)) {
+    uint32_t bad = 0;
+    if (__builtin_amdgcn_readfirstlane(sU[x].a.z) + 64 > __builtin_amdgcn_readfirstlane(sU[x].b.y)) {
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) kf[kk] = k_frag_at(sKc, kl0, hf, kk);
-        floatx16 t;                       // two chains: a product need not wait for the one before it
-#pragma unroll
-        for (int r = 0; r < 16; ++r) { sc[x][r] = 0.f; t[r] = 0.f; }
-#pragma unroll
-        for (int kk = 0; kk < D / 16; kk += 2) {
-          sc[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kk], qop[kk], sc[x], 0, 0, 0);
-          t = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kk + 1], qop[kk + 1], t, 0, 0, 0);
-        }
-#pragma unroll
-        for (int r = 0; r < 16; ++r) sc[x][r] += t[r];
-        if (__all(vis[x] == 0u || vis[x] == ~0u)) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) sc[x][r] = vis[x] ? sc[x][r] : -INFINITY;
-        } else {
-          const uint32_t vb = vis[x] >> (4 * hl);
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            sc[x][r] = (vb >> (8 * (r >> 2) + (r & 3))) & 1u ? sc[x][r] : -INFINITY;
-        }
-        float mraw = -INFINITY;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) mraw = fmaxf(mraw, sc[x][r]);
-        mloc = fmaxf(mloc, mraw * csc);
-      }
-      mloc = xor32_max(mloc);
-      // the reference moves only when a row's maximum exceeds it by more than 8
-      const bool up = mloc > m_run + 8.f;
-      if (__any(up)) {
-        const float alpha = up ? fast_exp2(m_run - mloc) : 1.f;
-        l_run *= alpha;
-#pragma unroll
-        for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) acc_o[dt][r] *= alpha;
-        m_run = up ? mloc : m_run;
-      }
-      const float off = m_run == -INFINITY ? 0.f : -m_run;
-#pragma unroll
-      for (int x = 0; x < NH; ++x) {
-        const int hf = KG == 2 ? kg : x;
-        bf16x8 vop[4][2];                 // V in registers before the weights are ready
-#pragma unroll
-        for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-          for (int jj = 0; jj < 2; ++jj) {
-            const char* vp = (const char*)sVc + (32 * hf + 16 * jj) * 256 + (vl0 ^ (uint32_t)(dt << 6));
-            const bf16x4 l4 = __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (lds_short4*)(__attribute__((address_space(3))) void*)vp));
-            const bf16x4 h4 = __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (lds_short4*)(__attribute__((address_space(3))) void*)(vp + 2048)));
-#pragma unroll
-            for (int e = 0; e < 4; ++e) { vop[dt][jj][e] = l4[e]; vop[dt][jj][e + 4] = h4[e]; }
-          }
-        uint32_t part[PARTS][2][4];
-#pragma unroll
-        for (int jj = 0; jj < 2; ++jj) {
-          float p[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) p[e] = fast_exp2(fmaf(sc[x][8 * jj + e], csc, off));
-          l_run += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-#pragma unroll
-            for (int n = 0; n < PARTS; ++n) {
-              bf16x2 y;
-              y[0] = (bf16)p[2 * e];
-              y[1] = (bf16)p[2 * e + 1];
-              const uint32_t w = __builtin_bit_cast(uint32_t, y);
-              part[n][jj][e] = w;
-              p[2 * e] -= __uint_as_float(w << 16);
-              p[2 * e + 1] -= __uint_as_float(w & 0xffff0000u);
-            }
-        }
-#pragma unroll
-        for (int jj = 0; jj < 2; ++jj)
-#pragma unroll
-          for (int n = PARTS - 1; n >= 0; --n) {       // smallest parts first
-            const bf16x8 w = __builtin_bit_cast(bf16x8, *(uint4*)part[n][jj]);
-#pragma unroll
-            for (int dt = 0; dt < 4; ++dt)
-              acc_o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vop[dt][jj], w, acc_o[dt], 0, 0, 0);
-          }
-      }
-      if (j0 + 64 <= e_all) return;
-      for (int w = 0; w < NW; ++w)
-        for (uint32_t todo = bad_of[w]; todo; todo &= todo - 1)
-          for (int q4 = 0; q4 < 4; ++q4) {
-            const int r = 4 * (NW * __builtin_ctz(todo) + w) + q4;
-            if (j0 + r >= g.k1 || (KG == 2 && r / 32 != kg)) continue;   // a repeated row
-            const bool sees = (vis[KG == 2 ? 0 : r / 32] >> (r & 31)) & 1u;
-            const bf16* vp = a.v + sOff[64 * x0 + r].y + 4 * hl;
-#pragma unroll
-            for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-              for (int n = 0; n < 4; ++n) {
-                const bf16x4 y = *(const bf16x4*)(vp + 32 * dt + 8 * n);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const float f = (float)y[e];
-                  if (sees && !(fabsf(f) <= 3.402823466e38f)) acc_o[dt][4 * n + e] += f;
-                }
-              }
-          }
-    };
-
-    for (int c0 = i_first; c0 < i_last; c0 += CH) {
-      const int c1 = min(c0 + CH, i_last);
-      if (c0 > i_first) __syncthreads();  // every wavefront left the units before
-      lay_out(c0, c1);
-      if (c0 == i_first) {
-#pragma unroll
-        for (int w = 0; w < NW; ++w) e_all = min(e_all, sEnd[w]);
-      }
-      if (ST == 1) {
-        for (int i = c0; i < c1; ++i) {
-          if (i > c0) __syncthreads();    // every wavefront left unit i - 1
-          fetch(i - c0, sK0, sV0);
-          __builtin_amdgcn_s_waitcnt(0);
-          clear(i, sV0, sBad[0]);
-          __syncthreads();                // unit i landed
-          item(i, i - c0, sK0, sV0, sBad[0]);
-        }
-        continue;
-      }
-      fetch(0, sK0, sV0);
-      auto step = [&](int i, auto par) __attribute__((always_inline)) {
-        constexpr int P = decltype(par)::value;
-        __builtin_amdgcn_s_waitcnt(0);
-        clear(i, P ? sV1 : sV0, sBad[P]);
-        __syncthreads();                  // unit i landed; every wavefront left unit i - 1
-        if (i + 1 < c1) fetch(i + 1 - c0, P ? sK0 : sK1, P ? sV0 : sV1);
-        item(i, i - c0, P ? sK1 : sK0, P ? sV1 : sV0, sBad[P]);
-      };
-      for (int i = c0; i < c1; i += 2) {
-        step(i, std::integral_constant<int, 0>{});
-        if (i + 1 < c1) step(i + 1, std::integral_constant<int, 1>{});
+      for (int n = 0; n < NG; ++n) {
+        uint4* p = (uint4*)(sVn + (NW * n + wv) * 4 * D) + lane;
+        uint4 y = *p;
+        bool is = false;
+        auto fix = [&](uint32_t& w) {
+          if ((w & 0x7f80u) == 0x7f80u) { w &= 0xffff0000u; is = true; }
+          if ((w & 0x7f800000u) == 0x7f800000u) { w &= 0xffffu; is = true; }
+        };
+        fix(y.x); fix(y.y); fix(y.z); fix(y.w);
+        if (is) *p = y;
+        if (__any(is)) bad |= 1u << n;
       }
     }
-
+    if (lane == 0) bad_of[wv] = bad;
+  };
+  // unit x: this wavefront's halves
+  auto item = [&](int x0, const bf16* sKc, const bf16* sVc,
+                  const uint32_t* bad_of) __attribute__((always_inline)) {
+    const int j0 = __builtin_amdgcn_readfirstlane(sU[x0].a.z);
+    uint32_t vis[NH];
+    bool any = false;
+    auto below = [](int y) -> uint32_t { return y >= 32 ? ~0u : y <= 0 ? 0u : (1u << y) - 1u; };
+#pragma unroll
+    for (int x = 0; x < NH; ++x) {
+      const int j = j0 + 32 * (KG == 2 ? kg : x);
+      vis[x] = rvalid ? (j + 32 <= e_min ? ~0u : below(end - j)) : 0u;
+      any = any || vis[x] != 0u;
+    }
+    if (!__any(any)) return;
+    floatx16 sc[NH];
+    float mloc = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < NH; ++x) {
+      const int hf = KG == 2 ? kg : x;
+      bf16x8 kf[D / 16];
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) kf[kk] = k_frag_at(sKc, kl0, hf, kk);
+      floatx16 t;                       // two chains: a product need not wait for the one before it
+#pragma unroll
+      for (int r = 0; r < 16; ++r) { sc[x][r] = 0.f; t[r] = 0.f; }
+#pragma unroll
+      for (int kk = 0; kk < D / 16; kk += 2) {
+        sc[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kk], qop[kk], sc[x], 0, 0, 0);
+        t = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kk + 1], qop[kk + 1], t, 0, 0, 0);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sc[x][r] += t[r];
+      if (__all(vis[x] == 0u || vis[x] == ~0u)) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sc[x][r] = vis[x] ? sc[x][r] : -INFINITY;
+      } else {
+        const uint32_t vb = vis[x] >> (4 * hl);
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          sc[x][r] = (vb >> (8 * (r >> 2) + (r & 3))) & 1u ? sc[x][r] : -INFINITY;
+      }
+      float mraw = -INFINITY;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mraw = fmaxf(mraw, sc[x][r]);
+      mloc = fmaxf(mloc, mraw * csc);
+    }
+    mloc = xor32_max(mloc);
+    // the reference moves only when a row's maximum exceeds it by more than 8
+    const bool up = mloc > m_run + 8.f;
+    if (__any(up)) {
+      const float alpha = up ? fast_exp2(m_run - mloc) : 1.f;
+      l_run *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc_o[dt][r] *= alpha;
+      m_run = up ? mloc : m_run;
+    }
+    const float off = m_run == -INFINITY ? 0.f : -m_run;
+#pragma unroll
+    for (int x = 0; x < NH; ++x) {
+      const int hf = KG == 2 ? kg : x;
+      bf16x8 vop[4][2];                 // V in registers before the weights are ready
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+        for (int jj = 0; jj < 2; ++jj) {
+          const char* vp = (const char*)sVc + (32 * hf + 16 * jj) * 256 + (vl0 ^ (uint32_t)(dt << 6));
+          const bf16x4 l4 = __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (lds_short4*)(__attribute__((address_space(3))) void*)vp));
+          const bf16x4 h4 = __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (lds_short4*)(__attribute__((address_space(3))) void*)(vp + 2048)));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) { vop[dt][jj][e] = l4[e]; vop[dt][jj][e + 4] = h4[e]; }
+        }
+      uint32_t part[PARTS][2][4];
+#pragma unroll
+      for (int jj = 0; jj < 2; ++jj) {
+        float p[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) p[e] = fast_exp2(fmaf(sc[x][8 * jj + e], csc, off));
+        l_run += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int n = 0; n < PARTS; ++n) {
+            bf16x2 y;
+            y[0] = (bf16)p[2 * e];
+            y[1] = (bf16)p[2 * e + 1];
+            const uint32_t w = __builtin_bit_cast(uint32_t, y);
+            part[n][jj][e] = w;
+            p[2 * e] -= __uint_as_float(w << 16);
+            p[2 * e + 1] -= __uint_as_float(w & 0xffff0000u);
+          }
+      }
+#pragma unroll
+      for (int jj = 0; jj < 2; ++jj)
+#pragma unroll
+        for (int n = PARTS - 1; n >= 0; --n) {       // smallest parts first
+          const bf16x8 w = __builtin_bit_cast(bf16x8, *(uint4*)part[n][jj]);
+#pragma unroll
+          for (int dt = 0; dt < 4; ++dt)
+            acc_o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vop[dt][jj], w, acc_o[dt], 0, 0, 0);
+        }
+    }
+    if (j0 + 64 <= __builtin_amdgcn_readfirstlane(sU[x0].b.y)) return;
+    for (int w = 0; w < NW; ++w)
+      for (uint32_t todo = bad_of[w]; todo; todo &= todo - 1)
+        for (int q4 = 0; q4 < 4; ++q4) {
+          const int r = 4 * (NW * __builtin_ctz(todo) + w) + q4;
+          if (j0 + r >= sU[x0].a.w || (KG == 2 && r / 32 != kg)) continue;   // a repeated row
+          const bool sees = (vis[KG == 2 ? 0 : r / 32] >> (r & 31)) & 1u;
+          const bf16* vp = vb + sOff[x0 / CH & 1][64 * (x0 % CH) + r].y + 4 * hl;
+#pragma unroll
+          for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+              const bf16x4 y = *(const bf16x4*)(vp + 32 * dt + 8 * n);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float f = (float)y[e];
+                if (sees && !(fabsf(f) <= 3.402823466e38f)) acc_o[dt][4 * n + e] += f;
+              }
+            }
+        }
+  };
+  // the end of a run; the stage of its last unit is free once every wavefront has left it
+  auto finish = [&](int x, bf16* sKc, bf16* sVc) __attribute__((always_inline)) {
     float l_tot = xor32_sum(l_run);
     if (KG == 2) {
       // the second half's wavefronts hand their sums to the first's
       __syncthreads();
-      float* so = (float*)(rt ? sK1 : sK0);
+      float* so = (float*)(rt ? sVc : sKc);
       if (kg == 1) {
 #pragma unroll
         for (int dt = 0; dt < D / 32; ++dt)
@@ -475,7 +497,7 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void shared_attn_kernel(SharedArgs
       }
     }
     if (kg == 0 && rvalid) {
-      const int64_t at = hk * a.parts + g.base + rr + (int64_t)turn * TR;
+      const int64_t at = hk * a.parts + sU[x].c.y + rr + (int64_t)turn * TR;
       float* po = a.part_o + at * D + 4 * hl;
 #pragma unroll
       for (int dt = 0; dt < D / 32; ++dt)
@@ -484,6 +506,44 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void shared_attn_kernel(SharedArgs
           *(float4*)(po + dt * 32 + 8 * n) = make_float4(acc_o[dt][4 * n], acc_o[dt][4 * n + 1],
                                                          acc_o[dt][4 * n + 2], acc_o[dt][4 * n + 3]);
       if (hl == 0) a.part_ml[at] = make_float2(m_run, l_tot);
+    }
+  };
+
+  for (int64_t u = u0; u < u_end; u += kShUnits) {
+    const int nu = (int)min((int64_t)kShUnits, u_end - u), chunks = (nu + CH - 1) / CH;
+    __syncthreads();                      // every wavefront left the batch before
+    if (wv == 0) sh_units(a, u0, u, u_end, TR, sU);
+    __syncthreads();
+    look_up(0, nu);
+    put(0, nu);
+    __syncthreads();
+    if (ST == 2) fetch(0, sK0, sV0);
+    auto step = [&](int x, auto par) __attribute__((always_inline)) {
+      constexpr int P = decltype(par)::value;
+      bf16* const sKc = P ? sK1 : sK0;
+      bf16* const sVc = P ? sV1 : sV0;
+      const int ends = __builtin_amdgcn_readfirstlane(sU[x].b.z), c = x / CH;
+      const bool ahead = x % CH == 0 && c + 1 < chunks;
+      if (ST == 1) {
+        __syncthreads();                  // every wavefront left unit x - 1
+        fetch(x, sKc, sVc);
+        if (ahead) look_up(c + 1, nu);
+      }
+      if (ends & 1) begin(x);
+      __builtin_amdgcn_s_waitcnt(0);      // unit x landed, and what was looked up
+      if (ST == 1 ? ahead : x % CH == 1 && c + 1 < chunks) put(c + 1, nu);
+      clear(x, sVc, sBad[P]);
+      __syncthreads();                    // every wavefront's part of it; and they left unit x - 1
+      if (ST == 2) {
+        if (x + 1 < nu) fetch(x + 1, P ? sK0 : sK1, P ? sV0 : sV1);
+        if (ahead) look_up(c + 1, nu);
+      }
+      item(x, sKc, sVc, sBad[P]);
+      if (ends & 2) finish(x, sKc, sVc);
+    };
+    for (int x = 0; x < nu; x += ST) {
+      step(x, std::integral_constant<int, 0>{});
+      if (ST == 2 && x + 1 < nu) step(x + 1, std::integral_constant<int, 1>{});
     }
   }
 }
