@@ -237,6 +237,7 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void shared_attn_kernel(SharedArgs
   constexpr int PER = 64 * CH / TH;       // offsets of a thread
   constexpr int ST = RT == 1 ? 1 : 2;     // stages
   constexpr int NG = 16 / NW;             // groups of four key rows that a wavefront loads
+  constexpr int kAux = RT == 4 ? 0 : 2;
   __shared__ __attribute__((aligned(16))) bf16 sK0[64 * D];
   __shared__ __attribute__((aligned(16))) bf16 sK1[ST == 2 ? 64 * D : 8];
   __shared__ __attribute__((aligned(16))) bf16 sV0[64 * D];
@@ -316,9 +317,9 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void shared_attn_kernel(SharedArgs
       const int grp = NW * n + wv, r = 4 * grp + (lane >> 4);
       const longlong2 o = sOff[x / CH & 1][64 * (x % CH) + r];
       __builtin_amdgcn_global_load_lds((const void*)(kb + o.x + k_slot(r, lane & 15) * 8),
-          (__attribute__((address_space(3))) void*)(sKn + grp * 4 * D), 16, 0, 0);
+          (__attribute__((address_space(3))) void*)(sKn + grp * 4 * D), 16, 0, kAux);
       __builtin_amdgcn_global_load_lds((const void*)(vb + o.y + v_slot(r, lane & 15) * 8),
-          (__attribute__((address_space(3))) void*)(sVn + grp * 4 * D), 16, 0, 0);
+          (__attribute__((address_space(3))) void*)(sVn + grp * 4 * D), 16, 0, kAux);
     }
   };
   // V values that are not finite would reach, through weights of 0, rows that do not see their keys.
