@@ -22,7 +22,7 @@
 namespace dash {
 
 constexpr int kRpThreads = 256;
-constexpr int kRpTokens = 4;        // of a work-group
+constexpr int kRpTokens = 4;        // of a work-group, one where there are few
 constexpr int kRpUnroll = 4;        // units of a thread in flight
 constexpr int kRpMaxPairs = 256;
 
@@ -42,6 +42,7 @@ struct RopeArgs {
   const int64_t* slots; int page; int64_t num_slots;
   int B, S, D, m, start;
   int units;                        // of a head row
+  int per;                          // tokens of a work-group
 };
 
 template <typename T, int E> struct RopeChunk {
@@ -58,14 +59,39 @@ __device__ __forceinline__ void rp_out(float x, float& y) { y = x; }
 __device__ __forceinline__ void rp_out(float x, bf16& y) { y = (bf16)x; }
 __device__ __forceinline__ void rp_out(float x, __half& y) { y = __float2half_rn(x); }
 
+// factor (cos, sin) of pos * f.  In turns, t = pos f / (2 pi) = pos (g + h) with g + h = f / (2 pi) to twice the
+// digits, so that t's own rounding is known and its whole part can go; then the nearest quarter turn, and the
+// series of sine and cosine on [-pi / 4, pi / 4], whose next terms are below 1.2e-10.
+__device__ __forceinline__ float2 rp_turn(double pos, double f, float factor) {
+  constexpr double c0 = 0.15915494309189535, c1 = -9.839338337591243e-18;   // 1 / (2 pi)
+  const double g = f * c0, h = fma(f, c0, -g) + f * c1;
+  const double t = pos * g, e = fma(pos, g, -t) + pos * h;
+  const double r = (t - __builtin_rint(t)) + e;
+  const double q = __builtin_rint(4.0 * r);
+  const double x = fma(q, -0.25, r) * 6.283185307179586, y = x * x;
+  double s = fma(y, -1.0 / 39916800.0, 1.0 / 362880.0);
+  s = fma(s, y, -1.0 / 5040.0);
+  s = fma(s, y, 1.0 / 120.0);
+  s = fma(s, y, -1.0 / 6.0);
+  s = fma(s * y, x, x);
+  double c = fma(y, -1.0 / 3628800.0, 1.0 / 40320.0);
+  c = fma(c, y, -1.0 / 720.0);
+  c = fma(c, y, 1.0 / 24.0);
+  c = fma(c, y, -0.5);
+  c = fma(c, y, 1.0);
+  const int k = (int)q & 3;
+  const double u = k & 1 ? s : c, v = k & 1 ? c : s;
+  return make_float2((float)((k == 1 || k == 2 ? -u : u) * factor), (float)((k & 2 ? -v : v) * factor));
+}
+
 template <typename T, int E, bool PAIRS>
 __global__ __launch_bounds__(kRpThreads) void rope_kernel(RopeArgs a) {
   typedef typename std::remove_reference<decltype(RopeChunk<T, E>::v)>::type V;
   __shared__ float2 sCs[kRpTokens * kRpMaxPairs];
   __shared__ int64_t sSlot[kRpTokens];
   const int tid = threadIdx.x;
-  const int64_t tokens = (int64_t)a.B * a.S, t0 = (int64_t)blockIdx.x * kRpTokens;
-  const int nt = (int)min((int64_t)kRpTokens, tokens - t0);
+  const int64_t tokens = (int64_t)a.B * a.S, t0 = (int64_t)blockIdx.x * a.per;
+  const int nt = (int)min((int64_t)a.per, tokens - t0);
   const int per_token = a.heads * a.units, total = nt * per_token;
   const int nturn = a.m / E;                 // units of a turned row that hold pairs
 
@@ -122,9 +148,7 @@ __global__ __launch_bounds__(kRpThreads) void rope_kernel(RopeArgs a) {
         const int b = a.B == 1 ? 0 : (int)((t0 + t) / a.S);
         const int64_t at = b * a.pos_sb + (t0 + t - (int64_t)b * a.S) * a.pos_st;
         const double pos = a.pos64 ? (double)((const int64_t*)a.pos)[at] : (double)((const int32_t*)a.pos)[at];
-        double s, c;
-        sincos(a.sign * pos * a.inv_freq[j], &s, &c);
-        sCs[t * kRpMaxPairs + j] = make_float2((float)(c * a.factor), (float)(s * a.factor));
+        sCs[t * kRpMaxPairs + j] = rp_turn(a.sign * pos, a.inv_freq[j], a.factor);
       }
       if (a.slots && tid < nt) sSlot[tid] = a.slots[t0 + tid];
       __syncthreads();
@@ -181,7 +205,9 @@ static int rope_launch(RopeArgs& a, bool pairs, hipStream_t st) {
   constexpr int E = 16 / sizeof(T);
   const bool wide = rope_fits(a, sizeof(T), 16);
   a.units = a.D / 2 / (wide ? E : 1);
-  const int64_t groups = ((int64_t)a.B * a.S + kRpTokens - 1) / kRpTokens;
+  const int64_t tokens = (int64_t)a.B * a.S;
+  a.per = tokens < 1024 ? 1 : kRpTokens;
+  const int64_t groups = (tokens + a.per - 1) / a.per;
   if (!fits_grid(groups, kRpThreads) || (int64_t)a.heads * a.units * kRpTokens > INT32_MAX / 2)
     return kErrUnsupported;
   const dim3 grid((unsigned)groups), block(kRpThreads);

@@ -128,7 +128,8 @@ class _RopeFn(torch.autograd.Function):
         interleaved, start, factor, back = ctx.how
         pos, freqs = ctx.saved_tensors
         if dq is not None or dk is not None:
-            dq, dk = _RopeFn.apply(dq, dk, pos, freqs, interleaved, start, factor, not back)
+            turn = _RopeFn.apply if torch.is_grad_enabled() else _turn     # (a graph of the gradients)
+            dq, dk = turn(dq, dk, pos, freqs, interleaved, start, factor, not back)
         return dq, dk, None, None, None, None, None, None
 
 
