@@ -10,9 +10,14 @@
 // whose 32-bit rounding alone is 4e-3.  They are rounded to 32 bits once a (token, pair), in LDS, for all
 // heads; the turn is two products and an addition in 32 bits, rounded once to the row's type.
 //
-// A work-group takes kRpTokens tokens and all their heads.  Its units are two 16-byte chunks: the two that a
-// pair of the halves' layout needs, or two neighbours (single elements where an address, a stride or the part
-// does not fit 16 bytes).  Their loads start before the sines are there.
+// A work-group takes a token, or a few of few heads, and all its heads.  Its units are two 16-byte chunks: the two
+// that a pair of the halves' layout needs, or two neighbours (single elements where an address, a stride or the
+// part does not fit 16 bytes).  Their loads start before the sines are there.
+//
+// Bound by HBM: 8,190 tokens of 10 + 10 + 10 heads of 128 bf16 in 38 us (126 MB read and written, 3.3 TB/s), 20 heads
+// turned as interleaved pairs 21.6 us (84 MB, 3.9 TB/s); with two or four units a thread in flight, or loads and stores
+// past the caches, 40 to 46 and 25 to 33.  Six wavefronts a SIMD: 38 us, five 44, eight (registers to memory) 46.
+// A few tokens 4 us, of latency.
 #include <hip/hip_fp16.h>
 
 #include <type_traits>
@@ -22,8 +27,7 @@
 namespace dash {
 
 constexpr int kRpThreads = 256;
-constexpr int kRpTokens = 4;        // of a work-group, one where there are few
-constexpr int kRpUnroll = 4;        // units of a thread in flight
+constexpr int kRpTokens = 4;        // of a work-group, at most
 constexpr int kRpMaxPairs = 256;
 
 struct RopeRows {                   // rows [B, S, heads, D] in elements; slots: y is a cache of pages
@@ -50,7 +54,8 @@ template <typename T, int E> struct RopeChunk {
   union { V v; T e[E]; };
 };
 template <typename T> struct RopeChunk<T, 1> {
-  union { T v; T e[1]; };
+  typedef typename std::conditional<sizeof(T) == 4, uint32_t, uint16_t>::type V;
+  union { V v; T e[1]; };
 };
 __device__ __forceinline__ float rp_in(float x) { return x; }
 __device__ __forceinline__ float rp_in(bf16 x) { return (float)x; }
@@ -85,7 +90,7 @@ __device__ __forceinline__ float2 rp_turn(double pos, double f, float factor) {
 }
 
 template <typename T, int E, bool PAIRS>
-__global__ __launch_bounds__(kRpThreads) void rope_kernel(RopeArgs a) {
+__global__ __launch_bounds__(kRpThreads, 6) void rope_kernel(RopeArgs a) {
   typedef typename std::remove_reference<decltype(RopeChunk<T, E>::v)>::type V;
   __shared__ float2 sCs[kRpTokens * kRpMaxPairs];
   __shared__ int64_t sSlot[kRpTokens];
@@ -130,18 +135,14 @@ __global__ __launch_bounds__(kRpThreads) void rope_kernel(RopeArgs a) {
     e0 = c * E;
     e1 = d * E;
   };
-  for (int i0 = 0; i0 < total; i0 += kRpThreads * kRpUnroll) {
-    Unit w[kRpUnroll];
-    RopeChunk<T, E> p[kRpUnroll], q[kRpUnroll];
-#pragma unroll
-    for (int k = 0; k < kRpUnroll; ++k) {
-      w[k] = unit_of(i0 + k * kRpThreads + tid);
-      int e0, e1;
-      chunks(w[k], e0, e1);
-      const T* x = (const T*)a.r[w[k].set].x + w[k].x;
-      p[k].v = *(const V*)(x + e0);
-      q[k].v = *(const V*)(x + e1);
-    }
+  for (int i0 = 0; i0 < total; i0 += kRpThreads) {
+    const Unit w = unit_of(i0 + tid);
+    const RopeRows& r = a.r[w.set];
+    int e0, e1;
+    chunks(w, e0, e1);
+    RopeChunk<T, E> p, q;
+    p.v = *(const V*)((const T*)r.x + w.x + e0);
+    q.v = *(const V*)((const T*)r.x + w.x + e1);
     if (i0 == 0) {
       for (int i = tid; i < nt * a.m; i += kRpThreads) {
         const int t = i / a.m, j = i - t * a.m;
@@ -153,36 +154,30 @@ __global__ __launch_bounds__(kRpThreads) void rope_kernel(RopeArgs a) {
       if (a.slots && tid < nt) sSlot[tid] = a.slots[t0 + tid];
       __syncthreads();
     }
+    if (!w.live) continue;
+    if (r.turn && w.u < nturn) {
+      const float2* cs = sCs + w.token * kRpMaxPairs + w.u * E;
 #pragma unroll
-    for (int k = 0; k < kRpUnroll; ++k) {
-      if (!w[k].live) continue;
-      const RopeRows& r = a.r[w[k].set];
-      int e0, e1;
-      chunks(w[k], e0, e1);
-      if (r.turn && w[k].u < nturn) {
-        const float2* cs = sCs + w[k].token * kRpMaxPairs + w[k].u * E;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          // pair e of the unit: element e of each chunk, or elements 2e, 2e + 1 of both in a row
-          T& xe = PAIRS ? (2 * e < E ? p[k].e[(2 * e) % E] : q[k].e[(2 * e) % E]) : p[k].e[e];
-          T& ye = PAIRS ? (2 * e + 1 < E ? p[k].e[(2 * e + 1) % E] : q[k].e[(2 * e + 1) % E]) : q[k].e[e];
-          const float2 z = cs[e];
-          const float x = rp_in(xe), y = rp_in(ye);
-          rp_out(fmaf(x, z.x, -(y * z.y)), xe);
-          rp_out(fmaf(y, z.x, x * z.y), ye);
-        }
+      for (int e = 0; e < E; ++e) {
+        // pair e of the unit: element e of each chunk, or elements 2e, 2e + 1 of both in a row
+        T& xe = PAIRS ? (2 * e < E ? p.e[(2 * e) % E] : q.e[(2 * e) % E]) : p.e[e];
+        T& ye = PAIRS ? (2 * e + 1 < E ? p.e[(2 * e + 1) % E] : q.e[(2 * e + 1) % E]) : q.e[e];
+        const float2 z = cs[e];
+        const float x = rp_in(xe), y = rp_in(ye);
+        rp_out(fmaf(x, z.x, -(y * z.y)), xe);
+        rp_out(fmaf(y, z.x, x * z.y), ye);
       }
-      int64_t y = w[k].y;
-      if (r.slots) {
-        const int64_t s = sSlot[w[k].token];
-        if (s < 0 || s >= a.num_slots) continue;
-        const int64_t pg = s / a.page;
-        y += pg * r.y_sb + (s - pg * a.page) * r.y_st;
-      }
-      T* out = (T*)r.y + y;
-      *(V*)(out + e0) = p[k].v;
-      *(V*)(out + e1) = q[k].v;
     }
+    int64_t y = w.y;
+    if (r.slots) {
+      const int64_t s = sSlot[w.token];
+      if (s < 0 || s >= a.num_slots) continue;
+      const int64_t pg = s / a.page;
+      y += pg * r.y_sb + (s - pg * a.page) * r.y_st;
+    }
+    T* out = (T*)r.y + y;
+    *(V*)(out + e0) = p.v;
+    *(V*)(out + e1) = q.v;
   }
 }
 
@@ -206,7 +201,10 @@ static int rope_launch(RopeArgs& a, bool pairs, hipStream_t st) {
   const bool wide = rope_fits(a, sizeof(T), 16);
   a.units = a.D / 2 / (wide ? E : 1);
   const int64_t tokens = (int64_t)a.B * a.S;
-  a.per = tokens < 1024 ? 1 : kRpTokens;
+  // four tokens (8,190 of 20 heads 21.6 us, one at a time 23.3), one where rows go to a cache (37.8 us, four 45.8)
+  // unless that leaves threads without a unit, or the CUs without a work-group
+  a.per = a.slots ? std::max(1, std::min(kRpTokens, kRpThreads / (a.heads * a.units))) : kRpTokens;
+  if (tokens < 1024) a.per = 1;
   const int64_t groups = (tokens + a.per - 1) / a.per;
   if (!fits_grid(groups, kRpThreads) || (int64_t)a.heads * a.units * kRpTokens > INT32_MAX / 2)
     return kErrUnsupported;
