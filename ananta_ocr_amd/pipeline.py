@@ -6,14 +6,18 @@ modeling_deepseekv2.py:481-498, except that the k_bar cache is refreshed only at
 the tail block instead of being rebuilt from the whole index-key cache every step
 (the summaries of complete blocks never change).  ``extend_prefill``, ``tree_step`` and
 ``commit_tree`` are the serving steps over a paged cache: a chunk of known tokens, and a tree of
-drafted ones with the update of the cache after its verification.
+drafted ones with the update of the cache after its verification.  ``start_step`` and
+``shared_step`` are a step of several answers to shared prompts (rows forked in the pool), for the
+layers that attend every key.
 """
 
 import math
 
+from typing import NamedTuple
+
 import torch
 
-from . import ops, tree
+from . import ops, rope, shared_prefix, tree
 
 
 def prefill(q, k, v, idx_q, idx_k, head_cls, block_size, local_blocks, idx_scale, floor,
@@ -264,6 +268,47 @@ def commit_tree(pool, path, count, context_lens, layers=()):
             else:
                 state.refresh_from(idx_k, head_cls, bs, pool.table, lens, ctx // bs)
     return new
+
+
+class StepRows(NamedTuple):
+    """The new tokens of a step, packed (kv_pages.step_rows)."""
+    ok: torch.Tensor             # int32 [1], 0 where the pool had no room: no token has a slot
+    context_lens: torch.Tensor   # [R] tokens of every pool row before the step
+    cu_seqlens_q: torch.Tensor   # [R + 1]
+    seq: torch.Tensor            # [rows] pool row, -1 past the last request's
+    positions: torch.Tensor      # [rows]
+    slots: torch.Tensor          # [rows] int64
+
+
+def start_step(pool, query_lens, rows):
+    """Room in the pool (kv_pages.PagePool) for query_lens [R] new tokens of its rows, one or more of a
+    row that takes part and 0 of the others, packed into a batch of `rows` rows: StepRows, once for
+    all layers.  Where the pool refuses (ok 0) its state stays, no token has a slot, and the step's
+    outputs mean nothing."""
+    with tree._device(pool.lens, query_lens):
+        n = ops._i32(query_lens).clamp(min=0)
+        ctx = pool.lens.clone()
+        ok = pool.reserve(ctx + n)
+        return StepRows(ok, ctx, *pool.step_rows(ctx, n, rows))
+
+
+def shared_step(step, q, k, v, k_cache, v_cache, block_table, inv_freq, cu_groups=None,
+                prefix_lens=None, scale=None, interleaved=False, start=0, factor=1.0,
+                out_dtype=torch.bfloat16):
+    """One layer of a step (start_step) whose tokens attend every key of their sequence: q [T,H,D]
+    and k, v [T,Hkv,D] bf16 as projected, T the step's rows.  The keys are turned by their positions
+    (rope.rope_append: inv_freq, interleaved, start, factor) and written with the values to the
+    layer's pages k_cache / v_cache [pages, page_size, Hkv, D], then the turned queries attend
+    (shared_prefix.attn_shared): the keys below prefix_lens[g] of the pool rows cu_groups[g] ..
+    cu_groups[g + 1] - 1, as pool.fork shared them, are read once for the group.  block_table [R,P] is
+    the pool's table.  Returns out [T,H,D] (out_dtype); rows of no sequence give 0."""
+    if scale is None:
+        scale = 1.0 / math.sqrt(q.shape[-1])
+    q = rope.rope_append(q, k, v, step.positions, step.slots, k_cache, v_cache, inv_freq, interleaved,
+                         start, factor)
+    return shared_prefix.attn_shared(q, k_cache, v_cache, block_table, step.context_lens,
+                                     step.cu_seqlens_q, cu_groups, prefix_lens, scale,
+                                     out_dtype=out_dtype)
 
 
 def init_decode_state(idx_k, head_cls, block_size, nblk_cap, seq_lens=None, block_table=None,
