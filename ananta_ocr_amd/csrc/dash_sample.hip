@@ -36,11 +36,12 @@ constexpr int kSmThreads = 256;           // of a chunk's
 constexpr int kSmBins = 512;
 constexpr int kSmMaxChunks = 16;
 constexpr int kSmList = 2048;             // tokens listed of a row
+constexpr int kSmFew = 1024;              // so many tokens are all listed
 constexpr int kSmMaxV = 1 << 20;
 constexpr int kSmTiles = 256;             // tiles of a row's work-group, or of a chunk's, at most
 constexpr int kSmShort = 32768;           // tokens of a row that one work-group takes
 constexpr int kSmMany = 256;              // rows that take a work-group each, however long
-constexpr int kSmCut = 256;               // threads, and steps a pass, of the search for a border
+constexpr int kSmCut = 256;               // steps a pass of the search for a border
 
 struct SampleState {                      // of a row, once its bins are known
   uint64_t k_mass, k_whole;               // weight of the bins before the k-th token's; of the first k, 0 if unknown
@@ -218,18 +219,21 @@ __device__ __forceinline__ int sm_bin(const SampleRow& w, float x) {
   return (int)fminf(sm_below(w, x), (float)(kSmBins - 1));
 }
 
-// Sum over the work-group's earlier threads; total: over all.
+// Sum over the earlier ones of the work-group's first NT threads (of the others: nothing in particular);
+// total: over all of them.
 template <int NT>
 __device__ __forceinline__ uint64_t sm_before(uint64_t v, uint64_t* sW, uint64_t& total) {
   const int lane = wave_lane(), wv = threadIdx.x / kWave;
   uint64_t x = v;
-#pragma unroll
-  for (int s = 1; s < kWave; s <<= 1) {
-    const uint64_t y = __shfl_up(x, s, kWave);
-    if (lane >= s) x += y;
-  }
   __syncthreads();
-  if (lane == kWave - 1) sW[wv] = x;
+  if (wv < NT / kWave) {
+#pragma unroll
+    for (int s = 1; s < kWave; s <<= 1) {
+      const uint64_t y = __shfl_up(x, s, kWave);
+      if (lane >= s) x += y;
+    }
+    if (lane == kWave - 1) sW[wv] = x;
+  }
   __syncthreads();
   uint64_t before = 0;
   total = 0;
@@ -291,7 +295,6 @@ struct SampleShared {
 // The row's borders as far as its bins tell, from the counts and weights in s.cnt and s.mass.  A thread adds up
 // kSmBins / kSmSelect bins of its own, of the first kSmSelect threads.
 constexpr int kSmSelect = 256;
-template <int NT>
 __device__ __forceinline__ void sm_select(const SampleRow& w, SampleShared& s) {
   constexpr int PER = kSmBins / kSmSelect;
   const int tid = threadIdx.x;
@@ -306,14 +309,15 @@ __device__ __forceinline__ void sm_select(const SampleRow& w, SampleShared& s) {
       c += cnt[i];
       m += mass[i];
     }
-    uint64_t cb = sm_before<NT>(c, s.sW, live), mb = sm_before<NT>(m, s.sW, all);
+    uint64_t cb = sm_before<kSmSelect>(c, s.sW, live), mb = sm_before<kSmSelect>(m, s.sW, all);
     const uint64_t mb0 = mb;
     const bool k_on = w.k > 0 && (uint64_t)w.k < live;
     if (tid == 0 && !k_on) s.st.k_whole = all;
-    if (tid <= kSmSelect) {
+    if (tid == 0) s.before[kSmBins] = (uint32_t)live;
+    if (tid < kSmSelect) {
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        if (tid < kSmSelect || i == 0) s.before[PER * tid + i] = (uint32_t)cb;
+        s.before[PER * tid + i] = (uint32_t)cb;
         if (k_on && cb < (uint64_t)w.k && cb + cnt[i] >= (uint64_t)w.k) {
           s.st.k_bin = PER * tid + i;
           s.st.k_count = (int)cb;
@@ -364,6 +368,7 @@ __device__ __forceinline__ void sm_select(const SampleRow& w, SampleShared& s) {
         st.sure = min(st.sure, max((int)d - 1, 0));
         st.end = min(st.end, (int)d + 2);
       }
+      if (s.before[st.end] <= (uint32_t)kSmFew) st.sure = 0;     // every token that may stay is listed
       int n = s.before[st.end] - s.before[min(st.sure, st.end)];
       if (part && kb >= st.end && st.p_lo >= 0 && st.p_lo < st.end) n += s.before[kb + 1] - s.before[kb];
       st.listed = n <= kSmList ? n : -1;
@@ -506,18 +511,23 @@ __global__ __launch_bounds__(kSmBins) void sample_select_kernel(SampleArgs a) {
   uint32_t cnt = 0;
   uint64_t mass = 0;
   if (w.filter) {
+    uint32_t c[kSmMaxChunks];
+    uint64_t m[kSmMaxChunks];
+#pragma unroll
+    for (int i = 0; i < kSmMaxChunks; ++i) {         // (every load before the first sum)
+      c[i] = cnts[min(i, a.S - 1) * kSmBins];
+      m[i] = masses[min(i, a.S - 1) * kSmBins];
+    }
 #pragma unroll
     for (int i = 0; i < kSmMaxChunks; ++i) {
-      if (i < a.S) {
-        cnt += cnts[i * kSmBins];
-        mass += masses[i * kSmBins];
-      }
+      cnt += i < a.S ? c[i] : 0;
+      mass += i < a.S ? m[i] : 0;
     }
   }
   s.cnt[tid] = cnt;
   s.mass[tid] = mass;
   __syncthreads();
-  sm_select<kSmBins>(w, s);
+  sm_select(w, s);
   if (tid == 0) {
     a.state[r] = s.st;
     a.n_list[r] = 0;
@@ -708,15 +718,21 @@ __device__ __forceinline__ int sm_draw(const SampleRow& w, const SmSrc<T, HELD>&
   if (nt > 1) {
     for (int i = tid; i < nt; i += NT) s.tile[i] = 0;
     __syncthreads();
-    sm_vectors<NT>(row, v0, v1, [&](const SmVec<T>& x, int v) {
-      uint64_t sum = 0;
+    for (int i = 0; i < nt; i += 2) {
+      const int v = v0 + i * kSmTile<T, NT> + E * tid, u = v + kSmTile<T, NT>;
+      SmVec<T> x, y;
+      if (v < v1) x = row.at(v, v1);
+      if (u < v1) y = row.at(u, v1);
+      uint64_t sum[2] = {0, 0};
 #pragma unroll
       for (int j = 0; j < E; ++j) {
         double f;
-        if (stays(x.at(j), v + j, f)) sum += sm_whole(w, f);
+        if (v < v1 && stays(x.at(j), v + j, f)) sum[0] += sm_whole(w, f);
+        if (u < v1 && stays(y.at(j), u + j, f)) sum[1] += sm_whole(w, f);
       }
-      if (sum > 0) atomicAdd(&s.tile[(v - v0) / kSmTile<T, NT>], (unsigned long long)sum);
-    });
+      if (__any(sum[0] > 0)) sm_add(sum[0], &s.tile[i]);
+      if (__any(sum[1] > 0)) sm_add(sum[1], &s.tile[i + 1]);
+    }
     __syncthreads();
     uint64_t before;
     t = sm_find<NT>(tid < nt ? s.tile[tid] : 0, ahead, want, s, before);
@@ -784,16 +800,16 @@ __device__ __forceinline__ double sm_want(float u, uint64_t total) {
   u = fmaxf(u, 0.f);
   return u < 1.f ? (double)u * (double)total : (double)INFINITY;
 }
-// f(place, weight) of the listed tokens of bins b0 .. b1 - 1.
+// f(place, weight) of the listed tokens of bins b0 .. b1 - 1; their weights in listw, where there is room for them.
 template <typename F>
-__device__ __forceinline__ void sm_listed(const SampleRow& w, int n, int b0, int b1, const SampleShared& s, F f) {
-  if (threadIdx.x < kSmCut)
-    for (int i = threadIdx.x; i < n; i += kSmCut) {
-      const uint64_t place = s.list[i];
-      const float x = sm_logit((uint32_t)(place >> 32));
-      const int b = sm_bin(w, x);
-      if (b >= b0 && b < b1) f(place, sm_whole(w, sm_weight(w, x)));
-    }
+__device__ __forceinline__ void sm_listed(const SampleRow& w, int n, int b0, int b1, const SampleShared& s,
+                                          const uint64_t* listw, F f) {
+  for (int i = threadIdx.x; i < n; i += blockDim.x) {
+    const uint64_t place = s.list[i];
+    const float x = sm_logit((uint32_t)(place >> 32));
+    const int b = sm_bin(w, x);
+    if (b >= b0 && b < b1) f(place, listw ? listw[i] : sm_whole(w, sm_weight(w, x)));
+  }
 }
 
 // The probabilities of tokens v0 .. v1 - 1.
@@ -813,23 +829,63 @@ __device__ __forceinline__ void sm_probs(const SampleArgs& a, const SampleRow& w
   });
 }
 
-template <typename T>
-__global__ __launch_bounds__(kSmThreads) void sample_draw_kernel(SampleArgs a) {
+// Every token that may stay is listed: the weight of those that do, and the token that u draws, by their ids as places.
+__device__ __forceinline__ uint64_t sm_few(const SampleArgs& a, const SampleRow& w, const SampleState& st,
+                                           uint64_t last, int64_t r, bool draw, const uint64_t* listw,
+                                           SampleShared& s) {
+  auto stay = [&](auto f) {
+    sm_listed(w, st.listed, 0, st.end, s, listw, [&](uint64_t place, uint64_t e) {
+      if (place >= last && (!(w.min_p > 0.f) || sm_weight(w, sm_logit((uint32_t)(place >> 32))) >= (double)w.min_p))
+        f((uint64_t)(uint32_t)place, e);
+    });
+  };
+  __syncthreads();
+  if (threadIdx.x == 0) s.chunk[0] = 0;
+  __syncthreads();
+  stay([&](uint64_t, uint64_t e) { atomicAdd(&s.chunk[0], (unsigned long long)e); });
+  __syncthreads();
+  const uint64_t total = s.chunk[0];
+  if (draw && a.u) {
+    // the first whose sum exceeds u times the whole is the last whose predecessors' sum does not
+    const double want = sm_want(a.u[r], total);
+    const SampleCut z = sm_cut(stay, 0, nextafter(want, (double)INFINITY), 0, 0, ~0ull, s);
+    if (threadIdx.x == 0) a.token[r] = (int)~(uint32_t)z.place;
+  }
+  return total;
+}
+
+// NT: kSmWide threads where a row's one work-group draws (64 rows: 27 us, kSmThreads 33), kSmThreads where every chunk's
+// has probabilities to write (each finds the borders by itself; 48 rows: 36.6 us, kSmWide 38).
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void sample_draw_kernel(SampleArgs a) {
   __shared__ SampleShared s;
+  __shared__ uint64_t sListw[kSmList];
   const int64_t r = blockIdx.y;
   const int c = blockIdx.x, tid = threadIdx.x;
   const SampleRow w = sm_row_of(a, r);
   const int v0 = c * a.chunk, v1 = min(a.V, v0 + a.chunk);
   if (!w.any || w.greedy) {
-    sm_one<kSmThreads>(a, w, r, c, v0, v1);
+    sm_one<NT>(a, w, r, c, v0, v1);
     return;
   }
   const SmSrc<T, false> row = {(const T*)a.x + r * a.x_st, nullptr};
   const SampleState st = a.state[r];
-  for (int i = tid; i < st.listed; i += kSmThreads) s.list[i] = a.list[r * kSmList + i];
+  for (int i = tid; i < st.listed; i += NT) {
+    s.list[i] = a.list[r * kSmList + i];
+    sListw[i] = sm_whole(w, sm_weight(w, sm_logit((uint32_t)(s.list[i] >> 32))));
+  }
   if (tid < a.S) s.chunk[tid] = a.sure[r * a.S + tid];
   __syncthreads();
-  uint64_t last = 0;
+  const SampleGate g = sm_gate(st);
+  uint64_t last = 0, total = 0;
+  auto stays = [&](float x, int v, double& e) { return sm_stays(w, g, last, x, v, e); };
+  auto listed = [&](int b0, int b1, auto f) { sm_listed(w, st.listed, b0, b1, s, sListw, f); };
+  if (st.sure == 0 && st.listed > 0) {
+    last = sm_borders(w, st, listed, s);
+    total = sm_few(a, w, st, last, r, c == 0, sListw, s);
+    if (a.probs) sm_probs<NT>(a, w, row, r, v0, v1, total, stays);
+    return;
+  }
   auto finish = [&](auto tokens) {
     last = sm_borders(w, st, tokens, s);
     tokens(st.sure, st.end, [&](uint64_t place, uint64_t e) {
@@ -839,12 +895,9 @@ __global__ __launch_bounds__(kSmThreads) void sample_draw_kernel(SampleArgs a) {
     __syncthreads();
   };
   if (st.listed > 0)
-    finish([&](int b0, int b1, auto f) { sm_listed(w, st.listed, b0, b1, s, f); });
+    finish(listed);
   else if (st.listed < 0)
-    finish([&](int b0, int b1, auto f) { sm_of_row<kSmThreads>(w, row, a.V, b0, b1, f); });
-  const SampleGate g = sm_gate(st);
-  auto stays = [&](float x, int v, double& e) { return sm_stays(w, g, last, x, v, e); };
-  uint64_t total = 0;
+    finish([&](int b0, int b1, auto f) { sm_of_row<NT>(w, row, a.V, b0, b1, f); });
   for (int i = 0; i < a.S; ++i) total += s.chunk[i];
   if (c == 0 && a.u) {
     const double want = sm_want(a.u[r], total);
@@ -867,10 +920,10 @@ __global__ __launch_bounds__(kSmThreads) void sample_draw_kernel(SampleArgs a) {
       ahead = any_ahead;
     }
     const int d0 = at * a.chunk, d1 = min(a.V, d0 + a.chunk);
-    const int token = sm_draw<kSmThreads>(w, row, want, ahead, d0, d1, s, stays);
+    const int token = sm_draw<NT>(w, row, want, ahead, d0, d1, s, stays);
     if (tid == 0) a.token[r] = token;
   }
-  if (a.probs) sm_probs<kSmThreads>(a, w, row, r, v0, v1, total, stays);
+  if (a.probs) sm_probs<NT>(a, w, row, r, v0, v1, total, stays);
 }
 
 // The same, a work-group a row.  A short row stays in LDS (HELD): one CU takes 5 us to read 128 KB, from the L2
@@ -909,11 +962,12 @@ __global__ __launch_bounds__(kSmWide) void sample_row_kernel(SampleArgs a) {
     sm_tokens<NT>(row, 0, a.V, [&](float x, int) { sum += sm_whole(w, sm_weight(w, x)); });
   __syncthreads();
   const uint64_t mass = tid < kSmBins ? s.mass[tid] : 0;
-  sm_select<NT>(w, s);
+  sm_select(w, s);
   const SampleState st = s.st;
   const SampleGate g = sm_gate(st);
   sm_add(!w.filter ? sum : tid < st.sure ? mass : 0, &s.chunk[0]);
   uint64_t last = 0;
+  auto stays = [&](float l, int v, double& e) { return sm_stays(w, g, last, l, v, e); };
   auto finish = [&](auto tokens) {
     last = sm_borders(w, st, tokens, s);
     tokens(st.sure, st.end, [&](uint64_t place, uint64_t e) {
@@ -924,13 +978,19 @@ __global__ __launch_bounds__(kSmWide) void sample_row_kernel(SampleArgs a) {
   if (st.listed > 0) {
     sm_tokens<NT>(row, 0, a.V, [&](float x, int v) { sm_take(w, g, x, v, s.list, &s.listed); });
     __syncthreads();
-    finish([&](int b0, int b1, auto f) { sm_listed(w, st.listed, b0, b1, s, f); });
+    auto listed = [&](int b0, int b1, auto f) { sm_listed(w, st.listed, b0, b1, s, nullptr, f); };
+    if (st.sure == 0) {
+      last = sm_borders(w, st, listed, s);
+      const uint64_t whole = sm_few(a, w, st, last, r, true, nullptr, s);
+      if (a.probs) sm_probs<NT>(a, w, row, r, 0, a.V, whole, stays);
+      return;
+    }
+    finish(listed);
   } else if (st.listed < 0) {
     finish([&](int b0, int b1, auto f) { sm_of_row<NT>(w, row, a.V, b0, b1, f); });
   }
   __syncthreads();
   const uint64_t total = s.chunk[0];
-  auto stays = [&](float l, int v, double& e) { return sm_stays(w, g, last, l, v, e); };
   if (a.u) {
     const int token = sm_draw<NT>(w, row, sm_want(a.u[r], total), 0, 0, a.V, s, stays);
     if (tid == 0) a.token[r] = token;
@@ -982,7 +1042,8 @@ static void sample_launch(const SampleArgs& a, int64_t R, hipStream_t st) {
   hipLaunchKernelGGL(sample_bins_kernel<T>, grid, block, 0, st, a);
   hipLaunchKernelGGL(sample_select_kernel, dim3((unsigned)R), dim3(kSmBins), 0, st, a);
   hipLaunchKernelGGL(sample_pick_kernel<T>, grid, block, 0, st, a);
-  hipLaunchKernelGGL(sample_draw_kernel<T>, dim3(a.probs ? a.S : 1, (unsigned)R), block, 0, st, a);
+  if (a.probs) hipLaunchKernelGGL((sample_draw_kernel<T, kSmThreads>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((sample_draw_kernel<T, kSmWide>), dim3(1, (unsigned)R), dim3(kSmWide), 0, st, a);
 }
 
 }  // namespace dash
