@@ -201,13 +201,13 @@ static int rope_launch(RopeArgs& a, bool pairs, hipStream_t st) {
   const bool wide = rope_fits(a, sizeof(T), 16);
   a.units = a.D / 2 / (wide ? E : 1);
   const int64_t tokens = (int64_t)a.B * a.S;
+  if ((int64_t)a.heads * a.units * kRpTokens > INT32_MAX / 2) return kErrUnsupported;
   // four tokens (8,190 of 20 heads 21.6 us, one at a time 23.3), one where rows go to a cache (37.8 us, four 45.8)
   // unless that leaves threads without a unit, or the CUs without a work-group
   a.per = a.slots ? std::max(1, std::min(kRpTokens, kRpThreads / (a.heads * a.units))) : kRpTokens;
   if (tokens < 1024) a.per = 1;
   const int64_t groups = (tokens + a.per - 1) / a.per;
-  if (!fits_grid(groups, kRpThreads) || (int64_t)a.heads * a.units * kRpTokens > INT32_MAX / 2)
-    return kErrUnsupported;
+  if (!fits_grid(groups, kRpThreads)) return kErrUnsupported;
   const dim3 grid((unsigned)groups), block(kRpThreads);
   if (wide && pairs) hipLaunchKernelGGL((rope_kernel<T, E, true>), grid, block, 0, st, a);
   else if (wide) hipLaunchKernelGGL((rope_kernel<T, E, false>), grid, block, 0, st, a);
