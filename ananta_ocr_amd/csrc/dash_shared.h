@@ -18,6 +18,7 @@
 namespace dash {
 
 constexpr int kShMaxSeqs = 8192;
+constexpr int kShMaxKeys = INT32_MAX - 127;      // (a tile's end past the last key is a number of 32 bits still)
 constexpr int kShThreads = 256;           // of the plan kernel
 
 struct SharedSeg {
@@ -661,7 +662,7 @@ inline SharedPlan shared_plan(int B, int G, int H, int Hkv, int64_t T) {
 extern "C" int dash_attn_shared_workspace_size(int B, int G, int H, int Hkv, int64_t T, int64_t* bytes) {
   using namespace dash;
   if (!bytes || B < 0 || G < 0 || H <= 0 || Hkv <= 0 || T < 0) return kErrInvalid;
-  if (H % Hkv != 0) return kErrUnsupported;
+  if (H % Hkv != 0 || B > kShMaxSeqs || G > kShMaxSeqs || T > INT32_MAX) return kErrUnsupported;
   *bytes = shared_plan(B, G, H, Hkv, T).total;
   return kOk;
 }
@@ -684,7 +685,7 @@ extern "C" int dash_attn_shared(const void* q, int64_t q_st, int64_t q_sh, const
   if (B > 0 && P > 0 && !block_table) return kErrInvalid;
   if (num_pages > 0 && (!k || !v)) return kErrInvalid;
   if (D != 128 || H % Hkv != 0 || B > kShMaxSeqs || G > kShMaxSeqs || !(scale > 0.f) ||
-      (int64_t)P * page_size > INT32_MAX)
+      (int64_t)P * page_size > kShMaxKeys)
     return kErrUnsupported;
   const int64_t strides[] = {q_st, q_sh, k_sp, k_st, k_sh, v_sp, v_st, v_sh};
   for (int64_t s : strides)
@@ -695,6 +696,7 @@ extern "C" int dash_attn_shared(const void* q, int64_t q_st, int64_t q_sh, const
   if (T > INT32_MAX - kShThreads || 2 * T * H > INT32_MAX || !fits_grid((T * H + 3) / 4, 256))
     return kErrUnsupported;
   const SharedPlan p = shared_plan(B, G, H, Hkv, T);
+  if (!fits_grid((int64_t)p.W * Hkv, 256)) return kErrUnsupported;
   if (!workspace || workspace_bytes < p.total || (uintptr_t)workspace % 256 != 0) return kErrWorkspace;
   char* w = (char*)workspace;
   SharedArgs a = {};

@@ -11,7 +11,7 @@ falling logits, of equals the lower id first,
 * of those the ones whose weight is at least min_p, which is min_p times the best token's (0 or below: all).
 
 The first always does.  A temperature that is not above 0 keeps the first alone.  Logits of -inf and NaN
-are masked; +inf counts as above every number.  Weights are whole numbers of 2^-s of the best token's, s =
+are masked; +inf counts as the largest number of 32 bits.  Weights are whole numbers of 2^-s of the best token's, s =
 62 - ceil(log2 V) but at most 51, so that sums are exact and no result depends on how a launch ran; a token
 below half of that counts as none.
 """
@@ -52,6 +52,8 @@ def _sample(logits, uniforms, temperature, top_k, top_p, min_p, probs_dtype):
         raise NotImplementedError(f"vocabularies of at most {MAX_VOCABULARY} tokens, got {V}")
     if probs_dtype is not None and probs_dtype not in _TYPES:
         raise NotImplementedError("probabilities in fp32, bf16 or fp16")
+    if probs_dtype is not None and logits.requires_grad and torch.is_grad_enabled():
+        raise ValueError("the probabilities have no gradients (detach the logits)")
     if uniforms is not None:
         _shape(uniforms, (R,), "uniforms")
     t, t0 = _floats(temperature, R, "temperature")
@@ -101,5 +103,5 @@ def sample(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, ret
 
 def token_probs(logits, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, dtype=torch.float32):
     """The probabilities [R, V] of the tokens after temperature, top-k, top-p and min-p (as sample draws
-    from them), 0 for those that do not stay: the target, or the draft, of tree.verify_tree."""
+    from them), 0 for those that do not stay: the target, or the draft, of tree.verify_tree.  No gradients."""
     return _sample(logits, None, temperature, top_k, top_p, min_p, dtype)[1]

@@ -13,6 +13,7 @@ from .ops import _bf16_rows, _i32, _ptr, _stream
 from .tree import _device, _shape
 
 MAX_SEQS = 8192
+MAX_TOKENS = 2 ** 31 - 128
 
 
 def attn_shared(q, k, v, block_table, context_lens, cu_seqlens_q, cu_groups, prefix_lens, scale,
@@ -30,7 +31,7 @@ def attn_shared(q, k, v, block_table, context_lens, cu_seqlens_q, cu_groups, pre
 
     Returns out [T,H,128] (fp32 or bf16) and with return_lse the log-sum-exp [T,H] fp32; a row that
     sees no key, or of no sequence (a batch padded to a fixed size), gives 0 and -inf.  At most 8,192
-    sequences; 2^31 - 1 tokens a table row."""
+    sequences; 2^31 - 128 tokens a table row.  For inference: no gradients."""
     if q.dim() != 3 or k.dim() != 4 or k.shape != v.shape:
         raise ValueError("q [T,H,D] and k, v of one shape [pages, page_size, Hkv, D] are needed")
     if out_dtype not in (torch.float32, torch.bfloat16):
@@ -54,8 +55,10 @@ def attn_shared(q, k, v, block_table, context_lens, cu_seqlens_q, cu_groups, pre
         _shape(prefix_lens, (G,), "prefix_lens")
     if B > MAX_SEQS or G > MAX_SEQS:
         raise NotImplementedError(f"at most {MAX_SEQS} sequences and groups")
-    if P * page_size > 2 ** 31 - 1:
-        raise NotImplementedError("a block_table of at most 2^31 - 1 tokens a sequence")
+    if P * page_size > MAX_TOKENS:
+        raise NotImplementedError("a block_table of at most 2^31 - 128 tokens a sequence")
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        raise ValueError("attn_shared has no gradients")
     with _device(q, k, v, block_table, context_lens, cu_seqlens_q, cu_groups, prefix_lens):
         q, k, v = _bf16_rows(q), _bf16_rows(k), _bf16_rows(v)
         bt, ctx, cu = _i32(block_table), _i32(context_lens), _i32(cu_seqlens_q)

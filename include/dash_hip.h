@@ -841,7 +841,7 @@ int dash_attn_shared_workspace_size(int B, int G, int H, int Hkv, int64_t T, int
  * read through the first one's table row, once for the group.  Sequences of no group share nothing.  Prefix sums
  * that do not fit the rows or sequences are cut to them.  out [T, H, 128] fp32 (out_bf16 = 0) or bf16, lse [T, H]
  * optional; a row that sees no key, and a row of no sequence, gives 0 and -inf.  B, G <= 8,192; any page size;
- * P * page_size < 2^31.  workspace: dash_attn_shared_workspace_size bytes, 256-byte aligned, any contents.
+ * P * page_size <= 2^31 - 128.  workspace: dash_attn_shared_workspace_size bytes, 256-byte aligned, any contents.
  */
 int dash_attn_shared(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_sp, int64_t k_st,
                      int64_t k_sh, const void* v, int64_t v_sp, int64_t v_st, int64_t v_sh,
