@@ -20,6 +20,7 @@ namespace dash {
 constexpr int kShMaxSeqs = 8192;
 constexpr int kShMaxKeys = INT32_MAX - 127;      // (a tile's end past the last key is a number of 32 bits still)
 constexpr int kShThreads = 256;           // of the plan kernel
+constexpr int kShFew = 64;                // sequences, and groups, whose plan every work-group makes for itself
 
 struct SharedSeg {
   int32_t r0, rows;                       // first packed row; rows times query heads of a key head
@@ -81,28 +82,72 @@ __device__ __forceinline__ int64_t sh_before(int64_t v, int64_t* sW, int64_t& to
   return before + x - v;
 }
 
+// The segment of a group of sequences from .. to - 1, whose rows start at cu(b); of sequence b with rows r0 .. r1 - 1, in
+// a batch of groups that start at cu_groups.
+template <typename Cu>
+__device__ __forceinline__ SharedSeg sh_group(const SharedArgs& a, int from, int to, int prefix, Cu cu) {
+  SharedSeg g = {0, 0, 0, 0, 0, -1, 0, 0, INT32_MAX, {0, 0, 0}};
+  const int b0 = min(max(from, 0), a.B), b1 = min(max(to, b0), a.B);
+  g.r0 = cu(b0);
+  g.rows = b1 > b0 ? max(cu(b1) - g.r0, 0) * (a.H / a.Hkv) : 0;
+  g.k1 = min(max(prefix, 0), a.S);
+  g.table_row = min(b0, a.B - 1);
+  return g;
+}
+__device__ __forceinline__ SharedSeg sh_sequence(const SharedArgs& a, int b, int r0, int r1, int ctx,
+                                                 const int* cu_groups, const int* prefix) {
+  SharedSeg g = {0, 0, 0, 0, 0, -1, 0, 0, 0, {0, 0, 0}};
+  const int n = max(r1 - r0, 0);
+  g.r0 = r0;
+  g.rows = n * (a.H / a.Hkv);
+  int lo = -1, hi = a.G;                  // the last group that starts at or before b
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (cu_groups[mid] <= b) lo = mid; else hi = mid;
+  }
+  if (lo >= 0 && b < cu_groups[lo + 1]) {
+    g.group = lo;
+    g.k0 = min(max(prefix[lo], 0), a.S);
+  }
+  ctx = min(max(ctx, 0), a.S);
+  g.k1 = (int)min((int64_t)ctx + n, (int64_t)a.S);
+  g.lo = ctx + 1;
+  g.table_row = b;
+  return g;
+}
+// With the partial rows before it, of groups or of sequences (those of sequences lie behind those of groups); its units.
+// Groups, or sequences, whose prefix sums are none could have more rows than the workspace holds.
+__device__ __forceinline__ int64_t sh_place(const SharedArgs& a, SharedSeg& g, bool group, int64_t before) {
+  const int64_t room = a.T * (a.H / a.Hkv);
+  if (before + g.rows > room) g.rows = 0;
+  g.base = (int)min(group ? before : room + before, 2 * room);
+  g.tiles = (g.rows + a.tile_rows - 1) / a.tile_rows;
+  return (int64_t)g.tiles * ((max(g.k1 - g.k0, 0) + 63) / 64);
+}
+// Row r's sequence and position, of sequences whose rows start at cu.
+__device__ __forceinline__ int2 sh_row(const SharedArgs& a, int64_t r, const int* cu, const int* ctx) {
+  if (r < cu[0] || r >= cu[a.B]) return make_int2(-1, -1);
+  int lo = 0, hi = a.B;                   // cu[lo] <= r < cu[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (cu[mid] <= r) lo = mid; else hi = mid;
+  }
+  return make_int2(lo, (int)min((int64_t)min(max(ctx[lo], 0), a.S) + (r - cu[lo]), (int64_t)INT32_MAX - 1));
+}
+
 // Work-group 0: the segments and their units.  The others: the sequence and position of every row.
 __global__ __launch_bounds__(kShThreads) void shared_plan_kernel(SharedArgs a) {
   __shared__ int sCu[kShMaxSeqs + 1], sLo[kShMaxSeqs];
   __shared__ int64_t sW[kShThreads / kWave];
-  const int tid = threadIdx.x, Gq = a.H / a.Hkv;
+  const int tid = threadIdx.x;
   if (blockIdx.x > 0) {
     for (int b = tid; b <= a.B; b += kShThreads) sCu[b] = sh_cu(a, b);
     __syncthreads();
     const int64_t r = (int64_t)(blockIdx.x - 1) * kShThreads + tid;
     if (r >= a.T) return;
-    int seq = -1, pos = -1;
-    if (r >= sCu[0] && r < sCu[a.B]) {
-      int lo = 0, hi = a.B;               // sCu[lo] <= r < sCu[hi]
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (sCu[mid] <= r) lo = mid; else hi = mid;
-      }
-      seq = lo;
-      pos = (int)min((int64_t)min(max(a.ctx[lo], 0), a.S) + (r - sCu[lo]), (int64_t)INT32_MAX - 1);
-    }
-    a.row_seq[r] = seq;
-    a.row_pos[r] = pos;
+    const int2 at = sh_row(a, r, sCu, a.ctx);
+    a.row_seq[r] = at.x;
+    a.row_pos[r] = at.y;
     return;
   }
   int64_t units_before = 0, rows_before = 0, own_before = 0;
@@ -117,45 +162,20 @@ __global__ __launch_bounds__(kShThreads) void shared_plan_kernel(SharedArgs a) {
     SharedSeg g = {0, 0, 0, 0, 0, -1, 0, 0, 0, {0, 0, 0}};
     const bool group = s < a.G;
     if (group) {
-      const int b0 = min(max(sCu[s], 0), a.B), b1 = min(max(sCu[s + 1], b0), a.B);
-      g.r0 = sh_cu(a, b0);
-      g.rows = b1 > b0 ? max(sh_cu(a, b1) - g.r0, 0) * Gq : 0;
-      g.k1 = min(max(a.prefix[s], 0), a.S);
-      g.table_row = min(b0, a.B - 1);
+      g = sh_group(a, sCu[s], sCu[s + 1], a.prefix[s], [&](int b) { return sh_cu(a, b); });
     } else if (s < ns) {
       const int b = s - a.G;
-      g.r0 = sh_cu(a, b);
-      const int n = max(sh_cu(a, b + 1) - g.r0, 0);
-      g.rows = n * Gq;
-      int lo = -1, hi = a.G;              // the last group that starts at or before b
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (sCu[mid] <= b) lo = mid; else hi = mid;
-      }
-      if (lo >= 0 && b < sCu[lo + 1]) {
-        g.group = lo;
-        g.k0 = min(max(a.prefix[lo], 0), a.S);
-      }
-      const int ctx = min(max(a.ctx[b], 0), a.S);
-      g.k1 = (int)min((int64_t)ctx + n, (int64_t)a.S);
-      g.lo = ctx + 1;
-      if (g.group >= 0 && n > 0) atomicMin(&sLo[g.group], g.lo);
-      g.table_row = b;
+      g = sh_sequence(a, b, sh_cu(a, b), sh_cu(a, b + 1), a.ctx[b], sCu, a.prefix);
+      if (g.group >= 0 && g.rows > 0) atomicMin(&sLo[g.group], g.lo);
     }
-    int64_t total;
-    int64_t before = sh_before(g.rows, sW, total);
-    // (groups, or sequences, whose prefix sums are none could have more rows than the workspace holds)
-    const int64_t mine = group ? 0 : g.rows, room = a.T * Gq;
-    int64_t own_total;
-    const int64_t own = sh_before(mine, sW, own_total) + own_before;
-    before += rows_before;               // (groups come first: of a group's thread, rows of groups)
-    if ((group ? before : own) + g.rows > room) g.rows = 0;
+    int64_t total, own_total;
+    // (groups come first: of a group's thread, rows of groups)
+    const int64_t rows = sh_before(g.rows, sW, total) + rows_before;
+    const int64_t own = sh_before(group ? 0 : g.rows, sW, own_total) + own_before;
     rows_before += total;
     own_before += own_total;
-    g.base = (int)min(group ? before : room + own, 2 * room);
-    g.tiles = (g.rows + a.tile_rows - 1) / a.tile_rows;
-    const int64_t units = (int64_t)g.tiles * ((max(g.k1 - g.k0, 0) + 63) / 64);
-    before = sh_before(units, sW, total);
+    const int64_t units = sh_place(a, g, group, group ? rows : own);
+    const int64_t before = sh_before(units, sW, total);
     if (s < ns) {
       a.starts[s] = units_before + before;
       a.seg[s] = g;
@@ -170,14 +190,71 @@ __global__ __launch_bounds__(kShThreads) void shared_plan_kernel(SharedArgs a) {
   for (int g = tid; g < a.G; g += kShThreads) a.seg[g].lo = sLo[g];
 }
 
+// The same of up to kShFew sequences and groups, by one wavefront, a lane for a group and for a sequence; every
+// work-group of the attention makes it for itself.  A segment's partial rows start where its packed rows do.  Returns
+// the units in all.
+struct SharedFew {
+  int64_t starts[2 * kShFew];
+  SharedSeg seg[2 * kShFew];
+  int lo[kShFew], prefix[kShFew], cu_groups[kShFew + 1];
+};
+__device__ __forceinline__ int64_t sh_plan_few(const SharedArgs& a, int* sCu, int* sCtx, SharedFew* few) {
+  const int lane = wave_lane(), Gq = a.H / a.Hkv;
+  {                                       // (every load before the first wait)
+    const int32_t* groups = a.G > 0 ? a.cu_groups : a.cu;
+    const int32_t* prefix = a.G > 0 ? a.prefix : a.cu;
+    const int c = sh_cu(a, min(lane, a.B)), c_last = sh_cu(a, a.B), x = a.ctx[min(lane, a.B - 1)];
+    const int g = groups[min(lane, a.G)], g_last = groups[a.G], pre = prefix[min(lane, max(a.G - 1, 0))];
+    few->lo[lane] = INT32_MAX;
+    sCtx[lane] = x;
+    few->prefix[lane] = pre;
+    sCu[lane] = c;
+    few->cu_groups[lane] = g;
+    if (lane == 0) { sCu[kShFew] = c_last; few->cu_groups[kShFew] = g_last; }
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  SharedSeg g = {0, 0, 0, 0, 0, -1, 0, 0, 0, {0, 0, 0}}, q = g;
+  if (lane < a.G)
+    g = sh_group(a, few->cu_groups[lane], few->cu_groups[lane + 1], few->prefix[lane], [&](int b) { return sCu[b]; });
+  if (lane < a.B) q = sh_sequence(a, lane, sCu[lane], sCu[lane + 1], sCtx[lane], few->cu_groups, few->prefix);
+  if (q.group >= 0 && q.rows > 0) atomicMin(&few->lo[q.group], q.lo);
+  g.base = g.r0 * Gq;
+  q.base = ((int)a.T + q.r0) * Gq;
+  g.tiles = (g.rows + a.tile_rows - 1) / a.tile_rows;
+  q.tiles = (q.rows + a.tile_rows - 1) / a.tile_rows;
+  const int64_t gu = (int64_t)g.tiles * ((max(g.k1 - g.k0, 0) + 63) / 64);
+  const int64_t qu = (int64_t)q.tiles * ((max(q.k1 - q.k0, 0) + 63) / 64);
+  int64_t gs = gu, qs = qu;
+#pragma unroll 1
+  for (int d = 1; d < kWave; d <<= 1) {
+    const int64_t x = __shfl_up((long long)gs, d, kWave), y = __shfl_up((long long)qs, d, kWave);
+    gs += lane >= d ? x : 0;
+    qs += lane >= d ? y : 0;
+  }
+  const int64_t g_units = __shfl((long long)gs, kWave - 1, kWave), units = g_units + __shfl((long long)qs, kWave - 1, kWave);
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  if (lane < a.G) {
+    g.lo = few->lo[lane];
+    few->seg[lane] = g;
+    few->starts[lane] = gs - gu;
+  }
+  if (lane < a.B) {
+    few->seg[a.G + lane] = q;
+    few->starts[a.G + lane] = g_units + qs - qu;
+  }
+  return units;
+}
+
 // The last segment that starts at or before unit u, over the wavefront.
-__device__ __forceinline__ int sh_find(const SharedArgs& a, int64_t u) {
+__device__ __forceinline__ int sh_find(const SharedArgs& a, const int64_t* starts, int64_t u) {
   const int lane = wave_lane();
   int lo = 0, n = a.G + a.B;
   while (n > 1) {
     const int step = (n + kWave - 1) / kWave;
     const int i = lane * step;
-    const bool at = i < n && a.starts[lo + i] <= u;
+    const bool at = i < n && starts[lo + i] <= u;
     const int c = max(__popcll(__ballot(at)) - 1, 0) * step;
     lo += c;
     n = min(step, n - c);
@@ -193,15 +270,15 @@ constexpr int kShUnits = 64;              // made at a time, a lane each
 
 // Units u .. of the work-group's u0 .. u_end - 1, by one wavefront: the segments that begin among them are met one
 // after another.
-__device__ __forceinline__ void sh_units(const SharedArgs& a, int64_t u0, int64_t u, int64_t u_end, int tr,
-                                         SharedUnit* sU) {
+__device__ __forceinline__ void sh_units(const SharedArgs& a, const int64_t* starts, const SharedSeg* segs,
+                                         int64_t u0, int64_t u, int64_t u_end, int tr, SharedUnit* sU) {
   const int lane = wave_lane(), ns = a.G + a.B, Gq = a.H / a.Hkv;
   const int n = (int)min((int64_t)kShUnits, u_end - u);
   const int64_t mine = u + min(lane, n - 1);
-  const int s0 = sh_find(a, u);
+  const int s0 = sh_find(a, starts, u);
   int s = s0;
   for (int k0 = s0 + 1; k0 < ns; k0 += kWave) {
-    const int64_t next = k0 + lane < ns ? a.starts[k0 + lane] : INT64_MAX;
+    const int64_t next = k0 + lane < ns ? starts[k0 + lane] : INT64_MAX;
     uint64_t some = __ballot(next < u + n);
     const bool more = some == ~0ull;
     for (; some; some &= some - 1) {
@@ -210,9 +287,9 @@ __device__ __forceinline__ void sh_units(const SharedArgs& a, int64_t u0, int64_
     }
     if (!more) break;
   }
-  const SharedSeg g = a.seg[s];
+  const SharedSeg g = segs[s];
   const int items = max((g.k1 - g.k0 + 63) / 64, 1);
-  const int64_t rel = mine - a.starts[s];
+  const int64_t rel = mine - starts[s];
   const int tile = (int)sh_div(rel, items), i = (int)(rel - (int64_t)tile * items), rb = tile * tr;
   const int j0 = g.k0 + 64 * i;
   const int seen = min(s >= a.G ? (int)min((int64_t)g.lo + rb / Gq, (int64_t)INT32_MAX) : g.lo, g.k1);
@@ -229,7 +306,8 @@ __device__ __forceinline__ void sh_units(const SharedArgs& a, int64_t u0, int64_
 // the second product as three bf16 parts (24 bits), so that a bf16 output is the fp32 one rounded once.
 // A work-group's units form one pipeline whatever runs they belong to: the next unit's keys and values are on their
 // way to LDS (two stages) and the pages of the units after looked up while one is multiplied.
-template <int RT, int KG>
+// FEW: the plan is made here.
+template <int RT, int KG, bool FEW>
 __global__ __launch_bounds__(64 * RT * KG, 2) void shared_attn_kernel(SharedArgs a) {
   constexpr int D = 128, NW = RT * KG, TH = 64 * NW, TR = 32 * RT;
   constexpr int NH = 2 / KG;              // halves of 64 keys that a wavefront takes
@@ -247,14 +325,23 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void shared_attn_kernel(SharedArgs
   __shared__ longlong2 sOff[2][64 * CH];  // offsets of a key row in K and V
   __shared__ uint32_t sBad[2][NW];
   __shared__ float2 sMl[32 * RT];
+  __shared__ int sCu[FEW ? kShFew + 1 : 1], sCtx[FEW ? kShFew : 1];
+  __shared__ int64_t sAll;
   const int tid = threadIdx.x, lane = wave_lane();
   const int wv = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int rt = wv % RT, kg = wv / RT;
   const int hl = lane >> 5, col = lane & 31;
   const int Gq = a.H / a.Hkv;
   const int hk = blockIdx.x % a.Hkv, turn = blockIdx.x / a.Hkv;
-  const int64_t u0 = turn * a.head[1], u_end = min(u0 + a.head[1], a.head[0]);
-  if (u0 >= u_end) return;
+  // (the plan of a few lies where keys will)
+  static_assert(sizeof(SharedFew) <= sizeof(sK0), "its room");
+  SharedFew* const few = (SharedFew*)sK0;
+  int64_t u0 = 0, u_end = 0;
+  auto mine = [&](int64_t all, int64_t per) { u0 = turn * per; u_end = min(u0 + per, all); };
+  if (!FEW) {
+    mine(a.head[0], a.head[1]);
+    if (u0 >= u_end) return;
+  }
   const uint32_t kl0 = k_lane_off(col, hl), vl0 = v_lane_off(lane);
   const float csc = a.scale_log2e;
   const bf16* const kb = a.k + hk * a.k_sh;
@@ -274,7 +361,8 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void shared_attn_kernel(SharedArgs
     rr = min(r, rows - 1);
     const int64_t row = uc.x + rr / Gq;
     const int h = hk * Gq + rr % Gq;
-    end = ua.x >= a.G ? (int)min((int64_t)uc.z + rr / Gq, (int64_t)INT32_MAX) : a.row_pos[row] + 1;
+    end = ua.x >= a.G ? (int)min((int64_t)uc.z + rr / Gq, (int64_t)INT32_MAX)
+                      : (FEW ? sh_row(a, row, sCu, sCtx).y : a.row_pos[row]) + 1;
     const bf16* qb = a.q + row * a.q_st + (int64_t)h * a.q_sh;
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) qop[kk] = *(const bf16x8*)(qb + kk * 16 + hl * 8);
@@ -511,10 +599,40 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void shared_attn_kernel(SharedArgs
     }
   };
 
-  for (int64_t u = u0; u < u_end; u += kShUnits) {
-    const int nu = (int)min((int64_t)kShUnits, u_end - u), chunks = (nu + CH - 1) / CH;
+  bool planned = !FEW;
+  for (int64_t u = u0; !planned || u < u_end; u += kShUnits) {
     __syncthreads();                      // every wavefront left the batch before
-    if (wv == 0) sh_units(a, u0, u, u_end, TR, sU);
+    SharedArgs b = a;
+    if (FEW) {
+      // (read again here: held from the start, the arguments would cost the loop registers)
+      auto* args = (const __attribute__((address_space(4))) SharedArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+      asm volatile("" : "+s"(args));
+      b.cu = args->cu; b.ctx = args->ctx; b.cu_groups = args->cu_groups; b.prefix = args->prefix;
+      b.B = args->B; b.G = args->G; b.H = args->H; b.Hkv = args->Hkv; b.S = args->S; b.tile_rows = args->tile_rows;
+      b.W = args->W; b.T = args->T;
+      b.head = args->head; b.starts = args->starts; b.seg = args->seg; b.row_seq = args->row_seq;
+      if (wv == 0) {
+        const int64_t all = sh_plan_few(b, sCu, sCtx, few);
+        if (lane == 0) sAll = all;
+      }
+      __syncthreads();
+    }
+    if (FEW && !planned) {
+      const int64_t all = sAll, per = max(sh_div(all + b.W - 1, b.W), (int64_t)1);
+      mine(all, per);
+      // what the merge needs of it
+      if (blockIdx.x == 0) {
+        if (tid == 0) { b.head[0] = all; b.head[1] = per; }
+        for (int s = tid; s < b.G + b.B; s += TH) { b.starts[s] = few->starts[s]; b.seg[s] = few->seg[s]; }
+      }
+      for (int64_t r = (int64_t)blockIdx.x * TH + tid; r < b.T; r += (int64_t)gridDim.x * TH)
+        b.row_seq[r] = sh_row(b, r, sCu, sCtx).x;
+      if (u0 >= u_end) return;
+      u = u0;
+      planned = true;
+    }
+    const int nu = (int)min((int64_t)kShUnits, u_end - u), chunks = (nu + CH - 1) / CH;
+    if (wv == 0) sh_units(b, FEW ? few->starts : a.starts, FEW ? few->seg : a.seg, u0, u, u_end, TR, sU);
     __syncthreads();
     look_up(0, nu);
     put(0, nu);
@@ -714,13 +832,16 @@ extern "C" int dash_attn_shared(const void* q, int64_t q_st, int64_t q_sh, const
   a.seg = (SharedSeg*)(w + p.seg); a.row_seq = (int32_t*)(w + p.rows); a.row_pos = a.row_seq + T;
   a.part_ml = (float2*)(w + p.ml); a.part_o = (float*)(w + p.o);
   hipStream_t st = (hipStream_t)stream;
-  hipLaunchKernelGGL(shared_plan_kernel, dim3((unsigned)(1 + (T + kShThreads - 1) / kShThreads)),
-                     dim3(kShThreads), 0, st, a);
+  const bool few = a.S > 0 && B > 0 && B <= kShFew && G <= kShFew;
+  if (!few)
+    hipLaunchKernelGGL(shared_plan_kernel, dim3((unsigned)(1 + (T + kShThreads - 1) / kShThreads)),
+                       dim3(kShThreads), 0, st, a);
   if (a.S > 0) {
-    const dim3 grid((unsigned)(p.W * Hkv));
-    if (p.rt == 1) hipLaunchKernelGGL((shared_attn_kernel<1, 2>), grid, dim3(128), 0, st, a);
-    else if (p.rt == 2) hipLaunchKernelGGL((shared_attn_kernel<2, 2>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((shared_attn_kernel<4, 1>), grid, dim3(256), 0, st, a);
+    const dim3 grid((unsigned)(p.W * Hkv)), block(p.rt == 1 ? 128 : 256);
+    auto* const kernel = p.rt == 1 ? few ? shared_attn_kernel<1, 2, true> : shared_attn_kernel<1, 2, false>
+                         : p.rt == 2 ? few ? shared_attn_kernel<2, 2, true> : shared_attn_kernel<2, 2, false>
+                                     : few ? shared_attn_kernel<4, 1, true> : shared_attn_kernel<4, 1, false>;
+    hipLaunchKernelGGL(kernel, grid, block, 0, st, a);
   }
   hipLaunchKernelGGL(shared_merge_kernel, dim3((unsigned)((T * H + 3) / 4)), dim3(256), 0, st, a);
   const hipError_t e = hipGetLastError();

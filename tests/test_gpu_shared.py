@@ -292,3 +292,56 @@ def test_offsets_past_32_bits():
     k[-n:], v[-n:] = c["k"].to(DEV), c["v"].to(DEV)
     d = dict(c, table=torch.where(c["table"] < n, c["table"] + (pages - n), c["table"]), k=k, v=v)
     assert torch.equal(_run(d), _run(c))
+
+
+def _padded(c, n):
+    """The same with n more sequences, without rows."""
+    more = dict(c)
+    more["table"] = torch.cat([c["table"], c["table"][:1].expand(n, -1)])
+    more["ctx"] = torch.cat([c["ctx"], torch.full((n,), 9, dtype=I32)])
+    more["cu"] = torch.cat([c["cu"], c["cu"][-1:].expand(n)])
+    return more
+
+
+@pytest.mark.parametrize("case", [1, 4, 5, 6, 8, 9, 14, 15])
+def test_more_sequences_than_a_wavefront_changes_nothing(case):
+    """A batch of up to 64 sequences plans its work inside of the attention, a larger one before it: the same units,
+    the same sums."""
+    groups, H, Hkv, page, alone = CASES[case]
+    c = _case(groups, H, Hkv, page, case, spare_rows=2, alone=alone)
+    B = len(c["ctx"])
+    out, lse = _run(c, return_lse=True)
+    _check(c, out, lse)
+    for n in (64 - B, 65 - B, 300):
+        o, l = _run(_padded(c, n), return_lse=True)
+        assert torch.equal(o, out) and torch.equal(l, lse), n
+
+
+def test_64_groups():
+    for n in (64, 65):
+        c = _case([(10 + i, [(12 + i, 1 + i % 2)]) for i in range(n)], 1, 1, 16, 3)
+        _check(c, *_run(c, return_lse=True))
+
+
+@pytest.mark.parametrize("B, n, ctx", [(40, 1, 4000), (1, 1000, 9000), (3, 60, 48000)])
+def test_more_units_than_a_pass(B, n, ctx):
+    """More than 64 units a work-group, at one, four and two row tiles: 32 key heads, whose sequences' tables name the
+    same pages."""
+    g = torch.Generator().manual_seed(B)
+    H, page = 32, 64
+    pages = 150
+    k, v = ((torch.randn(pages, page, H, 128, generator=g) * 0.7).bfloat16() for _ in range(2))
+    P = (ctx + n + page - 1) // page
+    c = dict(q=(torch.randn(B * n, H, 128, generator=g) * 0.7).bfloat16(), k=k, v=v,
+             table=torch.stack([torch.randint(0, pages, (P,), generator=g) for _ in range(B)]).to(I32),
+             ctx=torch.full((B,), ctx, dtype=I32), cu=torch.arange(B + 1, dtype=I32) * n, T=B * n,
+             groups=torch.tensor([0, 1], dtype=I32), prefix=torch.zeros(1, dtype=I32), new=[n] * B)
+    out, lse = _run(c, groups=False, return_lse=True)
+    more = _padded(c, 70)
+    # (an average of rows that keeps the row tile: padded by a group, of one sequence without a prompt)
+    o, l = _run(more, groups=B == 1, return_lse=True)
+    c["keys"] = [tuple(x[t.long()].reshape(-1, H, 128)[:ctx + n] for x in (k, v)) for t in c["table"][:1]]
+    first = {**c, "new": [n], "ctx": c["ctx"][:1], "T": n, "q": c["q"][:n]}
+    _check(first, out[:n], lse[:n])
+    tol = 6e-5 * float(v.float().abs().max())
+    assert float((o - out).abs().max()) <= tol and float((l - lse).abs().max()) <= 1e-4
