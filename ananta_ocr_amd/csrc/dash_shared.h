@@ -60,6 +60,12 @@ __device__ __forceinline__ int sh_cu(const SharedArgs& a, int b) {
 // doubles does not reach the next whole number).
 __device__ __forceinline__ int64_t sh_div(int64_t a, int64_t b) { return (int64_t)((double)a / (double)b); }
 
+// Units of a work-group.  Of larger tiles at least two: a run's partials are as many bytes as a unit's keys and more (128
+// rows: 64 KB; three groups of three sequences 28.3 us with one, 24.6 with two, 27.8 with four; 32 rows: 19.4 and 21.4).
+__device__ __forceinline__ int64_t sh_per(const SharedArgs& a, int64_t all) {
+  return max(sh_div(all + a.W - 1, a.W), (int64_t)(a.tile_rows > 32 ? 2 : 1));
+}
+
 // Sum over the work-group's earlier threads, and over all.
 __device__ __forceinline__ int64_t sh_before(int64_t v, int64_t* sW, int64_t& total) {
   const int lane = wave_lane(), wv = threadIdx.x / kWave;
@@ -184,7 +190,7 @@ __global__ __launch_bounds__(kShThreads) void shared_plan_kernel(SharedArgs a) {
   }
   if (tid == 0) {
     a.head[0] = units_before;
-    a.head[1] = max((units_before + a.W - 1) / a.W, (int64_t)1);
+    a.head[1] = sh_per(a, units_before);
   }
   __syncthreads();
   for (int g = tid; g < a.G; g += kShThreads) a.seg[g].lo = sLo[g];
@@ -618,7 +624,7 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void shared_attn_kernel(SharedArgs
       __syncthreads();
     }
     if (FEW && !planned) {
-      const int64_t all = sAll, per = max(sh_div(all + b.W - 1, b.W), (int64_t)1);
+      const int64_t all = sAll, per = sh_per(b, all);
       mine(all, per);
       // what the merge needs of it
       if (blockIdx.x == 0) {
