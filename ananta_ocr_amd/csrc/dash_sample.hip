@@ -771,12 +771,34 @@ __device__ __forceinline__ void sm_put(void* probs, int type, int64_t at, float 
   else if (type == 1) sm_out(x, ((bf16*)probs)[at]);
   else sm_out(x, ((__half*)probs)[at]);
 }
-// kN probabilities from v on.
+// kN probabilities from v on, in whole vectors at any element's boundary.
+template <int N, typename P>
+__device__ __forceinline__ void sm_put_all(P* to, const float* x) {
+  typedef uint32_t V __attribute__((ext_vector_type(N * sizeof(P) >= 16 ? 4 : 2), aligned(2)));
+  constexpr int PER = sizeof(V) / sizeof(P);
+#pragma unroll
+  for (int j = 0; j < N; j += PER) {
+    P e[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) sm_out(x[j + i], e[i]);
+    V b;
+    __builtin_memcpy(&b, e, sizeof(V));
+    *(V*)(to + j) = b;
+  }
+}
 template <typename T>
 __device__ __forceinline__ void sm_put_vec(const SampleArgs& a, int64_t r, int v, int v1, const float* x) {
+  constexpr int E = SmVec<T>::kN;
+  const int64_t at = r * a.p_st + v;
+  if (v + E <= v1) {
+    if (a.p_type == 0) sm_put_all<E>((float*)a.probs + at, x);
+    else if (a.p_type == 1) sm_put_all<E>((bf16*)a.probs + at, x);
+    else sm_put_all<E>((__half*)a.probs + at, x);
+    return;
+  }
 #pragma unroll
-  for (int j = 0; j < SmVec<T>::kN; ++j)
-    if (v + j < v1) sm_put(a.probs, a.p_type, r * a.p_st + v + j, x[j]);
+  for (int j = 0; j < E; ++j)
+    if (v + j < v1) sm_put(a.probs, a.p_type, at + j, x[j]);
 }
 
 // Whether a token stays, and its weight.
