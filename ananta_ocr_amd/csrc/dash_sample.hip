@@ -21,6 +21,12 @@
 //   sample_pick    the tokens between, listed
 //   sample_draw    the borders within the list, by the tokens' (logit, id); the chunk, the tile and then the
 //                  token that u falls into; the probabilities
+// Bound by the vector units and, a row a work-group, by latency.  64 rows of 131,072 bf16 (16.8 MB, from HBM once, then
+// from the L2s) 61 us: max 7.0, bins 15.6 (an exponential of 64 bits a token; its LDS atomics 1.5), select 6.2, pick
+// 11.3, draw 27.4 (the cut 8, the chunk's tokens again 11, for rows whose top-p leaves thousands).  48 rows of 100,003
+// fp32 with probabilities 67 us: 6.2, 12.2, 6.1, 9.8, 35.8.  One row of 32,000 27 to 30 us where it filters, 6.8 where it
+// is greedy; cut into chunks it took 34 where a work-group took 31.
+//
 // A list that would be too long (many tokens of one logit) is not made: its work-group reads the row again
 // instead, as often as the border needs.
 #include <hip/hip_fp16.h>
@@ -36,7 +42,7 @@ constexpr int kSmThreads = 256;           // of a chunk's
 constexpr int kSmBins = 512;
 constexpr int kSmMaxChunks = 16;
 constexpr int kSmList = 2048;             // tokens listed of a row
-constexpr int kSmFew = 1024;              // so many tokens are all listed
+constexpr int kSmFew = 1024;              // so many tokens are all listed (one row 27.9 us; 256: 29.6, 512: 31.3)
 constexpr int kSmMaxV = 1 << 20;
 constexpr int kSmTiles = 256;             // tiles of a row's work-group, or of a chunk's, at most
 constexpr int kSmShort = 32768;           // tokens of a row that one work-group takes
@@ -709,8 +715,8 @@ __device__ __forceinline__ int sm_find(uint64_t mine, uint64_t ahead, double wan
 
 // The token of v0 .. v1 - 1 that `want` falls into; `ahead` lies before.  The tile first, then its thread.
 template <int NT, typename T, bool HELD, typename Stays>
-__device__ __forceinline__ int sm_draw(const SampleRow& w, const SmSrc<T, HELD>& row, double want, uint64_t ahead, int v0, int v1,
-                                       SampleShared& s, Stays stays) {
+__device__ __forceinline__ int sm_draw(const SampleRow& w, const SmSrc<T, HELD>& row, double want, uint64_t ahead,
+                                       int v0, int v1, SampleShared& s, Stays stays) {
   const int tid = threadIdx.x;
   constexpr int E = SmVec<T>::kN;
   const int nt = (v1 - v0 + kSmTile<T, NT> - 1) / kSmTile<T, NT>;
@@ -877,7 +883,8 @@ __device__ __forceinline__ uint64_t sm_few(const SampleArgs& a, const SampleRow&
 }
 
 // NT: kSmWide threads where a row's one work-group draws (64 rows: 27 us, kSmThreads 33), kSmThreads where every chunk's
-// has probabilities to write (each finds the borders by itself; 48 rows: 36.6 us, kSmWide 38).
+// has probabilities to write (each finds the borders by itself; 48 rows: 35.8 us, kSmWide 38, a launch of their own for
+// them 36.5).
 template <typename T, int NT>
 __global__ __launch_bounds__(NT) void sample_draw_kernel(SampleArgs a) {
   __shared__ SampleShared s;
@@ -1023,7 +1030,7 @@ __global__ __launch_bounds__(kSmWide) void sample_row_kernel(SampleArgs a) {
 // Rows of up to kSmShort tokens, and batches of kSmMany rows and more, take a work-group a row.
 static bool sample_whole(int64_t R, int V) { return V <= kSmShort || R >= kSmMany; }
 
-// Chunks of a row: work-groups for four a CU in all, a tile each at least.
+// Chunks of a row: work-groups for four a CU in all (two: 78 us where four take 69), a tile each at least.
 struct SampleLayout {
   int S, chunk;
   int64_t best, low, cnt, mass, state, n_list, list, sure, total;
@@ -1074,7 +1081,8 @@ extern "C" int dash_sample_workspace_size(int64_t R, int V, int64_t* bytes) {
   using namespace dash;
   if (!bytes || R < 0 || V <= 0) return kErrInvalid;
   if (V > kSmMaxV) return kErrUnsupported;
-  *bytes = std::max(sample_layout(R, V, kSmTile<float, kSmThreads>).total, sample_layout(R, V, kSmTile<bf16, kSmThreads>).total);
+  *bytes = std::max(sample_layout(R, V, kSmTile<float, kSmThreads>).total,
+                    sample_layout(R, V, kSmTile<bf16, kSmThreads>).total);
   return kOk;
 }
 

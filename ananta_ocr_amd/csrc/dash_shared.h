@@ -7,12 +7,20 @@
 // others through the sequence's own row.  So there are G + B segments: rows of a group with the keys [0, prefix),
 // and rows of a sequence with the keys [prefix, ctx + n).  A row's result is the sum of two segments'.
 //
-// The lengths lie on the device, and a launch's grid cannot depend on them: the plan kernel adds up the
+// The lengths lie on the device, and a launch's grid cannot depend on them: a plan adds up the
 // segments' work in units of 64 keys and one tile of rows, the same for every key head, and each of the W
 // work-groups of a head takes the same number of units, one after another, over as many segments as that
 // reaches.  Each run of units within a (segment, row tile) leaves an unnormalised fp32 partial per row, and
 // the merge kernel adds a row's partials up.  Neighbouring work-groups take the heads of the same keys, whose
-// rows lie side by side in memory.
+// rows lie side by side in memory (each head's keys by work-groups of their own: 124 us for the 32 answers below, 95).
+//
+// Up to 64 sequences and groups, every work-group makes the plan for itself (1.5 us more of the attention, where a
+// launch before it takes 5: 4 answers 22.0 us and 19.4, 32 answers 100.4 and 97.8); more need the plan kernel.
+//
+// Bound by HBM where the cache is long: 32 answers to 4 prompts, 10 heads of 128, a call 98 us: attention 92.5, 475 MB
+// fetched (every key once, a prompt's for all its answers) at 5.1 TB/s, merge 6.6.  64 answers to one prompt 82 us:
+// 314 MB, whose 64 rows a tile need twice the products a key, 80 + 6.6.  Few keys are bound by the chain lengths, pages,
+// keys, sums, merge: 4 answers 13.3 + 6.7 us.
 #pragma once
 
 namespace dash {
@@ -322,7 +330,7 @@ __global__ __launch_bounds__(64 * RT * KG, 2) void shared_attn_kernel(SharedArgs
   constexpr int PER = 64 * CH / TH;       // offsets of a thread
   constexpr int ST = RT == 1 ? 1 : 2;     // stages
   constexpr int NG = 16 / NW;             // groups of four key rows that a wavefront loads
-  constexpr int kAux = RT == 4 ? 0 : 2;
+  constexpr int kAux = RT == 4 ? 0 : 2;   // past the caches, but where tiles of the same keys share them (112, 100 us)
   __shared__ __attribute__((aligned(16))) bf16 sK0[64 * D];
   __shared__ __attribute__((aligned(16))) bf16 sK1[ST == 2 ? 64 * D : 8];
   __shared__ __attribute__((aligned(16))) bf16 sV0[64 * D];
