@@ -23,9 +23,9 @@
 //                  token that u falls into; the probabilities
 // Bound by the vector units and, a row a work-group, by latency.  64 rows of 131,072 bf16 (16.8 MB, which each step
 // over them fetches again: little stays in the L2s from launch to launch) 61 us: max 7.0, bins 15.6 (an exponential of 64
-// bits a token; the LDS atomics 1.5), select 6.2, pick 11.3, draw 27.4 (the cut 8, the chunk's tokens again 11, for rows
-// whose top-p leaves thousands).  48 rows of 100,003 fp32 with probabilities 67 us: 6.2, 12.2, 6.1, 9.8, 35.8.  One row of
-// 32,000 27 to 30 us where it filters, 6.8 where it is greedy; cut into chunks it took 34 where a work-group took 31.
+// bits a token; the LDS atomics 1.5), select 6.2, pick 11.3, draw 27.4 (the rows whose top-p leaves thousands).  48 rows of
+// 100,003 fp32 with probabilities 67 us: 6.2, 12.2, 6.1, 9.8, 35.8.  One row of 32,000 27 to 30 us where it filters, 6.8
+// where it is greedy; cut into chunks it took 34 where a work-group took 31.
 //
 // A list that would be too long (many tokens of one logit) is not made: its work-group reads the row again
 // instead, as often as the border needs.
