@@ -730,22 +730,25 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(SharedArgs a) {
     M = Mn;
     L = L * al + wave_sum(seen ? ml.y * w : 0.f);
     acc *= al;
-    any = any || __any(seen);
+    const uint64_t live = __ballot(seen);
+    any = any || live != 0;
     const int m = min(kWave, all - e0);
     for (int i0 = 0; i0 < m; i0 += 2 * U) {
       floatx4 x[U];
       float f[U];
+      bool in_sum[U];
 #pragma unroll
       for (int i = 0; i < U; ++i) {
         const int l = i0 + 2 * i + hl;
         const int64_t pl = __shfl(p, min(l, m - 1), kWave);
         f[i] = __shfl(w, min(l, m - 1), kWave);
-        if (l >= m) f[i] = 0.f;
+        in_sum[i] = l < m && (live >> l) & 1u;
         x[i] = *(const floatx4*)(a.part_o + pl * D + 4 * (lane & 31));
       }
+      // (every run that saw a key: where its weight is 0 its values need not be finite)
 #pragma unroll
       for (int i = 0; i < U; ++i)
-        if (f[i] != 0.f) acc += f[i] * x[i];      // (a weight of 0: of a run that saw no key, or none)
+        if (in_sum[i]) acc += f[i] * x[i];
     }
   }
 #pragma unroll
