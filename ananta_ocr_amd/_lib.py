@@ -114,6 +114,7 @@ SIGNATURES = {
     "dash_copy_pages": (_i, [_i, _p, _p, _p, _p, _i, _i, _p]),
     "dash_keep_rows": (_i, [_i, _p, _p, _p, _l, _p, _p, _p, _l, _i, _i, _i, _i, _i, _p]),
     "dash_keep_lens": (_i, [_p, _l, _p, _p, _p, _i, _i, _p, _p, _p, _p, _p]),
+    "dash_step_lens": (_i, [_p, _p, _i, _i, _p, _p, _p, _p]),
     "dash_step_rows": (_i, [_p, _p, _p, _p, _l, _i, _i, _i, _i, _i, _p, _p, _p, _p, _p]),
     "dash_fork_pages": (_i, [_p, _i, _p, _l, _i, _i, _p, _p, _p, _i, _i, _p, _p, _p, _p]),
     "dash_reserve_pages": (_i, [_p, _i, _p, _l, _i, _i, _p, _p, _i, _p, _p, _p, _p]),

@@ -237,6 +237,30 @@ __global__ __launch_bounds__(kRowsThreads) void step_rows_kernel(
   slot[r] = at;
 }
 
+// What a step asks of the pages: n = its rows' new tokens (below 0: none), ctx = the rows' tokens, want = the tokens
+// that they are to hold.  New tokens that are more than the step's `rows` together have no place in its batch: the
+// rows that bring them then want more tokens than any table holds, which the reserve refuses as a whole.  One
+// work-group, a sum in 64 bits; bound by latency.
+__global__ __launch_bounds__(kKvThreads) void step_lens_kernel(const int32_t* query, const int32_t* lens, int R,
+                                                               int rows, int32_t* n, int32_t* ctx, int32_t* want) {
+  __shared__ int64_t sW[kKvThreads / kWave];
+  const int tid = threadIdx.x;
+  int64_t sum = 0;
+  for (int r = tid; r < R; r += kKvThreads) sum += max(query[r], 0);
+#pragma unroll
+  for (int m = kWave / 2; m >= 1; m >>= 1) sum += __shfl_xor((long long)sum, m, kWave);
+  if (wave_lane() == 0) sW[tid / kWave] = sum;
+  __syncthreads();
+  int64_t total = 0;
+  for (int w = 0; w < kKvThreads / kWave; ++w) total += sW[w];
+  for (int r = tid; r < R; r += kKvThreads) {
+    const int x = max(query[r], 0), len = lens[r];
+    n[r] = x;
+    ctx[r] = len;
+    want[r] = x == 0 ? len : total > rows ? INT32_MAX : (int)min((int64_t)len + x, (int64_t)INT32_MAX);
+  }
+}
+
 // Sum of v over the work-group's earlier threads; `total` gets the sum over all.
 __device__ __forceinline__ int block_exclusive(int v, int* sW, int& total) {
   const int lane = wave_lane(), wv = threadIdx.x / kWave;
@@ -670,6 +694,17 @@ extern "C" int dash_step_rows(const int32_t* query_lens, const int32_t* context_
   hipLaunchKernelGGL(step_rows_kernel, dim3((unsigned)groups), dim3(kRowsThreads), 0, (hipStream_t)stream,
                      query_lens, context_lens, lens, block_table, table_stride, B, P, page_size, num_pages,
                      rows, cu_seqlens_q, seq, positions, slots);
+  return kv_status();
+}
+
+extern "C" int dash_step_lens(const int32_t* query_lens, const int32_t* lens, int R, int rows, int32_t* new_tokens,
+                              int32_t* context_lens, int32_t* new_lens, void* stream) {
+  using namespace dash;
+  if (R < 0 || rows < 0) return kErrInvalid;
+  if (R == 0) return kOk;
+  if (!query_lens || !lens || !new_tokens || !context_lens || !new_lens) return kErrInvalid;
+  hipLaunchKernelGGL(step_lens_kernel, dim3(1), dim3(kKvThreads), 0, (hipStream_t)stream, query_lens, lens, R, rows,
+                     new_tokens, context_lens, new_lens);
   return kv_status();
 }
 

@@ -25,6 +25,7 @@ from .ops import _i32, _ptr, _stream
 from .tree import _device, _shape
 
 MAX_ROWS = 8192
+MAX_STEP_TOKENS = 2 ** 31 - 2       # of a table row, that a step's refusal must pass
 
 
 class PageCaches:
@@ -339,6 +340,24 @@ class PagePool:
         keep_rows(self.caches, path, step[0], context_lens, self.table)
         self.free(step[1])
         return step
+
+    def reserve_step(self, query_lens, rows):
+        """Room for query_lens [rows of the pool] new tokens (a number below 0 counts as 0) of a step whose
+        batch has `rows` rows.  Returns (ok, context_lens, query_lens): the tokens of every row before,
+        and the new ones.  ok is 0, and nothing changed, where the pool has no room or the batch has
+        fewer rows than there are new tokens."""
+        rows = int(rows)
+        if not 0 <= rows < 2 ** 31:
+            raise ValueError(f"a batch of {rows} rows")
+        _shape(query_lens, self.lens.shape, "query_lens")
+        if self.table.shape[1] * self.page_size > MAX_STEP_TOKENS:
+            raise NotImplementedError("steps over tables of at most 2^31 - 2 tokens a row")
+        with _device(self.lens, query_lens):
+            R, n = self.lens.numel(), _i32(query_lens)
+            new, ctx, want = _ints(n.device, R, R, R)
+            _lib.check(_lib.load().dash_step_lens(_ptr(n), _ptr(self.lens), R, rows, _ptr(new), _ptr(ctx),
+                                                  _ptr(want), _stream()), "dash_step_lens")
+            return self.reserve(want), ctx, new
 
     def step_rows(self, context_lens, query_lens, rows):
         """(cu_seqlens_q, seq, positions, slots) of a step's new tokens (step_rows), once reserve()

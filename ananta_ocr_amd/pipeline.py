@@ -272,7 +272,7 @@ def commit_tree(pool, path, count, context_lens, layers=()):
 
 class StepRows(NamedTuple):
     """The new tokens of a step, packed (kv_pages.step_rows)."""
-    ok: torch.Tensor             # int32 [1], 0 where the pool had no room: no token has a slot
+    ok: torch.Tensor             # int32 [1], 0 where pool or batch had no room: no token has a slot
     context_lens: torch.Tensor   # [R] tokens of every pool row before the step
     cu_seqlens_q: torch.Tensor   # [R + 1]
     seq: torch.Tensor            # [rows] pool row, -1 past the last request's
@@ -283,12 +283,10 @@ class StepRows(NamedTuple):
 def start_step(pool, query_lens, rows):
     """Room in the pool (kv_pages.PagePool) for query_lens [R] new tokens of its rows, one or more of a
     row that takes part and 0 of the others, packed into a batch of `rows` rows: StepRows, once for
-    all layers.  Where the pool refuses (ok 0) its state stays, no token has a slot, and the step's
-    outputs mean nothing."""
+    all layers.  Where the pool has no room, or the new tokens are more than `rows`, the step is refused
+    (ok 0): the pool's state stays, no token has a slot, and the step's outputs mean nothing."""
     with tree._device(pool.lens, query_lens):
-        n = ops._i32(query_lens).clamp(min=0)
-        ctx = pool.lens.clone()
-        ok = pool.reserve(ctx + n)
+        ok, ctx, n = pool.reserve_step(query_lens, rows)
         return StepRows(ok, ctx, *pool.step_rows(ctx, n, rows))
 
 

@@ -764,6 +764,12 @@ int dash_keep_lens(const int32_t* path, int64_t path_stride, const int32_t* coun
                    int32_t* stand, int32_t* kept, int32_t* new_context, int32_t* summed,
                    void* stream);
 
+/* What a step asks of a pool: new_tokens[r] = query_lens[r] (below 0: 0), context_lens[r] = lens[r] and new_lens[r] =
+ * their sum, for dash_reserve_pages.  Where the new tokens are more than `rows` together, new_lens is 2^31 - 1 for the
+ * rows that bring some, which a table of fewer tokens a row refuses as a whole. */
+int dash_step_lens(const int32_t* query_lens, const int32_t* lens, int R, int rows, int32_t* new_tokens,
+                   int32_t* context_lens, int32_t* new_lens, void* stream);
+
 /* The rows of a step: request b brings query_lens[b] new tokens (below 0: none) after its context_lens[b],
  * packed in order.  cu_seqlens_q [B + 1] gets their prefix sums, cut to `rows`; row r = cu_seqlens_q[b] + i
  * gets seq = b, positions = context_lens[b] + i (-1 outside 0 .. 2^31 - 1) and slots = the token's place in
