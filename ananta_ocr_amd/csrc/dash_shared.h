@@ -3,9 +3,10 @@
 //
 // Row r = cu[b] + i is new token i of sequence b, at position t = ctx[b] + i, and sees the keys j <= t.
 // The keys below prefix[g] of the sequences of group g (cu_groups[g] <= b < cu_groups[g + 1]) are read
-// through the block-table row of the group's first sequence, once for all rows of the group; the
-// others through the sequence's own row.  So there are G + B segments: rows of a group with the keys [0, prefix),
-// and rows of a sequence with the keys [prefix, ctx + n).  A row's result is the sum of two segments'.
+// through one block-table row, once for all rows of the group: that of the first sequence that has rows and holds the
+// prefix (an answer that left holds nothing), or the most of it.  The others are read through the sequence's own row.
+// So there are G + B segments: rows of a group with the keys [0, prefix), and rows of a sequence with the keys
+// [prefix, ctx + n).  A row's result is the sum of two segments'.
 //
 // The lengths lie on the device, and a launch's grid cannot depend on them: a plan adds up the
 // segments' work in units of 64 keys and one tile of rows, the same for every key head, and each of the W
@@ -105,7 +106,6 @@ __device__ __forceinline__ SharedSeg sh_group(const SharedArgs& a, int from, int
   g.r0 = cu(b0);
   g.rows = b1 > b0 ? max(cu(b1) - g.r0, 0) * (a.H / a.Hkv) : 0;
   g.k1 = min(max(prefix, 0), a.S);
-  g.table_row = min(b0, a.B - 1);
   return g;
 }
 __device__ __forceinline__ SharedSeg sh_sequence(const SharedArgs& a, int b, int r0, int r1, int ctx,
@@ -129,6 +129,9 @@ __device__ __forceinline__ SharedSeg sh_sequence(const SharedArgs& a, int b, int
   g.table_row = b;
   return g;
 }
+// How much of its group's prefix a sequence holds.
+__device__ __forceinline__ int sh_holds(const SharedSeg& g) { return min(g.k0, g.k1); }
+
 // With the partial rows before it, of groups or of sequences (those of sequences lie behind those of groups); its units.
 // Groups, or sequences, whose prefix sums are none could have more rows than the workspace holds.
 __device__ __forceinline__ int64_t sh_place(const SharedArgs& a, SharedSeg& g, bool group, int64_t before) {
@@ -152,6 +155,7 @@ __device__ __forceinline__ int2 sh_row(const SharedArgs& a, int64_t r, const int
 // Work-group 0: the segments and their units.  The others: the sequence and position of every row.
 __global__ __launch_bounds__(kShThreads) void shared_plan_kernel(SharedArgs a) {
   __shared__ int sCu[kShMaxSeqs + 1], sLo[kShMaxSeqs];
+  __shared__ unsigned long long sFrom[kShMaxSeqs];      // the most of a prefix that is held, and the first to hold it
   __shared__ int64_t sW[kShThreads / kWave];
   const int tid = threadIdx.x;
   if (blockIdx.x > 0) {
@@ -168,7 +172,7 @@ __global__ __launch_bounds__(kShThreads) void shared_plan_kernel(SharedArgs a) {
   const int ns = a.G + a.B;
   for (int g = tid; g <= a.G && a.G > 0; g += kShThreads) {
     sCu[g] = a.cu_groups[g];
-    if (g < a.G) sLo[g] = INT32_MAX;
+    if (g < a.G) { sLo[g] = INT32_MAX; sFrom[g] = 0; }
   }
   __syncthreads();
   for (int s0 = 0; s0 < ns; s0 += kShThreads) {
@@ -180,7 +184,10 @@ __global__ __launch_bounds__(kShThreads) void shared_plan_kernel(SharedArgs a) {
     } else if (s < ns) {
       const int b = s - a.G;
       g = sh_sequence(a, b, sh_cu(a, b), sh_cu(a, b + 1), a.ctx[b], sCu, a.prefix);
-      if (g.group >= 0 && g.rows > 0) atomicMin(&sLo[g.group], g.lo);
+      if (g.group >= 0 && g.rows > 0) {
+        atomicMin(&sLo[g.group], g.lo);
+        atomicMax(&sFrom[g.group], (unsigned long long)sh_holds(g) << 32 | (uint32_t)~g.table_row);
+      }
     }
     int64_t total, own_total;
     // (groups come first: of a group's thread, rows of groups)
@@ -201,7 +208,10 @@ __global__ __launch_bounds__(kShThreads) void shared_plan_kernel(SharedArgs a) {
     a.head[1] = sh_per(a, units_before);
   }
   __syncthreads();
-  for (int g = tid; g < a.G; g += kShThreads) a.seg[g].lo = sLo[g];
+  for (int g = tid; g < a.G; g += kShThreads) {
+    a.seg[g].lo = sLo[g];
+    a.seg[g].table_row = sFrom[g] ? (int)~(uint32_t)sFrom[g] : 0;     // (0: of a group without rows no key is read)
+  }
 }
 
 // The same of up to kShFew sequences and groups, by one wavefront, a lane for a group and for a sequence; every
@@ -210,7 +220,7 @@ __global__ __launch_bounds__(kShThreads) void shared_plan_kernel(SharedArgs a) {
 struct SharedFew {
   int64_t starts[2 * kShFew];
   SharedSeg seg[2 * kShFew];
-  int lo[kShFew], prefix[kShFew], cu_groups[kShFew + 1];
+  int most[kShFew], from[kShFew], lo[kShFew], prefix[kShFew], cu_groups[kShFew + 1];
 };
 __device__ __forceinline__ int64_t sh_plan_few(const SharedArgs& a, int* sCu, int* sCtx, SharedFew* few) {
   const int lane = wave_lane(), Gq = a.H / a.Hkv;
@@ -220,6 +230,8 @@ __device__ __forceinline__ int64_t sh_plan_few(const SharedArgs& a, int* sCu, in
     const int c = sh_cu(a, min(lane, a.B)), c_last = sh_cu(a, a.B), x = a.ctx[min(lane, a.B - 1)];
     const int g = groups[min(lane, a.G)], g_last = groups[a.G], pre = prefix[min(lane, max(a.G - 1, 0))];
     few->lo[lane] = INT32_MAX;
+    few->most[lane] = 0;
+    few->from[lane] = INT32_MAX;
     sCtx[lane] = x;
     few->prefix[lane] = pre;
     sCu[lane] = c;
@@ -232,7 +244,10 @@ __device__ __forceinline__ int64_t sh_plan_few(const SharedArgs& a, int* sCu, in
   if (lane < a.G)
     g = sh_group(a, few->cu_groups[lane], few->cu_groups[lane + 1], few->prefix[lane], [&](int b) { return sCu[b]; });
   if (lane < a.B) q = sh_sequence(a, lane, sCu[lane], sCu[lane + 1], sCtx[lane], few->cu_groups, few->prefix);
-  if (q.group >= 0 && q.rows > 0) atomicMin(&few->lo[q.group], q.lo);
+  if (q.group >= 0 && q.rows > 0) {
+    atomicMin(&few->lo[q.group], q.lo);
+    atomicMax(&few->most[q.group], sh_holds(q));
+  }
   g.base = g.r0 * Gq;
   q.base = ((int)a.T + q.r0) * Gq;
   g.tiles = (g.rows + a.tile_rows - 1) / a.tile_rows;
@@ -249,8 +264,13 @@ __device__ __forceinline__ int64_t sh_plan_few(const SharedArgs& a, int* sCu, in
   const int64_t g_units = __shfl((long long)gs, kWave - 1, kWave), units = g_units + __shfl((long long)qs, kWave - 1, kWave);
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
+  // (in two steps of 32 bits: one of 64, as in the plan kernel, costs the attention three registers that it lacks)
+  if (q.group >= 0 && q.rows > 0 && few->most[q.group] == sh_holds(q)) atomicMin(&few->from[q.group], lane);
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
   if (lane < a.G) {
     g.lo = few->lo[lane];
+    g.table_row = min(few->from[lane], a.B - 1);
     few->seg[lane] = g;
     few->starts[lane] = gs - gu;
   }

@@ -24,9 +24,10 @@ def attn_shared(q, k, v, block_table, context_lens, cu_seqlens_q, cu_groups, pre
     written (rope.rope_append); each attends every key of its sequence up to itself.
 
     Sequences cu_groups[g] .. cu_groups[g + 1] - 1 (cu_groups [G + 1], prefix sums over the batch) have
-    the keys below prefix_lens[g] in common: they are read through the first one's table row, once
-    for the group.  A forked row shares its full pages, and a copy of the partly filled one holds the
-    same keys.  Sequences of no group, or of one with a prefix of 0, share nothing; cu_groups and
+    the keys below prefix_lens[g] in common: they are read through one table row, once for the group,
+    that of the first sequence with new tokens that holds them all (or the most of them).  Sequences
+    without new tokens, as an answer that has left, may hold anything.  A forked row shares its full
+    pages, and a copy of the partly filled one holds the same keys.  Sequences of no group, or of one with a prefix of 0, share nothing; cu_groups and
     prefix_lens may be None.  Prefix sums past the rows or the batch are cut to them.
 
     Returns out [T,H,128] (fp32 or bf16) and with return_lse the log-sum-exp [T,H] fp32; a row that

@@ -844,8 +844,9 @@ int dash_attn_shared_workspace_size(int B, int G, int H, int Hkv, int64_t T, int
  * token and head; H a multiple of Hkv) through block_table [B, P].  Row cu_seqlens_q[b] + i is at position
  * context_lens[b] + i of sequence b and sees its keys up to itself, whose keys and values are written.  The
  * sequences cu_groups[g] .. cu_groups[g + 1] - 1 (cu_groups [G + 1]) share the keys below prefix_lens[g]: those are
- * read through the first one's table row, once for the group.  Sequences of no group share nothing.  Prefix sums
- * that do not fit the rows or sequences are cut to them.  out [T, H, 128] fp32 (out_bf16 = 0) or bf16, lse [T, H]
+ * read through one table row, once for the group, that of the first sequence with rows that holds them all (or the
+ * most of them); sequences without rows may hold anything.  Sequences of no group share nothing.  Prefix sums that
+ * do not fit the rows or sequences are cut to them.  out [T, H, 128] fp32 (out_bf16 = 0) or bf16, lse [T, H]
  * optional; a row that sees no key, and a row of no sequence, gives 0 and -inf.  B, G <= 8,192; any page size;
  * P * page_size <= 2^31 - 128.  workspace: dash_attn_shared_workspace_size bytes, 256-byte aligned, any contents.
  */
