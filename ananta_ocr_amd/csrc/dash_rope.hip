@@ -6,9 +6,9 @@
 //   (x, y) -> (x c - y s, y c + x s),   c = f cos(pos * inv_freq[j]), s = f sin(pos * inv_freq[j]).
 // The map's transpose is the turn by -pos with the same factor f, which is the gradient's.
 //
-// The angle is a product in 64 bits, and so are its sine and cosine: a position of 10^5 has 10^5 radians,
-// whose 32-bit rounding alone is 4e-3.  They are rounded to 32 bits once a (token, pair), in LDS, for all
-// heads; the turn is two products and an addition in 32 bits, rounded once to the row's type.
+// The angle is a product in 64 bits: a position of 10^5 has 10^5 radians, whose 32-bit rounding alone is 4e-3.  Its
+// sine and cosine are series in 64 bits, good to 1.2e-10 (33 bits, beside the 24 that they are rounded to), once a
+// (token, pair), in LDS, for all heads; the turn is two products and an addition in 32 bits, rounded once to the row's type.
 //
 // A work-group takes a token, or a few of few heads, and all its heads.  Its units are two 16-byte chunks: the two
 // that a pair of the halves' layout needs, or two neighbours (single elements where an address, a stride or the
@@ -16,7 +16,8 @@
 //
 // Bound by HBM: 8,190 tokens of 10 + 10 + 10 heads of 128 bf16 in 38 us (126 MB read and written, 3.3 TB/s), 20 heads
 // turned as interleaved pairs 21.6 us (84 MB, 3.9 TB/s); with two or four units a thread in flight, or loads and stores
-// past the caches, 40 to 46 and 25 to 33.  Six wavefronts a SIMD: 38 us, five 44, eight (registers to memory) 46.
+// past the caches, 40 to 46 and 25 to 33.  Six wavefronts a SIMD: 38 us, five 44, eight (registers to memory) 46; replayed
+// from a graph, seven 31.2, six 32.7.
 // A few tokens 4 us, of latency.
 #include <hip/hip_fp16.h>
 
@@ -64,20 +65,23 @@ __device__ __forceinline__ void rp_out(float x, float& y) { y = x; }
 __device__ __forceinline__ void rp_out(float x, bf16& y) { y = (bf16)x; }
 __device__ __forceinline__ void rp_out(float x, __half& y) { y = __float2half_rn(x); }
 
-// factor (cos, sin) of pos * f.  In turns, t = pos f / (2 pi) = pos (g + h) with g + h = f / (2 pi) to twice the
-// digits, so that t's own rounding is known and its whole part can go; then the nearest quarter turn, and the
-// series of sine and cosine on [-pi / 4, pi / 4], whose next terms are below 1.2e-10.
+// factor (cos, sin) of pos * f.  In turns: pos f / (2 pi) = pos (g + h) with g + h = f / (2 pi) to twice the digits.
+// Its whole part goes within one fused step, before anything is rounded (the product and its rounding apart, as two
+// terms of a sum, were fused by the compiler, which counted the rounding twice: a position of 2^31 was off by 2e-7, one
+// of 2^47 by 5e-3).  Then the nearest quarter turn, and the series of sine and cosine on [-pi / 4, pi / 4], whose next
+// terms are below 1.2e-10.
 __device__ __forceinline__ float2 rp_turn(double pos, double f, float factor) {
   constexpr double c0 = 0.15915494309189535, c1 = -9.839338337591243e-18;   // 1 / (2 pi)
   const double g = f * c0, h = fma(f, c0, -g) + f * c1;
-  const double t = pos * g, e = fma(pos, g, -t) + pos * h;
-  const double r = (t - __builtin_rint(t)) + e;
+  const double r = fma(pos, h, fma(pos, g, -__builtin_rint(pos * g)));
   const double q = __builtin_rint(4.0 * r);
   const double x = fma(q, -0.25, r) * 6.283185307179586, y = x * x;
-  double s = fma(y, -1.0 / 39916800.0, 1.0 / 362880.0);
-  s = fma(s, y, -1.0 / 5040.0);
-  s = fma(s, y, 1.0 / 120.0);
-  s = fma(s, y, -1.0 / 6.0);
+  double k3 = -1.0 / 6.0, k5 = 1.0 / 120.0, k7 = -1.0 / 5040.0, k9 = 1.0 / 362880.0;
+  asm("" : "+s"(k3), "+s"(k5), "+s"(k7), "+s"(k9));      // (in vector registers they would be spilled)
+  double s = fma(y, -1.0 / 39916800.0, k9);
+  s = fma(s, y, k7);
+  s = fma(s, y, k5);
+  s = fma(s, y, k3);
   s = fma(s * y, x, x);
   double c = fma(y, -1.0 / 3628800.0, 1.0 / 40320.0);
   c = fma(c, y, -1.0 / 720.0);
@@ -90,7 +94,7 @@ __device__ __forceinline__ float2 rp_turn(double pos, double f, float factor) {
 }
 
 template <typename T, int E, bool PAIRS>
-__global__ __launch_bounds__(kRpThreads, 6) void rope_kernel(RopeArgs a) {
+__global__ __launch_bounds__(kRpThreads, 7) void rope_kernel(RopeArgs a) {
   typedef typename std::remove_reference<decltype(RopeChunk<T, E>::v)>::type V;
   __shared__ float2 sCs[kRpTokens * kRpMaxPairs];
   __shared__ int64_t sSlot[kRpTokens];

@@ -3,9 +3,9 @@ positions, with a backward pass for training, or turned and written to a paged c
 for serving.
 
 A part [start, start + 2 m) of every head row is turned, m = len(inv_freq): pair j is elements (j,
-j + m) of the part, or (2 j, 2 j + 1) where ``interleaved``, its angle position * inv_freq[j].  Angles,
-sines and cosines are taken in 64 bits (a position of 10^5 is 10^5 radians, which 32 bits hold to
-4e-3) and rounded to 32 before the products, which are rounded once to the rows' type.
+j + m) of the part, or (2 j, 2 j + 1) where ``interleaved``, its angle position * inv_freq[j].  Angles
+are taken in 64 bits (a position of 10^5 is 10^5 radians, which 32 bits hold to 4e-3), their sines and
+cosines to 1.2e-10 and rounded to 32 bits before the products, which are rounded once to the rows' type.
 
 ``inv_freq`` gives the frequencies of a head with the usual scalings for long contexts; the cos/sin
 tables of two-axis positions are page_rope's.
@@ -162,7 +162,7 @@ def apply_rope(q, k, positions, inv_freq, interleaved=False, start=0, factor=1.0
     """q and k [T, heads, D] or [B, S, heads, D] (any strides; fp32, bf16 or fp16; k may be None) with
     the part [start, start + 2 len(inv_freq)) of every head row turned by its token's position times
     inv_freq, and scaled by factor; the rest as it is.  positions int32 or int64 [T], [S] or [B, S],
-    any whole numbers.  Returns new tensors (q', k'), or q' alone where k is None; differentiable in q
+    whole numbers of up to 2^53 of either sign.  Returns new tensors (q', k'), or q' alone where k is None; differentiable in q
     and k, to any order.  D even, at most 256 pairs.  Under capture a leaf that an eager graph still
     refers to is refused (a captured backward pass of it would end the process)."""
     if q.dim() not in (3, 4):
