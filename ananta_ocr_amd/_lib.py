@@ -14,6 +14,7 @@ _p = ctypes.c_void_p
 _i = ctypes.c_int
 _l = ctypes.c_int64
 _f = ctypes.c_float
+_d = ctypes.c_double
 
 # name -> (restype, argtypes); mirrors include/dash_hip.h
 SIGNATURES = {
@@ -121,9 +122,9 @@ SIGNATURES = {
     "dash_free_pages": (_i, [_p, _i, _p, _l, _i, _i, _p, _p, _i, _p]),
     "dash_compact_pages": (_i, [_p, _i, _p, _l, _i, _i, _p, _i, _p, _p, _p, _p, _p, _p]),
     "dash_rope": (_i, [_p, _l, _l, _l, _i, _p, _l, _l, _l, _p, _l, _l, _l, _i, _p, _l, _l, _l, _i, _p, _i, _l,
-                       _l, _p, _i, _i, _i, _i, _f, _i, _i, _i, _p]),
+                       _l, _p, _i, _i, _i, _i, _d, _i, _i, _i, _p]),
     "dash_rope_append": (_i, [_p, _l, _l, _i, _p, _l, _l, _p, _l, _l, _p, _l, _l, _i, _i, _p, _i, _p, _p, _l, _l,
-                              _l, _p, _l, _l, _l, _i, _i, _p, _i, _i, _i, _f, _i, _i, _p]),
+                              _l, _p, _l, _l, _l, _i, _i, _p, _i, _i, _i, _d, _i, _i, _p]),
     "dash_attn_shared_workspace_size": (_i, [_i, _i, _i, _i, _l, ctypes.POINTER(_l)]),
     "dash_attn_shared": (_i, [_p, _l, _l, _p, _l, _l, _l, _p, _l, _l, _l, _p, _l, _i, _i, _i, _p, _p, _p,
                               _p, _p, _i, _l, _l, _p, _l, _l, _i, _i, _i, _i, _l, _i, _f, _p, _l, _p]),

@@ -43,7 +43,7 @@ struct RopeArgs {
   int n, heads;                     // row sets and their heads
   const void* pos; int pos64; int64_t pos_sb, pos_st;
   const double* inv_freq;
-  double sign; float factor;
+  double sign, factor;
   const int64_t* slots; int page; int64_t num_slots;
   int B, S, D, m, start;
   int units;                        // of a head row
@@ -70,7 +70,7 @@ __device__ __forceinline__ void rp_out(float x, __half& y) { y = __float2half_rn
 // terms of a sum, were fused by the compiler, which counted the rounding twice: a position of 2^31 was off by 2e-7, one
 // of 2^47 by 5e-3).  Then the nearest quarter turn, and the series of sine and cosine on [-pi / 4, pi / 4], whose next
 // terms are below 1.2e-10.
-__device__ __forceinline__ float2 rp_turn(double pos, double f, float factor) {
+__device__ __forceinline__ float2 rp_turn(double pos, double f, double factor) {
   constexpr double c0 = 0.15915494309189535, c1 = -9.839338337591243e-18;   // 1 / (2 pi)
   const double g = f * c0, h = fma(f, c0, -g) + f * c1;
   const double r = fma(pos, h, fma(pos, g, -__builtin_rint(pos * g)));
@@ -252,7 +252,7 @@ extern "C" int dash_rope(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh
                          int64_t k_st, int64_t k_sh, int Hkv, void* k_out, int64_t ko_sb, int64_t ko_st,
                          int64_t ko_sh, int dtype, const void* positions, int positions_int64,
                          int64_t pos_sb, int64_t pos_st, const double* inv_freq, int pairs, int start,
-                         int interleaved, int back, float factor, int B, int S, int D, void* stream) {
+                         int interleaved, int back, double factor, int B, int S, int D, void* stream) {
   using namespace dash;
   RopeArgs a = {};
   a.r[0] = RopeRows{q, q_sb, q_st, q_sh, q_out, qo_sb, qo_st, qo_sh, H, 1, 0};
@@ -270,7 +270,7 @@ extern "C" int dash_rope_append(const void* q, int64_t q_st, int64_t q_sh, int H
                                 int positions_int64, const int64_t* slots, void* k_cache, int64_t kc_sp,
                                 int64_t kc_st, int64_t kc_sh, void* v_cache, int64_t vc_sp, int64_t vc_st,
                                 int64_t vc_sh, int page_size, int num_pages, const double* inv_freq,
-                                int pairs, int start, int interleaved, float factor, int T, int D,
+                                int pairs, int start, int interleaved, double factor, int T, int D,
                                 void* stream) {
   using namespace dash;
   if (page_size <= 0 || num_pages < 0 || (T > 0 && !slots)) return kErrInvalid;

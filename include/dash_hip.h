@@ -824,7 +824,7 @@ int dash_rope(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, int H, vo
               int64_t qo_st, int64_t qo_sh, const void* k, int64_t k_sb, int64_t k_st, int64_t k_sh, int Hkv,
               void* k_out, int64_t ko_sb, int64_t ko_st, int64_t ko_sh, int dtype, const void* positions,
               int positions_int64, int64_t pos_sb, int64_t pos_st, const double* inv_freq, int pairs, int start,
-              int interleaved, int back, float factor, int B, int S, int D, void* stream);
+              int interleaved, int back, double factor, int B, int S, int D, void* stream);
 
 /* The same of T tokens' q [T, H, D] into q_out, with k [T, Hkv, D] turned and v copied into the rows `slots` of
  * caches [num_pages, page_size, Hkv, D] (strides of page, token and head; slot = page * page_size + offset; a slot
@@ -834,7 +834,7 @@ int dash_rope_append(const void* q, int64_t q_st, int64_t q_sh, int H, void* q_o
                      int dtype, const void* positions, int positions_int64, const int64_t* slots, void* k_cache,
                      int64_t kc_sp, int64_t kc_st, int64_t kc_sh, void* v_cache, int64_t vc_sp, int64_t vc_st,
                      int64_t vc_sh, int page_size, int num_pages, const double* inv_freq, int pairs, int start,
-                     int interleaved, float factor, int T, int D, void* stream);
+                     int interleaved, double factor, int T, int D, void* stream);
 
 /* Workspace bytes dash_attn_shared needs. */
 int dash_attn_shared_workspace_size(int B, int G, int H, int Hkv, int64_t T, int64_t* bytes);

@@ -50,3 +50,16 @@ def test_far_positions(far):
     _check(pos, torch.cat((torch.ones(1, dtype=torch.float64), rope.inv_freq(64)[0])))
     if abs(far) < 2 ** 31:
         _check(pos.to(torch.int32), rope.inv_freq(64)[0])
+
+
+@pytest.mark.parametrize("factor", [1.3688879454113936, 1.0 / 3.0, -1.1, 1.0 + 2.0 ** -25])
+def test_factors_of_64_bits(factor):
+    """The first is that of a 40-fold stretch (0.1 ln 40 + 1).  Rounded to 32 bits it would be off by 3e-8 of
+    itself, half a step more; the last would be 1."""
+    _check(torch.arange(2000), rope.inv_freq(64)[0], factor)
+    f = rope.inv_freq(64, device=DEV)[0]
+    x = torch.ones(50, 1, 64, device=DEV)
+    caches = torch.zeros(2, 1, 64, 1, 64, device=DEV)
+    pos, slots = torch.arange(50, device=DEV), torch.arange(50, device=DEV)
+    rope.rope_append(x, x, x, pos, slots, *caches, f, factor=factor)
+    assert torch.equal(caches[0, 0, :50], rope.apply_rope(x, None, pos, f, factor=factor))
