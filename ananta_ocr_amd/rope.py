@@ -14,6 +14,7 @@ tables of two-axis positions are page_rope's.
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .ops import _need_gpu, _ptr, _stream
@@ -112,6 +113,12 @@ def _leaves_in_capture(*xs):
         node.metadata["dash_capture"] = stream
 
 
+def _tangents(*xs):
+    """Whether a tensor carries a tangent of forward-mode differentiation."""
+    return forward_ad._current_level >= 0 and any(
+        x is not None and forward_ad.unpack_dual(x).tangent is not None for x in xs)
+
+
 class _RopeFn(torch.autograd.Function):
     """The turn by position * inv_freq (back: by the negative), times factor.  Its gradient is the
     turn the other way, so that this function is its own backward, to any order."""
@@ -120,6 +127,8 @@ class _RopeFn(torch.autograd.Function):
     def forward(ctx, q, k, positions, freqs, interleaved, start, factor, back):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(positions, freqs)
+        ctx.save_for_forward(positions, freqs)
+        ctx.shapes = q is not None and q.shape, k is not None and k.shape
         ctx.how = interleaved, start, factor, back
         return _turn(q, k, positions, freqs, interleaved, start, factor, back)
 
@@ -128,9 +137,22 @@ class _RopeFn(torch.autograd.Function):
         interleaved, start, factor, back = ctx.how
         pos, freqs = ctx.saved_tensors
         if dq is not None or dk is not None:
-            turn = _RopeFn.apply if torch.is_grad_enabled() else _turn     # (a graph of the gradients)
-            dq, dk = turn(dq, dk, pos, freqs, interleaved, start, factor, not back)
+            dq, dk = _rope(dq, dk, pos, freqs, interleaved, start, factor, not back)
         return dq, dk, None, None, None, None, None, None
+
+    @staticmethod
+    def jvp(ctx, tq, tk, *_):
+        pos, freqs = ctx.saved_tensors
+        outs = _rope(tq, tk, pos, freqs, *ctx.how)
+        some = tq if tq is not None else tk      # (the tangent of an output whose input has none is 0)
+        return tuple(some.new_zeros(s) if y is None and s else y for s, y in zip(ctx.shapes, outs))
+
+
+def _rope(q, k, *how):
+    """_turn, recorded where a gradient or a tangent is."""
+    if (torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k))) or _tangents(q, k):
+        return _RopeFn.apply(q, k, *how)
+    return _turn(q, k, *how)
 
 
 def _turn(q, k, pos, freqs, interleaved, start, factor, back):
@@ -162,8 +184,9 @@ def apply_rope(q, k, positions, inv_freq, interleaved=False, start=0, factor=1.0
     """q and k [T, heads, D] or [B, S, heads, D] (any strides; fp32, bf16 or fp16; k may be None) with
     the part [start, start + 2 len(inv_freq)) of every head row turned by its token's position times
     inv_freq, and scaled by factor; the rest as it is.  positions int32 or int64 [T], [S] or [B, S],
-    whole numbers of up to 2^53 of either sign.  Returns new tensors (q', k'), or q' alone where k is None; differentiable in q
-    and k, to any order.  D even, at most 256 pairs.  Under capture a leaf that an eager graph still
+    whole numbers of up to 2^53 of either sign.  Returns new tensors (q', k'), or q' alone where k is
+    None; differentiable in q and k, to any order, in forward mode too (torch.func's transforms are
+    refused by torch).  D even, at most 256 pairs.  Under capture a leaf that an eager graph still
     refers to is refused (a captured backward pass of it would end the process)."""
     if q.dim() not in (3, 4):
         raise ValueError("q: [T, heads, D] or [B, S, heads, D] needed")
@@ -182,13 +205,9 @@ def apply_rope(q, k, positions, inv_freq, interleaved=False, start=0, factor=1.0
     _part(q.shape[-1], inv_freq.numel(), start)
     with _device(q, k, positions, inv_freq):
         freqs = _freqs(inv_freq)
-    how = q, k, positions, freqs, bool(interleaved), start, float(factor), False
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        fresh = list(_leaves_in_capture(q, k))
-        q, k2 = _RopeFn.apply(*how)
-        del fresh
-    else:
-        q, k2 = _turn(*how)
+    fresh = list(_leaves_in_capture(q, k)) if torch.is_grad_enabled() else ()
+    q, k2 = _rope(q, k, positions, freqs, bool(interleaved), start, float(factor), False)
+    del fresh
     return q if k is None else (q, k2)
 
 
