@@ -14,11 +14,10 @@ tables of two-axis positions are page_rope's.
 import math
 
 import torch
-from torch.autograd import forward_ad
 
 from . import _lib
 from .ops import _need_gpu, _ptr, _stream
-from .tree import _device, _shape
+from .tree import _derivatives, _device, _shape
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 MAX_PAIRS = 256
@@ -113,12 +112,6 @@ def _leaves_in_capture(*xs):
         node.metadata["dash_capture"] = stream
 
 
-def _tangents(*xs):
-    """Whether a tensor carries a tangent of forward-mode differentiation."""
-    return forward_ad._current_level >= 0 and any(
-        x is not None and forward_ad.unpack_dual(x).tangent is not None for x in xs)
-
-
 class _RopeFn(torch.autograd.Function):
     """The turn by position * inv_freq (back: by the negative), times factor.  Its gradient is the
     turn the other way, so that this function is its own backward, to any order."""
@@ -150,7 +143,7 @@ class _RopeFn(torch.autograd.Function):
 
 def _rope(q, k, *how):
     """_turn, recorded where a gradient or a tangent is."""
-    if (torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k))) or _tangents(q, k):
+    if _derivatives(q, k):
         return _RopeFn.apply(q, k, *how)
     return _turn(q, k, *how)
 
@@ -234,7 +227,7 @@ def rope_append(q, k, v, positions, slots, k_cache, v_cache, inv_freq, interleav
                          f"{tuple(v_cache.shape)}")
     if q.dtype not in _TYPES or any(x.dtype != q.dtype for x in (k, v, k_cache, v_cache)):
         raise NotImplementedError("q, k, v and the caches of one type: fp32, bf16 or fp16")
-    if torch.is_grad_enabled() and any(x.requires_grad for x in (q, k, v, k_cache, v_cache)):
+    if _derivatives(q, k, v, k_cache, v_cache):
         raise ValueError("rope_append writes a cache: no gradients (apply_rope has them)")
     for x in (k_cache, v_cache):
         if x.stride(3) != 1 and D > 1:

@@ -23,7 +23,7 @@ import torch
 
 from . import _lib
 from .ops import _ptr, _stream
-from .tree import _device, _shape
+from .tree import _derivatives, _device, _shape
 
 MAX_VOCABULARY = 2 ** 20
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
@@ -52,7 +52,7 @@ def _sample(logits, uniforms, temperature, top_k, top_p, min_p, probs_dtype):
         raise NotImplementedError(f"vocabularies of at most {MAX_VOCABULARY} tokens, got {V}")
     if probs_dtype is not None and probs_dtype not in _TYPES:
         raise NotImplementedError("probabilities in fp32, bf16 or fp16")
-    if probs_dtype is not None and logits.requires_grad and torch.is_grad_enabled():
+    if probs_dtype is not None and _derivatives(logits):
         raise ValueError("the probabilities have no gradients (detach the logits)")
     if uniforms is not None:
         _shape(uniforms, (R,), "uniforms")

@@ -10,7 +10,7 @@ import torch
 
 from . import _lib
 from .ops import _bf16_rows, _i32, _ptr, _stream
-from .tree import _device, _shape
+from .tree import _derivatives, _device, _shape
 
 MAX_SEQS = 8192
 MAX_TOKENS = 2 ** 31 - 128
@@ -58,7 +58,7 @@ def attn_shared(q, k, v, block_table, context_lens, cu_seqlens_q, cu_groups, pre
         raise NotImplementedError(f"at most {MAX_SEQS} sequences and groups")
     if P * page_size > MAX_TOKENS:
         raise NotImplementedError("a block_table of at most 2^31 - 128 tokens a sequence")
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if _derivatives(q, k, v):
         raise ValueError("attn_shared has no gradients")
     with _device(q, k, v, block_table, context_lens, cu_seqlens_q, cu_groups, prefix_lens):
         q, k, v = _bf16_rows(q), _bf16_rows(k), _bf16_rows(v)

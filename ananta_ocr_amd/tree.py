@@ -18,6 +18,7 @@ import ctypes
 import functools
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .ops import _bf16_rows, _i32, _need_gpu, _ptr, _stream, _u8
@@ -38,6 +39,14 @@ def _device(*ts):
     if index < 0:
         _need_gpu(*ts)
     return _HERE if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
+
+
+def _derivatives(*ts):
+    """Whether a gradient of a tensor is asked for, or it carries a tangent (forward mode)."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+        return True
+    return forward_ad._current_level >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts)
 
 
 def _shape(t, shape, what):
