@@ -33,15 +33,19 @@ def inv_freq(dim, base=10000.0, scaling=None, device=None):
     * {"type": "yarn", "factor": s, "original_max_position_embeddings": n, "beta_fast": 32,
       "beta_slow": 1, "mscale": 1, "mscale_all_dim": 0}: frequencies of fewer than beta_slow turns
       over n positions are divided by s, those of more than beta_fast kept, with a linear ramp over
-      the index between; factor is g(mscale) / g(mscale_all_dim), g(x) = 0.1 x ln s + 1 (1 where s <= 1).
+      the index between (from the whole index below to the one above, or with "truncate": False from
+      the border itself); factor is "attention_factor" where that is given, else g(mscale) /
+      g(mscale_all_dim), g(x) = 0.1 x ln s + 1 (1 where s <= 1).
 
-    `factor` scales cos and sin (1 for the others)."""
+    `factor` scales cos and sin (1 for the others, which refuse an "attention_factor" that is not).
+    Other settings are not read."""
     dim = int(dim)
     if dim < 0 or dim % 2:
         raise ValueError(f"a rotary part of {dim} elements")
     m = dim // 2
     kind = None if scaling is None else scaling.get("type", scaling.get("rope_type", "default"))
     s = 1.0 if scaling is None else float(scaling.get("factor", 1.0))
+    given = None if scaling is None else scaling.get("attention_factor")
     if not s > 0.0:
         raise ValueError(f"a scaling factor of {s}")
     base, factor = float(base), 1.0
@@ -56,17 +60,24 @@ def inv_freq(dim, base=10000.0, scaling=None, device=None):
         def at(turns):                       # the index whose frequency makes so many turns
             return m * math.log(n / (turns * 2 * math.pi)) / math.log(base)
 
-        lo = max(math.floor(at(float(scaling.get("beta_fast", 32)))), 0)
-        hi = min(math.ceil(at(float(scaling.get("beta_slow", 1)))), dim - 1)
+        lo, hi = at(float(scaling.get("beta_fast", 32))), at(float(scaling.get("beta_slow", 1)))
+        if scaling.get("truncate", True):
+            lo, hi = math.floor(lo), math.ceil(hi)
+        lo, hi = max(lo, 0), min(hi, dim - 1)
         ramp = ((torch.arange(m, dtype=torch.float64) - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
         f = f / s * ramp + f * (1 - ramp)
 
         def g(x):
             return 0.1 * x * math.log(s) + 1.0 if s > 1 else 1.0
 
-        factor = g(float(scaling.get("mscale", 1))) / g(float(scaling.get("mscale_all_dim", 0)))
+        if given is None:
+            factor = g(float(scaling.get("mscale", 1))) / g(float(scaling.get("mscale_all_dim", 0)))
+        else:
+            factor = float(given)
     elif kind not in (None, "default", "ntk"):
         raise NotImplementedError(f"rope scaling {kind!r}")
+    if kind != "yarn" and given is not None and float(given) != 1.0:
+        raise NotImplementedError(f"rope scaling {kind!r} with an attention factor of {given}")
     return f if device is None else f.to(device), factor
 
 
