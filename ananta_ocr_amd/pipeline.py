@@ -302,6 +302,7 @@ def shared_step(step, q, k, v, k_cache, v_cache, block_table, inv_freq, cu_group
     the pool's table.  Returns out [T,H,D] (out_dtype); rows of no sequence give 0."""
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
+    shared_prefix._bf16(q, k_cache, v_cache)         # (before anything is written)
     q = rope.rope_append(q, k, v, step.positions, step.slots, k_cache, v_cache, inv_freq, interleaved,
                          start, factor)
     return shared_prefix.attn_shared(q, k_cache, v_cache, block_table, step.context_lens,

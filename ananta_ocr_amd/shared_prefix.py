@@ -9,17 +9,23 @@ import functools
 import torch
 
 from . import _lib
-from .ops import _bf16_rows, _i32, _ptr, _stream
+from .ops import _i32, _ptr, _rows, _stream
 from .tree import _derivatives, _device, _shape
 
 MAX_SEQS = 8192
 MAX_TOKENS = 2 ** 31 - 128
 
 
+def _bf16(*ts):
+    """Refuses other types: a cast would round queries, and copy a whole pool at every call."""
+    if any(t.dtype != torch.bfloat16 for t in ts):
+        raise NotImplementedError(f"queries and caches in bf16: {', '.join(str(t.dtype) for t in ts)}")
+
+
 def attn_shared(q, k, v, block_table, context_lens, cu_seqlens_q, cu_groups, prefix_lens, scale,
                 out_dtype=torch.float32, return_lse=False):
-    """Attention of new tokens q [T,H,128] over pages k/v [pages, page_size, Hkv, 128] (H a multiple of
-    Hkv, any page size) through block_table [B,P].  Rows cu_seqlens_q[b] .. cu_seqlens_q[b + 1] - 1 are
+    """Attention of new tokens q [T,H,128] over pages k/v [pages, page_size, Hkv, 128] (bf16, H a
+    multiple of Hkv, any page size) through block_table [B,P].  Rows cu_seqlens_q[b] .. cu_seqlens_q[b + 1] - 1 are
     the new tokens of sequence b, at positions context_lens[b] + i, their keys and values already
     written (rope.rope_append); each attends every key of its sequence up to itself.
 
@@ -61,7 +67,8 @@ def attn_shared(q, k, v, block_table, context_lens, cu_seqlens_q, cu_groups, pre
     if _derivatives(q, k, v):
         raise ValueError("attn_shared has no gradients")
     with _device(q, k, v, block_table, context_lens, cu_seqlens_q, cu_groups, prefix_lens):
-        q, k, v = _bf16_rows(q), _bf16_rows(k), _bf16_rows(v)
+        _bf16(q, k, v)
+        q, k, v = _rows(q), _rows(k), _rows(v)
         bt, ctx, cu = _i32(block_table), _i32(context_lens), _i32(cu_seqlens_q)
         gr, pre = _i32(cu_groups), _i32(prefix_lens)
         out = torch.empty(T, H, D, dtype=out_dtype, device=q.device)
