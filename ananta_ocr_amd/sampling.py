@@ -73,7 +73,9 @@ def _sample(logits, uniforms, temperature, top_k, top_p, min_p, probs_dtype):
             x = x.contiguous()
         u, t, p, m = (None if y is None else y.float().contiguous() for y in (uniforms, t, p, m))
         if k is not None:
-            k = (k if k.dtype == torch.int32 else k.clamp(0, 2 ** 31 - 1).to(torch.int32)).contiguous()
+            if k.dtype != torch.int32:           # (widened first: the bound fits no narrower type)
+                k = k.to(torch.int64).clamp(0, 2 ** 31 - 1).to(torch.int32)
+            k = k.contiguous()
         token = None if u is None else torch.empty(R, dtype=torch.int64, device=x.device)
         probs = None if probs_dtype is None else torch.empty(R, V, dtype=probs_dtype, device=x.device)
         if R:
