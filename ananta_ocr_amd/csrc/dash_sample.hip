@@ -137,7 +137,8 @@ __device__ __forceinline__ uint64_t sm_place(uint32_t key, int v) {
 
 // What a row's tokens are measured by.
 struct SampleRow {
-  float top, t, bin_scale;
+  float top, t;
+  float half_top, bin_scale;              // half of the top; bins of half a logit's distance from it
   double c, scale;                        // log2(e) / T; 2^s
   float min_p;
   int k; float p;
@@ -164,8 +165,10 @@ __device__ __forceinline__ SampleRow sm_row(const A& a, int64_t r, uint64_t best
   if (w.k >= a.V) w.k = 0;
   w.filter = w.any && !w.greedy && (w.k > 0 || w.p < 1.f || w.min_p > 0.f);
   // past (s + 1) ln 2 T from the top a weight is none
-  const float range = fminf(w.top - low, (float)(a.bits + 1) * 0.6931472f * t);
-  w.bin_scale = range > 1e-30f ? fmaxf((float)kSmBins / range, 1e-37f) : 1e-37f;
+  // (halves: two logits may lie further apart than the largest number)
+  w.half_top = 0.5f * w.top;
+  const float range = fminf(fmaf(low, -0.5f, w.half_top), (float)(a.bits + 1) * 0.34657359f * t);
+  w.bin_scale = range > 5e-31f ? (float)kSmBins / range : 2e-37f;
   return w;
 }
 // The best token of a row and its lowest logit, from its chunks: a lane each.
@@ -220,7 +223,9 @@ __device__ __forceinline__ uint64_t sm_whole(const SampleRow& w, double e) {
   return __builtin_bit_cast(uint64_t, fma(e, w.scale, 4503599627370496.0)) - 0x4330000000000000ull;
 }
 // How far a logit lies below the top, in bins.
-__device__ __forceinline__ float sm_below(const SampleRow& w, float x) { return (w.top - x) * w.bin_scale; }
+__device__ __forceinline__ float sm_below(const SampleRow& w, float x) {
+  return fmaf(x, -0.5f, w.half_top) * w.bin_scale;
+}
 __device__ __forceinline__ int sm_bin(const SampleRow& w, float x) {
   return (int)fminf(sm_below(w, x), (float)(kSmBins - 1));
 }
@@ -370,7 +375,7 @@ __device__ __forceinline__ void sm_select(const SampleRow& w, SampleShared& s) {
       }
       if (w.min_p > 0.f) {
         // where exp((x - M) / T) = min_p, and the bins beside it, for what the logarithm may be off by
-        const float d = fminf(-logf(w.min_p) * w.t * w.bin_scale, (float)(kSmBins - 1));
+        const float d = fminf(-logf(w.min_p) * (0.5f * w.t * w.bin_scale), (float)(kSmBins - 1));
         st.sure = min(st.sure, max((int)d - 1, 0));
         st.end = min(st.end, (int)d + 2);
       }
