@@ -13,7 +13,10 @@ falling logits, of equals the lower id first,
 The first always does.  A temperature that is not above 0 keeps the first alone.  Logits of -inf and NaN
 are masked; +inf counts as the largest number of 32 bits.  Weights are whole numbers of 2^-s of the best token's, s =
 62 - ceil(log2 V) but at most 51, so that sums are exact and no result depends on how a launch ran; a token
-below half of that counts as none.
+below half of that counts as none (of 131,072, one more than 31.9 temperatures below the best).
+
+Uniforms, temperature, top_p and min_p are taken in 32 bits, as are logits of other types than fp32, bf16 and fp16:
+what has 64 is rounded.  (A uniform that so becomes 1 draws the last token that stays.)
 """
 
 import ctypes

@@ -42,3 +42,27 @@ def test_logits_further_apart_than_the_largest_number(V, dtype, t):
     for k, p, m in ((0, 1.0, 0.0), (V // 2, 1.0, 0.0), (0, 0.6, 0.0), (V // 2 + 1, 0.7, 0.0), (0, 1.0, 0.3),
                     (0, 0.9, 1e-4), (0, 1.0, 1.0)):
         _check(x, u, t, k, p, m)
+
+
+@pytest.mark.parametrize("V", [700, 32000, 131072])
+@pytest.mark.parametrize("spread, t", [(2.5, 1.0), (2.5, 0.05), (40.0, 1.0), (0.01, 1.0)])
+def test_what_whole_number_weights_leave_out(V, spread, t):
+    """Against a softmax that leaves no token out.  With s = 62 - ceil(log2 V), 51 at most, a weight below
+    2^-(s + 1) of the best token's is none: that much of a probability at most.  The V roundings of 2^-(s + 1) in
+    the sum, which is 1 at least, are V 2^-(s + 1) of the others, beside half a step of 32 bits and the
+    reference's own 2^-40."""
+    x, _ = _logits(3, V, V + 1, spread=spread)
+    z = x.double() / torch.tensor(t, dtype=torch.float32).double()
+    w = (z - z.max(1, keepdim=True).values).exp()
+    want = w / w.sum(1, keepdim=True)
+    s = min(51, 62 - (V - 1).bit_length())
+    got = sampling.token_probs(x.to(DEV), t).double().cpu()
+    tol = want * (2.0 ** -24 + V * 2.0 ** -(s + 1) + 2.0 ** -40) + 2.0 ** -(s + 1)
+    assert bool(((got - want).abs() <= tol).all())
+    # the k tokens of most weight
+    order = want.sort(1, descending=True)
+    k = min(V // 2, 40)
+    kept = torch.zeros_like(want).scatter(1, order.indices[:, :k], order.values[:, :k])
+    kept /= kept.sum(1, keepdim=True)
+    got = sampling.token_probs(x.to(DEV), t, k).double().cpu()
+    assert bool(((got - kept).abs() <= kept * (2.0 ** -24 + 2.0 ** -s * V + 2.0 ** -39) + 2.0 ** -s).all())
