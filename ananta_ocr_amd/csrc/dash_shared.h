@@ -812,12 +812,18 @@ inline SharedPlan shared_plan(int B, int G, int H, int Hkv, int64_t T) {
   return p;
 }
 
+// Sizes whose rows, partial rows and grids 32 bits hold (and whose workspace 64 do).
+inline bool shared_takes(int B, int G, int H, int Hkv, int64_t T) {
+  return H % Hkv == 0 && B <= kShMaxSeqs && G <= kShMaxSeqs && T <= INT32_MAX - kShThreads && 2 * T * H <= INT32_MAX &&
+         fits_grid((T * H + 3) / 4, 256) && fits_grid((int64_t)shared_plan(B, G, H, Hkv, T).W * Hkv, 256);
+}
+
 }  // namespace dash
 
 extern "C" int dash_attn_shared_workspace_size(int B, int G, int H, int Hkv, int64_t T, int64_t* bytes) {
   using namespace dash;
   if (!bytes || B < 0 || G < 0 || H <= 0 || Hkv <= 0 || T < 0) return kErrInvalid;
-  if (H % Hkv != 0 || B > kShMaxSeqs || G > kShMaxSeqs || T > INT32_MAX) return kErrUnsupported;
+  if (!shared_takes(B, G, H, Hkv, T)) return kErrUnsupported;
   *bytes = shared_plan(B, G, H, Hkv, T).total;
   return kOk;
 }
@@ -839,8 +845,7 @@ extern "C" int dash_attn_shared(const void* q, int64_t q_st, int64_t q_sh, const
     return kErrInvalid;
   if (B > 0 && P > 0 && !block_table) return kErrInvalid;
   if (num_pages > 0 && (!k || !v)) return kErrInvalid;
-  if (D != 128 || H % Hkv != 0 || B > kShMaxSeqs || G > kShMaxSeqs || !(scale > 0.f) ||
-      (int64_t)P * page_size > kShMaxKeys)
+  if (D != 128 || !(scale > 0.f) || (int64_t)P * page_size > kShMaxKeys || !shared_takes(B, G, H, Hkv, T))
     return kErrUnsupported;
   const int64_t strides[] = {q_st, q_sh, k_sp, k_st, k_sh, v_sp, v_st, v_sh};
   for (int64_t s : strides)
@@ -848,10 +853,7 @@ extern "C" int dash_attn_shared(const void* q, int64_t q_st, int64_t q_sh, const
   const void* ptrs[] = {q, k, v};
   for (const void* x : ptrs)
     if ((uintptr_t)x % 16 != 0) return kErrUnsupported;
-  if (T > INT32_MAX - kShThreads || 2 * T * H > INT32_MAX || !fits_grid((T * H + 3) / 4, 256))
-    return kErrUnsupported;
   const SharedPlan p = shared_plan(B, G, H, Hkv, T);
-  if (!fits_grid((int64_t)p.W * Hkv, 256)) return kErrUnsupported;
   if (!workspace || workspace_bytes < p.total || (uintptr_t)workspace % 256 != 0) return kErrWorkspace;
   char* w = (char*)workspace;
   SharedArgs a = {};
