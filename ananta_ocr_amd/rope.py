@@ -14,6 +14,7 @@ tables of two-axis positions are page_rope's.
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .ops import _need_gpu, _ptr, _stream
@@ -131,8 +132,9 @@ class _RopeFn(torch.autograd.Function):
     def forward(ctx, q, k, positions, freqs, interleaved, start, factor, back):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(positions, freqs)
-        ctx.save_for_forward(positions, freqs)
-        ctx.shapes = q is not None and q.shape, k is not None and k.shape
+        if forward_ad._current_level >= 0:
+            ctx.save_for_forward(positions, freqs)
+            ctx.shapes = q is not None and q.shape, k is not None and k.shape
         ctx.how = interleaved, start, factor, back
         return _turn(q, k, positions, freqs, interleaved, start, factor, back)
 
