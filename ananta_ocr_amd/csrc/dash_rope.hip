@@ -8,16 +8,17 @@
 //
 // The angle is a product in 64 bits: a position of 10^5 has 10^5 radians, whose 32-bit rounding alone is 4e-3.  Its
 // sine and cosine are series in 64 bits, good to 1.2e-10 (33 bits, beside the 24 that they are rounded to), once a
-// (token, pair), in LDS, for all heads; the turn is two products and an addition in 32 bits, rounded once to the row's type.
+// (token, pair), in LDS, for all heads; the turn is two products and an addition in 32 bits, rounded once to the row's
+// type.
 //
 // A work-group takes a token, or a few of few heads, and all its heads.  Its units are two 16-byte chunks: the two
 // that a pair of the halves' layout needs, or two neighbours (single elements where an address, a stride or the
 // part does not fit 16 bytes).  Their loads start before the sines are there.
 //
 // Bound by HBM: 8,190 tokens of 10 + 10 + 10 heads of 128 bf16 in 38 us (126 MB read and written, 3.3 TB/s), 20 heads
-// turned as interleaved pairs 21.6 us (84 MB, 3.9 TB/s); with two or four units a thread in flight, or loads and stores
-// past the caches, 40 to 46 and 25 to 33.  Six wavefronts a SIMD: 38 us, five 44, eight (registers to memory) 46; replayed
-// from a graph, seven 31.2, six 32.7.
+// turned as interleaved pairs 30.6 us (84 MB, 2.7 TB/s); replayed over the same rows, which the last cache then holds, 31
+// and 21.2.  With two or four units a thread in flight, or loads and stores past the caches, 40 to 46 and (replayed) 25 to
+// 33.  Six wavefronts a SIMD: 38 us, five 44, eight (registers to memory) 46; replayed, seven 31.2, six 32.7.
 // A few tokens 4 us, of latency.
 #include <hip/hip_fp16.h>
 
@@ -209,7 +210,7 @@ static int rope_launch(RopeArgs& a, bool pairs, hipStream_t st) {
   // four tokens (8,190 of 20 heads 21.6 us, one at a time 23.3), one where rows go to a cache (37.8 us, four 45.8)
   // unless that leaves threads without a unit, or the CUs without a work-group
   a.per = a.slots ? std::max(1, std::min(kRpTokens, kRpThreads / (a.heads * a.units))) : kRpTokens;
-  if (tokens < 1024) a.per = 1;
+  if (tokens < 1024) a.per = 1;      // (1,023 of 20 heads 16.2 us replayed, four at a time 16.9; 1,536: 16.9, 16.7)
   const int64_t groups = (tokens + a.per - 1) / a.per;
   if (!fits_grid(groups, kRpThreads)) return kErrUnsupported;
   const dim3 grid((unsigned)groups), block(kRpThreads);

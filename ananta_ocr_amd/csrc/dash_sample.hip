@@ -21,11 +21,13 @@
 //   sample_pick    the tokens between, listed
 //   sample_draw    the borders within the list, by the tokens' (logit, id); the chunk, the tile and then the
 //                  token that u falls into; the probabilities
-// Bound by the vector units and, a row a work-group, by latency.  64 rows of 131,072 bf16 (16.8 MB, which each step
-// over them fetches again: little stays in the L2s from launch to launch) 61 us: max 7.0, bins 15.6 (an exponential of 64
-// bits a token; the LDS atomics 1.5), select 6.2, pick 11.3, draw 27.4 (the rows whose top-p leaves thousands).  48 rows of
-// 100,003 fp32 with probabilities 67 us: 6.2, 12.2, 6.1, 9.8, 35.8.  One row of 32,000 27 to 30 us where it filters, 6.8
-// where it is greedy; cut into chunks it took 34 where a work-group took 31.
+// Bound by the latency of dependent launches, and of the passes and barriers within them; the bins' by the vector
+// units. 64 rows of 131,072 bf16 (16.8 MB, which each step over them fetches again: little stays in the L2s from launch
+// to launch) 63 us: max 7.0, bins 15.4 (an exponential of 64 bits a token; the LDS atomics 1.5), select 6.2, pick 11.3
+// (a read: only listed tokens are weighed), draw 27.7 (the rows whose top-p leaves thousands).  By the instructions
+// counted, four cycles each, the vector units are busy for 3.3, 8.5, 0.2, 3.4 and 0.8 us of these.  48 rows of 100,003
+// fp32 with probabilities 68 us: 6.2, 11.8, 6.3, 9.5, 35.9 (busy 2.0, 5.1, 0.2, 2.2, 4.1).  One row of 32,000 27 to 30
+// us where it filters, 6.8 where it is greedy; cut into chunks it took 34 where a work-group took 31.
 //
 // A list that would be too long (many tokens of one logit) is not made: its work-group reads the row again
 // instead, as often as the border needs.
@@ -46,7 +48,9 @@ constexpr int kSmFew = 1024;              // so many tokens are all listed (one 
 constexpr int kSmMaxV = 1 << 20;
 constexpr int kSmTiles = 256;             // tiles of a row's work-group, or of a chunk's, at most
 constexpr int kSmShort = 32768;           // tokens of a row that one work-group takes
-constexpr int kSmMany = 256;              // rows that take a work-group each, however long
+// Rows that take a work-group each, however long: as many as there are CUs.  (255 rows of 131,072 bf16 in chunks, and a
+// work-group a row: top-k 50 and top-p 109 us, 94; top-p alone 141, 170.  128 rows: 77, 90; 98, 165.)
+constexpr int kSmMany = 256;
 constexpr int kSmCut = 256;               // steps a pass of the search for a border
 
 struct SampleState {                      // of a row, once its bins are known
@@ -961,7 +965,8 @@ __global__ __launch_bounds__(NT) void sample_draw_kernel(SampleArgs a) {
 }
 
 // The same, a work-group a row.  A short row stays in LDS (HELD): one CU takes 5 us to read 128 KB, from the L2
-// too, and four of the five steps read the row.
+// too, and four of the five steps read the row.  The room is a row of kSmShort tokens' however short the row is, so that
+// a CU takes one at a time: 256 rows of 32,000 fp32 42 us (top-k and top-p), 2,048 of 4,096 160.
 template <typename T, bool HELD>
 __global__ __launch_bounds__(kSmWide) void sample_row_kernel(SampleArgs a) {
   constexpr int NT = kSmWide, E = SmVec<T>::kN, VECS = HELD ? kSmShort / E : 1;

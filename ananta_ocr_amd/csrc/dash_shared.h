@@ -19,9 +19,15 @@
 // launch before it takes 5: 4 answers 22.0 us and 19.4, 32 answers 100.4 and 97.8); more need the plan kernel.
 //
 // Bound by HBM where the cache is long: 32 answers to 4 prompts, 10 heads of 128, a call 98 us: attention 92.5, 475 MB
-// fetched (every key once, a prompt's for all its answers) at 5.1 TB/s, merge 6.6.  64 answers to one prompt 82 us:
-// 314 MB, whose 64 rows a tile need twice the products a key, 80 + 6.6.  Few keys are bound by the chain lengths, pages,
-// keys, sums, merge: 4 answers 13.3 + 6.7 us.
+// fetched (every key once, a prompt's for all its answers) at 5.1 TB/s, merge 6.6.  64 answers to one prompt 82 us, 314
+// MB at 3.9 TB/s in 81, merge 6.4: of its 1,011 units a head 585 are own keys, one row of a tile of 64, whose second
+// row tile's wavefronts leave at once, and a CU's two work-groups wait for a unit's keys, sums and barriers in turn
+// (matrix cores busy 14 % of the time, vector units 27 %; of the 32 answers 13 and 23).  Few keys are bound by the
+// chain lengths, pages, keys, sums, merge: 4 answers 13.4 + 6.6 us.
+//
+// A prompt itself: every row tile of a sequence takes the keys up to the last row's, and half of the units of one
+// without a context hold none that the tile sees: they are fetched, and left at once.  8,190 tokens of 10 heads 651 us
+// (2,730: 125).
 #pragma once
 
 namespace dash {
@@ -790,8 +796,9 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(SharedArgs a) {
     a.lse[row * a.lse_st + (int64_t)h * a.lse_sh] = any ? (M + log2f(L)) * 0.6931471805599453f : -INFINITY;
 }
 
-// Row tiles of a work-group by the rows that share a key head (a group's on average), and its work-groups:
-// four a CU of the one-stage kernel, two of the others.
+// Row tiles of a work-group by the rows that share a key head, and its work-groups: four a CU of the one-stage kernel,
+// two of the others.  The rows are a group's on average, all that the host knows: one group beside many sequences of no
+// group counts them as its own, which makes the tiles of their single rows larger than they need.
 struct SharedPlan { int rt, W; int64_t parts, head, starts, seg, rows, ml, o, total; };
 inline SharedPlan shared_plan(int B, int G, int H, int Hkv, int64_t T) {
   SharedPlan p;

@@ -1,6 +1,6 @@
 """Pages of a paged cache on the HIP kernels (csrc/dash_kvpages.hip): copied, shared between
-sequences (fork), handed out (reserve), given back (free) and moved together (compact), the rows of accepted drafted tokens
-moved up (keep), and the slots of a step's new tokens (step_rows).
+sequences (fork), handed out (reserve), given back (free) and moved together (compact), the rows of
+accepted drafted tokens moved up (keep), and the slots of a step's new tokens (step_rows).
 
 The state is three int32 tensors on the GPU: ``refs`` [num_pages], how many table entries name a
 page (0: free); ``table`` [R, P], the pages of every sequence row; ``lens`` [R], the tokens of a

@@ -25,16 +25,17 @@ def _bf16(*ts):
 def attn_shared(q, k, v, block_table, context_lens, cu_seqlens_q, cu_groups, prefix_lens, scale,
                 out_dtype=torch.float32, return_lse=False):
     """Attention of new tokens q [T,H,128] over pages k/v [pages, page_size, Hkv, 128] (bf16, H a
-    multiple of Hkv, any page size) through block_table [B,P].  Rows cu_seqlens_q[b] .. cu_seqlens_q[b + 1] - 1 are
-    the new tokens of sequence b, at positions context_lens[b] + i, their keys and values already
-    written (rope.rope_append); each attends every key of its sequence up to itself.
+    multiple of Hkv, any page size) through block_table [B,P].  Rows cu_seqlens_q[b] ..
+    cu_seqlens_q[b + 1] - 1 are the new tokens of sequence b, at positions context_lens[b] + i, their
+    keys and values already written (rope.rope_append); each attends every key of its sequence up to
+    itself.
 
     Sequences cu_groups[g] .. cu_groups[g + 1] - 1 (cu_groups [G + 1], prefix sums over the batch) have
     the keys below prefix_lens[g] in common: they are read through one table row, once for the group,
     that of the first sequence with new tokens that holds them all (or the most of them).  Sequences
     without new tokens, as an answer that has left, may hold anything.  A forked row shares its full
-    pages, and a copy of the partly filled one holds the same keys.  Sequences of no group, or of one with a prefix of 0, share nothing; cu_groups and
-    prefix_lens may be None.  Prefix sums past the rows or the batch are cut to them.
+    pages, and a copy of the partly filled one holds the same keys.  Sequences of no group, or of one
+    with a prefix of 0, share nothing; cu_groups and prefix_lens may be None.  Prefix sums past the rows or the batch are cut to them.
 
     Returns out [T,H,128] (fp32 or bf16) and with return_lse the log-sum-exp [T,H] fp32; a row that
     sees no key, or of no sequence (a batch padded to a fixed size), gives 0 and -inf.  At most 8,192
