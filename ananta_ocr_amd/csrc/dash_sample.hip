@@ -21,13 +21,13 @@
 //   sample_pick    the tokens between, listed
 //   sample_draw    the borders within the list, by the tokens' (logit, id); the chunk, the tile and then the
 //                  token that u falls into; the probabilities
-// Bound by the latency of dependent launches, and of the passes and barriers within them; the bins' by the vector
-// units. 64 rows of 131,072 bf16 (16.8 MB, which each step over them fetches again: little stays in the L2s from launch
-// to launch) 63 us: max 7.0, bins 15.4 (an exponential of 64 bits a token; the LDS atomics 1.5), select 6.2, pick 11.3
-// (a read: only listed tokens are weighed), draw 27.7 (the rows whose top-p leaves thousands).  By the instructions
-// counted, four cycles each, the vector units are busy for 3.3, 8.5, 0.2, 3.4 and 0.8 us of these.  48 rows of 100,003
-// fp32 with probabilities 68 us: 6.2, 11.8, 6.3, 9.5, 35.9 (busy 2.0, 5.1, 0.2, 2.2, 4.1).  One row of 32,000 27 to 30
-// us where it filters, 6.8 where it is greedy; cut into chunks it took 34 where a work-group took 31.
+// Bound by the latency of dependent launches, and of the passes and barriers within them; the bins' for more than half
+// by the vector units.  64 rows of 131,072 bf16 (16.8 MB, which each step over them fetches again: little stays in the
+// L2s from launch to launch) 63 us: max 7.0, bins 15.4 (an exponential of 64 bits a token; the LDS atomics 1.5), select
+// 6.2, pick 11.3 (a read: only listed tokens are weighed), draw 27.7 (the rows whose top-p leaves thousands).  By the
+// instructions counted, four cycles each, the vector units are busy for 3.3, 8.5, 0.2, 3.4 and 0.8 us of these.  48
+// rows of 100,003 fp32 with probabilities 68 us: 6.2, 11.8, 6.3, 9.5, 35.9 (busy 2.0, 5.1, 0.2, 2.2, 4.1).  One row of
+// 32,000 27 to 30 us where it filters, 6.8 where it is greedy; cut into chunks it took 34 where a work-group took 31.
 //
 // A list that would be too long (many tokens of one logit) is not made: its work-group reads the row again
 // instead, as often as the border needs.

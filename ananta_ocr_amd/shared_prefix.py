@@ -35,7 +35,8 @@ def attn_shared(q, k, v, block_table, context_lens, cu_seqlens_q, cu_groups, pre
     that of the first sequence with new tokens that holds them all (or the most of them).  Sequences
     without new tokens, as an answer that has left, may hold anything.  A forked row shares its full
     pages, and a copy of the partly filled one holds the same keys.  Sequences of no group, or of one
-    with a prefix of 0, share nothing; cu_groups and prefix_lens may be None.  Prefix sums past the rows or the batch are cut to them.
+    with a prefix of 0, share nothing; cu_groups and prefix_lens may be None.  Prefix sums past the
+    rows or the batch are cut to them.
 
     Returns out [T,H,128] (fp32 or bf16) and with return_lse the log-sum-exp [T,H] fp32; a row that
     sees no key, or of no sequence (a batch padded to a fixed size), gives 0 and -inf.  At most 8,192
